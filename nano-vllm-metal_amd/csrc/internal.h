@@ -227,6 +227,13 @@ hipError_t launch_paged_prefill(const float *q, int64_t B, int64_t L, int64_t D,
                                 float scale, int causal, int Hkv, int Hq, int out_dtype,
                                 void *out, hipStream_t st);
 
+// Microscaled operands (include/nvm_mx.h): argument checks of the entry
+// points (NVM_OK, or the status that set_error returned).
+constexpr int64_t kMxMaxRow = 1 << 20;  // values of a row
+int mx_check_rows(const char *op, int64_t rows, int64_t n, int format, const char *what);
+int mx_check_tensor(const char *op, const void *codes, const uint8_t *scales, int64_t scale_ld,
+                    int64_t n, const char *what);
+
 // Combine: y[t] = rnd(sum_j rnd(down[t*k+j] * score[t,j])).
 hipError_t launch_combine(int dtype, const void *down, const void *scores, int64_t T, int k,
                           int64_t H, void *y, hipStream_t st);

@@ -1,0 +1,175 @@
+// Microscaled formats on the device (include/nvm_mx.h): rounding of a block,
+// and the scaled matrix instruction's operands.
+#pragma once
+
+#include "common.h"
+#include "nvm_mx.h"
+
+namespace nvm {
+
+template <int FMT>
+struct Mx {
+  static constexpr int kEmax = FMT == NVM_MX_FP4 ? 2 : 8;  // exponent of the largest element
+  static constexpr int kBits = FMT == NVM_MX_FP4 ? 4 : 8;
+  static constexpr int kMfma = FMT == NVM_MX_FP4 ? 4 : 0;  // the instruction's format code
+};
+
+// Scale byte of a block from the float32 bits of its largest magnitude.
+template <int FMT>
+__device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {
+  const int e = (int)(amax_bits >> 23);
+  return e == 255 ? 255u : (uint32_t)max(0, e - Mx<FMT>::kEmax);
+}
+// 2^(127 - b), the factor that takes values to elements (b = 255, a block
+// with a NaN or an infinity: zero, after mx_quiet).
+__device__ __forceinline__ float mx_factor(uint32_t b) {
+  return b == 255u ? 0.f : __uint_as_float((254u - b) << 23);
+}
+// 2^(b - 127); NaN for 255.
+__device__ __forceinline__ float mx_scale(uint32_t b) {
+  return __uint_as_float(b == 0u ? 0x00400000u : b == 255u ? 0x7FC00000u : b << 23);
+}
+
+// Eight values to element codes (FP4: one dword, FP8: two).  x * factor is
+// exact (a power of two; results below float32's normal range round to zero
+// either way); the conversions round to nearest even.  E2M1 saturates in the
+// conversion, E4M3 is clamped before it (a conversion of larger values gives
+// NaN).  `bad`: a block of NaNs or infinities, whose codes are zero.
+template <int FMT>
+__device__ __forceinline__ u32x2 mx_encode8(const float (&x)[8], float factor, bool bad) {
+  u32x2 o = {0u, 0u};
+  if constexpr (FMT == NVM_MX_FP4) {
+    uint32_t d = 0;
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, x[0] * factor, x[1] * factor, 1.0f, 0);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, x[2] * factor, x[3] * factor, 1.0f, 1);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, x[4] * factor, x[5] * factor, 1.0f, 2);
+    d = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(d, x[6] * factor, x[7] * factor, 1.0f, 3);
+    o.x = bad ? 0u : d;
+  } else {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __builtin_amdgcn_fmed3f(x[i] * factor, -448.f, 448.f);
+    int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+    a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], a, true);
+    int b = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+    b = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], b, true);
+    o.x = bad ? 0u : (uint32_t)a;
+    o.y = bad ? 0u : (uint32_t)b;
+  }
+  return o;
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// Largest magnitude of eight values, as float32 bits (NaNs and infinities
+// come out largest).
+__device__ __forceinline__ uint32_t absmax8(const float (&x)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(x[i]));
+  return m;
+}
+
+// Operands of v_mfma_scale_f32_16x16x128_f8f6f4, row or column lane % 16.
+// Both operands' k-values 32 G .. 32 G + 31 are scaled by the byte that lane
+// group G = lane / 16 passes.  E2M1: the lane holds those 32 values, 16
+// bytes; E4M3: it holds k-values 16 G .. + 15 and 64 + 16 G .. + 15, 16 bytes
+// each.
+typedef int mx_operand __attribute__((ext_vector_type(8)));
+
+template <int FMT>
+struct MxFrag {
+  u32x4 v[FMT == NVM_MX_FP4 ? 1 : 2];
+  __device__ __forceinline__ mx_operand operand() const {
+    if constexpr (FMT == NVM_MX_FP4)
+      return mx_operand{(int)v[0].x, (int)v[0].y, (int)v[0].z, (int)v[0].w, 0, 0, 0, 0};
+    else
+      return mx_operand{(int)v[0].x, (int)v[0].y, (int)v[0].z, (int)v[0].w,
+                        (int)v[1].x, (int)v[1].y, (int)v[1].z, (int)v[1].w};
+  }
+};
+
+// c += w . x^T: rows (4 G + i of c) from the FP4 weights, columns (lane % 16)
+// from the activations.
+template <int FMT>
+__device__ __forceinline__ f32x4 mx_mfma(const MxFrag<NVM_MX_FP4> &w, uint32_t ws,
+                                         const MxFrag<FMT> &x, uint32_t xs, f32x4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+      w.operand(), x.operand(), c, Mx<NVM_MX_FP4>::kMfma, Mx<FMT>::kMfma, 0, (int)ws, 0, (int)xs);
+}
+
+// g / (1 + exp(-g)) * u
+__device__ __forceinline__ float mx_swiglu(float g, float u) { return g / (1.f + expf(-g)) * u; }
+
+// Four neighbouring outputs of a row (element i of out) in the output type;
+// `left` of them are inside the row; `whole`: rows are a multiple of four
+// outputs, so the four are aligned and all inside.
+__device__ __forceinline__ void mx_store4(void *out, int dt, int64_t i, f32x4 v, int left,
+                                          bool whole) {
+  if (left <= 0) return;
+  if (dt == NVM_MX_F32) {
+    float *o = (float *)out + i;
+    if (whole) {
+      *(f32x4 *)o = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < left) o[e] = v[e];
+    }
+    return;
+  }
+  const bool bf = dt == NVM_MX_BF16;
+  const u32x2 d = bf ? u32x2{Act<DT_BF16>::pack2(v[0], v[1]), Act<DT_BF16>::pack2(v[2], v[3])}
+                     : u32x2{Act<DT_F16>::pack2(v[0], v[1]), Act<DT_F16>::pack2(v[2], v[3])};
+  uint16_t *o = (uint16_t *)out + i;
+  if (whole) {
+    *(u32x2 *)o = d;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) o[e] = (uint16_t)((e & 2 ? d.y : d.x) >> (16 * (e & 1)));
+  }
+}
+
+// One block of 32 MX outputs of row m from column k on: lane group G holds
+// values 4 G .. + 3 and 16 + 4 G .. + 3 (h[0..3], h[4..7]); amax_bits: the
+// largest magnitude of the whole block.
+template <int OFMT>
+__device__ __forceinline__ void mx_store_block(const float (&h)[8], uint32_t amax_bits, int64_t m,
+                                               int k, int G, int K, void *codes, uint8_t *scales,
+                                               int64_t sld) {
+  const uint32_t b = mx_scale_byte<OFMT>(amax_bits);
+  const u32x2 o = mx_encode8<OFMT>(h, mx_factor(b), b == 255u);
+  if constexpr (OFMT == NVM_MX_FP4) {
+    uint16_t *c = (uint16_t *)codes + (m * K + k) / 4 + G;
+    c[0] = (uint16_t)o.x;
+    c[4] = (uint16_t)(o.x >> 16);
+  } else {
+    uint32_t *c = (uint32_t *)codes + (m * K + k) / 4 + G;
+    c[0] = o.x;
+    c[4] = o.y;
+  }
+  if (G == 0) scales[m * sld + k / 32] = (uint8_t)b;
+}
+
+// Arguments of the products (gate/up: two weights, MX output).
+struct MxMatmulArgs {
+  const uint8_t *a, *as;  // activations [M][N], scales
+  const uint8_t *w[2], *ws[2];
+  int64_t as_ld, ws_ld[2];
+  int64_t M;
+  int N, K;
+  int out_dtype;  // products: nvm_mx_dtype
+  void *out;      // [M][K], or MX codes
+  uint8_t *out_s;
+  int64_t out_sld;
+};
+// The products for few rows (mx_gemv.hip) and for many (mx_gemm.hip, at most
+// kMxMaxTiles output tiles: else hipErrorInvalidConfiguration).
+constexpr int64_t kMxMaxTiles = 1 << 22;
+hipError_t launch_mx_gemv(int format, bool dual, int out_format, const MxMatmulArgs &a,
+                          hipStream_t st);
+hipError_t launch_mx_gemm(int format, bool dual, int out_format, const MxMatmulArgs &a,
+                          hipStream_t st);
+
+}  // namespace nvm

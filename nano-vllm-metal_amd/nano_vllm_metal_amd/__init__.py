@@ -13,6 +13,8 @@ from .linear import QuantizedWeights, dequantize, quantize, quantized_linear, qu
 from .moe import Moe, grouped_expert_linear, moe_dispatch, route_and_dispatch, route_topk
 from .loader import load_moe_block, load_moe_blocks, read_config, sparse_layers
 from .attention import paged_attention
+from .mx import (MxTensor, mx_dequantize, mx_linear, mx_quantize, mx_swiglu,
+                 residual_rms_norm_mx)
 from .kv_cache import PagedKVCache
 from .qwen3 import Qwen3Config, Qwen3Model, qwen3_30b_a3b_config
 from .llm import LLM, GenerationOutput, SamplingParams
@@ -33,6 +35,12 @@ __all__ = [
     "read_config",
     "sparse_layers",
     "paged_attention",
+    "MxTensor",
+    "mx_quantize",
+    "mx_dequantize",
+    "mx_linear",
+    "mx_swiglu",
+    "residual_rms_norm_mx",
     "PagedKVCache",
     "Qwen3Config",
     "Qwen3Model",

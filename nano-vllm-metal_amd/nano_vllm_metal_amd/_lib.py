@@ -62,6 +62,13 @@ SIGNATURES = {
     "nvm_embedding": [_P, _I64, _P, _P, _P, _I64, _I64, _I, _I, _I, _P, _P],
     "nvm_qk_norm_rope_store": [_P, _I64, _I, _I, _I64, _P, _P, ctypes.c_float, _P, _P, _P, _I64,
                                _P, _P, _P, _P, _I64, _I64, _I, _P, _P, _P, _P],
+    "nvm_mx_quantize": [_P, _I64, _I64, _I64, _I, _I, _P, _P, _I64, _P],
+    "nvm_mx_dequantize": [_P, _P, _I64, _I64, _I64, _I, _I, _P, _P],
+    "nvm_residual_rms_norm_mx": [_P, _P, _P, _I64, _I64, ctypes.c_float, _I, _P, _I, _P, _P, _I64,
+                                 _P],
+    "nvm_mx_matmul": [_P, _P, _I64, _I, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P],
+    "nvm_mx_swiglu": [_P, _P, _I64, _I, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P,
+                      _I64, _P],
     "nvm_moe_forward_residual_norm": [_P, _I64, _I64, _I64, _I64, _I, _I, _I, _I, _I,
                                       _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                       _P, _P, ctypes.c_float, _P, _P, _I, _P, _SZ, _P],

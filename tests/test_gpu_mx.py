@@ -1,0 +1,492 @@
+"""GPU tests of the microscaled path (include/nvm_mx.h) against 64-bit results.
+
+Quantised codes and scales of given values are compared bit for bit.  Products:
+the scales are powers of two, and the sums are float32: at most N * 2^-23 *
+sum |a w| for N terms in some order, each addition off by at most one unit in
+the last place (2^-23, twice a rounding), plus one rounding of the result to
+its type (finfo.eps / 2).  With E4M3 activations the matrix instruction adds
+eight neighbouring products as integers in units of 2^-13 of (a power of two
+not above) the largest of them, and drops what lies below: less than 7 * 2^-13
+of that product for each eight, since the largest itself keeps its at most 6
+significant bits.  (E2M1 by E2M1 spans 2^-2 to 36, in multiples of 2^-2: nothing
+lies below.)  SwiGLU: the two sums' errors carried through
+g / (1 + e^-g) * u, whose factor has a derivative below 1.1 and is at most
+|g|, and 2^-20 of the result for exp, division and two products in float32
+(expf within 2 units, so 2^-22 each and a few of them).  The norm is float64:
+2^-40 covers a sum of 8192 terms.  Of those the codes have to be ones that a
+value within the error gets.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from oracle import mx_oracle as O
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+FMTS = ["mxfp4", "mxfp8"]
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _mx(x, fmt):
+    """An MxTensor of float values, by the oracle."""
+    from nano_vllm_metal_amd import MxTensor
+
+    c, b = O.quantize(x.double(), fmt)
+    return MxTensor(O.pack(c, fmt), b.to(torch.uint8), fmt)
+
+
+def _val(t):
+    return O.decode(t.codes, t.scales, t.fmt)
+
+
+def _same(t, x, fmt):
+    """t is the quantisation of x, bit for bit."""
+    c, b = O.quantize(x.double(), fmt)
+    assert t.fmt == fmt and t.shape == x.shape
+    assert torch.equal(t.scales.long(), b), "scales differ"
+    got = O.unpack(t.codes, fmt)
+    # (the sign of a zero stands for nothing)
+    zero = (c & (O.SIGN[fmt] - 1)) == 0
+    assert torch.equal(torch.where(zero, got & (O.SIGN[fmt] - 1), got),
+                       torch.where(zero, torch.zeros_like(c), c)), "codes differ"
+
+
+# ------------------------------------------------------------- quantisation
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+def test_quantize_every_16_bit_value(fmt, dt):
+    """All 65536 patterns: neighbours in a block, then shuffled (each block
+    with all sizes, most with a NaN or an infinity left out of the second
+    half), subnormals and both signs of zero among them."""
+    from nano_vllm_metal_amd import mx_quantize
+
+    bits = torch.arange(-2 ** 15, 2 ** 15, device=DEV, dtype=torch.int32).to(torch.int16)
+    x = bits.view(dt)
+    _same(mx_quantize(x.reshape(64, 1024), fmt), x.reshape(64, 1024), fmt)
+    y = x[torch.isfinite(x.float())]
+    y = y[torch.randperm(len(y), device=DEV, generator=_gen(1))]
+    y = y[:len(y) // 32 * 32].reshape(-1, 32)
+    _same(mx_quantize(y, fmt), y, fmt)
+    p = x[torch.randperm(len(x), device=DEV, generator=_gen(2))].reshape(-1, 32)
+    _same(mx_quantize(p, fmt), p, fmt)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantize_float32_borders(fmt):
+    """Values on and next to every rounding border of the elements, at scales
+    over the whole range, and random bit patterns."""
+    from nano_vllm_metal_amd import mx_quantize
+
+    grid = O.elements(fmt, DEV)
+    mid = ((grid[1:] + grid[:-1]) / 2).float()
+    v = torch.cat((mid, torch.nextafter(mid, mid + 1), torch.nextafter(mid, mid - 1), grid.float()))
+    v = torch.cat((v, -v))
+    pad = (-len(v)) % 31
+    v = torch.cat((v, v.new_zeros(pad))).reshape(-1, 31)
+    top = torch.full((len(v), 1), 4.0 if fmt == "mxfp4" else 256.0, device=DEV)
+    x = torch.cat((v, top), 1)
+    for e in (-140, -126, -100, -1, 0, 1, 60, 118):
+        y = torch.ldexp(x.double(), torch.tensor(e, device=DEV)).float()
+        _same(mx_quantize(y, fmt), y, fmt)
+    r = torch.randint(-2 ** 31, 2 ** 31 - 1, (999, 96), device=DEV, generator=_gen(3),
+                      dtype=torch.int32).view(torch.float32)
+    _same(mx_quantize(r, fmt), r, fmt)
+    r = torch.where(torch.isfinite(r), r, torch.zeros_like(r))
+    _same(mx_quantize(r, fmt), r, fmt)
+
+
+@pytest.mark.parametrize("M,n", [(1, 32), (3, 32), (1, 4096), (7, 96), (129, 544), (1000, 64)])
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_quantize_shapes(M, n, fmt, dt):
+    from nano_vllm_metal_amd import mx_quantize
+
+    x = (torch.randn(M, n, device=DEV, generator=_gen(M + n)) * 3).to(dt)
+    t = mx_quantize(x, fmt)
+    _same(t, x, fmt)
+    assert t.scales.stride(0) % 16 == 0
+
+
+def test_quantize_strides_and_leading_dimensions():
+    from nano_vllm_metal_amd import mx_quantize
+
+    big = torch.randn(40, 200, device=DEV, generator=_gen(5)).to(torch.bfloat16)
+    views = [big[:, :64], big[::2, 8:72], big[:, 3:67], big[1:, :96], big.t()[:64, :32],
+             big[:, :192].reshape(5, 8, 192), big[:, :192].reshape(5, 8, 192).transpose(0, 1),
+             big[:1, 8:40], big[3, 8:72], big[:, :32].expand(40, 32), big[:1, :64].expand(9, 64)]
+    for x in views:
+        _same(mx_quantize(x, "mxfp8"), x, "mxfp8")
+    t = mx_quantize(big[:0, :64], "mxfp4")
+    assert t.shape == (0, 64) and t.codes.shape == (0, 32)
+
+
+def test_quantize_writes_its_rows_only():
+    from nano_vllm_metal_amd import _lib
+
+    lib = _lib.load()
+    x = torch.randn(5, 96, device=DEV, generator=_gen(6))
+    codes = torch.full((7, 96), 0xAA, dtype=torch.uint8, device=DEV)
+    scales = torch.full((7, 32), 0xAA, dtype=torch.uint8, device=DEV)
+    _lib.check(lib.nvm_mx_quantize(x.data_ptr(), 5, 96, 96, 2, 1, codes.data_ptr(),
+                                   scales.data_ptr(), 32, _lib.stream_of(x.device)))
+    torch.cuda.synchronize()
+    assert (codes[5:] == 0xAA).all() and (scales[5:] == 0xAA).all()
+    assert (scales[:, 3:] == 0xAA).all()
+    c, b = O.quantize(x.double(), "mxfp8")
+    assert torch.equal(scales[:5, :3].long(), b)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_dequantize_every_code_and_scale(fmt, dt):
+    """(float32 holds every value but those at 2^127 and 2^126 that overflow;
+    the conversion to 16 bits is torch's own of the float32 value.)"""
+    from nano_vllm_metal_amd import MxTensor, mx_dequantize
+
+    s = torch.arange(256, device=DEV).reshape(256, 1).to(torch.uint8)
+    c = torch.arange(256, device=DEV).to(torch.uint8).expand(256, 256)
+    scales = s.expand(256, 256 * (2 if fmt == "mxfp4" else 1) // 32)
+    t = MxTensor(c, scales, fmt)
+    want = O.decode(c, scales, fmt).float().to(dt)
+    got = mx_dequantize(t, dt)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got.float(), 0.0), torch.nan_to_num(want.float(), 0.0))
+    assert got.dtype == dt and t.dequantize(dt).shape == t.shape
+
+
+def test_quantizing_what_was_dequantized_changes_nothing():
+    from nano_vllm_metal_amd import mx_dequantize, mx_quantize
+
+    x = torch.randn(33, 2048, device=DEV, generator=_gen(7))
+    for fmt in FMTS:
+        t = mx_quantize(x, fmt)
+        v = mx_dequantize(t, torch.float32)
+        assert torch.equal(mx_dequantize(mx_quantize(v, fmt)), v)
+
+
+# --------------------------------------------------------------------- norm
+
+
+def _norm_case(T, H, dt, seed, sparse=False):
+    g = _gen(seed)
+    h = (torch.randn(T, H, device=DEV, generator=g) * 3).to(dt)
+    if sparse:
+        h[0] = 0
+    r = torch.randn(T, H, device=DEV, generator=g).to(dt)
+    w = (1 + 0.1 * torch.randn(H, device=DEV, generator=g)).to(dt)
+    return h, r, w
+
+
+@pytest.mark.parametrize("T,H", [(1, 32), (5, 96), (3, 512), (2, 544), (8, 2048), (37, 2080),
+                                 (4, 4096), (3, 4128), (2, 8192), (301, 256)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_residual_rms_norm_mx(T, H, dt, fmt):
+    from nano_vllm_metal_amd import residual_rms_norm_mx
+
+    h, r, w = _norm_case(T, H, dt, T * H)
+    for res in (r, None):
+        h2, x = residual_rms_norm_mx(h, res, w, 1e-6, fmt)
+        want = (h.float() + r.float()).to(dt) if res is not None else h
+        assert torch.equal(h2, want)
+        v = want.double()
+        y = v / (v.square().mean(-1, keepdim=True) + float(torch.tensor(1e-6))).sqrt() * w.double()
+        O.check_quantized(x.codes, x.scales, fmt, y, y.abs() * 2.0 ** -40)
+
+
+def test_norm_rows_of_zeros_and_of_nothing_finite():
+    from nano_vllm_metal_amd import residual_rms_norm_mx
+
+    h, r, w = _norm_case(4, 2048, torch.bfloat16, 3)
+    h[0], r[0] = 0, 0
+    h[1, 7] = float("nan")
+    h[2, 9] = float("inf")
+    _, x = residual_rms_norm_mx(h, r, w, 1e-6)
+    v = _val(x)
+    assert (v[0] == 0).all() and torch.isnan(v[1]).all()
+    # (inf / inf where the infinity stood, finite / inf = 0 elsewhere: its block is not finite)
+    assert torch.isnan(v[2, :32]).all() and (v[2, 32:] == 0).all()
+    assert torch.isfinite(v[3]).all()
+
+
+# ----------------------------------------------------------------- products
+
+
+def _sum_bound(a, w, fmt):
+    """How far the float32 sums of a . w^T may be off (see above)."""
+    bound = a.shape[1] * 2.0 ** -23 * (a.abs() @ w.abs().t())
+    if fmt == "mxfp8":
+        rows = max(1, 2 ** 27 // w.numel())
+        for i in range(0, a.shape[0], rows):
+            p = (a[i:i + rows, None, :] * w[None]).abs()
+            bound[i:i + rows] += 7 * 2.0 ** -13 * p.unflatten(-1, (-1, 8)).amax(-1).sum(-1)
+    return bound
+
+
+def _close(got, a, w, dt, fmt):
+    y, sums = a @ w.t(), _sum_bound(a, w, fmt)
+    tol = sums + torch.finfo(dt).eps / 2 * (y.abs() + sums) + torch.finfo(dt).tiny
+    assert got.dtype == dt
+    off = (got.double() - y).abs() > tol
+    assert not off.any(), (f"{int(off.sum())} of {off.numel()} off, worst "
+                           f"{((got.double() - y).abs() / tol).max().item():.3g} of the bound")
+
+
+SHAPES = [(1, 32, 1), (1, 32, 64), (2, 64, 3), (1, 2048, 512), (5, 96, 33), (16, 128, 16),
+          (17, 160, 100), (15, 4096, 31), (33, 544, 257), (64, 512, 255), (64, 1024, 48),
+          (37, 6144, 65), (65, 128, 256), (65, 32, 5), (100, 160, 300), (128, 2048, 130),
+          (255, 64, 129), (256, 384, 256), (257, 512, 513), (300, 96, 1), (500, 2080, 260),
+          (1025, 640, 384), (70, 4128, 770)]
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_linear(M, N, K, fmt, dt):
+    from nano_vllm_metal_amd import mx_linear
+
+    g = _gen(M + N + K)
+    a = _mx(torch.randn(M, N, device=DEV, generator=g), fmt)
+    w = _mx(torch.randn(K, N, device=DEV, generator=g) * N ** -0.5, "mxfp4")
+    _close(mx_linear(a, w, dt), _val(a), _val(w), dt, fmt)
+
+
+@pytest.mark.parametrize("M", [3, 40, 300])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_linear_every_code_over_many_scales(M, fmt):
+    """All codes (but the NaN) and scales over 2^-30 .. 2^30, every operand
+    layout position: a wrong lane or scale shows as an error of the value."""
+    from nano_vllm_metal_amd import MxTensor, mx_linear
+
+    g, N, K = _gen(M), 672, 200
+    top = 256 if fmt == "mxfp8" else 256
+
+    def rnd(rows, f):
+        c = torch.randint(0, top, (rows, N if f == "mxfp8" else N // 2), device=DEV, generator=g,
+                          dtype=torch.int32)
+        if f == "mxfp8":
+            c = torch.where((c & 127) == 127, c - 1, c)
+        s = torch.randint(97, 158, (rows, N // 32), device=DEV, generator=g, dtype=torch.int32)
+        return MxTensor(c.to(torch.uint8), s.to(torch.uint8), f)
+
+    a, w = rnd(M, fmt), rnd(K, "mxfp4")
+    _close(mx_linear(a, w, torch.float32), _val(a), _val(w), torch.float32, fmt)
+
+
+@pytest.mark.parametrize("M", [9, 90])
+@pytest.mark.parametrize("N", [160, 512])
+def test_linear_what_lies_behind_a_row_does_not_matter(M, N):
+    """Scales of 255 (NaN) in the padding, and NaN codes in the next rows."""
+    from nano_vllm_metal_amd import MxTensor, mx_linear
+
+    g, K = _gen(N), 70
+    a0 = _mx(torch.randn(M, N, device=DEV, generator=g), "mxfp8")
+    w0 = _mx(torch.randn(K, N, device=DEV, generator=g), "mxfp4")
+
+    def hostile(t, rows):
+        codes = torch.full((rows + 3, t.codes.shape[1]), 0xFF, dtype=torch.uint8, device=DEV)
+        scales = torch.full((rows + 3, 32), 255, dtype=torch.uint8, device=DEV)
+        codes[:rows], scales[:rows, :N // 32] = t.codes, t.scales
+        return MxTensor(codes[:rows], scales[:rows, :N // 32], t.fmt)
+
+    a, w = hostile(a0, M), hostile(w0, K)
+    assert a.scales.stride(0) == 32 and a.scales.untyped_storage().nbytes() == (M + 3) * 32
+    y = mx_linear(a, w, torch.float32)
+    assert torch.equal(y, mx_linear(a0, w0, torch.float32))
+    _close(y, _val(a0), _val(w0), torch.float32, "mxfp8")
+
+
+@pytest.mark.parametrize("M", [5, 80])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_linear_nan_blocks_zeros_and_large_scales(M, fmt):
+    from nano_vllm_metal_amd import MxTensor, mx_linear
+
+    g, N, K = _gen(M), 256, 40
+    a = _mx(torch.randn(M, N, device=DEV, generator=g), fmt)
+    w = _mx(torch.randn(K, N, device=DEV, generator=g), "mxfp4")
+    y = mx_linear(a, w, torch.float32)
+    sa, sw = a.scales.clone(), w.scales.clone()
+    sa[2, 3], sw[7, 5] = 255, 255
+    z = mx_linear(MxTensor(a.codes, sa, fmt), MxTensor(w.codes, sw, "mxfp4"), torch.float32)
+    nan = torch.zeros_like(z, dtype=torch.bool)
+    nan[2], nan[:, 7] = True, True
+    assert torch.equal(torch.isnan(z), nan) and torch.equal(z[~nan], y[~nan])
+    zero = MxTensor(torch.zeros_like(a.codes), torch.zeros_like(a.scales), fmt)
+    assert (mx_linear(zero, w) == 0).all()
+    big = MxTensor(a.codes, torch.full_like(a.scales, 160), fmt)
+    huge = MxTensor(w.codes, torch.full_like(w.scales, 190), "mxfp4")
+    z = mx_linear(big, huge, torch.float32)  # 2^33 * 2^63 * sums: inside float32
+    _close(z, _val(big), _val(huge), torch.float32, fmt)
+
+
+def test_linear_takes_16_bit_activations_leading_dimensions_and_a_bias():
+    from nano_vllm_metal_amd import mx_linear, mx_quantize
+
+    g = _gen(11)
+    w = _mx(torch.randn(96, 256, device=DEV, generator=g) * 0.1, "mxfp4")
+    for dt in (torch.bfloat16, torch.float16):
+        x = torch.randn(2, 3, 256, device=DEV, generator=g).to(dt)
+        b = torch.randn(96, device=DEV, generator=g).to(dt)
+        y = mx_linear(x, w)
+        assert y.shape == (2, 3, 96) and y.dtype == dt
+        q = mx_quantize(x, "mxfp8")
+        assert torch.equal(y, mx_linear(q, w, dt))
+        assert torch.equal(y[0, 0], mx_linear(x[0, 0], w))
+        assert torch.equal(mx_linear(x, w, bias=b), y + b)
+    assert mx_linear(x[:0], w).shape == (0, 3, 96)
+
+
+def test_linear_rows_do_not_depend_on_their_batch():
+    """The same kernel for a row of a small and of a larger batch sums it in
+    the same order."""
+    from nano_vllm_metal_amd import MxTensor, mx_linear
+
+    g = _gen(12)
+    a = _mx(torch.randn(16, 2048, device=DEV, generator=g), "mxfp8")
+    w = _mx(torch.randn(80, 2048, device=DEV, generator=g), "mxfp4")
+    y = mx_linear(a, w, torch.float32)
+    for m in (1, 7, 15):
+        part = MxTensor(a.codes[:m], a.scales[:m], "mxfp8")
+        assert torch.equal(mx_linear(part, w, torch.float32), y[:m])
+
+
+def test_linear_writes_its_rows_only():
+    from nano_vllm_metal_amd import _lib
+
+    lib = _lib.load()
+    g = _gen(13)
+    for M, K in ((3, 50), (70, 50), (70, 258)):
+        a = _mx(torch.randn(M, 96, device=DEV, generator=g), "mxfp8")
+        w = _mx(torch.randn(K, 96, device=DEV, generator=g), "mxfp4")
+        for code, dt in ((1, torch.bfloat16), (2, torch.float32)):
+            out = torch.full((M + 2, K), 7.0, dtype=dt, device=DEV)
+            _lib.check(lib.nvm_mx_matmul(
+                a.codes.data_ptr(), a.scales.data_ptr(), a.scales.stride(0), 1,
+                w.codes.data_ptr(), w.scales.data_ptr(), w.scales.stride(0), M, 96, K, code,
+                out.data_ptr(), _lib.stream_of(out.device)))
+            torch.cuda.synchronize()
+            assert (out[M:] == 7).all()
+            _close(out[:M], _val(a), _val(w), dt, "mxfp8")
+
+
+# ------------------------------------------------------------------- SwiGLU
+
+
+def _swiglu_exact(x, gate, up):
+    a, wg, wu = _val(x), _val(gate), _val(up)
+    g, u = a @ wg.t(), a @ wu.t()
+    eg, eu = _sum_bound(a, wg, x.fmt), _sum_bound(a, wu, x.fmt)
+    h = g * torch.sigmoid(g) * u
+    d = 1.1 * eg * (u.abs() + eu) + (g * torch.sigmoid(g)).abs() * eu + 2.0 ** -20 * h.abs()
+    # (below 2^-126 float32 keeps absolute steps of 2^-149)
+    return h, d + 2.0 ** -146
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 32, 32), (1, 2048, 768), (8, 2048, 96), (17, 160, 128),
+                                   (40, 512, 160), (64, 96, 64), (65, 128, 128), (130, 544, 288),
+                                   (256, 256, 256), (300, 2048, 416), (515, 64, 32)])
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("ofmt", FMTS)
+def test_swiglu(M, N, K, fmt, ofmt):
+    from nano_vllm_metal_amd import mx_swiglu
+
+    g = _gen(M + N + K)
+    a = _mx(torch.randn(M, N, device=DEV, generator=g), fmt)
+    wg, wu = (_mx(torch.randn(K, N, device=DEV, generator=g) * 2 * N ** -0.5, "mxfp4")
+              for _ in range(2))
+    y = mx_swiglu(a, wg, wu, ofmt)
+    assert y.shape == (M, K) and y.fmt == ofmt
+    h, d = _swiglu_exact(a, wg, wu)
+    O.check_quantized(y.codes, y.scales, ofmt, h, d)
+
+
+@pytest.mark.parametrize("M", [6, 70])
+def test_swiglu_of_large_and_of_bad_values(M):
+    """Gates far from zero on both sides (exp overflows: the result is zero),
+    and a NaN block of an activation row."""
+    from nano_vllm_metal_amd import MxTensor, mx_swiglu
+
+    g, N, K = _gen(M), 128, 64
+    a = _mx(torch.randn(M, N, device=DEV, generator=g) * 40, "mxfp8")
+    wg, wu = (_mx(torch.randn(K, N, device=DEV, generator=g), "mxfp4") for _ in range(2))
+    y = mx_swiglu(a, wg, wu)
+    h, d = _swiglu_exact(a, wg, wu)
+    assert h.abs().max() > 1e4 and h.abs().min() < 1e-30
+    O.check_quantized(y.codes, y.scales, "mxfp8", h, d)
+    s = a.scales.clone()
+    s[3, 1] = 255
+    z = mx_swiglu(MxTensor(a.codes, s, "mxfp8"), wg, wu)
+    assert torch.isnan(_val(z)[3]).all()
+    keep = [i for i in range(M) if i != 3]
+    assert torch.equal(z.codes[keep], y.codes[keep]) and torch.equal(z.scales[keep], y.scales[keep])
+
+
+# ------------------------------------------------- together, streams, graphs
+
+
+def _layer(g, H=512, I=768, T=24, dt=torch.bfloat16):
+    h = torch.randn(T, H, device=DEV, generator=g).to(dt)
+    r = torch.randn(T, H, device=DEV, generator=g).to(dt)
+    w = (1 + 0.1 * torch.randn(H, device=DEV, generator=g)).to(dt)
+    wg, wu = (_mx(torch.randn(I, H, device=DEV, generator=g) * H ** -0.5, "mxfp4")
+              for _ in range(2))
+    wd = _mx(torch.randn(H, I, device=DEV, generator=g) * I ** -0.5, "mxfp4")
+    return h, r, w, wg, wu, wd
+
+
+def _mlp(h, r, w, wg, wu, wd):
+    from nano_vllm_metal_amd import mx_linear, mx_swiglu, residual_rms_norm_mx
+
+    h2, x = residual_rms_norm_mx(h, r, w, 1e-6)
+    m = mx_swiglu(x, wg, wu)
+    return h2, x, m, mx_linear(m, wd, h.dtype)
+
+
+@pytest.mark.parametrize("T", [1, 24, 200])
+def test_the_operators_in_a_row(T):
+    """Norm, gate/up and down as the dense MLP runs them, each step checked on
+    what the one before handed it."""
+    ops = _layer(_gen(T), T=T)
+    h2, x, m, y = _mlp(*ops)
+    v = h2.double()
+    n = v / (v.square().mean(-1, keepdim=True) + float(torch.tensor(1e-6))).sqrt() * ops[2].double()
+    O.check_quantized(x.codes, x.scales, "mxfp8", n, n.abs() * 2.0 ** -40)
+    hh, d = _swiglu_exact(x, ops[3], ops[4])
+    O.check_quantized(m.codes, m.scales, "mxfp8", hh, d)
+    _close(y, _val(m), _val(ops[5]), torch.bfloat16, "mxfp8")
+
+
+def _bits(out):
+    h2, x, m, y = out
+    return [h2, x.codes, x.scales.clone(), m.codes, m.scales.clone(), y]
+
+
+def test_on_another_stream_and_in_a_replayed_graph():
+    ops = _layer(_gen(21))
+    want = _bits(_mlp(*ops))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _bits(_mlp(*ops))
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _mlp(*ops)
+    for seed in (22, 23, 24):
+        new = _layer(_gen(seed))
+        ops[0].copy_(new[0])
+        ops[1].copy_(new[1])
+        graph.replay()
+        eager = _bits(_mlp(*ops))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(_bits(out), eager))
