@@ -171,12 +171,23 @@ def _plain(s):
 
 
 def _package():
+    if "nano_vllm_metal_amd" in sys.modules:
+        return sys.modules["nano_vllm_metal_amd"]
     at = str(Path(__file__).resolve().parent.parent / "nano-vllm-metal_amd")
     if at not in sys.path:
         sys.path.insert(0, at)
     import nano_vllm_metal_amd
 
     return nano_vllm_metal_amd
+
+
+def _mx(P, s, name):
+    """The handle that a program keeps of an operand (weights from loading on, activations from the
+    operator that made them); it refers to the state's own tensors."""
+    t = s.get("mx " + name)
+    if t is None:
+        t = s["mx " + name] = P.MxTensor(*s[name])
+    return t
 
 
 def _held(t):
@@ -193,8 +204,8 @@ def _own(s):
         h, x = P.residual_rms_norm_mx(s["h"], s["r"], s["w"], EPS, "mxfp8")
         return (h, *_held(x))
     if kind == "linear":
-        return P.mx_linear(P.MxTensor(*s["a"]), P.MxTensor(*s["w"]), s["dtype"])
-    return _held(P.mx_swiglu(P.MxTensor(*s["a"]), P.MxTensor(*s["g"]), P.MxTensor(*s["u"]), "mxfp8"))
+        return P.mx_linear(_mx(P, s, "a"), _mx(P, s, "w"), s["dtype"])
+    return _held(P.mx_swiglu(_mx(P, s, "a"), _mx(P, s, "g"), _mx(P, s, "u"), "mxfp8"))
 
 
 def run(state):
