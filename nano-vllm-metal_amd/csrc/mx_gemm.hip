@@ -38,185 +38,233 @@ __device__ __forceinline__ void lds_load4(rsrc_t r, void *lds, int voff, int sof
                                            voff, soff, 0, 0);
 }
 
+constexpr int round_up(int v, int m) { return (v + m - 1) / m * m; }
+
 // BN weight rows (DUAL: half of them gate, half up) and BM activation rows a
-// block, WF x WT wavefronts.
-template <int FMT, int BN_, int BM_, int WF_, int WT_, int ST_>
+// block, WF x WT wavefronts, two of them on a SIMD.
+template <int FMT, bool DUAL_, int BN_, int BM_, int WF_, int WT_, int ST_>
 struct Tile {
+  static constexpr bool DUAL = DUAL_;
   static constexpr int BN = BN_, BM = BM_, WF = WF_, WT = WT_, ST = ST_, NW = WF * WT;
+  static constexpr int NM = DUAL ? 2 : 1;        // matrices
+  static constexpr int BK = BN / NM;             // output columns
   static constexpr int XR = FMT == NVM_MX_FP4 ? 64 : 128;  // bytes of an activation row's step
-  static constexpr int kW = BN * 64, kX = BM * XR, kS = (BN + BM) * 4;
-  static constexpr int kStage = kW + kX + kS;
-  static constexpr int kLds = ST * kStage;
+  // pieces of a stage (1 KB of codes, 64 rows of scales: a load each)
+  static constexpr int PW = BN * 64 / 1024, PX = BM * XR / 1024;
+  static constexpr int PSM = (BK + 63) / 64, PSW = NM * PSM, PS = PSW + (BM + 63) / 64;
+  static constexpr int kW = PW * 1024, kX = PX * 1024, kS = PS * 256;
+  static constexpr int kStage = kW + kX + kS, kLds = ST * kStage;
   // a wavefront's loads of a stage
-  static constexpr int LW = kW / 1024 / NW, LX = kX / 1024 / NW, LS = (BN + BM) / 64;
+  static constexpr int LW = (PW + NW - 1) / NW, LX = (PX + NW - 1) / NW;
   static constexpr int kLoads = LW + LX + 1;
-  static_assert(kW % (1024 * NW) == 0 && kX % (1024 * NW) == 0 && LS <= NW, "whole loads");
   static constexpr int TF = BN / WF / 16, TM = BM / WT / 16;
+  static_assert(NW == 8 && PS <= NW && kLds <= 160 * 1024, "a block of eight wavefronts");
+  static_assert(BK % (16 * WF) == 0 && BM % (16 * WT) == 0 && (!DUAL || BK % (32 * WF) == 0),
+                "whole tiles of a wavefront");
 };
 
-template <int FMT, int OFMT, bool DUAL, class T>
-__global__ __launch_bounds__(64 * T::NW) void mx_gemm_kernel(const MxMatmulArgs p, int n_tiles,
-                                                             int total) {
+template <int FMT, int OFMT, class T>
+__global__ __launch_bounds__(64 * T::NW, 2) void mx_gemm_kernel(const MxMatmulArgs p, int n_tiles,
+                                                                int total) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   constexpr int NX = FMT == NVM_MX_FP4 ? 1 : 2;
-  constexpr int GR = T::BN / T::WF;          // LDS weight rows of a wavefront
-  constexpr int BK = DUAL ? T::BN / 2 : T::BN;  // output columns of a block
-  static_assert(!DUAL || GR % 128 == 0, "a scale load is of one matrix");
-  // tiles in contiguous runs per XCD (blocks go to the XCDs in turn)
-  const int per_xcd = (total + 7) >> 3;
-  const int tile = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
-  if (((int)blockIdx.x >> 3) >= per_xcd || tile >= total) return;
-  const int mt = tile / n_tiles, nt = tile - mt * n_tiles;
-  const int k0 = nt * BK;
-  const int64_t m0 = (int64_t)mt * T::BM;
-  const int nk = min(BK, p.K - k0), nm = (int)min((int64_t)T::BM, p.M - m0);
   const int lane = threadIdx.x & 63;
   const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int col = lane & 15, G = lane >> 4;
   const int wf = wv % T::WF, wt = wv / T::WF;
   const int WB = p.N / 2, XB = p.N * Mx<FMT>::kBits / 8, nb = p.N / 32;
-  const int steps = (p.N + 127) / 128, whole = p.N / 128;
+  const int steps = (p.N + 127) / 128;
+  // tiles in contiguous runs per XCD (blocks go to the XCDs in turn), a run
+  // dealt to the XCD's blocks
+  const int per_xcd = (total + 7) >> 3, stride = (int)gridDim.x >> 3;
+  const int run_end = min(((int)blockIdx.x & 7) * per_xcd + per_xcd, total);
+  const int first = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
+  if (first >= run_end) return;
 
-  // LDS weight row -> (matrix, row of the tile's columns)
-  auto matrix = [&](int row) { return DUAL ? (row / (GR / 2)) & 1 : 0; };
-  auto column = [&](int row) { return DUAL ? row / GR * (GR / 2) + row % (GR / 2) : row; };
+  struct Place {
+    int k0, nk, nm;
+    int64_t m0;
+  };
+  auto place = [&](int tile) {
+    Place q;
+    const int mt = tile / n_tiles;
+    q.k0 = (tile - mt * n_tiles) * T::BK;
+    q.m0 = (int64_t)mt * T::BM;
+    q.nk = min(T::BK, p.K - q.k0);
+    q.nm = (int)min((int64_t)T::BM, p.M - q.m0);
+    return q;
+  };
 
-  rsrc_t lw[T::LW];
-  int vw[T::LW], vx[T::LX];
+  // What the requests read: step r_step of tile r_tile, into stage r_slot.
+  // Weight row r of a stage is column r % BK of matrix r / BK.
+  int r_tile = first, r_step = 0, r_slot = 0;
+  rsrc_t rw[T::LW], rx, rs;
+  int vw[T::LW], vx[T::LX], vs;
+  const int sp = wv % T::PS;  // (left-over wavefronts load what others load)
+  auto aim = [&](int tile) {
+    const Place q = place(tile);
 #pragma unroll
-  for (int j = 0; j < T::LW; ++j) {
-    const int row = 16 * (wv * T::LW + j) + (lane >> 2), d = matrix(16 * (wv * T::LW + j));
-    lw[j] = make_rsrc(p.w[d] + (int64_t)k0 * WB, (uint32_t)(nk * WB));
-    vw[j] = min(column(row), nk - 1) * WB + 16 * ((lane & 3) ^ (lane >> 4));
-  }
-  const rsrc_t lx = make_rsrc(p.a + m0 * XB, (uint32_t)(nm * XB));
+    for (int j = 0; j < T::LW; ++j) {
+      const int row = 16 * min(wv + j * T::NW, T::PW - 1), d = T::DUAL && row >= T::BK;
+      rw[j] = make_rsrc(p.w[d] + (int64_t)q.k0 * WB, (uint32_t)(q.nk * WB));
+      vw[j] = min(row - d * T::BK + (lane >> 2), q.nk - 1) * WB + 16 * ((lane & 3) ^ (lane >> 4));
+    }
+    rx = make_rsrc(p.a + q.m0 * XB, (uint32_t)(q.nm * XB));
 #pragma unroll
-  for (int j = 0; j < T::LX; ++j) {
-    const int q = wv * T::LX + j;
-    if constexpr (FMT == NVM_MX_FP4)
-      vx[j] = min(16 * q + (lane >> 2), nm - 1) * XB + 16 * ((lane & 3) ^ (lane >> 4));
-    else
-      vx[j] = min(8 * q + (lane >> 3), nm - 1) * XB +
-              16 * ((lane & 7) ^ ((4 * (q & 1) + (lane >> 4)) & 7));
-  }
-  // one load of scales a wavefront: 64 rows' four bytes of the step (those
-  // wavefronts that are left over load what another loads)
-  const int sq = wv % T::LS, srow = 64 * sq;
-  const bool sw = srow < T::BN;
-  const int sd = sw ? matrix(srow) : 0;
-  const int sld = (int)(sw ? p.ws_ld[sd] : p.as_ld);
-  const rsrc_t ls = sw ? make_rsrc(p.ws[sd] + (int64_t)k0 * sld, (uint32_t)(nk * sld))
-                       : make_rsrc(p.as + m0 * sld, (uint32_t)(nm * sld));
-  const int vs = (sw ? min(column(srow + lane), nk - 1) : min(srow - T::BN + lane, nm - 1)) * sld;
-
-  auto request = [&](int s) {
-    // (steps past the end load the first again, into a stage that nothing
-    // reads any more: every step makes the same loads)
-    const int so = s < steps ? s : 0;
-    uint8_t *st = smem + s % T::ST * T::kStage;
+    for (int j = 0; j < T::LX; ++j) {
+      const int i = min(wv + j * T::NW, T::PX - 1);
+      if constexpr (FMT == NVM_MX_FP4)
+        vx[j] = min(16 * i + (lane >> 2), q.nm - 1) * XB + 16 * ((lane & 3) ^ (lane >> 4));
+      else
+        vx[j] = min(8 * i + (lane >> 3), q.nm - 1) * XB +
+                16 * ((lane & 7) ^ ((4 * i + (lane >> 4)) & 7));
+    }
+    if (sp < T::PSW) {
+      const int d = T::DUAL && sp >= T::PSM, ld = (int)p.ws_ld[d];
+      rs = make_rsrc(p.ws[d] + (int64_t)q.k0 * ld, (uint32_t)(q.nk * ld));
+      vs = min(64 * (sp - d * T::PSM) + lane, q.nk - 1) * ld;
+    } else {
+      const int ld = (int)p.as_ld;
+      rs = make_rsrc(p.as + q.m0 * ld, (uint32_t)(q.nm * ld));
+      vs = min(64 * (sp - T::PSW) + lane, q.nm - 1) * ld;
+    }
+  };
+  auto request = [&] {
+    uint8_t *st = smem + r_slot * T::kStage;
 #pragma unroll
-    for (int j = 0; j < T::LW; ++j) lds_load16(lw[j], st + (wv * T::LW + j) * 1024, vw[j], 64 * so);
+    for (int j = 0; j < T::LW; ++j)
+      lds_load16(rw[j], st + min(wv + j * T::NW, T::PW - 1) * 1024, vw[j], 64 * r_step);
 #pragma unroll
     for (int j = 0; j < T::LX; ++j)
-      lds_load16(lx, st + T::kW + (wv * T::LX + j) * 1024, vx[j], T::XR * so);
-    lds_load4(ls, st + T::kW + T::kX + sq * 256, vs, 4 * so);
+      lds_load16(rx, st + T::kW + min(wv + j * T::NW, T::PX - 1) * 1024, vx[j], T::XR * r_step);
+    lds_load4(rs, st + T::kW + T::kX + sp * 256, vs, 4 * r_step);
+    r_slot = r_slot + 1 == T::ST ? 0 : r_slot + 1;
+    if (++r_step == steps) {
+      r_step = 0;
+      r_tile += stride;
+      if (r_tile < run_end) aim(r_tile);
+    }
   };
 
-  f32x4 acc[T::TF][T::TM];
-#pragma unroll
-  for (int f = 0; f < T::TF; ++f)
-#pragma unroll
-    for (int t = 0; t < T::TM; ++t) acc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const int rw = (wf * GR + col) * 64 + 16 * (G ^ ((col >> 2) & 3));
-  const int xrow = wt * (T::BM / T::WT) + col;
-  int rx[NX];
+  // places in a stage that the wavefront's operands are read from
+  const int wrow = wf * (T::BK / T::WF) + col, xrow = wt * (T::BM / T::WT) + col;
+  const int aw = wrow * 64 + 16 * (G ^ ((col >> 2) & 3));
+  int ax[NX];
 #pragma unroll
   for (int c = 0; c < NX; ++c)
-    rx[c] = T::kW + xrow * T::XR +
+    ax[c] = T::kW + xrow * T::XR +
             16 * (FMT == NVM_MX_FP4 ? G ^ ((col >> 2) & 3) : (4 * c + G) ^ ((col >> 1) & 7));
-  const int rws = T::kW + T::kX + (wf * GR + col) * 4 + G;
-  const int rxs = T::kW + T::kX + (T::BN + xrow) * 4 + G;
-  auto compute = [&](int s, auto TAIL) {
-    constexpr bool tail = decltype(TAIL)::value;
-    const uint8_t *st = smem + s % T::ST * T::kStage;
-    MxFrag<FMT> x[T::TM];
-    uint32_t xs[T::TM];
-#pragma unroll
-    for (int t = 0; t < T::TM; ++t) {
-#pragma unroll
-      for (int c = 0; c < NX; ++c) {
-        x[t].v[c] = *(const u32x4 *)(st + rx[c] + t * 16 * T::XR);
-        if constexpr (tail)
-          if (128 * s + (FMT == NVM_MX_FP4 ? 32 * G : 64 * c + 16 * G) >= p.N)
-            x[t].v[c] = u32x4{0u, 0u, 0u, 0u};
-      }
-      xs[t] = st[rxs + t * 64];
-      if constexpr (tail) xs[t] = 4 * s + G < nb ? xs[t] : 127u;
-    }
-#pragma unroll
-    for (int f = 0; f < T::TF; ++f) {
-      MxFrag<NVM_MX_FP4> w;
-      w.v[0] = *(const u32x4 *)(st + rw + f * 1024);
-      uint32_t ws = st[rws + f * 64];
-      if constexpr (tail) ws = 4 * s + G < nb ? ws : 127u;
-#pragma unroll
-      for (int t = 0; t < T::TM; ++t) acc[f][t] = mx_mfma<FMT>(w, ws, x[t], xs[t], acc[f][t]);
-    }
+  const int aws = T::kW + T::kX + wrow * 4 + G;
+  const int axs = T::kW + T::kX + T::PSW * 256 + xrow * 4 + G;
+  // weight tile f of the wavefront: rows further on in the stage
+  auto ftile = [](int f) { return T::DUAL && f >= T::TF / 2 ? T::BK + 16 * (f - T::TF / 2) : 16 * f; };
+  auto fscale = [](int f) {
+    return T::DUAL && f >= T::TF / 2 ? T::PSM * 256 + 64 * (f - T::TF / 2) : 64 * f;
   };
-  // Stage s has arrived when at most the loads of the ST - 2 later ones are
-  // outstanding; the barrier extends that to every wavefront's share, and
-  // says that every wavefront has read stage s - 1, which the next request
-  // overwrites.
-  auto arrive = [&] {
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((T::ST - 2) * T::kLoads) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-  };
-#pragma unroll
-  for (int s = 0; s < T::ST - 1; ++s) request(s);
-  for (int s = 0; s < whole; ++s) {
-    arrive();
-    request(s + T::ST - 1);
-    compute(s, std::false_type{});
-  }
-  if (whole < steps) {
-    arrive();
-    compute(whole, std::true_type{});
-  }
-  // (no load may still be writing when the block's LDS is given back)
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
+  aim(first);
 #pragma unroll
-  for (int t = 0; t < T::TM; ++t) {
-    const int m = wt * (T::BM / T::WT) + 16 * t + col;
-    if constexpr (!DUAL) {
-      if (m >= nm) continue;
+  for (int s = 0; s < T::ST - 1; ++s)
+    if (r_tile < run_end) request();
+  // the first stage, of every wavefront
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  // wavefronts 4 to 7 run half a step behind the others
+  if (wv >= 4) __builtin_amdgcn_s_barrier();
+  int slot = 0;
+  for (int tile = first; tile < run_end; tile += stride) {
+    f32x4 acc[T::TF][T::TM];
+#pragma unroll
+    for (int f = 0; f < T::TF; ++f)
+#pragma unroll
+      for (int t = 0; t < T::TM; ++t) acc[f][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < steps; ++s) {
+      const uint8_t *st = smem + slot * T::kStage;
+      MxFrag<FMT> x[T::TM];
+      MxFrag<NVM_MX_FP4> w[T::TF];
+      uint32_t xs[T::TM], ws[T::TF];
+#pragma unroll
+      for (int t = 0; t < T::TM; ++t) {
+#pragma unroll
+        for (int c = 0; c < NX; ++c) x[t].v[c] = *(const u32x4 *)(st + ax[c] + t * 16 * T::XR);
+        xs[t] = st[axs + t * 64];
+      }
 #pragma unroll
       for (int f = 0; f < T::TF; ++f) {
-        const int k = wf * GR + 16 * f + 4 * G;
-        mx_store4(p.out, p.out_dtype, (m0 + m) * p.K + k0 + k, acc[f][t], nk - k, p.K % 4 == 0);
+        w[f].v[0] = *(const u32x4 *)(st + aw + ftile(f) * 64);
+        ws[f] = st[aws + fscale(f)];
       }
-    } else {
+      const bool more = r_tile < run_end;
+      if (more) request();
+      if (128 * s + 128 > p.N) {  // a last step that the row ends in
 #pragma unroll
-      for (int f = 0; f < T::TF / 2; f += 2) {
-        const int k = wf * (GR / 2) + 16 * f;
-        float h[8];
-        uint32_t mx = 0;
+        for (int t = 0; t < T::TM; ++t) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          h[e] = mx_swiglu(acc[f + (e >> 2)][t][e & 3], acc[T::TF / 2 + f + (e >> 2)][t][e & 3]);
-          mx = max(mx, abs_bits(h[e]));
+          for (int c = 0; c < NX; ++c)
+            if (128 * s + (FMT == NVM_MX_FP4 ? 32 * G : 64 * c + 16 * G) >= p.N)
+              x[t].v[c] = u32x4{0u, 0u, 0u, 0u};
+          if (4 * s + G >= nb) xs[t] = 127u;
         }
-        mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16));
-        mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
-        if (m < nm && k < nk)
-          mx_store_block<OFMT>(h, mx, m0 + m, k0 + k, G, p.K, p.out, p.out_s, p.out_sld);
+#pragma unroll
+        for (int f = 0; f < T::TF; ++f)
+          if (4 * s + G >= nb) ws[f] = 127u;
+      }
+      // The wavefront's share of the next step has arrived when at most the
+      // ST - 2 later requests are outstanding.  This step's operands are in
+      // registers, so its stage may be overwritten from the barrier on.
+      if (more)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((T::ST - 2) * T::kLoads) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+      for (int f = 0; f < T::TF; ++f)
+#pragma unroll
+        for (int t = 0; t < T::TM; ++t)
+          acc[f][t] = mx_mfma<FMT>(w[f], ws[f], x[t], xs[t], acc[f][t]);
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      slot = slot + 1 == T::ST ? 0 : slot + 1;
+    }
+
+    const Place q = place(tile);
+#pragma unroll
+    for (int t = 0; t < T::TM; ++t) {
+      const int m = wt * (T::BM / T::WT) + 16 * t + col;
+      if constexpr (!T::DUAL) {
+        if (m >= q.nm) continue;
+#pragma unroll
+        for (int f = 0; f < T::TF; ++f) {
+          const int k = wf * (T::BK / T::WF) + 16 * f + 4 * G;
+          mx_store4(p.out, p.out_dtype, (q.m0 + m) * p.K + q.k0 + k, acc[f][t], q.nk - k,
+                    p.K % 4 == 0);
+        }
+      } else {
+#pragma unroll
+        for (int f = 0; f < T::TF / 2; f += 2) {
+          const int k = wf * (T::BK / T::WF) + 16 * f;
+          float h[8];
+          uint32_t mx = 0;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            h[e] = mx_swiglu(acc[f + (e >> 2)][t][e & 3], acc[T::TF / 2 + f + (e >> 2)][t][e & 3]);
+            mx = max(mx, abs_bits(h[e]));
+          }
+          mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16));
+          mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
+          if (m < q.nm && k < q.nk)
+            mx_store_block<OFMT>(h, mx, q.m0 + m, q.k0 + k, G, p.K, p.out, p.out_s, p.out_sld);
+        }
       }
     }
   }
+  if (wv < 4) __builtin_amdgcn_s_barrier();
 }
 
 // more than 64 KB of dynamic LDS: allowed once per device and instance (a
@@ -231,26 +279,27 @@ void allow_lds(F kern, int bytes, bool (&done)[64]) {
   }
 }
 
-template <int FMT, int OFMT, bool DUAL, class T>
+template <int FMT, int OFMT, class T>
 hipError_t go(const MxMatmulArgs &a, hipStream_t st) {
   static bool done[64] = {false};
-  constexpr int BK = DUAL ? T::BN / 2 : T::BN;
-  auto kern = mx_gemm_kernel<FMT, OFMT, DUAL, T>;
+  auto kern = mx_gemm_kernel<FMT, OFMT, T>;
   allow_lds(kern, T::kLds, done);
-  const int n_tiles = (a.K + BK - 1) / BK;
+  const int n_tiles = (a.K + T::BK - 1) / T::BK;
   const int64_t total = (a.M + T::BM - 1) / T::BM * n_tiles;
   if (total > kMxMaxTiles) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(8 * ((total + 7) / 8))), dim3(64 * T::NW), T::kLds, st,
-                     a, n_tiles, (int)total);
+  const int64_t grid = std::min<int64_t>(8 * ((total + 7) / 8), cu_count() / 8 * 8);
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * T::NW), T::kLds, st, a, n_tiles,
+                     (int)total);
   return hipGetLastError();
 }
 
 template <int FMT>
 hipError_t launch_fmt(bool dual, int out_format, const MxMatmulArgs &a, hipStream_t st) {
-  using Large = Tile<FMT, 256, 256, 2, 4, FMT == NVM_MX_FP4 ? 4 : 3>;
-  if (!dual) return go<FMT, NVM_MX_FP8, false, Large>(a, st);
-  return out_format == NVM_MX_FP4 ? go<FMT, NVM_MX_FP4, true, Large>(a, st)
-                                  : go<FMT, NVM_MX_FP8, true, Large>(a, st);
+  constexpr int ST = FMT == NVM_MX_FP4 ? 4 : 3;
+  if (!dual) return go<FMT, NVM_MX_FP8, Tile<FMT, false, 256, 256, 2, 4, ST>>(a, st);
+  using Dual = Tile<FMT, true, 256, 256, 2, 4, ST>;
+  return out_format == NVM_MX_FP4 ? go<FMT, NVM_MX_FP4, Dual>(a, st)
+                                  : go<FMT, NVM_MX_FP8, Dual>(a, st);
 }
 
 }  // namespace

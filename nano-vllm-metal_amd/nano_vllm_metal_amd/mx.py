@@ -12,7 +12,6 @@ eight (or four) bits between them.  No CPU fallback.
 
 from __future__ import annotations
 
-import contextlib
 from typing import Optional, Tuple, Union
 
 import torch
@@ -48,7 +47,7 @@ class MxTensor:
     copied into that layout once, here.
     """
 
-    __slots__ = ("codes", "scales", "fmt", "shape")
+    __slots__ = ("codes", "scales", "fmt", "shape", "rows", "pitch")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str):
         _format(fmt)
@@ -63,27 +62,28 @@ class MxTensor:
                              f"{tuple(scales.shape)} are not rows of {fmt} blocks of {MX_BLOCK}")
         if codes.device != scales.device:
             raise ValueError("MxTensor: codes and scales must be on one device")
-        codes = codes.contiguous()
-        self.codes = codes if codes.data_ptr() % 16 == 0 else codes.clone()
-        self.scales = scales if _scales_laid_out(scales, n) else _lay_out(scales, n)
+        pitch = _row_pitch(scales, n)
+        if pitch is None:
+            scales, pitch = _lay_out(scales, n), _pitch(n)
+        self.codes = _packed(codes)
+        self.scales = scales
         self.fmt = fmt
         self.shape = torch.Size((*codes.shape[:-1], n))
+        self.rows = codes.shape[:-1].numel()
+        self.pitch = pitch
 
     @classmethod
-    def _of(cls, codes, scales, fmt, shape) -> "MxTensor":
-        """A tensor that a kernel wrote: nothing to check or to copy."""
+    def _empty(cls, lead, rows: int, n: int, fmt: str, device) -> "MxTensor":
+        """A tensor for a kernel to write: nothing to check or to copy."""
         t = cls.__new__(cls)
-        t.codes, t.scales, t.fmt, t.shape = codes, scales, fmt, shape
-        return t
-
-    @classmethod
-    def _empty(cls, lead, n: int, fmt: str, device) -> "MxTensor":
-        pitch = _pitch(n)
-        codes = torch.empty((*lead, n // _PER_BYTE[fmt]), dtype=torch.uint8, device=device)
+        t.pitch = pitch = _pitch(n)
+        t.codes = torch.empty((*lead, n // _PER_BYTE[fmt]), dtype=torch.uint8, device=device)
         scales = torch.empty((*lead, pitch), dtype=torch.uint8, device=device)
-        if pitch * MX_BLOCK != n:
-            scales = scales[..., :n // MX_BLOCK]
-        return cls._of(codes, scales, fmt, torch.Size((*lead, n)))
+        t.scales = scales if pitch * MX_BLOCK == n else scales[..., :n // MX_BLOCK]
+        t.fmt = fmt
+        t.shape = torch.Size((*lead, n))
+        t.rows = rows
+        return t
 
     @property
     def device(self) -> torch.device:
@@ -97,10 +97,6 @@ class MxTensor:
     def out_features(self) -> int:
         return self.shape[-2]
 
-    @property
-    def rows(self) -> int:
-        return self.shape[:-1].numel()
-
     def to(self, device) -> "MxTensor":
         return MxTensor(self.codes.to(device), self.scales.to(device), self.fmt)
 
@@ -111,27 +107,24 @@ class MxTensor:
         return f"MxTensor({self.fmt}, shape={tuple(self.shape)}, device={self.device})"
 
 
-def _row_pitch(scales: torch.Tensor, n: int) -> int:
-    """Bytes between rows of a scale tensor in the kernels' layout."""
-    return scales.stride(-2) if scales.dim() > 1 else _pitch(n)
-
-
-def _scales_laid_out(scales: torch.Tensor, n: int) -> bool:
-    """Whether rows start a multiple of 16 bytes apart, evenly over all leading
-    dimensions, and the last row's padding is inside the storage."""
+def _row_pitch(scales: torch.Tensor, n: int) -> Optional[int]:
+    """Bytes between rows of scales that lie as the kernels read them: rows a
+    multiple of 16 bytes apart, evenly over all leading dimensions, and the
+    last row's padding inside the storage.  None for others."""
     if scales.stride(-1) != 1 and scales.shape[-1] > 1 or scales.data_ptr() % 16:
-        return False
-    pitch = _row_pitch(scales, n)
-    if pitch % 16 or pitch < _pitch(n):
-        return False
+        return None
+    need = _pitch(n)
+    pitch = scales.stride(-2) if scales.dim() > 1 and scales.shape[-2] > 1 else need
+    if pitch % 16 or pitch < need:
+        return None
     step = pitch
     for size, stride in zip(reversed(scales.shape[:-1]), reversed(scales.stride()[:-1])):
-        if stride != step:
-            return False
+        if size > 1 and stride != step:
+            return None
         step *= size
     rows = scales.shape[:-1].numel()
-    last = scales.storage_offset() + max(rows - 1, 0) * pitch + _pitch(n)
-    return rows == 0 or last <= scales.untyped_storage().nbytes()
+    last = scales.storage_offset() + max(rows - 1, 0) * pitch + need
+    return pitch if rows == 0 or last <= scales.untyped_storage().nbytes() else None
 
 
 def _lay_out(scales: torch.Tensor, n: int) -> torch.Tensor:
@@ -142,23 +135,23 @@ def _lay_out(scales: torch.Tensor, n: int) -> torch.Tensor:
     return out
 
 
-def _rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """x as 16-byte aligned rows (a copy where it is not), and the values from
-    one row to the next."""
-    n, per16 = x.shape[-1], 16 // x.element_size()
-    if not x.is_contiguous() and not (x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= n
-                                      and x.stride(0) % per16 == 0):
-        x = x.contiguous()
-    if x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.contiguous_format)
-    return x, (x.stride(0) if x.dim() == 2 and x.shape[0] > 1 else n)
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and 16-byte aligned."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _on(device: torch.device):
-    """The launch's device is the tensors', whichever is current."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _launch(fn, dev: torch.device, *args) -> None:
+    """``fn(*args, stream)`` on the tensors' device, whichever is current, and
+    its current stream."""
+    index = dev.index
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status)
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "mxfp8") -> MxTensor:
@@ -170,18 +163,27 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp8") -> MxTensor:
     lib = _lib.load()
     code = _format(fmt)
     dev = _lib.require_device(x)
-    if x.dtype not in MX_DTYPES:
+    dtype = MX_DTYPES.get(x.dtype)
+    if dtype is None:
         raise ValueError(f"mx_quantize: x must be float16, bfloat16 or float32, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % MX_BLOCK:
+    shape = x.shape
+    n = shape[-1] if shape else 0
+    if n == 0 or n % MX_BLOCK:
         raise ValueError(f"mx_quantize: the last dimension must be a positive multiple of "
-                         f"{MX_BLOCK}, got shape {tuple(x.shape)}")
-    n = x.shape[-1]
-    xr, ld = _rows(x)
-    with _on(dev):
-        out = MxTensor._empty(x.shape[:-1], n, fmt, dev)
-        _lib.check(lib.nvm_mx_quantize(xr.data_ptr(), out.rows, n, ld, MX_DTYPES[x.dtype], code,
-                                       out.codes.data_ptr(), out.scales.data_ptr(), _pitch(n),
-                                       _lib.stream_of(dev)))
+                         f"{MX_BLOCK}, got shape {tuple(shape)}")
+    ld = n
+    if not x.is_contiguous():
+        if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= n \
+                and x.stride(0) * x.element_size() % 16 == 0:
+            ld = x.stride(0)
+        else:
+            x = x.contiguous()
+    if x.data_ptr() % 16:
+        x, ld = x.clone(memory_format=torch.contiguous_format), n
+    rows = x.numel() // n
+    out = MxTensor._empty(shape[:-1], rows, n, fmt, dev)
+    _launch(lib.nvm_mx_quantize, dev, x.data_ptr(), rows, n, ld, dtype, code,
+            out.codes.data_ptr(), out.scales.data_ptr(), out.pitch)
     return out
 
 
@@ -189,14 +191,12 @@ def mx_dequantize(t: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tens
     """The values that ``t`` stands for, rounded once to ``dtype``."""
     lib = _lib.load()
     dev = _lib.require_device(t.codes, t.scales)
-    if dtype not in MX_DTYPES:
+    code = MX_DTYPES.get(dtype)
+    if code is None:
         raise ValueError(f"mx_dequantize: dtype must be float16, bfloat16 or float32, got {dtype}")
-    n = t.shape[-1]
-    with _on(dev):
-        out = torch.empty(t.shape, dtype=dtype, device=dev)
-        _lib.check(lib.nvm_mx_dequantize(t.codes.data_ptr(), t.scales.data_ptr(),
-                                         _row_pitch(t.scales, n), t.rows, n, MX_FORMATS[t.fmt],
-                                         MX_DTYPES[dtype], out.data_ptr(), _lib.stream_of(dev)))
+    out = torch.empty(t.shape, dtype=dtype, device=dev)
+    _launch(lib.nvm_mx_dequantize, dev, t.codes.data_ptr(), t.scales.data_ptr(), t.pitch, t.rows,
+            t.shape[-1], MX_FORMATS[t.fmt], code, out.data_ptr())
     return out
 
 
@@ -209,71 +209,68 @@ def residual_rms_norm_mx(h: torch.Tensor, r: Optional[torch.Tensor], weight: tor
     lib = _lib.load()
     code = _format(fmt)
     dev = _lib.require_device(h, r, weight)
-    H = h.shape[-1]
-    if r is not None and (r.shape != h.shape or r.dtype != h.dtype):
-        raise ValueError("residual_rms_norm_mx: r must have the shape and dtype of h")
+    dtype = _lib.dtype_code(h.dtype)
+    shape = h.shape
+    H = shape[-1] if shape else 0
+    if H == 0 or H % MX_BLOCK:
+        raise ValueError(f"residual_rms_norm_mx: the last dimension must be a positive multiple "
+                         f"of {MX_BLOCK}, got shape {tuple(shape)}")
     if weight.numel() != H:
         raise ValueError(f"residual_rms_norm_mx: weight must have {H} elements")
     hc = _packed(h)
-    rc = None if r is None else _packed(r)
+    rc = h_out = None
+    if r is not None:
+        if r.shape != shape or r.dtype != h.dtype:
+            raise ValueError("residual_rms_norm_mx: r must have the shape and dtype of h")
+        rc = _packed(r)
+        h_out = torch.empty_like(hc)
     w = _packed(weight if weight.dtype == h.dtype else weight.to(h.dtype))
-    with _on(dev):
-        out = MxTensor._empty(h.shape[:-1], H, fmt, dev) if H % MX_BLOCK == 0 and H else None
-        if out is None:
-            raise ValueError(f"residual_rms_norm_mx: the last dimension must be a positive "
-                             f"multiple of {MX_BLOCK}, got {H}")
-        h_out = torch.empty_like(hc) if r is not None else None
-        _lib.check(lib.nvm_residual_rms_norm_mx(
-            hc.data_ptr(), _lib.ptr(rc), w.data_ptr(), out.rows, H, float(eps),
-            _lib.dtype_code(h.dtype), _lib.ptr(h_out), code, out.codes.data_ptr(),
-            out.scales.data_ptr(), _pitch(H), _lib.stream_of(dev)))
+    rows = hc.numel() // H
+    out = MxTensor._empty(shape[:-1], rows, H, fmt, dev)
+    _launch(lib.nvm_residual_rms_norm_mx, dev, hc.data_ptr(), _lib.ptr(rc), w.data_ptr(), rows, H,
+            float(eps), dtype, _lib.ptr(h_out), code, out.codes.data_ptr(), out.scales.data_ptr(),
+            out.pitch)
     return (h if h_out is None else h_out), out
 
 
-def _packed(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous and 16-byte aligned."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
 def _activations(x: Union[MxTensor, torch.Tensor], op: str) -> MxTensor:
-    if isinstance(x, MxTensor):
-        return x
-    if x.dtype not in (torch.float16, torch.bfloat16):
+    if x.dtype not in _lib.DTYPE_CODES:
         raise ValueError(f"{op}: x must be an MxTensor, float16 or bfloat16, got {x.dtype}")
     return mx_quantize(x, "mxfp8")
 
 
-def _check_weight(op: str, name: str, w: MxTensor, n: int) -> None:
-    if not isinstance(w, MxTensor) or w.fmt != "mxfp4" or len(w.shape) != 2:
+def _check_weight(op: str, name: str, w: MxTensor, a: MxTensor) -> None:
+    if type(w) is not MxTensor or w.fmt != "mxfp4" or len(w.shape) != 2:
         raise ValueError(f"{op}: {name} must be a two-dimensional mxfp4 MxTensor")
-    if w.shape[1] != n:
-        raise ValueError(f"{op}: {name} has {w.shape[1]} input features, x has {n}")
+    if w.shape[1] != a.shape[-1]:
+        raise ValueError(f"{op}: {name} has {w.shape[1]} input features, x has {a.shape[-1]}")
 
 
 def mx_linear(x: Union[MxTensor, torch.Tensor], w: MxTensor,
               dtype: Optional[torch.dtype] = None,
               bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x . w^T (+ bias)``: ``x [..., N]`` in MX (16-bit activations are
-    quantised to mxfp8 first), ``w [K, N]`` in mxfp4.  Exact products, float32
-    sums, one rounding to ``dtype`` (float16, bfloat16 or float32; by default
-    that of 16-bit activations, else bfloat16)."""
+    quantised to mxfp8 first), ``w [K, N]`` in mxfp4.  Float32 sums
+    (include/nvm_mx.h says what mxfp8 activations lose in them), one rounding
+    to ``dtype`` (float16, bfloat16 or float32; by default that of 16-bit
+    activations, else bfloat16)."""
     lib = _lib.load()
-    if dtype is None:
-        dtype = torch.bfloat16 if isinstance(x, MxTensor) else x.dtype
-    if dtype not in MX_DTYPES:
+    if type(x) is MxTensor:
+        a = x
+        dtype = torch.bfloat16 if dtype is None else dtype
+    else:
+        a = _activations(x, "mx_linear")
+        dtype = x.dtype if dtype is None else dtype
+    code = MX_DTYPES.get(dtype)
+    if code is None:
         raise ValueError(f"mx_linear: dtype must be float16, bfloat16 or float32, got {dtype}")
-    a = _activations(x, "mx_linear")
-    n = a.shape[-1]
-    _check_weight("mx_linear", "w", w, n)
-    dev = _lib.require_device(a.codes, w.codes)
-    K = w.shape[0]
-    with _on(dev):
-        out = torch.empty((*a.shape[:-1], K), dtype=dtype, device=dev)
-        _lib.check(lib.nvm_mx_matmul(
-            a.codes.data_ptr(), a.scales.data_ptr(), _row_pitch(a.scales, n), MX_FORMATS[a.fmt],
-            w.codes.data_ptr(), w.scales.data_ptr(), _row_pitch(w.scales, n), a.rows, n, K,
-            MX_DTYPES[dtype], out.data_ptr(), _lib.stream_of(dev)))
+    _check_weight("mx_linear", "w", w, a)
+    ac, wc, shape = a.codes, w.codes, w.shape
+    dev = _lib.require_device(ac, wc)
+    out = torch.empty((*a.shape[:-1], shape[0]), dtype=dtype, device=dev)
+    _launch(lib.nvm_mx_matmul, dev, ac.data_ptr(), a.scales.data_ptr(), a.pitch,
+            MX_FORMATS[a.fmt], wc.data_ptr(), w.scales.data_ptr(), w.pitch, a.rows, shape[1],
+            shape[0], code, out.data_ptr())
     return out if bias is None else out + bias
 
 
@@ -285,21 +282,17 @@ def mx_swiglu(x: Union[MxTensor, torch.Tensor], w_gate: MxTensor, w_up: MxTensor
     float32."""
     lib = _lib.load()
     code = _format(fmt)
-    a = _activations(x, "mx_swiglu")
-    n = a.shape[-1]
-    _check_weight("mx_swiglu", "w_gate", w_gate, n)
-    _check_weight("mx_swiglu", "w_up", w_up, n)
-    K = w_gate.shape[0]
+    a = x if type(x) is MxTensor else _activations(x, "mx_swiglu")
+    _check_weight("mx_swiglu", "w_gate", w_gate, a)
+    _check_weight("mx_swiglu", "w_up", w_up, a)
+    K, N = w_gate.shape
     if w_up.shape[0] != K or K == 0 or K % MX_BLOCK:
         raise ValueError(f"mx_swiglu: gate and up must have the same output features, a positive "
                          f"multiple of {MX_BLOCK}, got {K} and {w_up.shape[0]}")
     dev = _lib.require_device(a.codes, w_gate.codes, w_up.codes)
-    with _on(dev):
-        out = MxTensor._empty(a.shape[:-1], K, fmt, dev)
-        _lib.check(lib.nvm_mx_swiglu(
-            a.codes.data_ptr(), a.scales.data_ptr(), _row_pitch(a.scales, n), MX_FORMATS[a.fmt],
-            w_gate.codes.data_ptr(), w_gate.scales.data_ptr(), _row_pitch(w_gate.scales, n),
-            w_up.codes.data_ptr(), w_up.scales.data_ptr(), _row_pitch(w_up.scales, n), a.rows, n,
-            K, code, out.codes.data_ptr(), out.scales.data_ptr(), _pitch(K),
-            _lib.stream_of(dev)))
+    out = MxTensor._empty(a.shape[:-1], a.rows, K, fmt, dev)
+    _launch(lib.nvm_mx_swiglu, dev, a.codes.data_ptr(), a.scales.data_ptr(), a.pitch,
+            MX_FORMATS[a.fmt], w_gate.codes.data_ptr(), w_gate.scales.data_ptr(), w_gate.pitch,
+            w_up.codes.data_ptr(), w_up.scales.data_ptr(), w_up.pitch, a.rows, N, K, code,
+            out.codes.data_ptr(), out.scales.data_ptr(), out.pitch)
     return out

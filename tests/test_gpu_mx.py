@@ -112,7 +112,7 @@ def test_quantize_shapes(M, n, fmt, dt):
     x = (torch.randn(M, n, device=DEV, generator=_gen(M + n)) * 3).to(dt)
     t = mx_quantize(x, fmt)
     _same(t, x, fmt)
-    assert t.scales.stride(0) % 16 == 0
+    assert t.pitch % 16 == 0
 
 
 def test_quantize_strides_and_leading_dimensions():
