@@ -109,57 +109,6 @@ __device__ __forceinline__ float mx_swiglu(float g, float u) {
   return g * __builtin_amdgcn_rcpf(1.f + e) * u;
 }
 
-// Four neighbouring outputs of a row (element i of out) in the output type;
-// `left` of them are inside the row; `whole`: rows are a multiple of four
-// outputs, so the four are aligned and all inside.
-__device__ __forceinline__ void mx_store4(void *out, int dt, int64_t i, f32x4 v, int left,
-                                          bool whole) {
-  if (left <= 0) return;
-  if (dt == NVM_MX_F32) {
-    float *o = (float *)out + i;
-    if (whole) {
-      *(f32x4 *)o = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (e < left) o[e] = v[e];
-    }
-    return;
-  }
-  const bool bf = dt == NVM_MX_BF16;
-  const u32x2 d = bf ? u32x2{Act<DT_BF16>::pack2(v[0], v[1]), Act<DT_BF16>::pack2(v[2], v[3])}
-                     : u32x2{Act<DT_F16>::pack2(v[0], v[1]), Act<DT_F16>::pack2(v[2], v[3])};
-  uint16_t *o = (uint16_t *)out + i;
-  if (whole) {
-    *(u32x2 *)o = d;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (e < left) o[e] = (uint16_t)((e & 2 ? d.y : d.x) >> (16 * (e & 1)));
-  }
-}
-
-// One block of 32 MX outputs of row m from column k on: lane group G holds
-// values 4 G .. + 3 and 16 + 4 G .. + 3 (h[0..3], h[4..7]); amax_bits: the
-// largest magnitude of the whole block.
-template <int OFMT>
-__device__ __forceinline__ void mx_store_block(const float (&h)[8], uint32_t amax_bits, int64_t m,
-                                               int k, int G, int K, void *codes, uint8_t *scales,
-                                               int64_t sld) {
-  const uint32_t b = mx_scale_byte<OFMT>(amax_bits);
-  const u32x2 o = mx_encode8<OFMT>(h, mx_factor(b), b == 255u);
-  if constexpr (OFMT == NVM_MX_FP4) {
-    uint16_t *c = (uint16_t *)codes + (m * K + k) / 4 + G;
-    c[0] = (uint16_t)o.x;
-    c[4] = (uint16_t)(o.x >> 16);
-  } else {
-    uint32_t *c = (uint32_t *)codes + (m * K + k) / 4 + G;
-    c[0] = o.x;
-    c[4] = o.y;
-  }
-  if (G == 0) scales[m * sld + k / 32] = (uint8_t)b;
-}
-
 // Arguments of the products (gate/up: two weights, MX output).
 struct MxMatmulArgs {
   const uint8_t *a, *as;  // activations [M][N], scales
@@ -179,5 +128,82 @@ hipError_t launch_mx_gemv(int format, bool dual, int out_format, const MxMatmulA
                           hipStream_t st);
 hipError_t launch_mx_gemm(int format, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st);
+
+// f(integral constant) of an output type.
+template <int V>
+struct MxInt {
+  static constexpr int value = V;
+};
+template <class F>
+__host__ __device__ __forceinline__ void mx_by_dtype(int dtype, F f) {
+  if (dtype == NVM_MX_F32)
+    f(MxInt<NVM_MX_F32>{});
+  else if (dtype == NVM_MX_BF16)
+    f(MxInt<NVM_MX_BF16>{});
+  else
+    f(MxInt<NVM_MX_F16>{});
+}
+
+// Outputs k .. k + 3 of a row whose first is element `row` of out; those
+// below `end` are stored.
+template <int DT>
+__device__ __forceinline__ void mx_store4(void *out, int64_t row, int k, int end, f32x4 v) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (k + e >= end) break;
+    if constexpr (DT == NVM_MX_F32)
+      ((float *)out)[row + k + e] = v[e];
+    else
+      ((uint16_t *)out)[row + k + e] = Act<DT>::from_f32(v[e]);
+  }
+}
+
+// Two neighbouring 16-row weight tiles' outputs of one activation row, from
+// output k on: lane group G holds v0 = outputs 4 G .. + 3 and v1 = 16 + 4 G ..
+// + 3.  Rows are a multiple of eight outputs, and so is `end`.  16-bit
+// outputs trade places first (v_permlane16_swap: lane groups 1 and 3 of the
+// first with 0 and 2 of the second), which leaves a lane with eight
+// neighbours, 16 bytes: groups 0 and 2 of the first tile, 1 and 3 of the
+// second.  Every lane of the wavefront is active.
+template <int DT>
+__device__ __forceinline__ void mx_store_pair(void *out, int G, int64_t row, int k, int end, f32x4 v0,
+                                              f32x4 v1) {
+  if constexpr (DT == NVM_MX_F32) {
+    float *o = (float *)out + row + k + 4 * G;
+    if (k + 4 * G < end) *(f32x4 *)o = v0;
+    if (k + 16 + 4 * G < end) *(f32x4 *)(o + 16) = v1;
+  } else {
+    using A = Act<DT>;
+    const auto a = __builtin_amdgcn_permlane16_swap(A::pack2(v0[0], v0[1]), A::pack2(v1[0], v1[1]),
+                                                    false, false);
+    const auto b = __builtin_amdgcn_permlane16_swap(A::pack2(v0[2], v0[3]), A::pack2(v1[2], v1[3]),
+                                                    false, false);
+    k += 16 * (G & 1) + 8 * (G >> 1);
+    if (k < end) *(u32x4 *)((uint16_t *)out + row + k) = u32x4{a[0], b[0], a[1], b[1]};
+  }
+}
+
+// One block of 32 MX outputs of row m, from column k on: lane group G holds
+// values 4 G .. + 3 and 16 + 4 G .. + 3 (h[0..3], h[4..7]).  The codes trade
+// places as above, so a lane stores eight neighbours.  Every lane of the
+// wavefront is active; `on`: the block is inside the output.
+template <int OFMT>
+__device__ __forceinline__ void mx_store_block(const float (&h)[8], int G, bool on, int64_t m, int k,
+                                               const MxMatmulArgs &p) {
+  uint32_t mx = absmax8(h);
+  mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16));
+  mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
+  const uint32_t b = mx_scale_byte<OFMT>(mx);
+  const u32x2 o = mx_encode8<OFMT>(h, mx_factor(b), b == 255u);
+  const int64_t i = (m * p.K + k) / 8 + 2 * (G & 1) + (G >> 1);  // eight outputs
+  if constexpr (OFMT == NVM_MX_FP4) {
+    const auto a = __builtin_amdgcn_permlane16_swap(o.x & 0xFFFFu, o.x >> 16, false, false);
+    if (on) ((uint32_t *)p.out)[i] = a[0] | (a[1] << 16);
+  } else {
+    const auto a = __builtin_amdgcn_permlane16_swap(o.x, o.y, false, false);
+    if (on) ((u32x2 *)p.out)[i] = u32x2{a[0], a[1]};
+  }
+  if (on && G == 0) p.out_s[m * p.out_sld + k / 32] = (uint8_t)b;
+}
 
 }  // namespace nvm

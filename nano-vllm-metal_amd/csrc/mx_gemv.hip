@@ -5,12 +5,13 @@
 // 1.4 us of HBM time).  The scaled matrix instruction takes the codes as they
 // lie in memory, so a wavefront is loads, matrix instructions and one sum:
 //  * a block owns RT 16-row tiles of the weights and MT 16-row tiles of the
-//    activations; its NW wavefronts split the reduction in runs of whole
-//    128-value steps, and each requests up to RING steps (weights, their
-//    scales, activations) before it uses the first;
+//    activations; its NW wavefronts take runs of four 128-value steps in turn,
+//    and each requests a whole run (weights, their scales, activations) before
+//    it uses any of it, BUF runs at a time;
 //  * operands go from memory straight into the instruction's registers: a
-//    lane's 16 bytes of a weight row are its 32 values of a step, and the
-//    activations are few enough to come from L2;
+//    lane's 16 bytes of a weight row are its 32 values of a step, a row's 16
+//    scale bytes are the run's, and the activations are few enough to come
+//    from L2;
 //  * the wavefronts' sums meet in LDS once and are added in order.
 // Weights are the row operand, so a lane ends up with four neighbouring
 // outputs of one activation row, and a block of 32 outputs (SwiGLU's MX
@@ -26,7 +27,7 @@ namespace {
 
 // RT: weight tiles of a block (DUAL: RT / 2 of the gate and the same rows of
 // the up projection).
-template <int FMT, int OFMT, bool DUAL, int RT, int MT, int NW, int RING>
+template <int FMT, int OFMT, bool DUAL, int RT, int MT, int NW, int BUF>
 __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxMatmulArgs p) {
   constexpr int NX = FMT == NVM_MX_FP4 ? 1 : 2;  // 16-byte loads of a lane's 32 activations
   constexpr int RF = DUAL ? RT / 2 : RT;         // tiles of output columns
@@ -39,9 +40,7 @@ __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxMatmulArgs p) 
   const int nk = min(RF * 16, p.K - k0);
   const int nm = (int)min((int64_t)(MT * 16), p.M - m0);
   const int WB = p.N / 2, XB = p.N * Mx<FMT>::kBits / 8;  // bytes of a row
-  const int nb = p.N / 32;
-  const int steps = (p.N + 127) / 128, per = (steps + NW - 1) / NW;
-  const int s0 = wv * per, s1 = min(steps, s0 + per);
+  const int nb = p.N / 32, runs = (p.N + 511) / 512;
 
   rsrc_t wr[DUAL ? 2 : 1], wsr[DUAL ? 2 : 1];
 #pragma unroll
@@ -66,32 +65,36 @@ __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxMatmulArgs p) 
     xso[t] = r < nm ? r * (int)p.as_ld : kMaskedOffset;
   }
 
-  struct Step {
-    MxFrag<NVM_MX_FP4> w[RT];
-    MxFrag<FMT> x[MT];
-    uint32_t ws[RT], xs[MT];
+  struct Run {
+    MxFrag<NVM_MX_FP4> w[4][RT];
+    MxFrag<FMT> x[4][MT];
+    u32x4 ws[RT], xs[MT];  // dword j: step j, byte G of it the lane's block
   };
-  // (steps past the wavefront's run, and values past the row: zeros with the
-  // scale of one, whatever lies behind the row)
-  auto load = [&](Step &q, int s) {
-    const bool on = s < s1;
-    const int so = on ? s : 0;
-    const bool wk = on && 128 * so + 32 * G < p.N;
+  // (runs past the last, and values past the row: zeros)
+  auto load = [&](Run &q, int r) {
+    const bool on = r < runs;
+    const int r0 = on ? r : 0;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      q.w[t].v[0] = bload16(wr[DUAL && t >= RF], wk ? wo[t] : kMaskedOffset, 64 * so);
-      q.ws[t] = bload4(wsr[DUAL && t >= RF], wk ? wso[t] : kMaskedOffset, 4 * so);
-    }
+    for (int t = 0; t < RT; ++t)
+      q.ws[t] = bload16(wsr[DUAL && t >= RF], on ? wso[t] : kMaskedOffset, 16 * r0);
 #pragma unroll
-    for (int t = 0; t < MT; ++t) {
+    for (int t = 0; t < MT; ++t) q.xs[t] = bload16(xsr, on ? xso[t] : kMaskedOffset, 16 * r0);
 #pragma unroll
-      for (int c = 0; c < NX; ++c) {
-        // (FP4: the lane's 32 values; FP8: 16 at 16 G, 16 at 64 + 16 G)
-        const bool xk = FMT == NVM_MX_FP4 ? wk : on && 128 * so + 64 * c + 16 * G < p.N;
-        q.x[t].v[c] = bload16(xr, xk ? xo[t] : kMaskedOffset,
-                              FMT == NVM_MX_FP4 ? 64 * so : 128 * so + 64 * c);
-      }
-      q.xs[t] = bload4(xsr, wk ? xso[t] : kMaskedOffset, 4 * so);
+    for (int j = 0; j < 4; ++j) {
+      const int v = 512 * r0 + 128 * j;  // the step's first value
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        q.w[j][t].v[0] = bload16(wr[DUAL && t >= RF],
+                                 on && v + 32 * G < p.N ? wo[t] : kMaskedOffset, v / 2);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int c = 0; c < NX; ++c) {
+          // (FP4: the lane's 32 values; FP8: 16 at 16 G, 16 at 64 + 16 G)
+          const int o = FMT == NVM_MX_FP4 ? 32 * G : 64 * c + 16 * G;
+          q.x[j][t].v[c] = bload16(xr, on && v + o < p.N ? xo[t] : kMaskedOffset,
+                                   FMT == NVM_MX_FP4 ? v / 2 : v + 64 * c);
+        }
     }
   };
   f32x4 acc[RT][MT];
@@ -99,28 +102,31 @@ __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxMatmulArgs p) 
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto use = [&](const Step &q, int s) {
-    // the lane group's byte of the step's four
-    const bool in = s < s1 && 4 * s + G < nb;
-    auto pick = [&](uint32_t d) { return in ? d >> (8 * G) : 127u; };
-    uint32_t ws[RT], xs[MT];
+  auto use = [&](const Run &q, int r) {
 #pragma unroll
-    for (int t = 0; t < RT; ++t) ws[t] = pick(q.ws[t]);
+    for (int j = 0; j < 4; ++j) {
+      // (behind a row: the scale of one, whatever lies there)
+      const bool in = 16 * r + 4 * j + G < nb;
+      uint32_t xs[MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) xs[t] = pick(q.xs[t]);
+      for (int t = 0; t < MT; ++t) xs[t] = in ? q.xs[t][j] >> (8 * G) : 127u;
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+      for (int i = 0; i < RT; ++i) {
+        const uint32_t ws = in ? q.ws[i][j] >> (8 * G) : 127u;
 #pragma unroll
-      for (int t = 0; t < MT; ++t) acc[r][t] = mx_mfma<FMT>(q.w[r], ws[r], q.x[t], xs[t], acc[r][t]);
+        for (int t = 0; t < MT; ++t)
+          acc[i][t] = mx_mfma<FMT>(q.w[j][i], ws, q.x[j][t], xs[t], acc[i][t]);
+      }
+    }
   };
-  Step ring[RING];
+  Run buf[BUF];
 #pragma unroll
-  for (int j = 0; j < RING; ++j) load(ring[j], s0 + j);
-  for (int s = s0; s < s1; s += RING) {
+  for (int j = 0; j < BUF; ++j) load(buf[j], wv + j * NW);
+  for (int r = wv; r < runs; r += BUF * NW) {
 #pragma unroll
-    for (int j = 0; j < RING; ++j) {
-      use(ring[j], s + j);
-      load(ring[j], s + j + RING);
+    for (int j = 0; j < BUF; ++j) {
+      use(buf[j], r + j * NW);
+      load(buf[j], r + (j + BUF) * NW);
     }
   }
 
@@ -137,53 +143,82 @@ __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxMatmulArgs p) 
   };
   if constexpr (!DUAL) {
     for (int i = wv; i < RT * MT; i += NW) {
-      const int r = i / MT, t = i % MT;
+      const int r = i / MT, m = 16 * (i % MT) + col;
       const f32x4 v = sum(i);
-      const int k = 16 * r + 4 * G, m = 16 * t + col;
-      if (m >= nm) continue;
-      mx_store4(p.out, p.out_dtype, (m0 + m) * p.K + k0 + k, v, nk - k, p.K % 4 == 0);
+      if (m < nm)
+        mx_by_dtype(p.out_dtype, [&](auto DTYPE) {
+          mx_store4<decltype(DTYPE)::value>(p.out, (m0 + m) * p.K + k0, 16 * r + 4 * G, nk, v);
+        });
     }
   } else {
     // a block of 32 outputs of a row: two tiles, four lane groups
     for (int i = wv; i < RF / 2 * MT; i += NW) {
-      const int r = i / MT, t = i % MT;
+      const int r = i / MT, t = i % MT, m = 16 * t + col;
       float h[8];
-      uint32_t mx = 0;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const f32x4 g = sum((2 * r + j) * MT + t), u = sum((RF + 2 * r + j) * MT + t);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          h[4 * j + e] = mx_swiglu(g[e], u[e]);
-          mx = max(mx, abs_bits(h[4 * j + e]));
-        }
+        for (int e = 0; e < 4; ++e) h[4 * j + e] = mx_swiglu(g[e], u[e]);
       }
-      mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16));
-      mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));
-      const int m = 16 * t + col;
-      if (m >= nm || 32 * r >= nk) continue;
-      mx_store_block<OFMT>(h, mx, (m0 + m), k0 + 32 * r, G, p.K, p.out, p.out_s, p.out_sld);
+      mx_store_block<OFMT>(h, G, m < nm && 32 * r < nk, m0 + m, k0 + 32 * r, p);
     }
   }
 }
 
-template <int FMT, int OFMT, bool DUAL, int RT, int MT, int NW, int RING>
+template <int FMT, int OFMT, bool DUAL, int RT, int MT, int NW, int BUF>
 void go(const MxMatmulArgs &a, hipStream_t st) {
   constexpr int RF = DUAL ? RT / 2 : RT;
   const dim3 grid((unsigned)((a.K + 16 * RF - 1) / (16 * RF)),
                   (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
-  hipLaunchKernelGGL((mx_gemv_kernel<FMT, OFMT, DUAL, RT, MT, NW, RING>), grid, dim3(64 * NW), 0,
+  hipLaunchKernelGGL((mx_gemv_kernel<FMT, OFMT, DUAL, RT, MT, NW, BUF>), grid, dim3(64 * NW), 0,
                      st, a);
 }
 
+// The largest tile of a block that leaves kBlocks of them, without a half-used
+// activation tile.  Larger blocks read the activations, and a column of them
+// the weights, less often; too few leave CUs idle (2048 -> 5120 of 17 rows: 160
+// blocks of 2 x 2 tiles 5.6 us, 320 of 2 x 1 6.6; of 33 rows 240 of 4 x 1 7.1,
+// 480 of 2 x 1 7.5; of 64 rows 214 of 3 x 2 8.1, 640 of 2 x 1 10.0; 4096 ->
+// 2048 of 16 rows: 128 of 1 x 1 5.7, 64 of 2 x 1 7.0).
+constexpr int64_t kBlocks = 160;
+
 template <int FMT>
 void launch_fmt(bool dual, int out_format, const MxMatmulArgs &a, hipStream_t st) {
-  if (!dual)
-    go<FMT, NVM_MX_FP8, false, 1, 1, 8, 2>(a, st);
-  else if (out_format == NVM_MX_FP4)
-    go<FMT, NVM_MX_FP4, true, 4, 1, 8, 2>(a, st);
+  const int64_t mt = (a.M + 15) / 16;
+  auto fits = [&](int rt, int m) {
+    return mt % m == 0 && (a.K + 16 * rt - 1) / (16 * rt) * (mt / m) >= kBlocks;
+  };
+  if (!dual) {
+    if (fits(3, 2))
+      go<FMT, NVM_MX_FP8, false, 3, 2, 4, 1>(a, st);
+    else if (fits(4, 1))
+      go<FMT, NVM_MX_FP8, false, 4, 1, 4, 1>(a, st);
+    else if (fits(2, 2))
+      go<FMT, NVM_MX_FP8, false, 2, 2, 4, 1>(a, st);
+    else if (fits(2, 1))
+      go<FMT, NVM_MX_FP8, false, 2, 1, 4, 1>(a, st);
+    else
+      go<FMT, NVM_MX_FP8, false, 1, 1, 4, 1>(a, st);
+    return;
+  }
+  // SwiGLU: 32 outputs a block (its scale needs them), over all activation
+  // rows of up to four tiles (2048 -> 6144 of 8 rows: 6.9 us with eight
+  // wavefronts, 7.1 with four; of 17 rows 7.8 on 2 tiles, 10.2 on 1; of 64
+  // rows 11.9 on 4, 13.4 on 2)
+  auto swiglu = [&](auto OF) {
+    constexpr int OFMT = decltype(OF)::value;
+    if (mt == 1)
+      go<FMT, OFMT, true, 4, 1, 8, 1>(a, st);
+    else if (mt == 2)
+      go<FMT, OFMT, true, 4, 2, 8, 1>(a, st);
+    else
+      go<FMT, OFMT, true, 4, 4, 4, 1>(a, st);
+  };
+  if (out_format == NVM_MX_FP4)
+    swiglu(MxInt<NVM_MX_FP4>{});
   else
-    go<FMT, NVM_MX_FP8, true, 4, 1, 8, 2>(a, st);
+    swiglu(MxInt<NVM_MX_FP8>{});
 }
 
 }  // namespace

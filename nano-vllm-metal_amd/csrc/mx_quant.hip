@@ -223,26 +223,13 @@ void launch_norm_mx(const void *h, const void *r, const void *w, int64_t T, int6
     go(residual_rms_norm_mx_kernel<DT, FMT, 256, 4>, 256);
 }
 
-// Calls f(integral_constant...) with the constants of (dtype, format).
-template <int V>
-struct Int {
-  static constexpr int value = V;
-};
-template <class F>
-void by_dtype(int dtype, F f) {
-  if (dtype == NVM_MX_F32)
-    f(Int<NVM_MX_F32>{});
-  else if (dtype == NVM_MX_BF16)
-    f(Int<NVM_MX_BF16>{});
-  else
-    f(Int<NVM_MX_F16>{});
-}
+// f(integral constant) of a format.
 template <class F>
 void by_format(int format, F f) {
   if (format == NVM_MX_FP4)
-    f(Int<NVM_MX_FP4>{});
+    f(MxInt<NVM_MX_FP4>{});
   else
-    f(Int<NVM_MX_FP8>{});
+    f(MxInt<NVM_MX_FP8>{});
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -295,7 +282,7 @@ int nvm_mx_quantize(const void *x, int64_t rows, int64_t n, int64_t x_ld, int dt
   if (total > kMaxChunks)
     return set_error(NVM_ERR_UNSUPPORTED, "%s: more than 2^35 values in one call", op);
   const dim3 grid((unsigned)((total + kThreads - 1) / kThreads));
-  by_dtype(dtype, [&](auto D) {
+  mx_by_dtype(dtype, [&](auto D) {
     by_format(format, [&](auto F) {
       hipLaunchKernelGGL((mx_quantize_kernel<decltype(D)::value, decltype(F)::value>), grid,
                          dim3(kThreads), 0, (hipStream_t)stream, x, (uint32_t)total, (int)(n / 8), x_ld,
@@ -322,7 +309,7 @@ int nvm_mx_dequantize(const void *codes, const uint8_t *scales, int64_t scale_ld
   if (total > kMaxChunks)
     return set_error(NVM_ERR_UNSUPPORTED, "%s: more than 2^35 values in one call", op);
   const dim3 grid((unsigned)((total + kThreads - 1) / kThreads));
-  by_dtype(dtype, [&](auto D) {
+  mx_by_dtype(dtype, [&](auto D) {
     by_format(format, [&](auto F) {
       hipLaunchKernelGGL((mx_dequantize_kernel<decltype(F)::value, decltype(D)::value>), grid,
                          dim3(kThreads), 0, (hipStream_t)stream, codes, scales, scale_ld, (uint32_t)total,
