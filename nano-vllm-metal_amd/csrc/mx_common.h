@@ -90,12 +90,13 @@ struct MxFrag {
 };
 
 // c += w . x^T: rows (4 G + i of c) from the FP4 weights, columns (lane % 16)
-// from the activations.
-template <int FMT>
+// from the activations; the scales are byte BYTE of ws and xs.
+template <int FMT, int BYTE = 0>
 __device__ __forceinline__ f32x4 mx_mfma(const MxFrag<NVM_MX_FP4> &w, uint32_t ws,
                                          const MxFrag<FMT> &x, uint32_t xs, f32x4 c) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-      w.operand(), x.operand(), c, Mx<NVM_MX_FP4>::kMfma, Mx<FMT>::kMfma, 0, (int)ws, 0, (int)xs);
+      w.operand(), x.operand(), c, Mx<NVM_MX_FP4>::kMfma, Mx<FMT>::kMfma, BYTE, (int)ws, BYTE,
+      (int)xs);
 }
 
 // g / (1 + exp(-g)) * u.  exp(-g) = 2^t 2^d with t = -g log2(e) rounded and d
@@ -121,11 +122,15 @@ struct MxMatmulArgs {
   uint8_t *out_s;
   int64_t out_sld;
 };
-// The products for few rows (mx_gemv.hip) and for many (mx_gemm.hip, at most
-// kMxMaxTiles output tiles: else hipErrorInvalidConfiguration).
+// The products for few rows (mx_gemv.hip), for some (mx_gemm_pipe.hip: tiles of
+// 128 outputs by 128 rows, `wide` 256 by 128) and for many (mx_gemm.hip: 256 by
+// 256).  The latter two take at most kMxMaxTiles output tiles: else
+// hipErrorInvalidConfiguration.
 constexpr int64_t kMxMaxTiles = 1 << 22;
 hipError_t launch_mx_gemv(int format, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st);
+hipError_t launch_mx_gemm_pipe(int format, bool wide, bool dual, int out_format,
+                               const MxMatmulArgs &a, hipStream_t st);
 hipError_t launch_mx_gemm(int format, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st);
 

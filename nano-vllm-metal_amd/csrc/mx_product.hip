@@ -1,0 +1,128 @@
+// Products of MX rows with MXFP4 weights: which kernel, and the entry points
+// (include/nvm_mx.h).
+#include <algorithm>
+
+#include "internal.h"
+#include "mx_common.h"
+
+namespace nvm {
+
+// Few rows: mx_gemv.hip, whose time goes with rows x output columns (of both
+// matrices), while the tiles' goes with the steps along a row until they fill
+// the GPU.  2048 -> 5120: 64 rows (328 thousand outputs) 8.2 us there, 11.2 on
+// tiles; 96 rows (492) 12.9 and 11.4; 4096 -> 12288: 32 rows (393) 12.0 and
+// 17.2, 64 rows (786) 20.9 and 17.5; gate/up 2048 -> 6144: 32 rows (393) 8.7 and
+// 12.1, 96 rows 19.9 and 12.6.  One tile of 16 rows stays there whatever the
+// columns: 2048 -> 32768 of 16 rows 12.5 and 12.9 us, 2048 -> 151936 of 1 row
+// 43.7 and 48.3, of 16 rows 52.7 and 50.5.
+static bool few_rows(int64_t rows, int64_t columns) {
+  return rows <= 16 || rows * columns <= 3 << 17;
+}
+
+// Many rows: the tile whose rounds over the CUs cost least.  A step of the
+// larger ones costs less for its outputs, but they leave more CUs idle.  Their
+// costs, in steps of 256 x 256 at 20 (0.9 us each): E4M3 activations 13 and 9,
+// E2M1 11 and 8 for 256 x 128 and 128 x 128.  In us on 256 x 256, 256 x 128 and
+// 128 x 128, E4M3 unless said:
+//   2048 -> 5120    512 rows   24.0  17.2  13.2
+//                  1536 rows   26.3  21.0  24.8
+//                  2048 rows   27.0  30.3  35.2
+//                  4096 rows   47.5  46.4  59.0  (E2M1 42.4  38.3  46.3)
+//   6144 -> 2048   1024 rows   54    34    24
+//                  4096 rows   57    45.5  54
+//   8192 -> 8192   8192 rows   367   424   553   (E2M1  293   350   420)
+//   gate/up 2048 -> 6144
+//                   100 rows   24.0  16.8  12.6
+//                  1000 rows   27.7  31.7  35.9
+//                  4096 rows   82    94.7  134
+static hipError_t launch_mx_product(int format, bool dual, int out_format, const MxMatmulArgs &a,
+                                    hipStream_t st) {
+  const int64_t columns = (int64_t)a.K * (dual ? 2 : 1);
+  if (few_rows(a.M, columns)) return launch_mx_gemv(format, dual, out_format, a, st);
+  const int64_t cus = cu_count();
+  auto rounds = [&](int bn, int bm) {
+    return ((columns + bn - 1) / bn * ((a.M + bm - 1) / bm) + cus - 1) / cus;
+  };
+  const bool fp4 = format == NVM_MX_FP4;
+  const int64_t big = rounds(256, 256) * 20, wide = rounds(256, 128) * (fp4 ? 11 : 13),
+                small = rounds(128, 128) * (fp4 ? 8 : 9);
+  if (big <= std::min(wide, small)) return launch_mx_gemm(format, dual, out_format, a, st);
+  return launch_mx_gemm_pipe(format, wide <= small, dual, out_format, a, st);
+}
+
+}  // namespace nvm
+
+extern "C" {
+
+int nvm_mx_matmul(const void *a_codes, const uint8_t *a_scales, int64_t a_scale_ld, int a_format,
+                  const void *w_codes, const uint8_t *w_scales, int64_t w_scale_ld, int64_t M,
+                  int64_t N, int64_t K, int out_dtype, void *out, nvm_stream_t stream) {
+  using namespace nvm;
+  const char *op = "mx_matmul";
+  if (out_dtype != NVM_MX_F16 && out_dtype != NVM_MX_BF16 && out_dtype != NVM_MX_F32)
+    return set_error(NVM_ERR_INVALID, "%s: out_dtype must be f16, bf16 or f32", op);
+  if (int rc = mx_check_rows(op, M, N, a_format, "a")) return rc;
+  if (int rc = mx_check_rows(op, K, N, NVM_MX_FP4, "w")) return rc;
+  if (M == 0 || K == 0) return NVM_OK;
+  if (int rc = mx_check_tensor(op, a_codes, a_scales, a_scale_ld, N, "a")) return rc;
+  if (int rc = mx_check_tensor(op, w_codes, w_scales, w_scale_ld, N, "w")) return rc;
+  if (!out || ((uintptr_t)out & 15))
+    return set_error(NVM_ERR_INVALID, "%s: out must be a 16-byte aligned pointer", op);
+  MxMatmulArgs a{};
+  a.a = (const uint8_t *)a_codes;
+  a.as = a_scales;
+  a.as_ld = a_scale_ld;
+  a.w[0] = (const uint8_t *)w_codes;
+  a.ws[0] = w_scales;
+  a.ws_ld[0] = w_scale_ld;
+  a.M = M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.out_dtype = out_dtype;
+  a.out = out;
+  const hipError_t e = launch_mx_product(a_format, false, NVM_MX_FP8, a, (hipStream_t)stream);
+  if (e == hipErrorInvalidConfiguration)
+    return set_error(NVM_ERR_UNSUPPORTED, "%s: too many output tiles", op);
+  if (e != hipSuccess) return set_error(NVM_ERR_HIP, "%s: %s", op, hipGetErrorString(e));
+  return NVM_OK;
+}
+
+int nvm_mx_swiglu(const void *a_codes, const uint8_t *a_scales, int64_t a_scale_ld, int a_format,
+                  const void *gate_codes, const uint8_t *gate_scales, int64_t gate_scale_ld,
+                  const void *up_codes, const uint8_t *up_scales, int64_t up_scale_ld, int64_t M,
+                  int64_t N, int64_t K, int out_format, void *out_codes, uint8_t *out_scales,
+                  int64_t out_scale_ld, nvm_stream_t stream) {
+  using namespace nvm;
+  const char *op = "mx_swiglu";
+  if (int rc = mx_check_rows(op, M, N, a_format, "a")) return rc;
+  if (int rc = mx_check_rows(op, K, N, NVM_MX_FP4, "gate and up")) return rc;
+  if (int rc = mx_check_rows(op, M, K, out_format, "output")) return rc;
+  if (M == 0) return NVM_OK;
+  if (int rc = mx_check_tensor(op, a_codes, a_scales, a_scale_ld, N, "a")) return rc;
+  if (int rc = mx_check_tensor(op, gate_codes, gate_scales, gate_scale_ld, N, "gate")) return rc;
+  if (int rc = mx_check_tensor(op, up_codes, up_scales, up_scale_ld, N, "up")) return rc;
+  if (int rc = mx_check_tensor(op, out_codes, out_scales, out_scale_ld, K, "output")) return rc;
+  MxMatmulArgs a{};
+  a.a = (const uint8_t *)a_codes;
+  a.as = a_scales;
+  a.as_ld = a_scale_ld;
+  a.w[0] = (const uint8_t *)gate_codes;
+  a.ws[0] = gate_scales;
+  a.ws_ld[0] = gate_scale_ld;
+  a.w[1] = (const uint8_t *)up_codes;
+  a.ws[1] = up_scales;
+  a.ws_ld[1] = up_scale_ld;
+  a.M = M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.out = out_codes;
+  a.out_s = out_scales;
+  a.out_sld = out_scale_ld;
+  const hipError_t e = launch_mx_product(a_format, true, out_format, a, (hipStream_t)stream);
+  if (e == hipErrorInvalidConfiguration)
+    return set_error(NVM_ERR_UNSUPPORTED, "%s: too many output tiles", op);
+  if (e != hipSuccess) return set_error(NVM_ERR_HIP, "%s: %s", op, hipGetErrorString(e));
+  return NVM_OK;
+}
+
+}  // extern "C"

@@ -377,6 +377,63 @@ def test_linear_writes_its_rows_only():
             _close(out[:M], _val(a), _val(w), dt, "mxfp8")
 
 
+# Sizes at which each tile runs (on 256 CUs): of 128 x 128, of 256 x 128 (one and
+# several to a block), of 256 x 256 (one and two to a block); rows of one step,
+# of one run, of a step more than a run, and with a last step cut short.
+TILED = [(400, 32, 1000), (450, 640, 901), (521, 1184, 768), (1030, 96, 4000), (1030, 640, 4003),
+         (2600, 160, 8200), (1030, 512, 8200), (1030, 672, 8193), (3900, 32, 8104), (3900, 160, 8100)]
+
+
+@pytest.mark.parametrize("M,N,K", TILED)
+@pytest.mark.parametrize("fmt", FMTS)
+def test_linear_on_tiles(M, N, K, fmt):
+    from nano_vllm_metal_amd import MxTensor, mx_linear
+
+    g = _gen(M + N + K)
+    a = _mx(torch.randn(M, N, device=DEV, generator=g), fmt)
+    w = _mx(torch.randn(K, N, device=DEV, generator=g) * N ** -0.5, "mxfp4")
+    for dt in (torch.bfloat16, torch.float32):
+        y = mx_linear(a, w, dt)
+        _close(y, _val(a), _val(w), dt, fmt)
+    # a NaN block of a row and of a column leaves all others as they were
+    sa, sw = a.scales.clone(), w.scales.clone()
+    sa[M - 2, -1], sw[K - 3, 0] = 255, 255
+    z = mx_linear(MxTensor(a.codes, sa, fmt), MxTensor(w.codes, sw, "mxfp4"), torch.float32)
+    nan = torch.zeros_like(z, dtype=torch.bool)
+    nan[M - 2], nan[:, K - 3] = True, True
+    assert torch.equal(torch.isnan(z), nan) and torch.equal(z[~nan], y[~nan])
+
+
+@pytest.mark.parametrize("M,N,K", [(450, 160, 900), (450, 608, 900), (1030, 160, 4000),
+                                   (1030, 160, 8200), (1030, 608, 8200)])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_tiles_read_and_write_their_rows_only(M, N, K, fmt):
+    """What lies behind a row and behind the last one: NaN scales and codes in
+    the operands, a pattern in the output."""
+    from nano_vllm_metal_amd import MxTensor, _lib, mx_linear
+
+    g = _gen(N)
+    a0 = _mx(torch.randn(M, N, device=DEV, generator=g), fmt)
+    w0 = _mx(torch.randn(K, N, device=DEV, generator=g), "mxfp4")
+
+    def hostile(t):
+        rows = t.codes.shape[0]
+        codes = torch.full((rows + 3, t.codes.shape[1]), 0xFF, dtype=torch.uint8, device=DEV)
+        scales = torch.full((rows + 3, 32), 255, dtype=torch.uint8, device=DEV)
+        codes[:rows], scales[:rows, :N // 32] = t.codes, t.scales
+        return MxTensor(codes[:rows], scales[:rows, :N // 32], t.fmt)
+
+    a, w = hostile(a0), hostile(w0)
+    out = torch.full((M + 2, K), 7.0, device=DEV)
+    _lib.check(_lib.load().nvm_mx_matmul(
+        a.codes.data_ptr(), a.scales.data_ptr(), a.scales.stride(0), FMTS.index(fmt),
+        w.codes.data_ptr(), w.scales.data_ptr(), w.scales.stride(0), M, N, K, 2, out.data_ptr(),
+        _lib.stream_of(out.device)))
+    assert (out[M:] == 7).all()
+    assert torch.equal(out[:M], mx_linear(a0, w0, torch.float32))
+    _close(out[:M], _val(a0), _val(w0), torch.float32, fmt)
+
+
 # ------------------------------------------------------------------- SwiGLU
 
 
@@ -406,6 +463,14 @@ def test_swiglu(M, N, K, fmt, ofmt):
     assert y.shape == (M, K) and y.fmt == ofmt
     h, d = _swiglu_exact(a, wg, wu)
     O.check_quantized(y.codes, y.scales, ofmt, h, d)
+
+
+@pytest.mark.parametrize("M,N,K", [(300, 160, 800), (401, 640, 544), (1030, 160, 2016),
+                                   (2600, 96, 4128), (1030, 640, 4128), (3900, 96, 4064)])
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("ofmt", FMTS)
+def test_swiglu_on_tiles(M, N, K, fmt, ofmt):
+    test_swiglu(M, N, K, fmt, ofmt)
 
 
 @pytest.mark.parametrize("M", [6, 70])
