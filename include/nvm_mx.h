@@ -50,6 +50,12 @@ int nvm_mx_quantize(const void *x, int64_t rows, int64_t n, int64_t x_ld, int dt
 int nvm_mx_dequantize(const void *codes, const uint8_t *scales, int64_t scale_ld, int64_t rows,
                       int64_t n, int format, int dtype, void *out, nvm_stream_t stream);
 
+/* Rows ids[0], .. ids[T - 1] of a table [V, n] (an embedding), rounded once to
+ * `dtype`: out [T, n].  Ids outside [0, V) give zero rows. */
+int nvm_mx_embedding(const int32_t *ids, int64_t T, const void *codes, const uint8_t *scales,
+                     int64_t scale_ld, int64_t V, int64_t n, int format, int dtype, void *out,
+                     nvm_stream_t stream);
+
 /* nvm_residual_rms_norm with an MX output: h_out = rnd(h + r) (r NULL: h
  * itself, h_out not written), and the MX codes of rms_norm(h_out) * w.  The
  * norm is computed in float64 and not rounded to the activation dtype before

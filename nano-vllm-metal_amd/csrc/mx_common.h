@@ -124,8 +124,8 @@ struct MxMatmulArgs {
 };
 // The products for few rows (mx_gemv.hip), for some (mx_gemm_pipe.hip: tiles of
 // 128 outputs by 128 rows, `wide` 256 by 128) and for many (mx_gemm.hip: 256 by
-// 256).  The latter two take at most kMxMaxTiles output tiles: else
-// hipErrorInvalidConfiguration.
+// 256).  hipErrorInvalidConfiguration: more blocks than a launch has, more
+// than kMxMaxTiles output tiles.
 constexpr int64_t kMxMaxTiles = 1 << 22;
 hipError_t launch_mx_gemv(int format, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st);

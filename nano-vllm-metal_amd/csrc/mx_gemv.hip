@@ -167,12 +167,14 @@ __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxMatmulArgs p) 
 }
 
 template <int FMT, int OFMT, bool DUAL, int RT, int MT, int NW, int BUF>
-void go(const MxMatmulArgs &a, hipStream_t st) {
+hipError_t go(const MxMatmulArgs &a, hipStream_t st) {
   constexpr int RF = DUAL ? RT / 2 : RT;
-  const dim3 grid((unsigned)((a.K + 16 * RF - 1) / (16 * RF)),
-                  (unsigned)((a.M + 16 * MT - 1) / (16 * MT)));
-  hipLaunchKernelGGL((mx_gemv_kernel<FMT, OFMT, DUAL, RT, MT, NW, BUF>), grid, dim3(64 * NW), 0,
-                     st, a);
+  const int64_t x = ((int64_t)a.K + 16 * RF - 1) / (16 * RF), y = (a.M + 16 * MT - 1) / (16 * MT);
+  // (threads of a launch's dimension: below 2^32)
+  if (x * (64 * NW) > (int64_t)UINT32_MAX || y > 65535) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL((mx_gemv_kernel<FMT, OFMT, DUAL, RT, MT, NW, BUF>),
+                     dim3((unsigned)x, (unsigned)y), dim3(64 * NW), 0, st, a);
+  return hipGetLastError();
 }
 
 // The largest tile of a block that leaves kBlocks of them, without a half-used
@@ -184,23 +186,17 @@ void go(const MxMatmulArgs &a, hipStream_t st) {
 constexpr int64_t kBlocks = 160;
 
 template <int FMT>
-void launch_fmt(bool dual, int out_format, const MxMatmulArgs &a, hipStream_t st) {
+hipError_t launch_fmt(bool dual, int out_format, const MxMatmulArgs &a, hipStream_t st) {
   const int64_t mt = (a.M + 15) / 16;
   auto fits = [&](int rt, int m) {
-    return mt % m == 0 && (a.K + 16 * rt - 1) / (16 * rt) * (mt / m) >= kBlocks;
+    return mt % m == 0 && ((int64_t)a.K + 16 * rt - 1) / (16 * rt) * (mt / m) >= kBlocks;
   };
   if (!dual) {
-    if (fits(3, 2))
-      go<FMT, NVM_MX_FP8, false, 3, 2, 4, 1>(a, st);
-    else if (fits(4, 1))
-      go<FMT, NVM_MX_FP8, false, 4, 1, 4, 1>(a, st);
-    else if (fits(2, 2))
-      go<FMT, NVM_MX_FP8, false, 2, 2, 4, 1>(a, st);
-    else if (fits(2, 1))
-      go<FMT, NVM_MX_FP8, false, 2, 1, 4, 1>(a, st);
-    else
-      go<FMT, NVM_MX_FP8, false, 1, 1, 4, 1>(a, st);
-    return;
+    if (fits(3, 2)) return go<FMT, NVM_MX_FP8, false, 3, 2, 4, 1>(a, st);
+    if (fits(4, 1)) return go<FMT, NVM_MX_FP8, false, 4, 1, 4, 1>(a, st);
+    if (fits(2, 2)) return go<FMT, NVM_MX_FP8, false, 2, 2, 4, 1>(a, st);
+    if (fits(2, 1)) return go<FMT, NVM_MX_FP8, false, 2, 1, 4, 1>(a, st);
+    return go<FMT, NVM_MX_FP8, false, 1, 1, 4, 1>(a, st);
   }
   // SwiGLU: 32 outputs a block (its scale needs them), over all activation
   // rows of up to four tiles (2048 -> 6144 of 8 rows: 6.9 us with eight
@@ -208,28 +204,19 @@ void launch_fmt(bool dual, int out_format, const MxMatmulArgs &a, hipStream_t st
   // rows 11.9 on 4, 13.4 on 2)
   auto swiglu = [&](auto OF) {
     constexpr int OFMT = decltype(OF)::value;
-    if (mt == 1)
-      go<FMT, OFMT, true, 4, 1, 8, 1>(a, st);
-    else if (mt == 2)
-      go<FMT, OFMT, true, 4, 2, 8, 1>(a, st);
-    else
-      go<FMT, OFMT, true, 4, 4, 4, 1>(a, st);
+    if (mt == 1) return go<FMT, OFMT, true, 4, 1, 8, 1>(a, st);
+    if (mt == 2) return go<FMT, OFMT, true, 4, 2, 8, 1>(a, st);
+    return go<FMT, OFMT, true, 4, 4, 4, 1>(a, st);
   };
-  if (out_format == NVM_MX_FP4)
-    swiglu(MxInt<NVM_MX_FP4>{});
-  else
-    swiglu(MxInt<NVM_MX_FP8>{});
+  return out_format == NVM_MX_FP4 ? swiglu(MxInt<NVM_MX_FP4>{}) : swiglu(MxInt<NVM_MX_FP8>{});
 }
 
 }  // namespace
 
 hipError_t launch_mx_gemv(int format, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st) {
-  if (format == NVM_MX_FP4)
-    launch_fmt<NVM_MX_FP4>(dual, out_format, a, st);
-  else
-    launch_fmt<NVM_MX_FP8>(dual, out_format, a, st);
-  return hipGetLastError();
+  return format == NVM_MX_FP4 ? launch_fmt<NVM_MX_FP4>(dual, out_format, a, st)
+                              : launch_fmt<NVM_MX_FP8>(dual, out_format, a, st);
 }
 
 }  // namespace nvm

@@ -78,33 +78,45 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const void *x, ui
   store_block<FMT>(v, row, c, n8, codes, scales, sld);
 }
 
-template <int FMT, int DT>
-__global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(const void *codes,
-                                                                 const uint8_t *scales,
-                                                                 int64_t sld, uint32_t total,
-                                                                 int n8, void *out) {
+// Rows 0, 1, ..., or (IDS) rows ids[0], ids[1], ... of a table of `table_rows`:
+// of ids outside it zeros.
+template <int FMT, int DT, bool IDS>
+__global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(
+    const int32_t *ids, int table_rows, const void *codes, const uint8_t *scales, int64_t sld,
+    uint32_t total, int n8, void *out) {
   const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
   if (i >= total) return;
   int64_t row;
   int c;
   split_index(i, n8, row, c);
+  bool inside = true;
+  if constexpr (IDS) {
+    row = ids[row];
+    inside = row >= 0 && row < table_rows;
+    row = inside ? row : 0;
+  }
+  const int64_t at = IDS ? row * n8 + c : (int64_t)i;
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   f32x2 p[4];
   if constexpr (FMT == NVM_MX_FP4) {
-    const uint32_t d = ((const uint32_t *)codes)[i];
+    const uint32_t d = ((const uint32_t *)codes)[at];
     p[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d, 1.0f, 0);
     p[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d, 1.0f, 1);
     p[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d, 1.0f, 2);
     p[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(d, 1.0f, 3);
   } else {
-    const u32x2 d = ((const u32x2 *)codes)[i];
+    const u32x2 d = ((const u32x2 *)codes)[at];
     p[0] = __builtin_amdgcn_cvt_pk_f32_fp8((int)d.x, false);
     p[1] = __builtin_amdgcn_cvt_pk_f32_fp8((int)d.x, true);
     p[2] = __builtin_amdgcn_cvt_pk_f32_fp8((int)d.y, false);
     p[3] = __builtin_amdgcn_cvt_pk_f32_fp8((int)d.y, true);
   }
   // (the products are exact down to float32's subnormals: 2^-9 * 2^-127)
-  const float s = mx_scale(scales[row * sld + (c >> 2)]);
+  const float s = inside ? mx_scale(scales[row * sld + (c >> 2)]) : 0.f;
+  if (IDS && !inside) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p[j] = f32x2{0.f, 0.f};
+  }
   if constexpr (DT == NVM_MX_F32) {
     float *o = (float *)out + 8 * (int64_t)i;
     *(f32x4 *)o = f32x4{p[0].x * s, p[0].y * s, p[1].x * s, p[1].y * s};
@@ -261,6 +273,38 @@ int mx_check_tensor(const char *op, const void *codes, const uint8_t *scales, in
   return NVM_OK;
 }
 
+// Values of `rows` rows (all of the tensor's, or those that ids names) to out.
+static int mx_rows(const char *op, const int32_t *ids, int64_t rows, const void *codes,
+                   const uint8_t *scales, int64_t scale_ld, int64_t table_rows, int64_t n,
+                   int format, int dtype, void *out, hipStream_t st) {
+  if (dtype != NVM_MX_F16 && dtype != NVM_MX_BF16 && dtype != NVM_MX_F32)
+    return set_error(NVM_ERR_INVALID, "%s: dtype must be f16, bf16 or f32", op);
+  if (int rc = mx_check_rows(op, table_rows, n, format, "input")) return rc;
+  if (rows == 0) return NVM_OK;
+  if (int rc = mx_check_tensor(op, codes, scales, scale_ld, n, "input")) return rc;
+  if (!out || !aligned16(out))
+    return set_error(NVM_ERR_INVALID, "%s: out must be a 16-byte aligned pointer", op);
+  const int64_t total = rows * (n / 8);
+  if (total > kMaxChunks)
+    return set_error(NVM_ERR_UNSUPPORTED, "%s: more than 2^35 values in one call", op);
+  const dim3 grid((unsigned)((total + kThreads - 1) / kThreads));
+  mx_by_dtype(dtype, [&](auto D) {
+    by_format(format, [&](auto F) {
+      auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, grid, dim3(kThreads), 0, st, ids, (int)table_rows, codes, scales,
+                           scale_ld, (uint32_t)total, (int)(n / 8), out);
+      };
+      if (ids)
+        go(mx_dequantize_kernel<decltype(F)::value, decltype(D)::value, true>);
+      else
+        go(mx_dequantize_kernel<decltype(F)::value, decltype(D)::value, false>);
+    });
+  });
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return set_error(NVM_ERR_HIP, "%s: %s", op, hipGetErrorString(e));
+  return NVM_OK;
+}
+
 }  // namespace nvm
 
 extern "C" {
@@ -296,29 +340,20 @@ int nvm_mx_quantize(const void *x, int64_t rows, int64_t n, int64_t x_ld, int dt
 
 int nvm_mx_dequantize(const void *codes, const uint8_t *scales, int64_t scale_ld, int64_t rows,
                       int64_t n, int format, int dtype, void *out, nvm_stream_t stream) {
+  return nvm::mx_rows("mx_dequantize", nullptr, rows, codes, scales, scale_ld, rows, n, format,
+                      dtype, out, (hipStream_t)stream);
+}
+
+int nvm_mx_embedding(const int32_t *ids, int64_t T, const void *codes, const uint8_t *scales,
+                     int64_t scale_ld, int64_t V, int64_t n, int format, int dtype, void *out,
+                     nvm_stream_t stream) {
   using namespace nvm;
-  const char *op = "mx_dequantize";
-  if (dtype != NVM_MX_F16 && dtype != NVM_MX_BF16 && dtype != NVM_MX_F32)
-    return set_error(NVM_ERR_INVALID, "%s: dtype must be f16, bf16 or f32", op);
-  if (int rc = mx_check_rows(op, rows, n, format, "input")) return rc;
-  if (rows == 0) return NVM_OK;
-  if (int rc = mx_check_tensor(op, codes, scales, scale_ld, n, "input")) return rc;
-  if (!out || !aligned16(out))
-    return set_error(NVM_ERR_INVALID, "%s: out must be a 16-byte aligned pointer", op);
-  const int64_t total = rows * (n / 8);
-  if (total > kMaxChunks)
-    return set_error(NVM_ERR_UNSUPPORTED, "%s: more than 2^35 values in one call", op);
-  const dim3 grid((unsigned)((total + kThreads - 1) / kThreads));
-  mx_by_dtype(dtype, [&](auto D) {
-    by_format(format, [&](auto F) {
-      hipLaunchKernelGGL((mx_dequantize_kernel<decltype(F)::value, decltype(D)::value>), grid,
-                         dim3(kThreads), 0, (hipStream_t)stream, codes, scales, scale_ld, (uint32_t)total,
-                         (int)(n / 8), out);
-    });
-  });
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return set_error(NVM_ERR_HIP, "%s: %s", op, hipGetErrorString(e));
-  return NVM_OK;
+  if (T < 0 || T > INT32_MAX || V <= 0)
+    return set_error(NVM_ERR_INVALID, "mx_embedding: bad shape T=%lld V=%lld", (long long)T,
+                     (long long)V);
+  if (T > 0 && !ids) return set_error(NVM_ERR_INVALID, "mx_embedding: null pointer (ids)");
+  return mx_rows("mx_embedding", ids, T, codes, scales, scale_ld, V, n, format, dtype, out,
+                 (hipStream_t)stream);
 }
 
 int nvm_residual_rms_norm_mx(const void *h, const void *r, const void *w, int64_t T, int64_t H,

@@ -281,15 +281,15 @@ struct MxTile {
 template <class T, class F>
 hipError_t mx_launch_tiles(F kern, bool single, bool (&allowed)[64], const MxMatmulArgs &a,
                            hipStream_t st) {
+  const int n_tiles = (int)(((int64_t)a.K + T::BK - 1) / T::BK);
+  const int64_t m_tiles = (a.M + T::BM - 1) / T::BM, total = m_tiles * n_tiles;
+  if (total > kMxMaxTiles) return hipErrorInvalidConfiguration;
   int dev = 0;
   if (hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < 64 && !allowed[dev]) {
     (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
                               T::kLds);
     allowed[dev] = true;
   }
-  const int n_tiles = (a.K + T::BK - 1) / T::BK;
-  const int64_t m_tiles = (a.M + T::BM - 1) / T::BM, total = m_tiles * n_tiles;
-  if (total > kMxMaxTiles) return hipErrorInvalidConfiguration;
   const int64_t all = 8 * ((total + 7) / 8);
   const int64_t grid = single ? all : std::min<int64_t>(all, cu_count() / 8 * 8);
   hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * T::NW), T::kLds, st, a, n_tiles,

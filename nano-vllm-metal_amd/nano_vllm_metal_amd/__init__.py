@@ -5,7 +5,9 @@ Public names mirror the reference's package root for this path
 ``quantized_matmul``, ``quantized_linear``, ``route_topk``,
 ``grouped_expert_linear`` and ``Moe``, plus ``paged_attention``
 (``layers/attention.py:154``), the Qwen3 model with its paged KV cache and
-``LLM``/``SamplingParams`` (``llm.py``).  All compute runs in HIP kernels on the GPU
+``LLM``/``SamplingParams`` (``llm.py``).  Beyond the reference: the microscaled
+path (``mx.py``), ``MxTensor`` weights in ``mxfp4`` with activations in eight or
+four bits, on its own and in the model's dense layers.  All compute runs in HIP kernels on the GPU
 (libnvm_moe.so); nothing falls back to the CPU.
 """
 
@@ -13,7 +15,7 @@ from .linear import QuantizedWeights, dequantize, quantize, quantized_linear, qu
 from .moe import Moe, grouped_expert_linear, moe_dispatch, route_and_dispatch, route_topk
 from .loader import load_moe_block, load_moe_blocks, read_config, sparse_layers
 from .attention import paged_attention
-from .mx import (MxTensor, mx_dequantize, mx_linear, mx_quantize, mx_swiglu,
+from .mx import (MxTensor, mx_dequantize, mx_embedding, mx_linear, mx_quantize, mx_swiglu,
                  residual_rms_norm_mx)
 from .kv_cache import PagedKVCache
 from .qwen3 import Qwen3Config, Qwen3Model, qwen3_30b_a3b_config
@@ -38,6 +40,7 @@ __all__ = [
     "MxTensor",
     "mx_quantize",
     "mx_dequantize",
+    "mx_embedding",
     "mx_linear",
     "mx_swiglu",
     "residual_rms_norm_mx",

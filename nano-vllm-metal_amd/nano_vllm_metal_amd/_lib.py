@@ -64,6 +64,7 @@ SIGNATURES = {
                                _P, _P, _P, _P, _I64, _I64, _I, _P, _P, _P, _P],
     "nvm_mx_quantize": [_P, _I64, _I64, _I64, _I, _I, _P, _P, _I64, _P],
     "nvm_mx_dequantize": [_P, _P, _I64, _I64, _I64, _I, _I, _P, _P],
+    "nvm_mx_embedding": [_P, _I64, _P, _P, _I64, _I64, _I64, _I, _I, _P, _P],
     "nvm_residual_rms_norm_mx": [_P, _P, _P, _I64, _I64, ctypes.c_float, _I, _P, _I, _P, _P, _I64,
                                  _P],
     "nvm_mx_matmul": [_P, _P, _I64, _I, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P],

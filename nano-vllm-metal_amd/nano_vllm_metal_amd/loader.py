@@ -17,6 +17,10 @@ This module reads the same tensors straight from a local checkpoint directory
   ``bits``; an entry keyed by a module path (for example
   ``"model.layers.3.mlp.gate"``) overrides them for that module, and ``false``
   there marks it unquantised (not supported: the kernels take 4-bit weights).
+* ``mode`` there is ``affine`` (the default) or, for all but the sparse blocks,
+  ``mxfp4`` (blocks of 32 values with one power-of-two scale): the words of
+  ``weight`` are the codes of an ``MxTensor``, ``scales`` are uint8, and there
+  are no ``biases``.
 * Expert projections stored per expert (``mlp.experts.{j}.gate_proj.*``, the
   layout before MLX stacks them) are stacked along a new leading axis, so they
   land in the same ``[E, out, in/8]`` layout as ``switch_mlp``.
@@ -36,6 +40,7 @@ import torch
 
 from .linear import QuantizedWeights
 from .moe import Moe
+from .mx import MX_BLOCK, MxTensor
 
 _PROJS = ("gate_proj", "up_proj", "down_proj")
 
@@ -57,9 +62,9 @@ def sparse_layers(config: dict) -> List[int]:
     return [i for i in range(n) if i not in only and (i + 1) % step == 0]
 
 
-def quant_params(config: dict, module: str):
-    """``(group_size, bits)`` of a module: the per-module entry of
-    ``quantization`` if there is one, else the checkpoint default."""
+def _quantization(config: dict, module: str) -> dict:
+    """The entry of ``quantization`` that holds for a module: its own if there
+    is one, else the checkpoint default."""
     q = config.get("quantization", config.get("quantization_config"))
     if not isinstance(q, dict):
         raise ValueError("checkpoint has no 'quantization' entry: not an MLX quantised model")
@@ -69,7 +74,22 @@ def quant_params(config: dict, module: str):
     src = own if isinstance(own, dict) else q
     if "group_size" not in src or "bits" not in src:
         raise ValueError(f"no group_size/bits for {module} in 'quantization'")
+    return src
+
+
+def quant_params(config: dict, module: str):
+    """``(group_size, bits)`` of a module: the per-module entry of
+    ``quantization`` if there is one, else the checkpoint default."""
+    src = _quantization(config, module)
     return int(src["group_size"]), int(src["bits"])
+
+
+def quant_mode(config: dict, module: str) -> str:
+    """``affine`` or ``mxfp4``, from the same entry as ``quant_params``."""
+    mode = _quantization(config, module).get("mode", "affine")
+    if mode not in ("affine", "mxfp4"):
+        raise ValueError(f"{module}: quantisation mode {mode!r} is neither 'affine' nor 'mxfp4'")
+    return mode
 
 
 class _Tensors:
@@ -116,7 +136,10 @@ def _words(t: torch.Tensor) -> torch.Tensor:
 
 
 def _qweights(ts: _Tensors, prefix: str, config: dict, device, stack: Optional[int] = None):
-    gs, bits = quant_params(config, prefix if stack is None else prefix.replace("{j}", "0"))
+    module = prefix if stack is None else prefix.replace("{j}", "0")
+    gs, bits = quant_params(config, module)
+    if quant_mode(config, module) != "affine":
+        raise ValueError(f"{prefix}: mxfp4 weights; the sparse blocks take affine ones")
     if bits != 4:
         raise ValueError(f"{prefix}: {bits}-bit weights; the MoE kernels take 4-bit weights")
 
@@ -133,6 +156,29 @@ def _qweights(ts: _Tensors, prefix: str, config: dict, device, stack: Optional[i
         raise ValueError(f"{prefix}: weight and scales disagree with group_size {gs}")
     return QuantizedWeights(s.contiguous().to(device), b.contiguous().to(device), gs, bits,
                             w.contiguous().to(device))
+
+
+def _mx_weights(ts: _Tensors, prefix: str, config: dict, device) -> MxTensor:
+    gs, bits = quant_params(config, prefix)
+    if (gs, bits) != (MX_BLOCK, 4):
+        raise ValueError(f"{prefix}: mxfp4 has groups of {MX_BLOCK} and 4 bits, got {gs} and {bits}")
+    if ts.has(f"{prefix}.biases"):
+        raise ValueError(f"{prefix}: mxfp4 weights have no biases")
+    w, s = _words(ts.get(f"{prefix}.weight")), ts.get(f"{prefix}.scales")
+    if s.dtype != torch.uint8:
+        raise ValueError(f"{prefix}: scales of mxfp4 must be uint8, got {s.dtype}")
+    if w.dim() != 2 or s.dim() != 2 or s.shape[0] != w.shape[0] \
+            or w.shape[1] * 8 != s.shape[1] * MX_BLOCK:
+        raise ValueError(f"{prefix}: inconsistent shapes {tuple(w.shape)}, {tuple(s.shape)}")
+    codes = w.contiguous().view(torch.uint8)
+    return MxTensor(codes.to(device), s.to(device), "mxfp4")
+
+
+def _weights(ts: _Tensors, prefix: str, config: dict, device):
+    """``QuantizedWeights`` or, in ``mxfp4`` mode, an ``MxTensor``."""
+    if quant_mode(config, prefix) == "mxfp4":
+        return _mx_weights(ts, prefix, config, device)
+    return _qweights(ts, prefix, config, device)
 
 
 def load_moe_block(path, layer: int, device="cuda", config: Optional[dict] = None,

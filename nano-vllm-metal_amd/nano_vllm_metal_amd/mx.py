@@ -200,6 +200,30 @@ def mx_dequantize(t: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tens
     return out
 
 
+def mx_embedding(tokens: torch.Tensor, table: MxTensor, dtype: torch.dtype) -> torch.Tensor:
+    """The rows of ``table [V, D]`` for ``tokens``, rounded once to ``dtype``,
+    ``[*tokens.shape, D]``: ``embedding`` of a table in MX.  Ids outside ``[0,
+    V)`` give zero rows."""
+    lib = _lib.load()
+    if type(table) is not MxTensor or len(table.shape) != 2:
+        raise ValueError("mx_embedding: table must be a two-dimensional MxTensor")
+    dev = _lib.require_device(tokens, table.codes, table.scales)
+    code = MX_DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"mx_embedding: dtype must be float16, bfloat16 or float32, got {dtype}")
+    if tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"mx_embedding: tokens must be int32 or int64, got {tokens.dtype}")
+    V, D = table.shape
+    if tokens.dtype == torch.int64:  # (an id that 32 bits would wrap stays outside)
+        tokens = tokens.clamp(-1, V)
+    ids = tokens.reshape(-1).to(torch.int32).contiguous()
+    out = torch.empty((*tokens.shape, D), dtype=dtype, device=dev)
+    _launch(lib.nvm_mx_embedding, dev, ids.data_ptr(), ids.numel(), table.codes.data_ptr(),
+            table.scales.data_ptr(), table.pitch, V, D, MX_FORMATS[table.fmt], code,
+            out.data_ptr())
+    return out
+
+
 def residual_rms_norm_mx(h: torch.Tensor, r: Optional[torch.Tensor], weight: torch.Tensor,
                          eps: float, fmt: str = "mxfp8") -> Tuple[torch.Tensor, MxTensor]:
     """``residual_rms_norm`` with an MX output: ``(h + r, rms_norm(h + r) *
@@ -231,6 +255,14 @@ def residual_rms_norm_mx(h: torch.Tensor, r: Optional[torch.Tensor], weight: tor
             float(eps), dtype, _lib.ptr(h_out), code, out.codes.data_ptr(), out.scales.data_ptr(),
             out.pitch)
     return (h if h_out is None else h_out), out
+
+
+def mx_stack_outputs(*ws: MxTensor) -> MxTensor:
+    """One weight for several projections of the same input: rows one behind
+    the other."""
+    if any(w.fmt != ws[0].fmt or w.shape[1:] != ws[0].shape[1:] for w in ws):
+        raise ValueError("mx_stack_outputs: projections differ in format or input features")
+    return MxTensor(torch.cat([w.codes for w in ws]), torch.cat([w.scales for w in ws]), ws[0].fmt)
 
 
 def _activations(x: Union[MxTensor, torch.Tensor], op: str) -> MxTensor:

@@ -21,13 +21,20 @@ the new tokens is torch's SDPA (float32, as the reference's
 ``mx.fast.scaled_dot_product_attention``).  Activations are bf16 (or fp16)
 like the reference's ``precision``; norms and RoPE compute in float32 and
 round where the reference materialises a tensor.
+
+Projections, dense MLPs, the embedding and the lm head may instead be
+``MxTensor`` weights (``mxfp4``, ``mx.py``), each on its own.  Where a norm's
+output goes into such weights only, it is computed in MX (``mxfp8``) and never
+stored in 16 bits: norm -> q/k/v product, and norm -> gate/up -> down product;
+the attention's output and the lm head's input are quantised by ``mx_linear``.
 """
 
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass, field
 from pathlib import Path
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Union
 
 import torch
 
@@ -37,6 +44,10 @@ from .kv_cache import PagedKVCache
 from .linear import (QuantizedWeights, quantized_linear, quantized_swiglu,
                      swiglu_supports)
 from .moe import Moe
+from .mx import (MxTensor, mx_embedding, mx_linear, mx_stack_outputs, mx_swiglu,
+                 residual_rms_norm_mx)
+
+Weights = Union[QuantizedWeights, MxTensor]
 
 
 @dataclass
@@ -89,13 +100,36 @@ class RoPE:
         self.sin = torch.sin(freqs).to(device).contiguous()
 
 
+def linear(x, w: Weights, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``x . w^T`` by the weight's kind; ``dtype``: of the output of an ``x`` in
+    MX."""
+    return mx_linear(x, w, dtype) if isinstance(w, MxTensor) else quantized_linear(x, w)
+
+
+def norm_for(consumer: object, h: torch.Tensor, r: Optional[torch.Tensor], weight: torch.Tensor,
+             eps: float):
+    """``residual_rms_norm``, in MX if what reads the norm takes that."""
+    if isinstance(consumer, MxTensor) or isinstance(consumer, DenseMLP) and consumer.mx:
+        return residual_rms_norm_mx(h, r, weight, eps)
+    return residual_rms_norm(h, r, weight, eps)
+
+
 class DenseMLP:
-    """``Qwen3MLP`` (models/qwen3.py:176-184): down(silu(gate(x)) * up(x))."""
+    """``Qwen3MLP`` (models/qwen3.py:176-184): down(silu(gate(x)) * up(x)).
+    With ``MxTensor`` weights, ``x`` may be one too (``dtype``: of the output
+    then), and the product of the two is in MX."""
 
-    def __init__(self, w_gate: QuantizedWeights, w_up: QuantizedWeights, w_down: QuantizedWeights):
+    def __init__(self, w_gate: Weights, w_up: Weights, w_down: Weights):
         self.w_gate, self.w_up, self.w_down = w_gate, w_up, w_down
+        mx = [isinstance(w, MxTensor) for w in (w_gate, w_up, w_down)]
+        if any(mx) and not all(mx):
+            raise ValueError("DenseMLP: gate, up and down must all be MxTensors, or none")
+        self.mx = all(mx)
 
-    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+    def __call__(self, x, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        if self.mx:
+            out = dtype if isinstance(x, MxTensor) else x.dtype
+            return mx_linear(mx_swiglu(x, self.w_gate, self.w_up), self.w_down, out)
         if swiglu_supports(x, self.w_gate, self.w_up):
             h = quantized_swiglu(x, self.w_gate, self.w_up)
         else:
@@ -125,21 +159,26 @@ class StepInputs:
 
 @dataclass
 class Qwen3Layer:
-    wq: QuantizedWeights
-    wk: QuantizedWeights
-    wv: QuantizedWeights
-    wo: QuantizedWeights
+    wq: Weights
+    wk: Weights
+    wv: Weights
+    wo: Weights
     q_norm: torch.Tensor
     k_norm: torch.Tensor
     input_norm: torch.Tensor
     post_norm: torch.Tensor
     mlp: object  # Moe or DenseMLP
-    wqkv: Optional[QuantizedWeights] = None  # q, k and v stacked along the output rows
+    wqkv: Optional[Weights] = None  # q, k and v stacked along the output rows
 
 
-def stack_outputs(*ws: QuantizedWeights) -> QuantizedWeights:
+def stack_outputs(*ws: Weights) -> Weights:
     """One product for several projections of the same input: rows, scales
     and biases concatenated along the output dimension."""
+    mx = [isinstance(w, MxTensor) for w in ws]
+    if all(mx):
+        return mx_stack_outputs(*ws)
+    if any(mx):
+        raise ValueError("stack_outputs: projections must all be MxTensors, or none")
     gs, bits = ws[0].group_size, ws[0].bits
     if any(w.group_size != gs or w.bits != bits for w in ws):
         raise ValueError("stack_outputs: projections differ in group_size or bits")
@@ -148,8 +187,8 @@ def stack_outputs(*ws: QuantizedWeights) -> QuantizedWeights:
 
 
 class Qwen3Model:
-    def __init__(self, config: Qwen3Config, embed: QuantizedWeights, layers: Sequence[Qwen3Layer],
-                 norm: torch.Tensor, lm_head: Optional[QuantizedWeights],
+    def __init__(self, config: Qwen3Config, embed: Weights, layers: Sequence[Qwen3Layer],
+                 norm: torch.Tensor, lm_head: Optional[Weights],
                  dtype: torch.dtype = torch.bfloat16):
         self.config = config
         self.embed_w = embed
@@ -157,7 +196,7 @@ class Qwen3Model:
         self.norm = norm
         self.lm_head = lm_head
         self.dtype = dtype
-        self.device = embed.weight.device
+        self.device = embed.device if isinstance(embed, MxTensor) else embed.weight.device
         self.rope = RoPE(config.head_dim, config.max_position_embeddings, config.rope_theta,
                          self.device)
         for layer in self.layers:
@@ -177,14 +216,16 @@ class Qwen3Model:
         # (mx.dequantize returns the scales' dtype; a table stored in another
         # dtype than the model's is then cast, as the reference's next op does)
         w = self.embed_w
+        if isinstance(w, MxTensor):
+            return mx_embedding(tokens, w, self.dtype)
         return embedding(tokens, w, w.scales.dtype).to(self.dtype)
 
-    def _attention(self, li: int, layer: Qwen3Layer, x: torch.Tensor, step: "StepInputs",
+    def _attention(self, li: int, layer: Qwen3Layer, x, step: "StepInputs",
                    cache: PagedKVCache) -> torch.Tensor:
         c = self.config
         B, L, _ = x.shape
         Hq, Hkv, D = c.num_attention_heads, c.num_key_value_heads, c.head_dim
-        qkv = quantized_linear(x, layer.wqkv)
+        qkv = linear(x, layer.wqkv, self.dtype)
         q, k, v = qk_norm_rope_store(qkv, Hq, Hkv, D, layer.q_norm, layer.k_norm, c.rms_norm_eps,
                                      step.positions, self.rope.cos, self.rope.sin, step.page_ids,
                                      step.slots, cache.key_pages[li], cache.value_pages[li],
@@ -195,15 +236,15 @@ class Qwen3Model:
             # the new tokens only (models/qwen3.py:134-141); the grouped query
             # heads share each key/value read
             o = causal_attention(q.view(B, L, Hq, D), k.view(B, L, Hkv, D), v.view(B, L, Hkv, D),
-                                 scale, self.dtype, out_dtype=x.dtype)
+                                 scale, self.dtype, out_dtype=qkv.dtype)
             o = o.reshape(B, L, Hq * D)
         else:
             # (the k/v of an initial step are in the pages as well)
             o = paged_attention(q.view(B, L, Hq, D).transpose(1, 2), cache.key_pages[li],
                                 cache.value_pages[li], step.block_table, step.lens,
-                                cache.page_size, scale=scale, mask="causal", out_dtype=x.dtype)
+                                cache.page_size, scale=scale, mask="causal", out_dtype=qkv.dtype)
             o = o.transpose(1, 2).reshape(B, L, Hq * D)
-        return quantized_linear(o, layer.wo)
+        return linear(o, layer.wo)
 
     # ---------------------------------------------------------------- forward
 
@@ -228,20 +269,22 @@ class Qwen3Model:
         eps = self.config.rms_norm_eps
         h = self.embed(tokens)
         # residual adds fused with the norm that follows them
-        _, x = residual_rms_norm(h, None, self.layers[0].input_norm, eps)
+        _, x = norm_for(self.layers[0].wqkv, h, None, self.layers[0].input_norm, eps)
         n = len(self.layers)
         for li, layer in enumerate(self.layers):
-            h, x = residual_rms_norm(h, self._attention(li, layer, x, step, cache),
-                                     layer.post_norm, eps)
-            nxt = self.layers[li + 1].input_norm if li + 1 < n else self.norm
+            h, x = norm_for(layer.mlp, h, self._attention(li, layer, x, step, cache),
+                            layer.post_norm, eps)
+            follow = self.layers[li + 1] if li + 1 < n else None
+            nxt = follow.input_norm if follow else self.norm
             if isinstance(layer.mlp, Moe):
                 # the MoE combine fused into this residual add and norm
                 h, x = moe_residual_rms_norm(layer.mlp, x, h, nxt, eps)
             else:
-                h, x = residual_rms_norm(h, layer.mlp(x), nxt, eps)
+                y = layer.mlp(x, self.dtype) if isinstance(x, MxTensor) else layer.mlp(x)
+                h, x = norm_for(follow.wqkv if follow else None, h, y, nxt, eps)
         if last_only:
             x = x[:, -1]
-        return quantized_linear(x, self.lm_head if self.lm_head is not None else self.embed_w)
+        return linear(x, self.lm_head if self.lm_head is not None else self.embed_w)
 
     def forward(self, tokens: torch.Tensor, cache: PagedKVCache, seq_ids: Sequence[int],
                 last_only: bool = True) -> torch.Tensor:
@@ -263,8 +306,9 @@ class Qwen3Model:
     @classmethod
     def from_checkpoint(cls, path, device="cuda", dtype: torch.dtype = torch.bfloat16):
         """Load an MLX 4-bit Qwen3 / Qwen3-MoE checkpoint from a local directory
-        (``config.json`` plus safetensors, sharded or not)."""
-        from .loader import _Tensors, _qweights, load_moe_block, read_config
+        (``config.json`` plus safetensors, sharded or not); modules in ``mxfp4``
+        mode as ``MxTensor`` weights (the sparse blocks have to be affine)."""
+        from .loader import _Tensors, _weights, load_moe_block, read_config
 
         path = Path(path)
         raw = read_config(path)
@@ -281,27 +325,31 @@ class Qwen3Model:
             if cfg.is_sparse(i):
                 mlp = load_moe_block(path, i, device, raw, ts)
             else:
-                mlp = DenseMLP(*[_qweights(ts, f"{base}.mlp.{p}", raw, device)
+                mlp = DenseMLP(*[_weights(ts, f"{base}.mlp.{p}", raw, device)
                                  for p in ("gate_proj", "up_proj", "down_proj")])
             layers.append(Qwen3Layer(
-                *[_qweights(ts, f"{att}.{p}", raw, device)
+                *[_weights(ts, f"{att}.{p}", raw, device)
                   for p in ("q_proj", "k_proj", "v_proj", "o_proj")],
                 vec(f"{att}.q_norm.weight"), vec(f"{att}.k_norm.weight"),
                 vec(f"{base}.input_layernorm.weight"),
                 vec(f"{base}.post_attention_layernorm.weight"), mlp))
-        embed = _qweights(ts, "model.embed_tokens", raw, device)
+        embed = _weights(ts, "model.embed_tokens", raw, device)
         lm_head = None
         if not cfg.tie_word_embeddings and ts.has("lm_head.weight"):
-            lm_head = _qweights(ts, "lm_head", raw, device)
+            lm_head = _weights(ts, "lm_head", raw, device)
         return cls(cfg, embed, layers, vec("model.norm.weight"), lm_head, dtype)
 
     @classmethod
     def random(cls, config: Qwen3Config, device="cuda", dtype: torch.dtype = torch.bfloat16,
-               seed: int = 0, group_size: int = 64, std: float = 0.02):
+               seed: int = 0, group_size: int = 64, std: float = 0.02, mode: str = "affine"):
         """Synthetic weights of the configured architecture, drawn directly in
         the packed int4 domain (uniform codes; per-group scales and biases of
         an N(0, std) group) - for benchmarks, where quantising billions of
-        floats would only cost time."""
+        floats would only cost time.  ``mode`` "mxfp4": all but the sparse
+        blocks in MX (uniform codes, whose root mean square is 2.94, over
+        scales of the two powers of two around ``std`` of that)."""
+        if mode not in ("affine", "mxfp4"):
+            raise ValueError(f"random: mode must be 'affine' or 'mxfp4', got {mode!r}")
         gen = torch.Generator(device=device)
         gen.manual_seed(seed)
         c = config
@@ -314,6 +362,16 @@ class Qwen3Model:
                  * 0.5 + 0.75) * (std * 6.0 / 15.0)
             b = -7.5 * s
             return QuantizedWeights(s.to(dtype), b.to(dtype), group_size, 4, words)
+
+        def mw(out, inn):
+            codes = torch.randint(0, 256, (out, inn // 2), dtype=torch.uint8, device=device,
+                                  generator=gen)
+            low = 127 + math.floor(math.log2(std / 2.94))
+            scales = torch.randint(low, low + 2, (out, inn // 32), dtype=torch.uint8,
+                                   device=device, generator=gen)
+            return MxTensor(codes, scales, "mxfp4")
+
+        w = mw if mode == "mxfp4" else qw
 
         def ones(n):
             return torch.ones(n, dtype=dtype, device=device)
@@ -328,14 +386,14 @@ class Qwen3Model:
                           norm_topk_prob=c.norm_topk_prob)
             else:
                 I = c.intermediate_size
-                mlp = DenseMLP(qw(I, H), qw(I, H), qw(H, I))
-            layers.append(Qwen3Layer(qw(c.num_attention_heads * D, H),
-                                     qw(c.num_key_value_heads * D, H),
-                                     qw(c.num_key_value_heads * D, H),
-                                     qw(H, c.num_attention_heads * D),
+                mlp = DenseMLP(w(I, H), w(I, H), w(H, I))
+            layers.append(Qwen3Layer(w(c.num_attention_heads * D, H),
+                                     w(c.num_key_value_heads * D, H),
+                                     w(c.num_key_value_heads * D, H),
+                                     w(H, c.num_attention_heads * D),
                                      ones(D), ones(D), ones(H), ones(H), mlp))
-        embed = qw(c.vocab_size, H)
-        lm_head = None if c.tie_word_embeddings else qw(c.vocab_size, H)
+        embed = w(c.vocab_size, H)
+        lm_head = None if c.tie_word_embeddings else w(c.vocab_size, H)
         return cls(c, embed, layers, ones(H), lm_head, dtype)
 
 

@@ -555,3 +555,173 @@ def test_on_another_stream_and_in_a_replayed_graph():
         eager = _bits(_mlp(*ops))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(_bits(out), eager))
+
+
+# ------------------------------------------------------------------- the model
+
+
+@pytest.mark.parametrize("V,D", [(1, 32), (50, 96), (1000, 2048)])
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+def test_embedding(V, D, fmt, dt):
+    from nano_vllm_metal_amd import MxTensor, mx_embedding
+
+    g = _gen(V)
+    t = _mx(torch.randn(V, D, device=DEV, generator=g), fmt)
+    s = t.scales.clone()
+    s[0, 0] = 255  # (a NaN of row 0 stays there)
+    t = MxTensor(t.codes, s, fmt)
+    ids = torch.randint(0, V, (3, 7), device=DEV, generator=g)
+    ids[0, 0], ids[1, 2], ids[1, 3], ids[2, 6] = 0, -1, V, 2 ** 32 + V - 1
+    for tok in (ids, ids.clamp(-5, V + 5).to(torch.int32), ids.t()):
+        y = mx_embedding(tok, t, dt)
+        out = (tok < 0) | (tok >= V)
+        want = _val(t).to(dt)[torch.where(out, 0, tok).long()]  # (float64 to dtype: one rounding)
+        want[out] = 0
+        assert y.dtype == dt and torch.equal(torch.isnan(y), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(y), torch.nan_to_num(want))
+    assert mx_embedding(ids[:0], t, dt).shape == (0, 7, D)
+
+
+def _mx_model(seed=3, mixed=False, **kw):
+    from nano_vllm_metal_amd import Qwen3Config, Qwen3Model
+
+    d = dict(hidden_size=256, num_hidden_layers=3 if mixed else 2, num_attention_heads=4,
+             num_key_value_heads=2, head_dim=64, vocab_size=1024, intermediate_size=640,
+             rms_norm_eps=1e-6, rope_theta=10000.0, max_position_embeddings=512)
+    if mixed:  # layer 1 is a sparse block, of affine weights
+        d.update(moe_intermediate_size=128, num_experts=8, num_experts_per_tok=2,
+                 norm_topk_prob=True, mlp_only_layers=[0, 2])
+    d.update(kw)
+    m = Qwen3Model.random(Qwen3Config.from_dict(d), device=DEV, seed=seed, std=0.06, mode="mxfp4")
+    g = _gen(seed)
+    for layer in m.layers:
+        for n in ("q_norm", "k_norm", "input_norm", "post_norm"):
+            w = getattr(layer, n)
+            w += (0.1 * torch.randn(w.shape, device=DEV, generator=g)).to(w.dtype)
+    return m
+
+
+def _by_hand(m, tokens, step, cache):
+    """Qwen3Model.run as calls of the public operators."""
+    from nano_vllm_metal_amd import (Moe, mx_embedding, mx_linear, mx_quantize, mx_swiglu,
+                                     paged_attention, residual_rms_norm_mx)
+    from nano_vllm_metal_amd.attention import causal_attention
+    from nano_vllm_metal_amd.fused import qk_norm_rope_store, residual_rms_norm
+
+    c, eps, dt = m.config, m.config.rms_norm_eps, m.dtype
+    B, L = tokens.shape
+    Hq, Hkv, D = c.num_attention_heads, c.num_key_value_heads, c.head_dim
+    h, r = mx_embedding(tokens, m.embed_w, dt), None
+    for li, layer in enumerate(m.layers):
+        h, x = residual_rms_norm_mx(h, r, layer.input_norm, eps)
+        if li and isinstance(m.layers[li - 1].mlp, Moe):  # (that norm was in 16 bits)
+            x = mx_quantize(residual_rms_norm(h, None, layer.input_norm, eps)[1])
+        qkv = mx_linear(x, layer.wqkv, dt)
+        q, k, v = qk_norm_rope_store(qkv, Hq, Hkv, D, layer.q_norm, layer.k_norm, eps,
+                                     step.positions, m.rope.cos, m.rope.sin, step.page_ids,
+                                     step.slots, cache.key_pages[li], cache.value_pages[li],
+                                     want_kv=step.initial)
+        if step.initial:
+            o = causal_attention(q.view(B, L, Hq, D), k.view(B, L, Hkv, D), v.view(B, L, Hkv, D),
+                                 D ** -0.5, dt, out_dtype=dt).reshape(B, L, Hq * D)
+        else:
+            o = paged_attention(q.view(B, L, Hq, D).transpose(1, 2), cache.key_pages[li],
+                                cache.value_pages[li], step.block_table, step.lens,
+                                cache.page_size, scale=D ** -0.5, mask="causal", out_dtype=dt)
+            o = o.transpose(1, 2).reshape(B, L, Hq * D)
+        r = mx_linear(mx_quantize(o, "mxfp8"), layer.wo, dt)
+        if isinstance(layer.mlp, Moe):
+            h, x = residual_rms_norm(h, r, layer.post_norm, eps)
+            r = layer.mlp(x)
+        else:
+            h, x = residual_rms_norm_mx(h, r, layer.post_norm, eps)
+            r = mx_linear(mx_swiglu(x, layer.mlp.w_gate, layer.mlp.w_up), layer.mlp.w_down, dt)
+    _, x = residual_rms_norm(h, r, m.norm, eps)
+    return mx_linear(x[:, -1], m.lm_head if m.lm_head is not None else m.embed_w)
+
+
+@pytest.mark.parametrize("kw", [{}, {"tie_word_embeddings": True}, {"mixed": True}])
+@pytest.mark.parametrize("B,L", [(1, 1), (3, 1), (2, 70), (1, 300)])
+def test_model_is_its_operators(B, L, kw):
+    """Prefill, then a decode step on what it left in the pages, bit for bit."""
+    m = _mx_model(**kw)
+    for layer in m.layers:
+        assert torch.equal(_val(layer.wqkv), torch.cat([_val(layer.wq), _val(layer.wk),
+                                                        _val(layer.wv)]))
+    tokens = torch.randint(0, 1024, (B, L), device=DEV, generator=_gen(B + L))
+    got = []
+    for run in (m.run, lambda *a: _by_hand(m, *a)):
+        cache, ids, out = m.create_kv_cache(64, 16), list(range(B)), []
+        for s in ids:
+            cache.add(s)
+        for t in (tokens, tokens[:, :1]):
+            step = m.prepare(cache, ids, t.shape[1])
+            out.append(run(t, step, cache))
+            cache.advance(ids, t.shape[1])
+        got.append(out)
+    for a, b in zip(*got):
+        assert a.shape == (B, 1024) and torch.isfinite(a).all() and a.std() > 0
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("mixed", [False, True])
+def test_generate_with_mx_weights(mixed):
+    """Greedy generation with graphs is that without, for several batches; the
+    mixed model has a sparse block between two dense layers."""
+    from nano_vllm_metal_amd import LLM, SamplingParams
+
+    m = _mx_model(mixed=mixed)
+    g = _gen(5)
+    prompts = [torch.randint(0, 1024, (n,), device=DEV, generator=g).tolist()
+               for n in (5, 40, 5, 130)]
+    outs = []
+    for graphs in (False, True):
+        llm = LLM(m, max_num_seqs=3, max_model_len=256, page_size=16, use_graphs=graphs)
+        outs.append([o.token_ids for o in llm.generate(
+            prompts, SamplingParams(max_tokens=12, ignore_eos=True))])
+    assert outs[0] == outs[1] and all(len(o) == 12 for o in outs[0])
+
+
+def test_mx_layers_beside_the_same_weights_in_float():
+    """Logits of a dense model near those of its decoded weights without any
+    rounding of activations.  Each activation's rounding to E4M3 is off by at
+    most 2^-4 of it, as good as independent from value to value, so a product of
+    N of them is off by at most about 2^-4 / sqrt(3) of its own size; of the
+    eight products in a row of two layers, the errors of all of them add up to
+    at most 8 * 2^-4 / sqrt(3) = 0.29 of the logits' size, and a wrong scale,
+    lane or operand is off by 1 and more."""
+    m = _mx_model()
+    c = m.config
+    B, L, D, Hq, Hkv = 1, 50, c.head_dim, c.num_attention_heads, c.num_key_value_heads
+    tokens = torch.randint(0, 1024, (B, L), device=DEV, generator=_gen(6))
+    cache = m.create_kv_cache(16, 16)
+    cache.add(0)
+    got = m.forward(tokens, cache, [0], last_only=False)[0].double()
+
+    def norm(x, w):
+        return x / (x.square().mean(-1, keepdim=True) + c.rms_norm_eps).sqrt() * w.double()
+
+    def rope(x):  # [L, heads, D]
+        a, b = x[..., :D // 2], x[..., D // 2:]
+        cs, sn = m.rope.cos[:L, None].double(), m.rope.sin[:L, None].double()
+        return torch.cat((a * cs - b * sn, b * cs + a * sn), -1)
+
+    h = _val(m.embed_w)[tokens[0]]
+    mask = torch.ones(L, L, dtype=torch.bool, device=DEV).tril()
+    for layer in m.layers:
+        x = norm(h, layer.input_norm)
+        q, k, v = (x @ _val(w).t() for w in (layer.wq, layer.wk, layer.wv))
+        q = rope(norm(q.view(L, Hq, D), layer.q_norm)).transpose(0, 1)
+        k = rope(norm(k.view(L, Hkv, D), layer.k_norm)).transpose(0, 1)
+        v = v.view(L, Hkv, D).transpose(0, 1)
+        k, v = (t.repeat_interleave(Hq // Hkv, 0).contiguous() for t in (k, v))
+        s = (q @ k.transpose(1, 2).contiguous() * D ** -0.5).masked_fill(~mask, float("-inf"))
+        o = (torch.softmax(s, -1) @ v).transpose(0, 1).reshape(L, Hq * D)
+        h = h + o @ _val(layer.wo).t()
+        x = norm(h, layer.post_norm)
+        a = x @ _val(layer.mlp.w_gate).t()
+        u = x @ _val(layer.mlp.w_up).t()
+        h = h + (a * torch.sigmoid(a) * u) @ _val(layer.mlp.w_down).t()
+    want = norm(h, m.norm) @ _val(m.lm_head).t()
+    assert (got - want).norm() < 0.3 * want.norm()
