@@ -7,17 +7,14 @@
 
 namespace nvm {
 
-// Few rows: mx_gemv.hip, whose time goes with rows x output columns (of both
-// matrices), while the tiles' goes with the steps along a row until they fill
-// the GPU.  2048 -> 5120: 64 rows (328 thousand outputs) 8.2 us there, 11.2 on
-// tiles; 96 rows (492) 12.9 and 11.4; 4096 -> 12288: 32 rows (393) 12.0 and
-// 17.2, 64 rows (786) 20.9 and 17.5; gate/up 2048 -> 6144: 32 rows (393) 8.7 and
-// 12.1, 96 rows 19.9 and 12.6.  One tile of 16 rows stays there whatever the
-// columns: 2048 -> 32768 of 16 rows 12.5 and 12.9 us, 2048 -> 151936 of 1 row
-// 43.7 and 48.3, of 16 rows 52.7 and 50.5.
-static bool few_rows(int64_t rows, int64_t columns) {
-  return rows <= 16 || rows * columns <= 3 << 17;
-}
+// Few rows: mx_gemv.hip, whose time goes with rows x output columns, while the
+// tiles' goes with the steps along a row until they fill the GPU.  2048 -> 5120:
+// 80 rows (410 thousand outputs) 9.4 us there, 11.3 on tiles; 96 rows (492) 11.5
+// and 11.3; 4096 -> 12288: 32 rows (393) 11.6 and 17.0, 64 rows (786) 19.5 and
+// 17.5; gate/up 2048 -> 6144: 64 rows (393) 10.6 and 12.6; 4096 -> 14336: 32 rows
+// (459) 21.5 and 20.5.  One tile of 16 rows stays there whatever the columns:
+// 2048 -> 151936 of 1 row 31 and 50 us, of 16 rows 42 and 49.
+static bool few_rows(const MxMatmulArgs &a) { return a.M <= 16 || a.M * a.K <= 3 << 17; }
 
 // Many rows: the tile whose rounds over the CUs cost least.  A step of the
 // larger ones costs less for its outputs, but they leave more CUs idle.  Their
@@ -38,7 +35,7 @@ static bool few_rows(int64_t rows, int64_t columns) {
 static hipError_t launch_mx_product(int format, bool dual, int out_format, const MxMatmulArgs &a,
                                     hipStream_t st) {
   const int64_t columns = (int64_t)a.K * (dual ? 2 : 1);
-  if (few_rows(a.M, columns)) return launch_mx_gemv(format, dual, out_format, a, st);
+  if (few_rows(a)) return launch_mx_gemv(format, dual, out_format, a, st);
   const int64_t cus = cu_count();
   auto rounds = [&](int bn, int bm) {
     return ((columns + bn - 1) / bn * ((a.M + bm - 1) / bm) + cus - 1) / cus;
