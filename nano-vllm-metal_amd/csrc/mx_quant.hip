@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kThreads) void mx_quantize_kernel(const void *x, ui
   store_block<FMT>(v, row, c, n8, codes, scales, sld);
 }
 
-// Rows 0, 1, ..., or (IDS) rows ids[0], ids[1], ... of a table of `table_rows`:
+// The values of rows 0, 1, ..., or (IDS) of rows ids[0], ids[1], ... of a table of `table_rows`:
 // of ids outside it zeros.
 template <int FMT, int DT, bool IDS>
 __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(
@@ -146,7 +146,10 @@ __device__ __forceinline__ float round_to_odd(double d) {
 // goes out before the first is used.  The sum of squares, its root and the
 // scaled values are float64: squares of 16-bit values are exact there, and
 // an E4M3 or E2M1 rounding border is then missed by 2^-52 instead of the
-// sum's 2^-22 (one value in some 10^5 changed its code).
+// sum's 2^-22 (one value in some 10^5 changed its code).  Bound: HBM and the
+// ramp (4096 x 2048 14.9 us, 4.0 TB/s; 16384 x 2048 46 us, 5.1 TB/s), at few rows
+// latency: 8 rows of 2048 in 2.65 us, with 128 threads of two chunks 3.4, with
+// 64 of four 4.4.
 template <int DT, int FMT, int NT, int NC>
 __global__ __launch_bounds__(NT) void residual_rms_norm_mx_kernel(
     const uint16_t *h, const uint16_t *r, const uint16_t *w, int H8, float eps, uint16_t *h_out,
