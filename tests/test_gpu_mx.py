@@ -557,6 +557,115 @@ def test_on_another_stream_and_in_a_replayed_graph():
         assert all(torch.equal(a, b) for a, b in zip(_bits(out), eager))
 
 
+# ---------------------------------------------------------------- large tensors
+
+
+def _random_mx(rows, n, fmt, g):
+    """Any finite codes, scales of one to four (drawn a part at a time)."""
+    from nano_vllm_metal_amd import MxTensor
+
+    codes = torch.empty(rows, n // 2 if fmt == "mxfp4" else n, dtype=torch.uint8, device=DEV)
+    for part in codes.split(1 << 13):
+        part.copy_(torch.randint(0, 256, part.shape, dtype=torch.uint8, device=DEV, generator=g))
+        if fmt == "mxfp8":
+            part.bitwise_and_(0xBF)  # (below 2, so none is a NaN)
+    scales = torch.randint(127, 130, (rows, n // 32), dtype=torch.uint8, device=DEV, generator=g)
+    return MxTensor(codes, scales, fmt)
+
+
+def _rows(t, i):
+    return O.decode(t.codes[i], t.scales[i], t.fmt)
+
+
+@pytest.mark.parametrize("M", [1, 300])
+def test_linear_of_weights_past_32_bits(M):
+    """2.6 GB of codes: rows on both sides of 2^31 bytes, and the last."""
+    from nano_vllm_metal_amd import mx_linear
+
+    N, K = 32768, 160000
+    g = _gen(M)
+    w, a = _random_mx(K, N, "mxfp4", g), _random_mx(M, N, "mxfp8", g)
+    assert w.codes.numel() > 2 ** 31
+    y = mx_linear(a, w, torch.float32)
+    i = torch.tensor([0, 77777, 131070, 131071, 131072, 131073, K - 1], device=DEV)
+    for r in (0, M // 2, M - 1):
+        _close(y[r:r + 1, i], _rows(a, slice(r, r + 1)), _rows(w, i), torch.float32, "mxfp8")
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_linear_of_outputs_past_32_bits(dt):
+    from nano_vllm_metal_amd import mx_linear
+
+    M, N, K = 70001, 64, 32768
+    g = _gen(1)
+    a, w = _random_mx(M, N, "mxfp8", g), _random_mx(K, N, "mxfp4", g)
+    y = mx_linear(a, w, dt)
+    assert y.numel() > 2 ** 31
+    i = torch.tensor([0, 32767, 32768, 65535, 65536, 65537, M - 1], device=DEV)
+    _close(y[i], _rows(a, i), _val(w), dt, "mxfp8")
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantize_past_32_bits(fmt):
+    from nano_vllm_metal_amd import MxTensor, mx_dequantize, mx_embedding, mx_quantize
+
+    M, n = 70001, 32768
+    g = _gen(2)
+    x = torch.empty(M, n, dtype=torch.bfloat16, device=DEV)
+    for part in x.split(1 << 13):
+        part.copy_(torch.randn(part.shape, device=DEV, generator=g))
+    assert x.numel() > 2 ** 31
+    t = mx_quantize(x, fmt)
+    i = torch.tensor([0, 32767, 32768, 65535, 65536, M - 1], device=DEV)
+    part = MxTensor(t.codes[i], t.scales[i], fmt)
+    _same(part, x[i], fmt)
+    assert torch.equal(mx_embedding(i, t, torch.float32).double(), _val(part))
+    del x
+    y = mx_dequantize(t, torch.bfloat16)
+    assert torch.equal(y[i].double(), _val(part).to(torch.bfloat16).double())
+
+
+def test_a_first_call_may_be_a_captured_one():
+    """In a process of its own: nothing has been launched, and no kernel's LDS
+    been allowed, before the capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parent.parent
+    code = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch
+from nano_vllm_metal_amd import MxTensor, mx_linear, mx_quantize, mx_swiglu
+dev = "cuda:0"
+x = torch.zeros(1030, 256, dtype=torch.bfloat16, device=dev)
+def mx(rows):
+    return MxTensor(torch.full((rows, 128), 0x23, dtype=torch.uint8, device=dev),
+                    torch.full((rows, 16), 120, dtype=torch.uint8, device=dev)[:, :8], "mxfp4")
+ws = mx(1000), mx(4000), mx(8200)
+u = mx(4128)
+torch.cuda.synchronize()
+side = torch.cuda.Stream()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph, stream=side):
+    q = mx_quantize(x)
+    out = [mx_linear(q, w) for w in ws] + [mx_linear(x[:3], ws[0]), mx_swiglu(q, u, u).codes]
+for n in (1, 2, 3):
+    x.fill_(float(n))
+    graph.replay()
+    torch.cuda.synchronize()
+    q2 = mx_quantize(x)
+    want = [mx_linear(q2, w) for w in ws] + [mx_linear(x[:3], ws[0]), mx_swiglu(q2, u, u).codes]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want)), n
+    assert out[0].float().abs().min() > 0
+print("captured first: ok", flush=True)
+""" % (str(root), str(root / "nano-vllm-metal_amd"))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "captured first: ok" in r.stdout, r.stderr[-2000:]
+
+
 # ------------------------------------------------------------------- the model
 
 
