@@ -21,7 +21,7 @@ __device__ __forceinline__ uint32_t mx_scale_byte(uint32_t amax_bits) {
   return e == 255 ? 255u : (uint32_t)max(0, e - Mx<FMT>::kEmax);
 }
 // 2^(127 - b), the factor that takes values to elements (b = 255, a block
-// with a NaN or an infinity: zero, after mx_quiet).
+// with a NaN or an infinity: zero; its codes do not come from the products).
 __device__ __forceinline__ float mx_factor(uint32_t b) {
   return b == 255u ? 0.f : __uint_as_float((254u - b) << 23);
 }

@@ -21,7 +21,6 @@
 // Weights are the row operand, so a lane ends up with four neighbouring
 // outputs of one activation row, and a block of 32 outputs (SwiGLU's MX
 // output) is two tiles of four lane groups.
-#include <algorithm>
 #include <type_traits>
 
 #include "internal.h"

@@ -47,7 +47,10 @@ class MxTensor:
     copied into that layout once, here.
     """
 
-    __slots__ = ("codes", "scales", "fmt", "shape", "rows", "pitch")
+    # _base holds the codes; where a kernel wrote the tensor, the scales too, from
+    # byte _split on, and codes and scales are views that are made when asked for
+    # (each takes as long as an allocation, and operators pass pointers on).
+    __slots__ = ("_base", "_split", "_codes", "_scales", "fmt", "shape", "rows", "pitch")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, fmt: str):
         _format(fmt)
@@ -65,8 +68,9 @@ class MxTensor:
         pitch = _row_pitch(scales, n)
         if pitch is None:
             scales, pitch = _lay_out(scales, n), _pitch(n)
-        self.codes = _packed(codes)
-        self.scales = scales
+        self._base = self._codes = _packed(codes)
+        self._split = None
+        self._scales = scales
         self.fmt = fmt
         self.shape = torch.Size((*codes.shape[:-1], n))
         self.rows = codes.shape[:-1].numel()
@@ -77,17 +81,46 @@ class MxTensor:
         """A tensor for a kernel to write: nothing to check or to copy."""
         t = cls.__new__(cls)
         t.pitch = pitch = _pitch(n)
-        t.codes = torch.empty((*lead, n // _PER_BYTE[fmt]), dtype=torch.uint8, device=device)
-        scales = torch.empty((*lead, pitch), dtype=torch.uint8, device=device)
-        t.scales = scales if pitch * MX_BLOCK == n else scales[..., :n // MX_BLOCK]
+        t._split = split = rows * (n // _PER_BYTE[fmt])
+        t._base = torch.empty(split + rows * pitch, dtype=torch.uint8, device=device)
+        t._codes = t._scales = None
         t.fmt = fmt
         t.shape = torch.Size((*lead, n))
         t.rows = rows
         return t
 
+    def _view(self, width: int, pitch: int, offset: int) -> torch.Tensor:
+        """Rows of ``width`` bytes, ``pitch`` apart, from a byte of the base on."""
+        shape = self.shape
+        if len(shape) == 2:
+            return self._base.as_strided((shape[0], width), (pitch, 1), offset)
+        lead, strides = shape[:-1], [1]
+        for size in reversed(lead):
+            strides.append(pitch)
+            pitch *= max(size, 1)
+        return self._base.as_strided((*lead, width), strides[::-1], offset)
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            width = self.shape[-1] // _PER_BYTE[self.fmt]
+            self._codes = self._view(width, width, 0)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._view(self.shape[-1] // MX_BLOCK, self.pitch, self._split)
+        return self._scales
+
+    def _pointers(self) -> Tuple[int, int]:
+        """Addresses of codes and scales."""
+        at = self._base.data_ptr()
+        return at, self._scales.data_ptr() if self._split is None else at + self._split
+
     @property
     def device(self) -> torch.device:
-        return self.codes.device
+        return self._base.device
 
     @property
     def in_features(self) -> int:
@@ -102,6 +135,9 @@ class MxTensor:
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         return mx_dequantize(self, dtype)
+
+    def __reduce__(self):  # (copies: of what the views show, not of the views beside their base)
+        return MxTensor, (self.codes, self.scales, self.fmt)
 
     def __repr__(self) -> str:
         return f"MxTensor({self.fmt}, shape={tuple(self.shape)}, device={self.device})"
@@ -182,21 +218,21 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp8") -> MxTensor:
         x, ld = x.clone(memory_format=torch.contiguous_format), n
     rows = x.numel() // n
     out = MxTensor._empty(shape[:-1], rows, n, fmt, dev)
-    _launch(lib.nvm_mx_quantize, dev, x.data_ptr(), rows, n, ld, dtype, code,
-            out.codes.data_ptr(), out.scales.data_ptr(), out.pitch)
+    _launch(lib.nvm_mx_quantize, dev, x.data_ptr(), rows, n, ld, dtype, code, *out._pointers(),
+            out.pitch)
     return out
 
 
 def mx_dequantize(t: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values that ``t`` stands for, rounded once to ``dtype``."""
     lib = _lib.load()
-    dev = _lib.require_device(t.codes, t.scales)
+    dev = _lib.require_device(t._base)
     code = MX_DTYPES.get(dtype)
     if code is None:
         raise ValueError(f"mx_dequantize: dtype must be float16, bfloat16 or float32, got {dtype}")
     out = torch.empty(t.shape, dtype=dtype, device=dev)
-    _launch(lib.nvm_mx_dequantize, dev, t.codes.data_ptr(), t.scales.data_ptr(), t.pitch, t.rows,
-            t.shape[-1], MX_FORMATS[t.fmt], code, out.data_ptr())
+    _launch(lib.nvm_mx_dequantize, dev, *t._pointers(), t.pitch, t.rows, t.shape[-1],
+            MX_FORMATS[t.fmt], code, out.data_ptr())
     return out
 
 
@@ -207,7 +243,7 @@ def mx_embedding(tokens: torch.Tensor, table: MxTensor, dtype: torch.dtype) -> t
     lib = _lib.load()
     if type(table) is not MxTensor or len(table.shape) != 2:
         raise ValueError("mx_embedding: table must be a two-dimensional MxTensor")
-    dev = _lib.require_device(tokens, table.codes, table.scales)
+    dev = _lib.require_device(tokens, table._base)
     code = MX_DTYPES.get(dtype)
     if code is None:
         raise ValueError(f"mx_embedding: dtype must be float16, bfloat16 or float32, got {dtype}")
@@ -218,9 +254,8 @@ def mx_embedding(tokens: torch.Tensor, table: MxTensor, dtype: torch.dtype) -> t
         tokens = tokens.clamp(-1, V)
     ids = tokens.reshape(-1).to(torch.int32).contiguous()
     out = torch.empty((*tokens.shape, D), dtype=dtype, device=dev)
-    _launch(lib.nvm_mx_embedding, dev, ids.data_ptr(), ids.numel(), table.codes.data_ptr(),
-            table.scales.data_ptr(), table.pitch, V, D, MX_FORMATS[table.fmt], code,
-            out.data_ptr())
+    _launch(lib.nvm_mx_embedding, dev, ids.data_ptr(), ids.numel(), *table._pointers(),
+            table.pitch, V, D, MX_FORMATS[table.fmt], code, out.data_ptr())
     return out
 
 
@@ -252,8 +287,7 @@ def residual_rms_norm_mx(h: torch.Tensor, r: Optional[torch.Tensor], weight: tor
     rows = hc.numel() // H
     out = MxTensor._empty(shape[:-1], rows, H, fmt, dev)
     _launch(lib.nvm_residual_rms_norm_mx, dev, hc.data_ptr(), _lib.ptr(rc), w.data_ptr(), rows, H,
-            float(eps), dtype, _lib.ptr(h_out), code, out.codes.data_ptr(), out.scales.data_ptr(),
-            out.pitch)
+            float(eps), dtype, _lib.ptr(h_out), code, *out._pointers(), out.pitch)
     return (h if h_out is None else h_out), out
 
 
@@ -297,12 +331,11 @@ def mx_linear(x: Union[MxTensor, torch.Tensor], w: MxTensor,
     if code is None:
         raise ValueError(f"mx_linear: dtype must be float16, bfloat16 or float32, got {dtype}")
     _check_weight("mx_linear", "w", w, a)
-    ac, wc, shape = a.codes, w.codes, w.shape
-    dev = _lib.require_device(ac, wc)
-    out = torch.empty((*a.shape[:-1], shape[0]), dtype=dtype, device=dev)
-    _launch(lib.nvm_mx_matmul, dev, ac.data_ptr(), a.scales.data_ptr(), a.pitch,
-            MX_FORMATS[a.fmt], wc.data_ptr(), w.scales.data_ptr(), w.pitch, a.rows, shape[1],
-            shape[0], code, out.data_ptr())
+    K, N = w.shape
+    dev = _lib.require_device(a._base, w._base)
+    out = torch.empty((*a.shape[:-1], K), dtype=dtype, device=dev)
+    _launch(lib.nvm_mx_matmul, dev, *a._pointers(), a.pitch, MX_FORMATS[a.fmt], *w._pointers(),
+            w.pitch, a.rows, N, K, code, out.data_ptr())
     return out if bias is None else out + bias
 
 
@@ -321,10 +354,9 @@ def mx_swiglu(x: Union[MxTensor, torch.Tensor], w_gate: MxTensor, w_up: MxTensor
     if w_up.shape[0] != K or K == 0 or K % MX_BLOCK:
         raise ValueError(f"mx_swiglu: gate and up must have the same output features, a positive "
                          f"multiple of {MX_BLOCK}, got {K} and {w_up.shape[0]}")
-    dev = _lib.require_device(a.codes, w_gate.codes, w_up.codes)
+    dev = _lib.require_device(a._base, w_gate._base, w_up._base)
     out = MxTensor._empty(a.shape[:-1], a.rows, K, fmt, dev)
-    _launch(lib.nvm_mx_swiglu, dev, a.codes.data_ptr(), a.scales.data_ptr(), a.pitch,
-            MX_FORMATS[a.fmt], w_gate.codes.data_ptr(), w_gate.scales.data_ptr(), w_gate.pitch,
-            w_up.codes.data_ptr(), w_up.scales.data_ptr(), w_up.pitch, a.rows, N, K, code,
-            out.codes.data_ptr(), out.scales.data_ptr(), out.pitch)
+    _launch(lib.nvm_mx_swiglu, dev, *a._pointers(), a.pitch, MX_FORMATS[a.fmt],
+            *w_gate._pointers(), w_gate.pitch, *w_up._pointers(), w_up.pitch, a.rows, N, K, code,
+            *out._pointers(), out.pitch)
     return out

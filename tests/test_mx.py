@@ -181,6 +181,41 @@ def test_tensor_of_more_dimensions_and_of_none():
     assert moved.shape == t.shape and "mxfp8" in repr(moved)
 
 
+@pytest.mark.parametrize("lead", [(), (1,), (5,), (2, 3), (2, 0, 3), (0,)])
+@pytest.mark.parametrize("n", [32, 544, 2048])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_tensor_that_a_kernel_writes(lead, n, fmt):
+    """Codes and scales are views of one buffer, codes first, of the layout that
+    an MxTensor of tensors has."""
+    import copy
+    import pickle
+
+    from nano_vllm_metal_amd import MxTensor
+
+    rows = int(np.prod(lead, dtype=np.int64))
+    t = MxTensor._empty(lead, rows, n, fmt, "cpu")
+    width, pitch = n // (2 if fmt == "mxfp4" else 1), -(-n // 512) * 16
+    t._base.copy_(torch.randint(0, 256, t._base.shape, dtype=torch.uint8))
+    assert t._base.numel() == rows * (width + pitch) and t.pitch == pitch and t.rows == rows
+    codes, scales = t.codes, t.scales
+    assert codes.shape == (*lead, width) and scales.shape == (*lead, n // 32)
+    assert codes.is_contiguous() and t.codes is codes and t.scales is scales
+    assert torch.equal(codes.reshape(-1), t._base[:rows * width])
+    assert torch.equal(scales.reshape(rows, n // 32),
+                       t._base[rows * width:].view(rows, pitch)[:, :n // 32])
+    assert t._pointers() == (t._base.data_ptr(), t._base.data_ptr() + rows * width)
+    again = MxTensor(codes, scales, fmt)
+    assert again.pitch == pitch and again.shape == t.shape and again.rows == rows
+    if rows:
+        assert again._pointers() == t._pointers()  # (nothing was copied)
+    for other in (copy.deepcopy(t), pickle.loads(pickle.dumps(t)), copy.deepcopy(again)):
+        assert torch.equal(other.codes, codes) and torch.equal(other.scales, scales)
+        if rows:
+            assert other._pointers()[0] != t._pointers()[0]
+        codes2, scales2 = other._pointers()
+        assert codes2 == other.codes.data_ptr() and (not rows or scales2 == other.scales.data_ptr())
+
+
 def test_tensor_refuses():
     from nano_vllm_metal_amd import MxTensor
 
