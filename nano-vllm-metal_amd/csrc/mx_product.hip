@@ -7,14 +7,24 @@
 
 namespace nvm {
 
-// Few rows: mx_gemv.hip, whose time goes with rows x output columns, while the
-// tiles' goes with the steps along a row until they fill the GPU.  2048 -> 5120:
-// 80 rows (410 thousand outputs) 9.4 us there, 11.3 on tiles; 96 rows (492) 11.5
-// and 11.3; 4096 -> 12288: 32 rows (393) 11.6 and 17.0, 64 rows (786) 19.5 and
-// 17.5; gate/up 2048 -> 6144: 64 rows (393) 10.6 and 12.6; 4096 -> 14336: 32 rows
-// (459) 21.5 and 20.5.  One tile of 16 rows stays there whatever the columns:
-// 2048 -> 151936 of 1 row 31 and 50 us, of 16 rows 42 and 49.
-static bool few_rows(const MxMatmulArgs &a) { return a.M <= 16 || a.M * a.K <= 3 << 17; }
+// Few rows: mx_gemv.hip, whose time goes with rows x outputs x steps, some 6 us
+// for 10^9 of them; that of a tile goes with the steps along a row alone until
+// tiles fill the GPU, 3.4 us for 1000 values, and 1 to 2 us more at any size.  So
+// the border is a number of outputs, a little more for short rows (rows padded
+// to the kernel's own tiles):
+//   2048 -> 5120, 80 rows (410 thousand outputs) 9.4 and 11.3 us, 96 rows (492)
+//   11.5 and 11.3; 4096 -> 12288, 32 rows (393) 11.6 and 17.0, 64 rows (786) 19.5
+//   and 17.5; 928 -> 11616, 62 rows (743) 6.4 and 8.8; 4928 -> 3296, 132 rows
+//   (475) 14.0 and 21.4; 8192 -> 8192, 64 rows (524) 33.3 and 27.7; 512 -> 2048,
+//   384 rows (786) 7.25 and 7.3, 512 rows (1049) 7.7 and 7.3
+//   gate/up 2048 -> 6144, 64 rows (393) 10.6 and 12.6, 96 rows (786) 19.9 and 12.6
+// One tile of 16 rows stays there whatever the columns: 2048 -> 151936 of 1 row
+// 31 and 50 us, of 16 rows 42 and 49.
+static bool few_rows(bool dual, const MxMatmulArgs &a) {
+  if (a.M <= 16) return true;
+  const int64_t tile = dual && a.M > 32 ? 64 : 16, rows = (a.M + tile - 1) / tile * tile;
+  return rows * a.K < (7 << 16) + (1 << 28) / std::max(a.N, 512);
+}
 
 // Many rows: the tile whose rounds over the CUs cost least.  A step of the
 // larger ones costs less for its outputs, but they leave more CUs idle.  Their
@@ -35,7 +45,7 @@ static bool few_rows(const MxMatmulArgs &a) { return a.M <= 16 || a.M * a.K <= 3
 static hipError_t launch_mx_product(int format, bool dual, int out_format, const MxMatmulArgs &a,
                                     hipStream_t st) {
   const int64_t columns = (int64_t)a.K * (dual ? 2 : 1);
-  if (few_rows(a)) return launch_mx_gemv(format, dual, out_format, a, st);
+  if (few_rows(dual, a)) return launch_mx_gemv(format, dual, out_format, a, st);
   const int64_t cus = cu_count();
   auto rounds = [&](int bn, int bm) {
     return ((columns + bn - 1) / bn * ((a.M + bm - 1) / bm) + cus - 1) / cus;
