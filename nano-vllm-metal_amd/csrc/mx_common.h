@@ -124,14 +124,15 @@ struct MxMatmulArgs {
 };
 // The products for few rows (mx_gemv.hip), for some (mx_gemm_pipe.hip: tiles of
 // 128 outputs by 128 rows, `wide` 256 by 128) and for many (mx_gemm.hip: 256 by
-// 256).  hipErrorInvalidConfiguration: more blocks than a launch has, more
-// than kMxMaxTiles output tiles.
+// 256, those past whole rounds in `parts`: 0, 2 or 4, a part a block).
+// hipErrorInvalidConfiguration: more blocks than a launch has, more than
+// kMxMaxTiles output tiles.
 constexpr int64_t kMxMaxTiles = 1 << 22;
 hipError_t launch_mx_gemv(int format, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st);
 hipError_t launch_mx_gemm_pipe(int format, bool wide, bool dual, int out_format,
                                const MxMatmulArgs &a, hipStream_t st);
-hipError_t launch_mx_gemm(int format, bool dual, int out_format, const MxMatmulArgs &a,
+hipError_t launch_mx_gemm(int format, int parts, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st);
 
 // f(integral constant) of an output type.
@@ -171,8 +172,8 @@ __device__ __forceinline__ void mx_store4(void *out, int64_t row, int k, int end
 // neighbours, 16 bytes: groups 0 and 2 of the first tile, 1 and 3 of the
 // second.  Every lane of the wavefront is active.
 template <int DT>
-__device__ __forceinline__ void mx_store_pair(void *out, int G, int64_t row, int k, int end, f32x4 v0,
-                                              f32x4 v1) {
+__device__ __forceinline__ void mx_store_pair(void *out, int G, int64_t row, int k, int end,
+                                              f32x4 v0, f32x4 v1) {
   if constexpr (DT == NVM_MX_F32) {
     float *o = (float *)out + row + k + 4 * G;
     if (k + 4 * G < end) *(f32x4 *)o = v0;
@@ -193,8 +194,8 @@ __device__ __forceinline__ void mx_store_pair(void *out, int G, int64_t row, int
 // places as above, so a lane stores eight neighbours.  Every lane of the
 // wavefront is active; `on`: the block is inside the output.
 template <int OFMT>
-__device__ __forceinline__ void mx_store_block(const float (&h)[8], int G, bool on, int64_t m, int k,
-                                               const MxMatmulArgs &p) {
+__device__ __forceinline__ void mx_store_block(const float (&h)[8], int G, bool on, int64_t m,
+                                               int k, const MxMatmulArgs &p) {
   uint32_t mx = absmax8(h);
   mx = max(mx, (uint32_t)__shfl_xor((int)mx, 16));
   mx = max(mx, (uint32_t)__shfl_xor((int)mx, 32));

@@ -18,6 +18,10 @@
 //    side (mx_gemm_pipe.hip) two steps' operands only fit beside 4 x 4 sums.
 //  * Blocks are persistent and requests run on across tiles, so a tile's first
 //    steps arrive during the epilogue of the one before.
+//  * Tiles that would be a last round of at most a quarter (half) of the CUs are
+//    computed in quarters (halves) by all of them, with the code of mx_pipe.h
+//    (3000 rows of 4096 -> 6144, 288 tiles: 66.5 us with quarters, 82 without;
+//    8192 rows of 2048 -> 5120, 640 tiles: 73 with halves, 77 without).
 //  * A last step of less than 128 values is computed with the activations
 //    behind the row replaced by zeros and scales by one in registers, so what
 //    lies there does not matter (a weight code is finite whatever its bits).
@@ -25,15 +29,22 @@
 // 8192 x 8192 x 8192: 367 us, 3.0 PFLOP/s (E2M1: 293 us, 3.75); 4096 rows of
 // 2048 through a gate/up pair of 6144: 82 us, 2.5 PFLOP/s.  Left there: 768 tiles
 // of 16 steps each, whose epilogues the other half of the block hides in part.
-#include "mx_tile.h"
+#include "mx_pipe.h"
 
 namespace nvm {
 
 namespace {
 
+template <class X>
+struct TypeOf {
+  using type = X;
+};
+
+// The first `whole` tiles in turn; the others, if `parts` is not zero, in that
+// many parts (2 or 4), a part a block.
 template <int FMT, int OFMT, class T>
 __global__ __launch_bounds__(64 * T::NW, 2) void mx_gemm_kernel(const MxMatmulArgs p, int n_tiles,
-                                                                int m_tiles) {
+                                                                int m_tiles, int whole, int parts) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   constexpr int NX = FMT == NVM_MX_FP4 ? 1 : 2;
   const int lane = threadIdx.x & 63, G = lane >> 4;
@@ -46,8 +57,8 @@ __global__ __launch_bounds__(64 * T::NW, 2) void mx_gemm_kernel(const MxMatmulAr
   if (T::SL < T::ST) steps += steps % 4 == 1;
   // tiles in contiguous runs per XCD (blocks go to the XCDs in turn), dealt to
   // the XCD's blocks
-  const int total = n_tiles * m_tiles, per_xcd = (total + 7) >> 3, stride = (int)gridDim.x >> 3;
-  const int last = min(((int)blockIdx.x & 7) * per_xcd + per_xcd, total);
+  const int per_xcd = (whole + 7) >> 3, stride = (int)gridDim.x >> 3;
+  const int last = min(((int)blockIdx.x & 7) * per_xcd + per_xcd, whole);
   const int first = ((int)blockIdx.x & 7) * per_xcd + ((int)blockIdx.x >> 3);
   if (first >= last) return;
 
@@ -203,30 +214,65 @@ __global__ __launch_bounds__(64 * T::NW, 2) void mx_gemm_kernel(const MxMatmulAr
   // (no load may write to LDS behind the block's end)
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   if (!late) __builtin_amdgcn_s_barrier();
+  // The tiles past whole rounds, in parts: one to a block.
+  if (parts == 0) return;
+  const int part = ((int)blockIdx.x & 7) * stride + ((int)blockIdx.x >> 3);
+  const int tile = whole + part / parts, sub = part % parts;
+  if (tile >= n_tiles * m_tiles) return;
+  __syncthreads();  // (LDS changes hands)
+  auto finish = [&](auto TILE) {
+    using S = typename decltype(TILE)::type;
+    constexpr int across = T::BK / S::BK;
+    const typename T::Place from = T::place(p, tile, n_tiles, m_tiles);
+    typename S::Place q;
+    q.k0 = from.k0 + sub % across * S::BK;
+    q.m0 = from.m0 + sub / across * S::BM;
+    q.nk = min(S::BK, p.K - q.k0);
+    q.nm = (int)min((int64_t)S::BM, p.M - q.m0);
+    if (q.nk > 0 && q.nm > 0)
+      mx_pipe_tiles<FMT, OFMT, S>(p, smem, 0, 1, 1, [&](int) { return q; });
+  };
+  if (parts == 4)
+    finish(TypeOf<MxSmallTile<FMT, T::DUAL>>{});
+  else
+    finish(TypeOf<MxWideTile<FMT, T::DUAL>>{});
 }
 
 template <int FMT, int OFMT, bool DUAL>
-hipError_t go(const MxMatmulArgs &a, hipStream_t st) {
+hipError_t go(int parts, const MxMatmulArgs &a, hipStream_t st) {
   // (the rings fill the 160 KB of LDS)
   using T = std::conditional_t<FMT == NVM_MX_FP4, MxTile<FMT, DUAL, 256, 256, 2, 4, 1, 4, 4>,
                                MxTile<FMT, DUAL, 256, 256, 2, 4, 1, 3, 2>>;
+  constexpr int kLds =
+      std::max({T::kLds, MxSmallTile<FMT, DUAL>::kLds, MxWideTile<FMT, DUAL>::kLds});
   static bool allowed[64] = {false};
-  return mx_launch_tiles<T>(mx_gemm_kernel<FMT, OFMT, T>, false, allowed, a, st);
+  int n_tiles, m_tiles;
+  if (!mx_count_tiles<T>(a, n_tiles, m_tiles)) return hipErrorInvalidConfiguration;
+  auto kern = mx_gemm_kernel<FMT, OFMT, T>;
+  mx_allow_lds(kern, kLds, allowed);
+  // blocks that walk tiles, one to a CU
+  const int total = n_tiles * m_tiles;
+  const int grid = std::min(8 * ((total + 7) / 8), cu_count() / 8 * 8);
+  const int whole = parts ? total / grid * grid : total;
+  if (parts && (whole == 0 || (total - whole) * parts > grid)) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * T::NW), kLds, st, a, n_tiles, m_tiles,
+                     whole, parts);
+  return hipGetLastError();
 }
 
 template <int FMT>
-hipError_t launch_fmt(bool dual, int out_format, const MxMatmulArgs &a, hipStream_t st) {
-  if (!dual) return go<FMT, NVM_MX_FP8, false>(a, st);
-  return out_format == NVM_MX_FP4 ? go<FMT, NVM_MX_FP4, true>(a, st)
-                                  : go<FMT, NVM_MX_FP8, true>(a, st);
+hipError_t launch_fmt(int parts, bool dual, int out_format, const MxMatmulArgs &a, hipStream_t st) {
+  if (!dual) return go<FMT, NVM_MX_FP8, false>(parts, a, st);
+  return out_format == NVM_MX_FP4 ? go<FMT, NVM_MX_FP4, true>(parts, a, st)
+                                  : go<FMT, NVM_MX_FP8, true>(parts, a, st);
 }
 
 }  // namespace
 
-hipError_t launch_mx_gemm(int format, bool dual, int out_format, const MxMatmulArgs &a,
+hipError_t launch_mx_gemm(int format, int parts, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st) {
-  return format == NVM_MX_FP4 ? launch_fmt<NVM_MX_FP4>(dual, out_format, a, st)
-                              : launch_fmt<NVM_MX_FP8>(dual, out_format, a, st);
+  return format == NVM_MX_FP4 ? launch_fmt<NVM_MX_FP4>(parts, dual, out_format, a, st)
+                              : launch_fmt<NVM_MX_FP8>(parts, dual, out_format, a, st);
 }
 
 }  // namespace nvm

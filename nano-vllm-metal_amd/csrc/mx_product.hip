@@ -26,34 +26,42 @@ static bool few_rows(bool dual, const MxMatmulArgs &a) {
   return rows * a.K < (7 << 16) + (1 << 28) / std::max(a.N, 512);
 }
 
-// Many rows: the tile whose rounds over the CUs cost least.  A step of the
+// Many rows: the tiles whose rounds over the CUs cost least.  A step of the
 // larger ones costs less for its outputs, but they leave more CUs idle.  Their
 // costs, in steps of 256 x 256 at 20 (0.9 us each): E4M3 activations 13 and 9,
-// E2M1 11 and 8 for 256 x 128 and 128 x 128.  In us on 256 x 256, 256 x 128 and
-// 128 x 128, E4M3 unless said:
-//   2048 -> 5120    512 rows   24.0  17.2  13.2
-//                  1536 rows   26.3  21.0  24.8
-//                  2048 rows   27.0  30.3  35.2
-//                  4096 rows   47.5  46.4  59.0  (E2M1 42.4  38.3  46.3)
-//   6144 -> 2048   1024 rows   54    34    24
-//                  4096 rows   57    45.5  54
-//   8192 -> 8192   8192 rows   367   424   553   (E2M1  293   350   420)
+// E2M1 11 and 8 for 256 x 128 and 128 x 128.  A last round of 256 x 256 that no
+// more than a quarter (half) of the CUs would have is computed in parts of those
+// sizes.  In us on 256 x 256 in whole tiles, in parts, on 256 x 128 and 128 x 128,
+// E4M3 unless said:
+//   2048 -> 5120    512 rows   24.0   -    17.2  13.2
+//                  1536 rows   26.3   -    21.0  24.8
+//                  2048 rows   27.0   -    30.3  35.2
+//                  4096 rows   48.9  44.4  47.0  59.0  (E2M1 42.0  35.8  35.7  46.3)
+//                  8192 rows   77.3  73.1  78.7   -    (E2M1 67.1  61.7  61.8)
+//   6144 -> 2048   1024 rows   54     -    34    24
+//                  4096 rows   57     -    45.5  54
+//   4096 -> 6144   3000 rows   82.2  66.4  78.2   -
+//   8192 -> 8192   8192 rows   367    -    424   553   (E2M1  293   -   350   420)
 //   gate/up 2048 -> 6144
-//                   100 rows   24.0  16.8  12.6
-//                  1000 rows   27.7  31.7  35.9
-//                  4096 rows   82    94.7  134
+//                   100 rows   24.0   -    16.8  12.6
+//                  1000 rows   27.7   -    31.7  35.9
+//                  1500 rows   50.5  40.4  46.0   -
+//                  4096 rows   82     -    94.7  134
 static hipError_t launch_mx_product(int format, bool dual, int out_format, const MxMatmulArgs &a,
                                     hipStream_t st) {
-  const int64_t columns = (int64_t)a.K * (dual ? 2 : 1);
   if (few_rows(dual, a)) return launch_mx_gemv(format, dual, out_format, a, st);
-  const int64_t cus = cu_count();
-  auto rounds = [&](int bn, int bm) {
-    return ((columns + bn - 1) / bn * ((a.M + bm - 1) / bm) + cus - 1) / cus;
-  };
   const bool fp4 = format == NVM_MX_FP4;
-  const int64_t big = rounds(256, 256) * 20, wide = rounds(256, 128) * (fp4 ? 11 : 13),
-                small = rounds(128, 128) * (fp4 ? 8 : 9);
-  if (big <= std::min(wide, small)) return launch_mx_gemm(format, dual, out_format, a, st);
+  const int64_t columns = (int64_t)a.K * (dual ? 2 : 1), cus = cu_count() / 8 * 8;
+  auto tiles = [&](int bn, int bm) { return (columns + bn - 1) / bn * ((a.M + bm - 1) / bm); };
+  auto rounds = [&](int64_t n) { return (n + cus - 1) / cus; };
+  const int64_t wide_round = fp4 ? 11 : 13, small_round = fp4 ? 8 : 9;
+  const int64_t wide = rounds(tiles(256, 128)) * wide_round;
+  const int64_t small = rounds(tiles(128, 128)) * small_round;
+  const int64_t n = tiles(256, 256), rest = n % cus;
+  const int parts = n < cus || rest == 0 || 2 * rest > cus ? 0 : 4 * rest > cus ? 2 : 4;
+  const int64_t big = parts ? n / cus * 20 + (parts == 4 ? small_round : wide_round)
+                            : rounds(n) * 20;
+  if (big <= std::min(wide, small)) return launch_mx_gemm(format, parts, dual, out_format, a, st);
   return launch_mx_gemm_pipe(format, wide <= small, dual, out_format, a, st);
 }
 

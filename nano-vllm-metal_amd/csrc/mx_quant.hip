@@ -333,8 +333,8 @@ int nvm_mx_quantize(const void *x, int64_t rows, int64_t n, int64_t x_ld, int dt
   mx_by_dtype(dtype, [&](auto D) {
     by_format(format, [&](auto F) {
       hipLaunchKernelGGL((mx_quantize_kernel<decltype(D)::value, decltype(F)::value>), grid,
-                         dim3(kThreads), 0, (hipStream_t)stream, x, (uint32_t)total, (int)(n / 8), x_ld,
-                         codes, scales, scale_ld);
+                         dim3(kThreads), 0, (hipStream_t)stream, x, (uint32_t)total, (int)(n / 8),
+                         x_ld, codes, scales, scale_ld);
     });
   });
   const hipError_t e = hipGetLastError();

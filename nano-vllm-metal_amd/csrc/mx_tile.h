@@ -1,6 +1,6 @@
-// What the two kernels for many MX rows share (mx_gemm.hip, mx_gemm_pipe.hip):
-// a block's tile and its layout in LDS, the order of the tiles, the turn of
-// the scales, the epilogue, the launch.
+// What the products of many MX rows share (mx_gemm.hip, mx_pipe.h): a block's
+// tile and its layout in LDS, the order of the tiles, the turn of the scales,
+// the epilogue.
 #pragma once
 
 #include <algorithm>
@@ -275,26 +275,32 @@ struct MxTile {
   }
 };
 
-// The launch of a kernel of T's tiles: a block a tile if `single`, else blocks
-// that walk tiles, one to a CU.  (More than 64 KB of dynamic LDS is allowed
-// once per device and instance; a failure shows up as a failed launch.)
-template <class T, class F>
-hipError_t mx_launch_tiles(F kern, bool single, bool (&allowed)[64], const MxMatmulArgs &a,
-                           hipStream_t st) {
-  const int n_tiles = (int)(((int64_t)a.K + T::BK - 1) / T::BK);
-  const int64_t m_tiles = (a.M + T::BM - 1) / T::BM, total = m_tiles * n_tiles;
-  if (total > kMxMaxTiles) return hipErrorInvalidConfiguration;
+// 128 outputs (gate/up: 64 of each) by 128 rows, and 256 by 128 (mx_pipe.h).
+template <int FMT, bool DUAL>
+using MxSmallTile = MxTile<FMT, DUAL, 128, 128, 2, 2, 2, 3, 2>;
+template <int FMT, bool DUAL>
+using MxWideTile = MxTile<FMT, DUAL, 256, 128, 4, 2, 1, 4, 2>;
+
+// Output tiles of T; false: more than kMxMaxTiles.
+template <class T>
+bool mx_count_tiles(const MxMatmulArgs &a, int &n_tiles, int &m_tiles) {
+  const int64_t n = ((int64_t)a.K + T::BK - 1) / T::BK, m = (a.M + T::BM - 1) / T::BM;
+  if (n * m > kMxMaxTiles) return false;
+  n_tiles = (int)n;
+  m_tiles = (int)m;
+  return true;
+}
+
+// More than 64 KB of dynamic LDS is allowed once per device and kernel (a
+// failure shows up as a failed launch).
+template <class F>
+void mx_allow_lds(F kern, int bytes, bool (&allowed)[64]) {
   int dev = 0;
   if (hipGetDevice(&dev) == hipSuccess && dev >= 0 && dev < 64 && !allowed[dev]) {
     (void)hipFuncSetAttribute((const void *)kern, hipFuncAttributeMaxDynamicSharedMemorySize,
-                              T::kLds);
+                              bytes);
     allowed[dev] = true;
   }
-  const int64_t all = 8 * ((total + 7) / 8);
-  const int64_t grid = single ? all : std::min<int64_t>(all, cu_count() / 8 * 8);
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * T::NW), T::kLds, st, a, n_tiles,
-                     (int)m_tiles);
-  return hipGetLastError();
 }
 
 }  // namespace nvm

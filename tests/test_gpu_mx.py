@@ -382,7 +382,8 @@ def test_linear_writes_its_rows_only():
 # of one run, of a step more than a run, and with a last step cut short.
 TILED = [(400, 32, 1000), (450, 640, 901), (521, 1184, 768), (1030, 96, 4000), (1030, 640, 4003),
          (2600, 160, 8200), (1030, 512, 8200), (1030, 672, 8193), (3900, 32, 8104), (3900, 160, 8100),
-         (1000, 32, 1200), (1100, 96, 1001), (1000, 544, 1250), (700, 1056, 1600), (513, 512, 2500)]
+         (1000, 32, 1200), (1100, 96, 1001), (1000, 544, 1250), (700, 1056, 1600), (513, 512, 2500),
+         (1100, 160, 15200), (1100, 544, 15301), (2600, 672, 8200)]
 
 
 @pytest.mark.parametrize("M,N,K", TILED)
@@ -407,7 +408,7 @@ def test_linear_on_tiles(M, N, K, fmt):
 
 @pytest.mark.parametrize("M,N,K", [(450, 160, 900), (450, 608, 900), (1030, 160, 4000),
                                    (1030, 160, 8200), (1030, 608, 8200), (1000, 160, 1200),
-                                   (1000, 608, 1201)])
+                                   (1000, 608, 1201), (1100, 160, 15201)])
 @pytest.mark.parametrize("fmt", FMTS)
 def test_tiles_read_and_write_their_rows_only(M, N, K, fmt):
     """What lies behind a row and behind the last one: NaN scales and codes in
@@ -469,7 +470,8 @@ def test_swiglu(M, N, K, fmt, ofmt):
 
 @pytest.mark.parametrize("M,N,K", [(300, 160, 800), (401, 640, 544), (1030, 160, 2016),
                                    (2600, 96, 4128), (1030, 640, 4128), (3900, 96, 4064),
-                                   (1000, 96, 1216), (1000, 544, 1056), (650, 640, 1600)])
+                                   (1000, 96, 1216), (1000, 544, 1056), (650, 640, 1600),
+                                   (1100, 160, 7616), (2600, 672, 4128)])
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("ofmt", FMTS)
 def test_swiglu_on_tiles(M, N, K, fmt, ofmt):
