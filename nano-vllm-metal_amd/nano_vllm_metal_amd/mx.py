@@ -115,8 +115,10 @@ class MxTensor:
 
     def _pointers(self) -> Tuple[int, int]:
         """Addresses of codes and scales."""
+        if self._split is None:
+            return self._base.data_ptr(), self._scales.data_ptr()
         at = self._base.data_ptr()
-        return at, self._scales.data_ptr() if self._split is None else at + self._split
+        return at, at + self._split
 
     @property
     def device(self) -> torch.device:
@@ -218,7 +220,8 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp8") -> MxTensor:
         x, ld = x.clone(memory_format=torch.contiguous_format), n
     rows = x.numel() // n
     out = MxTensor._empty(shape[:-1], rows, n, fmt, dev)
-    _launch(lib.nvm_mx_quantize, dev, x.data_ptr(), rows, n, ld, dtype, code, *out._pointers(),
+    codes, scales = out._pointers()
+    _launch(lib.nvm_mx_quantize, dev, x.data_ptr(), rows, n, ld, dtype, code, codes, scales,
             out.pitch)
     return out
 
@@ -286,8 +289,9 @@ def residual_rms_norm_mx(h: torch.Tensor, r: Optional[torch.Tensor], weight: tor
     w = _packed(weight if weight.dtype == h.dtype else weight.to(h.dtype))
     rows = hc.numel() // H
     out = MxTensor._empty(shape[:-1], rows, H, fmt, dev)
+    codes, scales = out._pointers()
     _launch(lib.nvm_residual_rms_norm_mx, dev, hc.data_ptr(), _lib.ptr(rc), w.data_ptr(), rows, H,
-            float(eps), dtype, _lib.ptr(h_out), code, *out._pointers(), out.pitch)
+            float(eps), dtype, _lib.ptr(h_out), code, codes, scales, out.pitch)
     return (h if h_out is None else h_out), out
 
 
@@ -334,8 +338,10 @@ def mx_linear(x: Union[MxTensor, torch.Tensor], w: MxTensor,
     K, N = w.shape
     dev = _lib.require_device(a._base, w._base)
     out = torch.empty((*a.shape[:-1], K), dtype=dtype, device=dev)
-    _launch(lib.nvm_mx_matmul, dev, *a._pointers(), a.pitch, MX_FORMATS[a.fmt], *w._pointers(),
-            w.pitch, a.rows, N, K, code, out.data_ptr())
+    ac, asc = a._pointers()
+    wc, wsc = w._pointers()
+    _launch(lib.nvm_mx_matmul, dev, ac, asc, a.pitch, MX_FORMATS[a.fmt], wc, wsc, w.pitch, a.rows,
+            N, K, code, out.data_ptr())
     return out if bias is None else out + bias
 
 
@@ -356,7 +362,10 @@ def mx_swiglu(x: Union[MxTensor, torch.Tensor], w_gate: MxTensor, w_up: MxTensor
                          f"multiple of {MX_BLOCK}, got {K} and {w_up.shape[0]}")
     dev = _lib.require_device(a._base, w_gate._base, w_up._base)
     out = MxTensor._empty(a.shape[:-1], a.rows, K, fmt, dev)
-    _launch(lib.nvm_mx_swiglu, dev, *a._pointers(), a.pitch, MX_FORMATS[a.fmt],
-            *w_gate._pointers(), w_gate.pitch, *w_up._pointers(), w_up.pitch, a.rows, N, K, code,
-            *out._pointers(), out.pitch)
+    ac, asc = a._pointers()
+    gc, gsc = w_gate._pointers()
+    uc, usc = w_up._pointers()
+    oc, osc = out._pointers()
+    _launch(lib.nvm_mx_swiglu, dev, ac, asc, a.pitch, MX_FORMATS[a.fmt], gc, gsc, w_gate.pitch, uc,
+            usc, w_up.pitch, a.rows, N, K, code, oc, osc, out.pitch)
     return out
