@@ -21,6 +21,8 @@
 // Weights are the row operand, so a lane ends up with four neighbouring
 // outputs of one activation row, and a block of 32 outputs (SwiGLU's MX
 // output) is two tiles of four lane groups.
+#include <math.h>
+
 #include <type_traits>
 
 #include "internal.h"
@@ -183,45 +185,74 @@ hipError_t go(const MxMatmulArgs &a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// The largest tile of a block that leaves kBlocks of them, without a half-used
-// activation tile.  Larger blocks read the activations, and a column of them
-// the weights, less often; too few leave CUs idle (2048 -> 5120 of 16 rows: 160
-// blocks of 2 x 1 tiles 4.6 us, 320 of 1 x 1 5.2, 80 of 4 x 1 5.6; of 64 rows 214
-// of 3 x 2 7.6, 320 of 4 x 1 9.2; 4096 -> 2048 of 32 rows: 256 of 1 x 1 5.4, 128
-// of 2 x 1 6.7).
-constexpr int64_t kBlocks = 160;
+// Tiles of a block, and the time of a launch of such blocks: `fixed` + `round` x
+// rounds over the CUs x N / 2048 microseconds, for E2M1 and E4M3 activations
+// (least squares over 390 products of 17 to 512 rows; the residual is 3 to 9 %).
+// Larger blocks read the activations, and a column of them the weights, less
+// often, but a round of them is longer: 4096 -> 4096 of 128 rows 12.4 us on 256
+// blocks of 4 x 2 tiles, 15.3 on 192 of 4 x 3, 15.7 on 512 of 2 x 2, 18.8 on 688
+// of 3 x 2; 2048 -> 2048 of 32 rows 3.7 on 256 of 1 x 1, 4.4 on 128 of 2 x 1, 5.7
+// on 64 of 2 x 2.
+struct Blocks {
+  int rt, mt;
+  double fixed[2], round[2];  // by nvm_mx_format
+};
+constexpr Blocks kLinear[] = {
+    {1, 1, {2, 2.2}, {1.15, 1.5}}, {2, 1, {2.1, 2.3}, {1.8, 2.05}}, {4, 1, {2.3, 2.6}, {3, 3.25}},
+    {2, 2, {2.4, 2.6}, {2.4, 3.3}}, {2, 3, {2.7, 2.7}, {2.9, 4.5}}, {4, 2, {3, 3.3}, {3.6, 4.5}},
+    {4, 3, {3.5, 3.6}, {4.1, 6}}};
+// (SwiGLU: 32 outputs a block, which its scale needs: two tiles of each matrix.
+// 2048 -> 6144 of 8 rows 6.2 us; of 32 rows 8.1 on 192 blocks of 2 tiles of
+// rows, 10.2 on 384 of 1; 2048 -> 768 of 64 rows 5.8 on 96 of 1, 10.5 on 24 of 4)
+constexpr Blocks kSwiglu[] = {{4, 1, {2.6, 2.5}, {2.9, 3.3}},
+                              {4, 2, {2.8, 3}, {3.5, 4.3}},
+                              {4, 3, {3.2, 2.9}, {3.8, 5.6}},
+                              {4, 4, {3.2, 3.4}, {4.7, 6.2}}};
+
+template <int FMT, int OFMT, bool DUAL, int I>
+hipError_t launch_tile(int tile, const MxMatmulArgs &a, hipStream_t st) {
+  constexpr const Blocks &b = DUAL ? kSwiglu[I] : kLinear[I];
+  if constexpr (I > 0)
+    if (tile != I) return launch_tile<FMT, OFMT, DUAL, I - 1>(tile, a, st);
+  return go<FMT, OFMT, DUAL, b.rt, b.mt>(a, st);
+}
 
 template <int FMT>
-hipError_t launch_fmt(bool dual, int out_format, const MxMatmulArgs &a, hipStream_t st) {
-  const int64_t mt = (a.M + 15) / 16;
-  auto fits = [&](int rt, int m) {
-    return mt % m == 0 && ((int64_t)a.K + 16 * rt - 1) / (16 * rt) * (mt / m) >= kBlocks;
-  };
-  if (!dual) {
-    if (fits(3, 2)) return go<FMT, NVM_MX_FP8, false, 3, 2>(a, st);
-    if (fits(4, 1)) return go<FMT, NVM_MX_FP8, false, 4, 1>(a, st);
-    if (fits(2, 2)) return go<FMT, NVM_MX_FP8, false, 2, 2>(a, st);
-    if (fits(2, 1)) return go<FMT, NVM_MX_FP8, false, 2, 1>(a, st);
-    return go<FMT, NVM_MX_FP8, false, 1, 1>(a, st);
+hipError_t launch_fmt(int tile, bool dual, int out_format, const MxMatmulArgs &a,
+                      hipStream_t st) {
+  constexpr int nl = sizeof(kLinear) / sizeof(Blocks), ns = sizeof(kSwiglu) / sizeof(Blocks);
+  if (!dual) return launch_tile<FMT, NVM_MX_FP8, false, nl - 1>(tile, a, st);
+  return out_format == NVM_MX_FP4 ? launch_tile<FMT, NVM_MX_FP4, true, ns - 1>(tile, a, st)
+                                  : launch_tile<FMT, NVM_MX_FP8, true, ns - 1>(tile, a, st);
+}
+
+template <int N>
+double best_of(const Blocks (&blocks)[N], int format, bool dual, const MxMatmulArgs &a, int *tile) {
+  const int64_t cus = cu_count();
+  double best = INFINITY;
+  for (int i = 0; i < N; ++i) {
+    const Blocks &b = blocks[i];
+    const int64_t columns = 16 * (dual ? b.rt / 2 : b.rt), rows = 16 * b.mt;
+    const int64_t n = (a.K + columns - 1) / columns * ((a.M + rows - 1) / rows);
+    const double t = b.fixed[format] + b.round[format] * ((n + cus - 1) / cus) * (a.N / 2048.0);
+    if (t < best) {
+      best = t;
+      *tile = i;
+    }
   }
-  // SwiGLU: 32 outputs a block (its scale needs them), over all activation
-  // rows of up to four tiles (2048 -> 6144 of 8 rows 6.2 us; of 17 rows 7.4 on 2
-  // tiles, 10.2 on 1; of 64 rows 11.9 on 4, 13.4 on 2)
-  auto swiglu = [&](auto OF) {
-    constexpr int OFMT = decltype(OF)::value;
-    if (mt == 1) return go<FMT, OFMT, true, 4, 1>(a, st);
-    if (mt == 2) return go<FMT, OFMT, true, 4, 2>(a, st);
-    return go<FMT, OFMT, true, 4, 4>(a, st);
-  };
-  return out_format == NVM_MX_FP4 ? swiglu(MxInt<NVM_MX_FP4>{}) : swiglu(MxInt<NVM_MX_FP8>{});
+  return best;
 }
 
 }  // namespace
 
-hipError_t launch_mx_gemv(int format, bool dual, int out_format, const MxMatmulArgs &a,
+double mx_gemv_time(int format, bool dual, const MxMatmulArgs &a, int *tile) {
+  return dual ? best_of(kSwiglu, format, dual, a, tile) : best_of(kLinear, format, dual, a, tile);
+}
+
+hipError_t launch_mx_gemv(int format, int tile, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st) {
-  return format == NVM_MX_FP4 ? launch_fmt<NVM_MX_FP4>(dual, out_format, a, st)
-                              : launch_fmt<NVM_MX_FP8>(dual, out_format, a, st);
+  return format == NVM_MX_FP4 ? launch_fmt<NVM_MX_FP4>(tile, dual, out_format, a, st)
+                              : launch_fmt<NVM_MX_FP8>(tile, dual, out_format, a, st);
 }
 
 }  // namespace nvm

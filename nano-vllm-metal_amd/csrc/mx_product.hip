@@ -7,25 +7,14 @@
 
 namespace nvm {
 
-// Few rows: mx_gemv.hip, whose time goes with rows x outputs x steps, some 6 us
-// for 10^9 of them; that of a tile goes with the steps along a row alone until
-// tiles fill the GPU, 3.4 us for 1000 values, and 1 to 2 us more at any size.  So
-// the border is a number of outputs, a little more for short rows (rows padded
-// to the kernel's own tiles):
-//   2048 -> 5120, 80 rows (410 thousand outputs) 9.4 and 11.3 us, 96 rows (492)
-//   11.5 and 11.3; 4096 -> 12288, 32 rows (393) 11.6 and 17.0, 64 rows (786) 19.5
-//   and 17.5; 928 -> 11616, 62 rows (743) 6.4 and 8.8; 4928 -> 3296, 132 rows
-//   (475) 14.0 and 21.4; 8192 -> 8192, 64 rows (524) 33.3 and 27.7; 512 -> 2048,
-//   384 rows (786) 7.25 and 7.3, 512 rows (1049) 7.7 and 7.3
-//   gate/up 2048 -> 6144, 64 rows (393) 10.6 and 12.6, 96 rows (786) 19.9 and 12.6
-// One tile of 16 rows stays there whatever the columns: 2048 -> 151936 of 1 row
-// 31 and 50 us, of 16 rows 42 and 49.
-static bool few_rows(bool dual, const MxMatmulArgs &a) {
-  if (a.M <= 16) return true;
-  const int64_t tile = dual && a.M > 32 ? 64 : 16, rows = (a.M + tile - 1) / tile * tile;
-  return rows * a.K < (7 << 16) + (1 << 28) / std::max(a.N, 512);
-}
-
+// Few rows: mx_gemv.hip, while its time as fitted (mx_gemv_time) is the least;
+// that of tiles goes with the steps along a row alone until they fill the GPU.
+// In us there and on tiles: 2048 -> 5120, 64 rows 7.6 and 10.8, 96 rows 8.0 and
+// 11.3, 128 rows 9.8 and 12.0, 192 rows 12.7 and 12.5; 4096 -> 4096, 192 rows 15.5
+// and 17; gate/up 2048 -> 6144, 64 rows 10.5 and 12.6, 80 rows 15.2 and 12.6.  16
+// rows stay there whatever the columns, where reading the weights is all:
+// 2048 -> 151936 of 1 row 31 and 50 us, of 16 rows 42 and 49.
+//
 // Many rows: the tiles whose rounds over the CUs cost least.  A step of the
 // larger ones costs less for its outputs, but they leave more CUs idle.  Their
 // costs, in steps of 256 x 256 at 20 (0.9 us each): E4M3 activations 13 and 9,
@@ -49,14 +38,22 @@ static bool few_rows(bool dual, const MxMatmulArgs &a) {
 //                  4096 rows   82     -    94.7  134
 static hipError_t launch_mx_product(int format, bool dual, int out_format, const MxMatmulArgs &a,
                                     hipStream_t st) {
-  if (few_rows(dual, a)) return launch_mx_gemv(format, dual, out_format, a, st);
   const bool fp4 = format == NVM_MX_FP4;
   const int64_t columns = (int64_t)a.K * (dual ? 2 : 1), cus = cu_count() / 8 * 8;
   auto tiles = [&](int bn, int bm) { return (columns + bn - 1) / bn * ((a.M + bm - 1) / bm); };
   auto rounds = [&](int64_t n) { return (n + cus - 1) / cus; };
   const int64_t wide_round = fp4 ? 11 : 13, small_round = fp4 ? 8 : 9;
-  const int64_t wide = rounds(tiles(256, 128)) * wide_round;
-  const int64_t small = rounds(tiles(128, 128)) * small_round;
+  const int64_t wide_rounds = rounds(tiles(256, 128)), small_rounds = rounds(tiles(128, 128));
+  // (Fitted likewise, for rows of 2048 values.  Where a few rows' tiles read many
+  // weights they take longer than that, and blocks of a second round less: a
+  // tenth in favour of the former.)
+  const double n2048 = a.N / 2048.0;
+  const double wide_time = (fp4 ? 5.0 : 7.0) + (fp4 ? 6.4 : 9.0) * wide_rounds * n2048;
+  const double small_time = (fp4 ? 5.0 : 5.5) + (fp4 ? 4.1 : 5.9) * small_rounds * n2048;
+  int tile = 0;
+  if (mx_gemv_time(format, dual, a, &tile) <= 1.1 * std::min(wide_time, small_time) || a.M <= 16)
+    return launch_mx_gemv(format, tile, dual, out_format, a, st);
+  const int64_t wide = wide_rounds * wide_round, small = small_rounds * small_round;
   const int64_t n = tiles(256, 256), rest = n % cus;
   const int parts = n < cus || rest == 0 || 2 * rest > cus ? 0 : 4 * rest > cus ? 2 : 4;
   const int64_t big = parts ? n / cus * 20 + (parts == 4 ? small_round : wide_round)

@@ -383,7 +383,10 @@ def test_linear_writes_its_rows_only():
 TILED = [(400, 32, 1000), (450, 640, 901), (521, 1184, 768), (1030, 96, 4000), (1030, 640, 4003),
          (2600, 160, 8200), (1030, 512, 8200), (1030, 672, 8193), (3900, 32, 8104), (3900, 160, 8100),
          (1000, 32, 1200), (1100, 96, 1001), (1000, 544, 1250), (700, 1056, 1600), (513, 512, 2500),
-         (1100, 160, 15200), (1100, 544, 15301), (2600, 672, 8200)]
+         (1100, 160, 15200), (1100, 544, 15301), (2600, 672, 8200),
+         # few rows: blocks of 2 x 1 tiles of 16, 4 x 1, 2 x 2, 2 x 3, 4 x 2 and 4 x 3
+         (16, 2080, 4201), (11, 2080, 9001), (30, 2080, 4200), (48, 2592, 8003), (60, 2080, 8100),
+         (90, 2080, 8100), (33, 992, 8008)]
 
 
 @pytest.mark.parametrize("M,N,K", TILED)
@@ -408,7 +411,8 @@ def test_linear_on_tiles(M, N, K, fmt):
 
 @pytest.mark.parametrize("M,N,K", [(450, 160, 900), (450, 608, 900), (1030, 160, 4000),
                                    (1030, 160, 8200), (1030, 608, 8200), (1000, 160, 1200),
-                                   (1000, 608, 1201), (1100, 160, 15201)])
+                                   (1000, 608, 1201), (1100, 160, 15201), (48, 992, 8003),
+                                   (60, 992, 8100), (90, 992, 8100), (30, 1024, 4199)])
 @pytest.mark.parametrize("fmt", FMTS)
 def test_tiles_read_and_write_their_rows_only(M, N, K, fmt):
     """What lies behind a row and behind the last one: NaN scales and codes in
@@ -471,7 +475,9 @@ def test_swiglu(M, N, K, fmt, ofmt):
 @pytest.mark.parametrize("M,N,K", [(300, 160, 800), (401, 640, 544), (1030, 160, 2016),
                                    (2600, 96, 4128), (1030, 640, 4128), (3900, 96, 4064),
                                    (1000, 96, 1216), (1000, 544, 1056), (650, 640, 1600),
-                                   (1100, 160, 7616), (2600, 672, 4128)])
+                                   (1100, 160, 7616), (2600, 672, 4128),
+                                   (30, 2080, 6144), (48, 2080, 6144), (60, 2080, 6144),
+                                   (33, 992, 6080), (64, 2592, 768)])
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("ofmt", FMTS)
 def test_swiglu_on_tiles(M, N, K, fmt, ofmt):
