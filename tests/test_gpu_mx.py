@@ -568,6 +568,24 @@ def test_on_another_stream_and_in_a_replayed_graph():
         assert all(torch.equal(a, b) for a, b in zip(_bits(out), eager))
 
 
+def test_calls_on_two_streams_at_once():
+    """Nothing is shared between calls: on two streams, with no wait between
+    them, each gives what it gives alone."""
+    shapes = [(6, 512, 768), (48, 2080, 1536), (700, 512, 1024), (1030, 320, 4128)]
+    layers = [_layer(_gen(T), H=H, I=I, T=T) for T, H, I in shapes]
+    want = [_bits(_mlp(*ops)) for ops in layers]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(4):
+        for i, ops in enumerate(layers):
+            with torch.cuda.stream(streams[(i + turn) % 2]):
+                got.append((i, _mlp(*ops)))
+    torch.cuda.synchronize()
+    for i, out in got:
+        assert all(torch.equal(a, b) for a, b in zip(_bits(out), want[i]))
+
+
 # ---------------------------------------------------------------- large tensors
 
 
