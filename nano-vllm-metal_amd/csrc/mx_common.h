@@ -124,15 +124,15 @@ struct MxMatmulArgs {
 };
 // The products for few rows (mx_gemv.hip, with the block's `tile` that
 // mx_gemv_time names: the one of the least time, which it returns in us), for some
-// (mx_gemm_pipe.hip: tiles of 128 outputs by 128 rows, `wide` 256 by 128) and for
-// many (mx_gemm.hip: 256 by 256, those past whole rounds in `parts`: 0, 2 or 4, a
-// part a block).  hipErrorInvalidConfiguration: more blocks than a launch
-// has, more than kMxMaxTiles output tiles.
+// (mx_gemm_pipe.hip, in tiles of bn outputs by bm rows) and for many (mx_gemm.hip:
+// 256 by 256, those past whole rounds in `parts`: 0, 2 or 4, a part a block).
+// hipErrorInvalidConfiguration: more blocks than a launch has, more than
+// kMxMaxTiles output tiles.
 constexpr int64_t kMxMaxTiles = 1 << 22;
 double mx_gemv_time(int format, bool dual, const MxMatmulArgs &a, int *tile);
 hipError_t launch_mx_gemv(int format, int tile, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st);
-hipError_t launch_mx_gemm_pipe(int format, bool wide, bool dual, int out_format,
+hipError_t launch_mx_gemm_pipe(int format, int bn, int bm, bool dual, int out_format,
                                const MxMatmulArgs &a, hipStream_t st);
 hipError_t launch_mx_gemm(int format, int parts, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st);

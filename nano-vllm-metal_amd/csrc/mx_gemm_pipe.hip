@@ -35,26 +35,30 @@ hipError_t go(const MxMatmulArgs &a, hipStream_t st) {
   return hipGetLastError();
 }
 
+// (mx_product.hip chooses; 64 x 64 has no room for two matrices' scale pieces)
 template <int FMT, int OFMT, bool DUAL>
-hipError_t launch_tile(bool wide, const MxMatmulArgs &a, hipStream_t st) {
-  return wide ? go<FMT, OFMT, MxWideTile<FMT, DUAL>>(a, st)
-              : go<FMT, OFMT, MxSmallTile<FMT, DUAL>>(a, st);
+hipError_t launch_tile(int bn, int bm, const MxMatmulArgs &a, hipStream_t st) {
+  if (bn == 256) return go<FMT, OFMT, MxWideTile<FMT, DUAL>>(a, st);
+  if (bm == 128) return go<FMT, OFMT, MxSmallTile<FMT, DUAL>>(a, st);
+  if constexpr (!DUAL)
+    if (bn == 64) return go<FMT, OFMT, MxTile<FMT, DUAL, 64, 64, 2, 2, 2, 3, 2>>(a, st);
+  return go<FMT, OFMT, MxTile<FMT, DUAL, 128, 64, 2, 2, 2, 3, 2>>(a, st);
 }
 
 template <int FMT>
-hipError_t launch_fmt(bool wide, bool dual, int out_format, const MxMatmulArgs &a,
+hipError_t launch_fmt(int bn, int bm, bool dual, int out_format, const MxMatmulArgs &a,
                       hipStream_t st) {
-  if (!dual) return launch_tile<FMT, NVM_MX_FP8, false>(wide, a, st);
-  return out_format == NVM_MX_FP4 ? launch_tile<FMT, NVM_MX_FP4, true>(wide, a, st)
-                                  : launch_tile<FMT, NVM_MX_FP8, true>(wide, a, st);
+  if (!dual) return launch_tile<FMT, NVM_MX_FP8, false>(bn, bm, a, st);
+  return out_format == NVM_MX_FP4 ? launch_tile<FMT, NVM_MX_FP4, true>(bn, bm, a, st)
+                                  : launch_tile<FMT, NVM_MX_FP8, true>(bn, bm, a, st);
 }
 
 }  // namespace
 
-hipError_t launch_mx_gemm_pipe(int format, bool wide, bool dual, int out_format,
+hipError_t launch_mx_gemm_pipe(int format, int bn, int bm, bool dual, int out_format,
                                const MxMatmulArgs &a, hipStream_t st) {
-  return format == NVM_MX_FP4 ? launch_fmt<NVM_MX_FP4>(wide, dual, out_format, a, st)
-                              : launch_fmt<NVM_MX_FP8>(wide, dual, out_format, a, st);
+  return format == NVM_MX_FP4 ? launch_fmt<NVM_MX_FP4>(bn, bm, dual, out_format, a, st)
+                              : launch_fmt<NVM_MX_FP8>(bn, bm, dual, out_format, a, st);
 }
 
 }  // namespace nvm

@@ -188,11 +188,13 @@ hipError_t go(const MxMatmulArgs &a, hipStream_t st) {
 // Tiles of a block, and the time of a launch of such blocks: `fixed` + `round` x
 // rounds over the CUs x N / 2048 microseconds, for E2M1 and E4M3 activations
 // (least squares over 390 products of 17 to 512 rows; the residual is 3 to 9 %).
-// Larger blocks read the activations, and a column of them the weights, less
-// often, but a round of them is longer: 4096 -> 4096 of 128 rows 12.4 us on 256
-// blocks of 4 x 2 tiles, 15.3 on 192 of 4 x 3, 15.7 on 512 of 2 x 2, 18.8 on 688
-// of 3 x 2; 2048 -> 2048 of 32 rows 3.7 on 256 of 1 x 1, 4.4 on 128 of 2 x 1, 5.7
-// on 64 of 2 x 2.
+// A round after the first takes kLeastRound, however short the rows (32 -> 2048 of
+// 2048 rows, 11 rounds of 3 x 2 tiles: 17.3 us).  Larger blocks read the
+// activations, and a column of them the weights, less often, but a round of them
+// is longer: 4096 -> 4096 of 128 rows 12.4 us on 256 blocks of 4 x 2 tiles, 15.3
+// on 192 of 4 x 3, 15.7 on 512 of 2 x 2, 18.8 on 688 of 3 x 2; 2048 -> 2048 of 32
+// rows 3.7 on 256 of 1 x 1, 4.4 on 128 of 2 x 1, 5.7 on 64 of 2 x 2.
+constexpr double kLeastRound = 1.8;
 struct Blocks {
   int rt, mt;
   double fixed[2], round[2];  // by nvm_mx_format
@@ -207,7 +209,7 @@ constexpr Blocks kLinear[] = {
 constexpr Blocks kSwiglu[] = {{4, 1, {2.6, 2.5}, {2.9, 3.3}},
                               {4, 2, {2.8, 3}, {3.5, 4.3}},
                               {4, 3, {3.2, 2.9}, {3.8, 5.6}},
-                              {4, 4, {3.2, 3.4}, {4.7, 6.2}}};
+                              {4, 4, {3.2, 3.4}, {4.7, 6.8}}};
 
 template <int FMT, int OFMT, bool DUAL, int I>
 hipError_t launch_tile(int tile, const MxMatmulArgs &a, hipStream_t st) {
@@ -234,7 +236,8 @@ double best_of(const Blocks (&blocks)[N], int format, bool dual, const MxMatmulA
     const Blocks &b = blocks[i];
     const int64_t columns = 16 * (dual ? b.rt / 2 : b.rt), rows = 16 * b.mt;
     const int64_t n = (a.K + columns - 1) / columns * ((a.M + rows - 1) / rows);
-    const double t = b.fixed[format] + b.round[format] * ((n + cus - 1) / cus) * (a.N / 2048.0);
+    const double round = b.round[format] * (a.N / 2048.0);
+    const double t = b.fixed[format] + round + ((n - 1) / cus) * fmax(round, kLeastRound);
     if (t < best) {
       best = t;
       *tile = i;

@@ -1,65 +1,79 @@
 // Products of MX rows with MXFP4 weights: which kernel, and the entry points
 // (include/nvm_mx.h).
-#include <algorithm>
-
 #include "internal.h"
 #include "mx_common.h"
 
 namespace nvm {
 
-// Few rows: mx_gemv.hip, while its time as fitted (mx_gemv_time) is the least;
-// that of tiles goes with the steps along a row alone until they fill the GPU.
-// In us there and on tiles: 2048 -> 5120, 64 rows 7.6 and 10.8, 96 rows 8.0 and
-// 11.3, 128 rows 9.8 and 12.0, 192 rows 12.7 and 12.5; 4096 -> 4096, 192 rows 15.5
-// and 17; gate/up 2048 -> 6144, 64 rows 10.5 and 12.6, 80 rows 15.2 and 12.6.  16
-// rows stay there whatever the columns, where reading the weights is all:
-// 2048 -> 151936 of 1 row 31 and 50 us, of 16 rows 42 and 49.
-//
-// Many rows: the tiles whose rounds over the CUs cost least.  A step of the
-// larger ones costs less for its outputs, but they leave more CUs idle.  Their
-// costs, in steps of 256 x 256 at 20 (0.9 us each): E4M3 activations 13 and 9,
-// E2M1 11 and 8 for 256 x 128 and 128 x 128.  A last round of 256 x 256 that no
-// more than a quarter (half) of the CUs would have is computed in parts of those
-// sizes.  In us on 256 x 256 in whole tiles, in parts, on 256 x 128 and 128 x 128,
-// E4M3 unless said:
-//   2048 -> 5120    512 rows   24.0   -    17.2  13.2
+// Tiles of the larger kernels (of outputs, for gate/up of both matrices', by
+// rows), and the time of a launch: `fixed` + rounds over the CUs x (`start` +
+// `row` x N / 2048) microseconds, for E2M1 and E4M3 activations (fitted; some 10 %
+// off, more where the clock falls under the load, for all alike).  A step of the
+// larger ones costs less for its outputs, but they leave more CUs idle.  In us on
+// 256 x 256 in whole tiles, in parts (below), on 256 x 128, 128 x 128, 128 x 64 and
+// 64 x 64, E4M3 unless said:
+//   2048 -> 2048    512 rows    -     -     -    12.2   9.1   7.9
+//                  1024 rows    -     -     -    12.7  10.0  11.2
+//   2048 -> 5120    256 rows    -     -     -    12.4   9.4  10.3
+//                   512 rows   24.0   -    17.2  13.2  16.6  15.4
 //                  1536 rows   26.3   -    21.0  24.8
 //                  2048 rows   27.0   -    30.3  35.2
-//                  4096 rows   48.9  44.4  47.0  59.0  (E2M1 42.0  35.8  35.7  46.3)
-//                  8192 rows   77.3  73.1  78.7   -    (E2M1 67.1  61.7  61.8)
-//   6144 -> 2048   1024 rows   54     -    34    24
+//                  4096 rows   48.9  44.4  47.0  59.0        (E2M1 42.0  35.8  35.7  46.3)
+//                  8192 rows   77.3  73.1  78.7   -          (E2M1 67.1  61.7  61.8)
+//   6144 -> 2048    512 rows    -     -     -    22.9  16.5  14.1
+//                  1024 rows   54     -    34    23.9  20.2  23.2
 //                  4096 rows   57     -    45.5  54
 //   4096 -> 6144   3000 rows   82.2  66.4  78.2   -
-//   8192 -> 8192   8192 rows   367    -    424   553   (E2M1  293   -   350   420)
+//   8192 -> 8192   8192 rows   367    -    424   553         (E2M1  293   -   350   420)
 //   gate/up 2048 -> 6144
-//                   100 rows   24.0   -    16.8  12.6
+//                   128 rows   24.0   -    16.8  13.0   9.7
+//                   256 rows    -     -     -    13.6  16.8
 //                  1000 rows   27.7   -    31.7  35.9
 //                  1500 rows   50.5  40.4  46.0   -
 //                  4096 rows   82     -    94.7  134
+struct Tiles {
+  int bn, bm;
+  double fixed[2], start[2], row[2];  // by nvm_mx_format
+  double round(int format, int N) const { return start[format] + row[format] * (N / 2048.0); }
+};
+constexpr Tiles kBig = {256, 256, {3.0, 3.0}, {4.5, 7.5}, {14.0, 15.5}};
+constexpr Tiles kTiles[] = {{256, 128, {2.5, 3.5}, {4.0, 3.5}, {7.0, 9.2}},
+                            {128, 128, {1.0, 1.5}, {4.0, 4.0}, {4.1, 6.3}},
+                            {128, 64, {3.0, 2.5}, {1.8, 2.8}, {3.2, 4.3}},
+                            {64, 64, {3.5, 3.5}, {1.0, 0.9}, {2.1, 3.1}}};
+
+// The kernel of the least time.  Few rows: mx_gemv.hip (2048 -> 5120, 64 rows 7.6
+// us, on 64 x 64 tiles 6.9, 48 rows 6.1 and 6.8; gate/up 2048 -> 6144, 48 rows 9.4,
+// on 128 x 64 9.2), and 32 rows always: there reading the weights is more of the
+// time than the fit knows (2048 -> 151936 of 16 rows 42 us, on 256 x 128 49; gate/up
+// 2912 -> 14240 of 27 rows 13.2 and 17.4).
 static hipError_t launch_mx_product(int format, bool dual, int out_format, const MxMatmulArgs &a,
                                     hipStream_t st) {
-  const bool fp4 = format == NVM_MX_FP4;
   const int64_t columns = (int64_t)a.K * (dual ? 2 : 1), cus = cu_count() / 8 * 8;
-  auto tiles = [&](int bn, int bm) { return (columns + bn - 1) / bn * ((a.M + bm - 1) / bm); };
-  auto rounds = [&](int64_t n) { return (n + cus - 1) / cus; };
-  const int64_t wide_round = fp4 ? 11 : 13, small_round = fp4 ? 8 : 9;
-  const int64_t wide_rounds = rounds(tiles(256, 128)), small_rounds = rounds(tiles(128, 128));
-  // (Fitted likewise, for rows of 2048 values.  Where a few rows' tiles read many
-  // weights they take longer than that, and blocks of a second round less: a
-  // tenth in favour of the former.)
-  const double n2048 = a.N / 2048.0;
-  const double wide_time = (fp4 ? 5.0 : 7.0) + (fp4 ? 6.4 : 9.0) * wide_rounds * n2048;
-  const double small_time = (fp4 ? 5.0 : 5.5) + (fp4 ? 4.1 : 5.9) * small_rounds * n2048;
-  int tile = 0;
-  if (mx_gemv_time(format, dual, a, &tile) <= 1.1 * std::min(wide_time, small_time) || a.M <= 16)
-    return launch_mx_gemv(format, tile, dual, out_format, a, st);
-  const int64_t wide = wide_rounds * wide_round, small = small_rounds * small_round;
-  const int64_t n = tiles(256, 256), rest = n % cus;
+  auto count = [&](const Tiles &t) {
+    return (columns + t.bn - 1) / t.bn * ((a.M + t.bm - 1) / t.bm);
+  };
+  // A last round of 256 x 256 that no more than a quarter (half) of the CUs would
+  // have is computed in parts, of 128 x 128 (256 x 128), by all of them.
+  const int64_t n = count(kBig), rest = n % cus;
   const int parts = n < cus || rest == 0 || 2 * rest > cus ? 0 : 4 * rest > cus ? 2 : 4;
-  const int64_t big = parts ? n / cus * 20 + (parts == 4 ? small_round : wide_round)
-                            : rounds(n) * 20;
-  if (big <= std::min(wide, small)) return launch_mx_gemm(format, parts, dual, out_format, a, st);
-  return launch_mx_gemm_pipe(format, wide <= small, dual, out_format, a, st);
+  double least = kBig.fixed[format] +
+                 (parts ? n / cus : (n + cus - 1) / cus) * kBig.round(format, a.N) +
+                 (parts ? kTiles[parts == 4].round(format, a.N) : 0.0);
+  const Tiles *best = &kBig;
+  for (const Tiles &t : kTiles) {
+    if (dual && t.bn == 64) continue;
+    const double time = t.fixed[format] + (count(t) + cus - 1) / cus * t.round(format, a.N);
+    if (time < least) {
+      least = time;
+      best = &t;
+    }
+  }
+  int tile = 0;
+  if (mx_gemv_time(format, dual, a, &tile) <= least || a.M <= 32)
+    return launch_mx_gemv(format, tile, dual, out_format, a, st);
+  if (best == &kBig) return launch_mx_gemm(format, parts, dual, out_format, a, st);
+  return launch_mx_gemm_pipe(format, best->bn, best->bm, dual, out_format, a, st);
 }
 
 }  // namespace nvm

@@ -377,16 +377,19 @@ def test_linear_writes_its_rows_only():
             _close(out[:M], _val(a), _val(w), dt, "mxfp8")
 
 
-# Sizes at which each tile runs (on 256 CUs): of 128 x 128, of 256 x 128 (one and
-# several to a block), of 256 x 256 (one and two to a block); rows of one step,
-# of one run, of a step more than a run, and with a last step cut short.
+# Sizes at which every tile of every kernel runs (on 256 CUs), one and several to
+# a block, whole and in parts; rows of one step, of one run, of a step more than a
+# run, and with a last step cut short.
 TILED = [(400, 32, 1000), (450, 640, 901), (521, 1184, 768), (1030, 96, 4000), (1030, 640, 4003),
          (2600, 160, 8200), (1030, 512, 8200), (1030, 672, 8193), (3900, 32, 8104), (3900, 160, 8100),
          (1000, 32, 1200), (1100, 96, 1001), (1000, 544, 1250), (700, 1056, 1600), (513, 512, 2500),
          (1100, 160, 15200), (1100, 544, 15301), (2600, 672, 8200),
          # few rows: blocks of 2 x 1 tiles of 16, 4 x 1, 2 x 2, 2 x 3, 4 x 2 and 4 x 3
          (16, 2080, 4201), (11, 2080, 9001), (30, 2080, 4200), (48, 2592, 8003), (60, 2080, 8100),
-         (90, 2080, 8100), (33, 992, 8008)]
+         (90, 2080, 8100), (33, 992, 8008),
+         # 4 x 3; tiles of 64 x 64, 128 x 64, 128 x 128; two rounds of 256 x 256
+         (48, 448, 12200), (127, 1024, 6100), (256, 2080, 5121), (512, 160, 5121), (510, 544, 5120),
+         (390, 1184, 6001), (3900, 672, 8100), (96, 1184, 2720)]
 
 
 @pytest.mark.parametrize("M,N,K", TILED)
@@ -412,7 +415,8 @@ def test_linear_on_tiles(M, N, K, fmt):
 @pytest.mark.parametrize("M,N,K", [(450, 160, 900), (450, 608, 900), (1030, 160, 4000),
                                    (1030, 160, 8200), (1030, 608, 8200), (1000, 160, 1200),
                                    (1000, 608, 1201), (1100, 160, 15201), (48, 992, 8003),
-                                   (60, 992, 8100), (90, 992, 8100), (30, 1024, 4199)])
+                                   (60, 992, 8100), (90, 992, 8100), (30, 1024, 4199), (512, 160, 5121),
+                                   (510, 608, 5120), (128, 992, 6101), (127, 1024, 6100)])
 @pytest.mark.parametrize("fmt", FMTS)
 def test_tiles_read_and_write_their_rows_only(M, N, K, fmt):
     """What lies behind a row and behind the last one: NaN scales and codes in
@@ -477,7 +481,9 @@ def test_swiglu(M, N, K, fmt, ofmt):
                                    (1000, 96, 1216), (1000, 544, 1056), (650, 640, 1600),
                                    (1100, 160, 7616), (2600, 672, 4128),
                                    (30, 2080, 6144), (48, 2080, 6144), (60, 2080, 6144),
-                                   (33, 992, 6080), (64, 2592, 768)])
+                                   (33, 992, 6080), (64, 2592, 768), (60, 992, 6080),
+                                   (130, 2080, 4096), (100, 2592, 4064), (3900, 672, 4064),
+                                   (1100, 672, 7616)])
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("ofmt", FMTS)
 def test_swiglu_on_tiles(M, N, K, fmt, ofmt):
