@@ -7,7 +7,9 @@
 // Bound: the loads into LDS.  128 x 128 with KG = 2 (24 stages, 6144 -> 2048 of
 // 512 rows, 23 us): 9 us without reading or multiplying, products alone 19, LDS
 // reads alone 12, loads alone 22; a deeper ring changes nothing (2 stages 29
-// us, 3 23, and of E2M1, which leaves room, 3 as fast as 4).
+// us, 3 23, and of E2M1, which leaves room, 3 as fast as 4).  So where 128 x 128
+// leaves CUs idle, smaller tiles are faster though they load more: those 512 rows
+// 16.5 us on 128 x 64, 14.1 on 64 x 64, of which two blocks fit a CU.
 //  * Every wavefront reads stage j + 1's operands from LDS into registers and
 //    requests stage j + ST while it multiplies stage j's, instruction by
 //    instruction side by side: one barrier a stage.
@@ -20,8 +22,8 @@
 //  * A last run of less than 512 values is computed with the activations behind
 //    the row replaced by zeros and scales by one in registers.
 //
-// 6144 -> 2048: 512 rows 23.0 us (0.56 PFLOP/s; 64 tiles for 256 CUs, 24 stages
-// of 0.8 us one after the other), 4096 rows 45.5 us (2.3 PFLOP/s).
+// 6144 -> 2048: 512 rows 14.1 us (0.91 PFLOP/s), 1024 rows 20.2 us on 128 x 64
+// (1.28), 4096 rows 45.5 us on 256 x 128 (2.3).
 #pragma once
 
 #include "mx_tile.h"
