@@ -23,6 +23,7 @@ MX_BLOCK = 32
 MX_FORMATS = {"mxfp4": 0, "mxfp8": 1}
 MX_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _PER_BYTE = {"mxfp4": 2, "mxfp8": 1}
+_MAX_PITCH = 1 << 20
 
 
 def _pitch(n: int) -> int:
@@ -147,13 +148,13 @@ class MxTensor:
 
 def _row_pitch(scales: torch.Tensor, n: int) -> Optional[int]:
     """Bytes between rows of scales that lie as the kernels read them: rows a
-    multiple of 16 bytes apart, evenly over all leading dimensions, and the
-    last row's padding inside the storage.  None for others."""
+    multiple of 16 bytes apart, up to ``_MAX_PITCH``, evenly over all leading
+    dimensions, and the last row's padding inside the storage.  None for others."""
     if scales.stride(-1) != 1 and scales.shape[-1] > 1 or scales.data_ptr() % 16:
         return None
     need = _pitch(n)
     pitch = scales.stride(-2) if scales.dim() > 1 and scales.shape[-2] > 1 else need
-    if pitch % 16 or pitch < need:
+    if pitch % 16 or not need <= pitch <= _MAX_PITCH:
         return None
     step = pitch
     for size, stride in zip(reversed(scales.shape[:-1]), reversed(scales.stride()[:-1])):

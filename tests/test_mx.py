@@ -157,6 +157,11 @@ def test_tensor_copies_what_the_kernels_could_not_read():
         assert torch.equal(t.scales, scales) and t.pitch % 16 == 0
         assert t.scales.data_ptr() % 16 == 0 and t.scales.stride(-1) in (1, 16)
         assert t.scales.untyped_storage().nbytes() - t.scales.storage_offset() >= 16 * t.rows
+    # rows further apart than the kernels take: copied
+    far = torch.zeros(2, (1 << 20) + 16, dtype=torch.uint8)[:, :2]
+    assert MxTensor(codes[:2], far, "mxfp8").pitch == 16
+    near = torch.zeros(2, 1 << 20, dtype=torch.uint8)[:, :2]
+    assert MxTensor(codes[:2], near, "mxfp8").pitch == 1 << 20
     # the last row's padding would lie behind the storage: copied
     tight = torch.zeros(5 * 16 + 2, dtype=torch.uint8).as_strided((6, 2), (16, 1))
     assert MxTensor(codes, tight, "mxfp8").scales.data_ptr() != tight.data_ptr()
