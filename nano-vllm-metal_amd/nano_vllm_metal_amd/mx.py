@@ -180,17 +180,17 @@ def _packed(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _launch(fn, dev: torch.device, *args) -> None:
-    """``fn(*args, stream)`` on the tensors' device, whichever is current, and
-    its current stream."""
-    index = dev.index
-    if index == torch._C._cuda_getDevice():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if status:
-        _lib.check(status)
+# (each operator: its tensors' device, whichever is current, and its stream)
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _index(a: torch.Tensor, b: torch.Tensor) -> int:
+    """The one GPU of both."""
+    index = a.get_device()
+    if index < 0 or b.get_device() != index:
+        _lib.require_device(a, b)
+    return index
 
 
 def mx_quantize(x: torch.Tensor, fmt: str = "mxfp8") -> MxTensor:
@@ -220,10 +220,14 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp8") -> MxTensor:
     if x.data_ptr() % 16:
         x, ld = x.clone(memory_format=torch.contiguous_format), n
     rows = x.numel() // n
+    index = dev.index
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return mx_quantize(x, fmt)
     out = MxTensor._empty(shape[:-1], rows, n, fmt, dev)
     codes, scales = out._pointers()
-    _launch(lib.nvm_mx_quantize, dev, x.data_ptr(), rows, n, ld, dtype, code, codes, scales,
-            out.pitch)
+    _lib.check(lib.nvm_mx_quantize(x.data_ptr(), rows, n, ld, dtype, code, codes, scales, out.pitch,
+                                   _raw_stream(index)))
     return out
 
 
@@ -234,9 +238,14 @@ def mx_dequantize(t: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tens
     code = MX_DTYPES.get(dtype)
     if code is None:
         raise ValueError(f"mx_dequantize: dtype must be float16, bfloat16 or float32, got {dtype}")
+    index = dev.index
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return mx_dequantize(t, dtype)
     out = torch.empty(t.shape, dtype=dtype, device=dev)
-    _launch(lib.nvm_mx_dequantize, dev, *t._pointers(), t.pitch, t.rows, t.shape[-1],
-            MX_FORMATS[t.fmt], code, out.data_ptr())
+    codes, scales = t._pointers()
+    _lib.check(lib.nvm_mx_dequantize(codes, scales, t.pitch, t.rows, t.shape[-1], MX_FORMATS[t.fmt],
+                                     code, out.data_ptr(), _raw_stream(index)))
     return out
 
 
@@ -247,19 +256,24 @@ def mx_embedding(tokens: torch.Tensor, table: MxTensor, dtype: torch.dtype) -> t
     lib = _lib.load()
     if type(table) is not MxTensor or len(table.shape) != 2:
         raise ValueError("mx_embedding: table must be a two-dimensional MxTensor")
-    dev = _lib.require_device(tokens, table._base)
+    index = _index(tokens, table._base)
     code = MX_DTYPES.get(dtype)
     if code is None:
         raise ValueError(f"mx_embedding: dtype must be float16, bfloat16 or float32, got {dtype}")
     if tokens.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"mx_embedding: tokens must be int32 or int64, got {tokens.dtype}")
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return mx_embedding(tokens, table, dtype)
     V, D = table.shape
     if tokens.dtype == torch.int64:  # (an id that 32 bits would wrap stays outside)
         tokens = tokens.clamp(-1, V)
     ids = tokens.reshape(-1).to(torch.int32).contiguous()
-    out = torch.empty((*tokens.shape, D), dtype=dtype, device=dev)
-    _launch(lib.nvm_mx_embedding, dev, ids.data_ptr(), ids.numel(), *table._pointers(),
-            table.pitch, V, D, MX_FORMATS[table.fmt], code, out.data_ptr())
+    out = torch.empty((*tokens.shape, D), dtype=dtype, device=ids.device)
+    codes, scales = table._pointers()
+    _lib.check(lib.nvm_mx_embedding(ids.data_ptr(), ids.numel(), codes, scales, table.pitch, V, D,
+                                    MX_FORMATS[table.fmt], code, out.data_ptr(),
+                                    _raw_stream(index)))
     return out
 
 
@@ -280,6 +294,10 @@ def residual_rms_norm_mx(h: torch.Tensor, r: Optional[torch.Tensor], weight: tor
                          f"of {MX_BLOCK}, got shape {tuple(shape)}")
     if weight.numel() != H:
         raise ValueError(f"residual_rms_norm_mx: weight must have {H} elements")
+    index = dev.index
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return residual_rms_norm_mx(h, r, weight, eps, fmt)
     hc = _packed(h)
     rc = h_out = None
     if r is not None:
@@ -291,8 +309,9 @@ def residual_rms_norm_mx(h: torch.Tensor, r: Optional[torch.Tensor], weight: tor
     rows = hc.numel() // H
     out = MxTensor._empty(shape[:-1], rows, H, fmt, dev)
     codes, scales = out._pointers()
-    _launch(lib.nvm_residual_rms_norm_mx, dev, hc.data_ptr(), _lib.ptr(rc), w.data_ptr(), rows, H,
-            float(eps), dtype, _lib.ptr(h_out), code, codes, scales, out.pitch)
+    _lib.check(lib.nvm_residual_rms_norm_mx(
+        hc.data_ptr(), _lib.ptr(rc), w.data_ptr(), rows, H, float(eps), dtype, _lib.ptr(h_out),
+        code, codes, scales, out.pitch, _raw_stream(index)))
     return (h if h_out is None else h_out), out
 
 
@@ -336,13 +355,18 @@ def mx_linear(x: Union[MxTensor, torch.Tensor], w: MxTensor,
     if code is None:
         raise ValueError(f"mx_linear: dtype must be float16, bfloat16 or float32, got {dtype}")
     _check_weight("mx_linear", "w", w, a)
+    index = _index(a._base, w._base)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return mx_linear(a, w, dtype, bias)
     K, N = w.shape
-    dev = _lib.require_device(a._base, w._base)
-    out = torch.empty((*a.shape[:-1], K), dtype=dtype, device=dev)
+    lead = a.shape
+    out = torch.empty((lead[0], K) if len(lead) == 2 else (*lead[:-1], K), dtype=dtype,
+                      device=a._base.device)
     ac, asc = a._pointers()
     wc, wsc = w._pointers()
-    _launch(lib.nvm_mx_matmul, dev, ac, asc, a.pitch, MX_FORMATS[a.fmt], wc, wsc, w.pitch, a.rows,
-            N, K, code, out.data_ptr())
+    _lib.check(lib.nvm_mx_matmul(ac, asc, a.pitch, MX_FORMATS[a.fmt], wc, wsc, w.pitch, a.rows, N,
+                                 K, code, out.data_ptr(), _raw_stream(index)))
     return out if bias is None else out + bias
 
 
@@ -361,12 +385,18 @@ def mx_swiglu(x: Union[MxTensor, torch.Tensor], w_gate: MxTensor, w_up: MxTensor
     if w_up.shape[0] != K or K == 0 or K % MX_BLOCK:
         raise ValueError(f"mx_swiglu: gate and up must have the same output features, a positive "
                          f"multiple of {MX_BLOCK}, got {K} and {w_up.shape[0]}")
-    dev = _lib.require_device(a._base, w_gate._base, w_up._base)
-    out = MxTensor._empty(a.shape[:-1], a.rows, K, fmt, dev)
+    index = _index(a._base, w_gate._base)
+    if w_up._base.get_device() != index:
+        _lib.require_device(a._base, w_up._base)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return mx_swiglu(a, w_gate, w_up, fmt)
+    out = MxTensor._empty(a.shape[:-1], a.rows, K, fmt, a._base.device)
     ac, asc = a._pointers()
     gc, gsc = w_gate._pointers()
     uc, usc = w_up._pointers()
     oc, osc = out._pointers()
-    _launch(lib.nvm_mx_swiglu, dev, ac, asc, a.pitch, MX_FORMATS[a.fmt], gc, gsc, w_gate.pitch, uc,
-            usc, w_up.pitch, a.rows, N, K, code, oc, osc, out.pitch)
+    _lib.check(lib.nvm_mx_swiglu(ac, asc, a.pitch, MX_FORMATS[a.fmt], gc, gsc, w_gate.pitch, uc,
+                                 usc, w_up.pitch, a.rows, N, K, code, oc, osc, out.pitch,
+                                 _raw_stream(index)))
     return out

@@ -592,6 +592,30 @@ def test_calls_on_two_streams_at_once():
         assert all(torch.equal(a, b) for a, b in zip(_bits(out), want[i]))
 
 
+def test_tensors_of_a_device_that_is_not_the_current_one(monkeypatch):
+    """Each operator makes its tensors' device the current one for the call (on
+    one GPU: with the current one reported as another, once a call)."""
+    from nano_vllm_metal_amd import mx, mx_dequantize, mx_embedding, mx_quantize
+
+    ops = _layer(_gen(3))
+    x, tok = ops[0], torch.tensor([3, 1], device=DEV)
+
+    def all_of_them():
+        q = mx_quantize(x)
+        return _bits(_mlp(*ops)) + [q.codes, q.scales.clone(), mx_dequantize(q),
+                                    mx_embedding(tok, ops[3], x.dtype), mx.mx_linear(x, ops[3])]
+
+    want, calls = all_of_them(), []
+
+    def current():
+        calls.append(torch.cuda.current_device())
+        return calls[-1] + len(calls) % 2  # every other call: another device
+
+    monkeypatch.setattr(mx, "_current_device", current)
+    got = all_of_them()
+    assert len(calls) == 2 * 8 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 # ---------------------------------------------------------------- large tensors
 
 
