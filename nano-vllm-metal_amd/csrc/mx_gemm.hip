@@ -2,11 +2,11 @@
 // 256 x 256 fill the GPU: long prompts through the projections and through the
 // dense MLP's gate/up pair.  (Fewer rows: mx_gemm_pipe.hip.)
 //
-// Bound: the scaled matrix instruction, 32 cycles a 16x16x128 product where an
-// operand is E4M3 and 16 where both are E2M1, so feeding it.
-//  * Nothing is unpacked: codes and scale bytes go from memory into LDS as
-//    they are (buffer loads with an LDS target) and from there into the
-//    instruction's operands.
+// Bound: the matrix instructions.  A 16x16x128 product is one scaled instruction
+// where both operands are E2M1, 16 cycles, or for short sums of E4M3, 32; E4M3
+// otherwise takes four bf16 ones, 64 cycles, and conversions beside them.
+//  * Codes and scale bytes go from memory into LDS as they are (buffer loads with
+//    an LDS target) and from there into registers.
 //  * A stage is one 128-value step of the tile: weight rows of 64 bytes and
 //    activation rows of 128 (E4M3) or 64.  Scales come 16 bytes a row, for
 //    four steps at once, into a ring of their own.
@@ -20,15 +20,15 @@
 //    steps arrive during the epilogue of the one before.
 //  * Tiles that would be a last round of at most a quarter (half) of the CUs are
 //    computed in quarters (halves) by all of them, with the code of mx_pipe.h
-//    (3000 rows of 4096 -> 6144, 288 tiles: 66.5 us with quarters, 82 without;
-//    8192 rows of 2048 -> 5120, 640 tiles: 73 with halves, 77 without).
+//    (3000 rows of 4096 -> 6144, 288 tiles: 127 us with quarters, 176 without;
+//    8192 rows of 2048 -> 5120, 640 tiles: 134 with halves, 141 without).
 //  * A last step of less than 128 values is computed with the activations
 //    behind the row replaced by zeros and scales by one in registers, so what
 //    lies there does not matter (a weight code is finite whatever its bits).
 //
-// 8192 x 8192 x 8192: 367 us, 3.0 PFLOP/s (E2M1: 293 us, 3.75); 4096 rows of
-// 2048 through a gate/up pair of 6144: 82 us, 2.5 PFLOP/s.  Left there: 768 tiles
-// of 16 steps each, whose epilogues the other half of the block hides in part.
+// 8192 x 8192 x 8192: 743 us, 1.48 PFLOP/s, the rate of a bf16 library product
+// there (1.41); E2M1 293 us, 3.75; short sums 367 us, 3.0.  4096 rows of 2048
+// through a gate/up pair of 6144: 153 us, 1.35 PFLOP/s; short sums 84 us, 2.5.
 #include "mx_pipe.h"
 
 namespace nvm {
@@ -137,9 +137,11 @@ __global__ __launch_bounds__(64 * T::NW, 2) void mx_gemm_kernel(const MxMatmulAr
     // (the matrix instruction takes a register's low byte).
     typename T::Scales sc;
     for (int s = 0;; ++s) {
-      if (s % 4 == 0) {
-        chunk = chunk + 1 == T::SL ? 0 : chunk + 1;
-        sc.read(smem, at, chunk, 0);
+      if (s % 4 == 0) chunk = chunk + 1 == T::SL ? 0 : chunk + 1;
+      if (s % 4 == 0 || FMT == NVM_MX_FP8) {
+        // (bf16 operands leave no registers to keep a run's scales in beside
+        // them: a step reads them again)
+        sc.read(smem, at, chunk, FMT == NVM_MX_FP8 ? s % 4 : 0);
       } else {
 #pragma unroll
         for (int f = 0; f < T::TF; ++f) sc.w[f] >>= 8;
@@ -174,7 +176,7 @@ __global__ __launch_bounds__(64 * T::NW, 2) void mx_gemm_kernel(const MxMatmulAr
         for (int t = 0; t < T::TM; ++t) {
 #pragma unroll
           for (int c = 0; c < NX; ++c)
-            if (128 * s + (FMT == NVM_MX_FP4 ? 32 * G : 64 * c + 16 * G) >= p.N)
+            if (128 * s + mx_act_at<FMT>(G, c) >= p.N)
               x[t].v[c] = u32x4{0u, 0u, 0u, 0u};
           if (4 * s + G >= nb) sc.x[t] = 127u;
         }
@@ -191,12 +193,9 @@ __global__ __launch_bounds__(64 * T::NW, 2) void mx_gemm_kernel(const MxMatmulAr
       asm volatile("" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-      for (int f = 0; f < T::TF; ++f) {
-#pragma unroll
-        for (int t = 0; t < T::TM; ++t)
-          acc[f][t] = mx_mfma<FMT>(w[f], sc.w[f], x[t], sc.x[t], acc[f][t]);
-      }
+      mx_products<FMT, 0>(w, sc.w, x, sc.x, acc, [](int) {
+        if constexpr (FMT == NVM_MX_FP8) __builtin_amdgcn_sched_barrier(0);
+      });
       __builtin_amdgcn_s_setprio(0);
       __builtin_amdgcn_sched_barrier(0);
       slot = slot + 1 == T::ST ? 0 : slot + 1;
@@ -271,8 +270,9 @@ hipError_t launch_fmt(int parts, bool dual, int out_format, const MxMatmulArgs &
 
 hipError_t launch_mx_gemm(int format, int parts, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st) {
-  return format == NVM_MX_FP4 ? launch_fmt<NVM_MX_FP4>(parts, dual, out_format, a, st)
-                              : launch_fmt<NVM_MX_FP8>(parts, dual, out_format, a, st);
+  return format == NVM_MX_FP4   ? launch_fmt<NVM_MX_FP4>(parts, dual, out_format, a, st)
+         : format == NVM_MX_FP8 ? launch_fmt<NVM_MX_FP8>(parts, dual, out_format, a, st)
+                                : launch_fmt<kMxShort>(parts, dual, out_format, a, st);
 }
 
 }  // namespace nvm

@@ -57,8 +57,9 @@ hipError_t launch_fmt(int bn, int bm, bool dual, int out_format, const MxMatmulA
 
 hipError_t launch_mx_gemm_pipe(int format, int bn, int bm, bool dual, int out_format,
                                const MxMatmulArgs &a, hipStream_t st) {
-  return format == NVM_MX_FP4 ? launch_fmt<NVM_MX_FP4>(bn, bm, dual, out_format, a, st)
-                              : launch_fmt<NVM_MX_FP8>(bn, bm, dual, out_format, a, st);
+  return format == NVM_MX_FP4   ? launch_fmt<NVM_MX_FP4>(bn, bm, dual, out_format, a, st)
+         : format == NVM_MX_FP8 ? launch_fmt<NVM_MX_FP8>(bn, bm, dual, out_format, a, st)
+                                : launch_fmt<kMxShort>(bn, bm, dual, out_format, a, st);
 }
 
 }  // namespace nvm

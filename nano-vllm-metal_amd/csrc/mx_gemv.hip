@@ -2,8 +2,10 @@
 // batches of the projections and of the dense MLP's gate/up pair.
 //
 // Bound: latency, then the weight stream (a projection's 5 to 7 MB are 1 to
-// 1.4 us of HBM time).  The scaled matrix instruction takes the codes as they
-// lie in memory, so a wavefront is loads, matrix instructions and one sum:
+// 1.4 us of HBM time).  Codes go from memory into registers and from there, E2M1
+// as it is, E4M3 by way of bf16 (mx_common.h), into matrix instructions, so a
+// wavefront is loads, products and one sum (E4M3, 2048 -> 5120: one row 4.1 us, 8
+// rows 4.4; in short sums 3.6 and 3.9):
 //  * a block owns RT 16-row tiles of the weights and MT 16-row tiles of the
 //    activations; its four wavefronts take runs of four 128-value steps in
 //    turn, and each requests a whole run (scales, weights, activations) before
@@ -12,11 +14,11 @@
 //    compiler's own order instead of row by row, cost 2048 -> 151936 of one row
 //    12 of 44 us), and only the last run is compared with the row's end.  Eight
 //    wavefronts, or runs of two steps, or a run requested ahead, were slower
-//    nearly everywhere (2048 -> 5120 of 8 rows 4.0, 4.1 and 4.1 us for 3.9);
-//  * operands go from memory straight into the instruction's registers: a
-//    lane's 16 bytes of a weight row are its 32 values of a step, a row's 16
-//    scale bytes are the run's, and the activations are few enough to come
-//    from L2;
+//    nearly everywhere (short sums, 2048 -> 5120 of 8 rows: 4.0, 4.1 and 4.1 us for
+//    3.9);
+//  * operands go from memory straight into registers: a lane's 16 bytes of a
+//    weight row are its 32 values of a step, a row's 16 scale bytes are the run's,
+//    and the activations are few enough to come from L2;
 //  * the wavefronts' sums meet in LDS once and are added in order.
 // Weights are the row operand, so a lane ends up with four neighbouring
 // outputs of one activation row, and a block of 32 outputs (SwiGLU's MX
@@ -70,7 +72,7 @@ __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxMatmulArgs p) 
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     const int r = 16 * t + col;
-    xo[t] = r < nm ? r * XB + 16 * G : kMaskedOffset;
+    xo[t] = r < nm ? r * XB + (FMT == NVM_MX_FP4 ? 16 * G : mx_act_at<FMT>(G, 0)) : kMaskedOffset;
     xso[t] = r < nm ? r * (int)p.as_ld : kMaskedOffset;
   }
 
@@ -102,11 +104,10 @@ __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxMatmulArgs p) 
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int c = 0; c < NX; ++c)
-          // (FP4: the lane's 32 values; FP8: 16 at 16 G, 16 at 64 + 16 G)
           q.x[j][t].v[c] =
-              FMT == NVM_MX_FP4
-                  ? bload16(xr, at(xo[t], 128 * j + 32 * G), 256 * r + 64 * j)
-                  : bload16(xr, at(xo[t], 128 * j + 64 * c + 16 * G), 512 * r + 128 * j + 64 * c);
+              bload16(xr, at(xo[t], 128 * j + mx_act_at<FMT>(G, c)),
+                      FMT == NVM_MX_FP4 ? 256 * r + 64 * j
+                                        : 512 * r + 128 * j + mx_act_at<FMT>(0, c));
     __builtin_amdgcn_sched_barrier(0);
   };
   f32x4 acc[RT][MT];
@@ -121,16 +122,12 @@ __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxMatmulArgs p) 
     for (int j = 0; j < 4; ++j) {
       // (behind a row: the scale of one, whatever lies there)
       const bool in = !decltype(TAIL)::value || 16 * r + 4 * j + G < nb;
-      uint32_t xs[MT];
+      uint32_t xs[MT], ws[RT];
 #pragma unroll
       for (int t = 0; t < MT; ++t) xs[t] = in ? q.xs[t][j] >> (8 * G) : 127u;
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        const uint32_t ws = in ? q.ws[i][j] >> (8 * G) : 127u;
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-          acc[i][t] = mx_mfma<FMT>(q.w[j][i], ws, q.x[j][t], xs[t], acc[i][t]);
-      }
+      for (int i = 0; i < RT; ++i) ws[i] = in ? q.ws[i][j] >> (8 * G) : 127u;
+      mx_products<FMT, 0>(q.w[j], ws, q.x[j], xs, acc, [](int) {});
     }
   };
   const int full = p.N / 512;
@@ -186,30 +183,32 @@ hipError_t go(const MxMatmulArgs &a, hipStream_t st) {
 }
 
 // Tiles of a block, and the time of a launch of such blocks: `fixed` + `round` x
-// rounds over the CUs x N / 2048 microseconds, for E2M1 and E4M3 activations
-// (least squares over 390 products of 17 to 512 rows; the residual is 3 to 9 %).
-// A round after the first takes kLeastRound, however short the rows (32 -> 2048 of
-// 2048 rows, 11 rounds of 3 x 2 tiles: 17.3 us).  Larger blocks read the
-// activations, and a column of them the weights, less often, but a round of them
-// is longer: 4096 -> 4096 of 128 rows 12.4 us on 256 blocks of 4 x 2 tiles, 15.3
-// on 192 of 4 x 3, 15.7 on 512 of 2 x 2, 18.8 on 688 of 3 x 2; 2048 -> 2048 of 32
-// rows 3.7 on 256 of 1 x 1, 4.4 on 128 of 2 x 1, 5.7 on 64 of 2 x 2.
+// rounds over the CUs x N / 2048 microseconds, for E2M1 activations, E4M3, and E4M3
+// in short sums (least squares over some hundred products of 16 to 512 rows each;
+// the residual is 3 to 9 %, for 1 x 1 tiles of E4M3 14).  A round after the first
+// takes kLeastRound, however short the rows (in short sums 32 -> 2048 of 2048 rows,
+// 11 rounds of 3 x 2 tiles: 17.3 us).  Larger blocks read the activations, and a
+// column of them the weights, less often, but a round of them is longer: 4096 ->
+// 4096 of 128 rows 14.3 us on 256 blocks of 4 x 2 tiles, 16.9 on 192 of 4 x 3, 16.5
+// on 512 of 2 x 2, 20.1 on 1024 of 2 x 1; 2048 -> 2048 of 32 rows 4.2 on 256 of 1 x
+// 1, 4.7 on 128 of 2 x 1, 6.5 on 64 of 2 x 2.
 constexpr double kLeastRound = 1.8;
 struct Blocks {
   int rt, mt;
-  double fixed[2], round[2];  // by nvm_mx_format
+  double fixed[3], round[3];  // by the activations: an nvm_mx_format or kMxShort
 };
 constexpr Blocks kLinear[] = {
-    {1, 1, {2, 2.2}, {1.15, 1.5}}, {2, 1, {2.1, 2.3}, {1.8, 2.05}}, {4, 1, {2.3, 2.6}, {3, 3.25}},
-    {2, 2, {2.4, 2.6}, {2.4, 3.3}}, {2, 3, {2.7, 2.7}, {2.9, 4.5}}, {4, 2, {3, 3.3}, {3.6, 4.5}},
-    {4, 3, {3.5, 3.6}, {4.1, 6}}};
+    {1, 1, {2, 1.9, 2.2}, {1.15, 1.8, 1.5}}, {2, 1, {2.1, 2.6, 2.3}, {1.8, 2.2, 2.05}},
+    {4, 1, {2.3, 3.5, 2.6}, {3, 3.2, 3.25}}, {2, 2, {2.4, 3.4, 2.6}, {2.4, 3.1, 3.3}},
+    {2, 3, {2.7, 3.9, 2.7}, {2.9, 3.6, 4.5}}, {4, 2, {3, 4.6, 3.3}, {3.6, 4.3, 4.5}},
+    {4, 3, {3.5, 5.3, 3.6}, {4.1, 5, 6}}};
 // (SwiGLU: 32 outputs a block, which its scale needs: two tiles of each matrix.
-// 2048 -> 6144 of 8 rows 6.2 us; of 32 rows 8.1 on 192 blocks of 2 tiles of
-// rows, 10.2 on 384 of 1; 2048 -> 768 of 64 rows 5.8 on 96 of 1, 10.5 on 24 of 4)
-constexpr Blocks kSwiglu[] = {{4, 1, {2.6, 2.5}, {2.9, 3.3}},
-                              {4, 2, {2.8, 3}, {3.5, 4.3}},
-                              {4, 3, {3.2, 2.9}, {3.8, 5.6}},
-                              {4, 4, {3.2, 3.4}, {4.7, 6.8}}};
+// 2048 -> 6144 of 32 rows 9.3 us on 192 blocks of 2 tiles of rows, 10.4 on 384 of
+// 1; 2048 -> 768 of 64 rows 6.5 on 96 of 1, 11.6 on 24 of 4)
+constexpr Blocks kSwiglu[] = {{4, 1, {2.6, 2.9, 2.5}, {2.9, 3.6, 3.3}},
+                              {4, 2, {2.8, 3.6, 3}, {3.5, 4.9, 4.3}},
+                              {4, 3, {3.2, 2.7, 2.9}, {3.8, 7, 5.6}},
+                              {4, 4, {3.2, 3, 3.4}, {4.7, 7.8, 6.8}}};
 
 template <int FMT, int OFMT, bool DUAL, int I>
 hipError_t launch_tile(int tile, const MxMatmulArgs &a, hipStream_t st) {
@@ -254,8 +253,9 @@ double mx_gemv_time(int format, bool dual, const MxMatmulArgs &a, int *tile) {
 
 hipError_t launch_mx_gemv(int format, int tile, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st) {
-  return format == NVM_MX_FP4 ? launch_fmt<NVM_MX_FP4>(tile, dual, out_format, a, st)
-                              : launch_fmt<NVM_MX_FP8>(tile, dual, out_format, a, st);
+  return format == NVM_MX_FP4   ? launch_fmt<NVM_MX_FP4>(tile, dual, out_format, a, st)
+         : format == NVM_MX_FP8 ? launch_fmt<NVM_MX_FP8>(tile, dual, out_format, a, st)
+                                : launch_fmt<kMxShort>(tile, dual, out_format, a, st);
 }
 
 }  // namespace nvm

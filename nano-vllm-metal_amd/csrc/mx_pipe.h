@@ -1,10 +1,12 @@
 // Products of MX rows with MXFP4 weights (include/nvm_mx.h) between decode
 // batches (mx_gemv.hip) and grids that tiles of 256 x 256 fill (mx_gemm.hip):
 // prompts of some hundred rows.  Codes and scales go through LDS into the
-// scaled matrix instruction as they do there; the tiles are smaller, so that
-// there are enough of them, and time goes by stages.
+// matrix instructions as they do there; the tiles are smaller, so that there are
+// enough of them, and time goes by stages.
 //
-// Bound: the loads into LDS.  128 x 128 with KG = 2 (24 stages, 6144 -> 2048 of
+// Bound: of E4M3 the bf16 products (256 x 128, a round of 16 stages in 25 us: 1.4
+// PFLOP/s, the library's rate).  Of E2M1, and in short sums, of which the figures
+// to come are, the loads into LDS.  128 x 128 with KG = 2 (24 stages, 6144 -> 2048 of
 // 512 rows, 23 us): 9 us without reading or multiplying, products alone 19, LDS
 // reads alone 12, loads alone 22; a deeper ring changes nothing (2 stages 29
 // us, 3 23, and of E2M1, which leaves room, 3 as fast as 4).  So where 128 x 128
@@ -13,8 +15,8 @@
 //  * Every wavefront reads stage j + 1's operands from LDS into registers and
 //    requests stage j + ST while it multiplies stage j's, instruction by
 //    instruction side by side: one barrier a stage.
-//  * A run of four steps is unrolled, because the matrix instruction takes the
-//    scale byte of a step as an immediate.  Its scales are requested two runs
+//  * A run of four steps is unrolled, because the scaled matrix instruction takes
+//    the scale byte of a step as an immediate.  Its scales are requested two runs
 //    ahead, turned (MxTile::turn) one ahead, read at the end of the run before.
 //  * KG = 2: rows are loaded 128 bytes at a time, and few tiles still have
 //    eight wavefronts, each with a 64 x 64 piece of the tile to multiply.
@@ -22,8 +24,8 @@
 //  * A last run of less than 512 values is computed with the activations behind
 //    the row replaced by zeros and scales by one in registers.
 //
-// 6144 -> 2048: 512 rows 14.1 us (0.91 PFLOP/s), 1024 rows 20.2 us on 128 x 64
-// (1.28), 4096 rows 45.5 us on 256 x 128 (2.3).
+// 6144 -> 2048: 512 rows 20.7 us (0.62 PFLOP/s), 1024 rows 30.2 us on 128 x 64
+// (0.85), 4096 rows 79.8 us on 256 x 128 (1.29); in short sums 14.1, 20.2 and 45.5.
 #pragma once
 
 #include "mx_tile.h"
@@ -165,7 +167,7 @@ __device__ __forceinline__ void mx_pipe_tiles(const MxMatmulArgs &p, uint8_t *sm
         for (int t = 0; t < T::TM; ++t)
 #pragma unroll
           for (int c = 0; c < NX; ++c)
-            if (128 * step + (FMT == NVM_MX_FP4 ? 32 * G : 64 * c + 16 * G) >= p.N)
+            if (128 * step + mx_act_at<FMT>(G, c) >= p.N)
               q.x[t].v[c] = u32x4{0u, 0u, 0u, 0u};
         if constexpr (J == 0) {
           const int in = min(max((nb - 16 * r - G + 3) >> 2, 0), 4);  // steps inside
@@ -178,18 +180,16 @@ __device__ __forceinline__ void mx_pipe_tiles(const MxMatmulArgs &p, uint8_t *sm
       }
       if constexpr (J + 1 == T::RUN) sc[1].read(smem, at, chunk ^ 1, kg);
       __builtin_amdgcn_sched_barrier(0);
+      mx_products<FMT, T::KG * J>(q.w, sc[0].w, q.x, sc[0].x, acc, [&](int part) {
+        constexpr int of = mx_parts<FMT, T::TF>;
+        if (part > 0) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int f = 0; f < T::TF; ++f) {
+        for (int i = part * NR / of; i < (part + 1) * NR / of; ++i) read(n, i, from);
 #pragma unroll
-        for (int i = f * NR / T::TF; i < (f + 1) * NR / T::TF; ++i) read(n, i, from);
-#pragma unroll
-        for (int i = f * T::kLoads / T::TF; i < (f + 1) * T::kLoads / T::TF; ++i)
+        for (int i = part * T::kLoads / of; i < (part + 1) * T::kLoads / of; ++i)
           load(i, (J + T::ST) % T::RUN, to);
-#pragma unroll
-        for (int t = 0; t < T::TM; ++t)
-          acc[f][t] = mx_mfma<FMT, T::KG * J>(q.w[f], sc[0].w[f], q.x[t], sc[0].x[t], acc[f][t]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      });
+      __builtin_amdgcn_sched_barrier(0);
       // (computed here: the compiler would move products whose sums it needs
       // later only past the next barrier)
 #pragma unroll

@@ -7,46 +7,58 @@ namespace nvm {
 
 // Tiles of the larger kernels (of outputs, for gate/up of both matrices', by
 // rows), and the time of a launch: `fixed` + rounds over the CUs x (`start` +
-// `row` x N / 2048) microseconds, for E2M1 and E4M3 activations (fitted; some 10 %
-// off, more where the clock falls under the load, for all alike).  A step of the
-// larger ones costs less for its outputs, but they leave more CUs idle.  In us on
-// 256 x 256 in whole tiles, in parts (below), on 256 x 128, 128 x 128, 128 x 64 and
-// 64 x 64, E4M3 unless said:
+// `row` x N / 2048) microseconds, for E2M1 activations, E4M3, and E4M3 in short
+// sums (fitted; some 10 % off, more where the clock falls under the load, for all
+// alike).  A step of the larger ones costs less for its outputs, but they leave
+// more CUs idle.  In us on 256 x 256 in whole tiles, in parts (below), on 256 x
+// 128, 128 x 128, 128 x 64 and 64 x 64:
+//   E4M3
+//   2048 -> 2048    512 rows   47.8   -    27.5  18.2  13.0  10.5
+//                  1024 rows   48.5   -    28.0  19.2  13.9  15.3
+//   2048 -> 5120    512 rows   48.2   -    29.0  19.5  24.2  20.1
+//                  1536 rows   49.6   -    35.8  37.6  45.0
+//                  4096 rows   97.0  73.7  87.5  95.1
+//                  8192 rows  141.1 133.7 148.2 169.4
+//   6144 -> 2048    512 rows  129.4   -    68.0  39.9  27.6  20.7
+//                  1024 rows  127.4   -    68.2  41.2  30.2  32.5
+//                  8192 rows  147.7   -   166.8 179.5
+//   4096 -> 6144   3000 rows  176.1 127.5 142.5 142.4
+//   8192 -> 8192   8192 rows  743     -   800   892
+//   gate/up 2048 -> 6144
+//                   128 rows    -     -    28.9  19.0  13.5
+//                  1500 rows   97.5  75.5  82.2  84.5
+//                  4096 rows  153     -   169   204
+//   E4M3 in short sums
 //   2048 -> 2048    512 rows    -     -     -    12.2   9.1   7.9
 //                  1024 rows    -     -     -    12.7  10.0  11.2
-//   2048 -> 5120    256 rows    -     -     -    12.4   9.4  10.3
-//                   512 rows   24.0   -    17.2  13.2  16.6  15.4
+//   2048 -> 5120    512 rows   24.0   -    17.2  13.2  16.6  15.4
 //                  1536 rows   26.3   -    21.0  24.8
-//                  2048 rows   27.0   -    30.3  35.2
 //                  4096 rows   48.9  44.4  47.0  59.0        (E2M1 42.0  35.8  35.7  46.3)
 //                  8192 rows   77.3  73.1  78.7   -          (E2M1 67.1  61.7  61.8)
 //   6144 -> 2048    512 rows    -     -     -    22.9  16.5  14.1
-//                  1024 rows   54     -    34    23.9  20.2  23.2
 //                  4096 rows   57     -    45.5  54
 //   4096 -> 6144   3000 rows   82.2  66.4  78.2   -
 //   8192 -> 8192   8192 rows   367    -    424   553         (E2M1  293   -   350   420)
 //   gate/up 2048 -> 6144
 //                   128 rows   24.0   -    16.8  13.0   9.7
-//                   256 rows    -     -     -    13.6  16.8
-//                  1000 rows   27.7   -    31.7  35.9
 //                  1500 rows   50.5  40.4  46.0   -
 //                  4096 rows   82     -    94.7  134
 struct Tiles {
   int bn, bm;
-  double fixed[2], start[2], row[2];  // by nvm_mx_format
+  double fixed[3], start[3], row[3];  // by the activations: an nvm_mx_format or kMxShort
   double round(int format, int N) const { return start[format] + row[format] * (N / 2048.0); }
 };
-constexpr Tiles kBig = {256, 256, {3.0, 3.0}, {4.5, 7.5}, {14.0, 15.5}};
-constexpr Tiles kTiles[] = {{256, 128, {2.5, 3.5}, {4.0, 3.5}, {7.0, 9.2}},
-                            {128, 128, {1.0, 1.5}, {4.0, 4.0}, {4.1, 6.3}},
-                            {128, 64, {3.0, 2.5}, {1.8, 2.8}, {3.2, 4.3}},
-                            {64, 64, {3.5, 3.5}, {1.0, 0.9}, {2.1, 3.1}}};
+constexpr Tiles kBig = {256, 256, {3.0, 1.0, 3.0}, {4.5, 6.5, 7.5}, {14.0, 41.4, 15.5}};
+constexpr Tiles kTiles[] = {{256, 128, {2.5, 1.0, 3.5}, {4.0, 5.6, 3.5}, {7.0, 20.7, 9.2}},
+                            {128, 128, {1.0, 1.0, 1.5}, {4.0, 5.5, 4.0}, {4.1, 11.3, 6.3}},
+                            {128, 64, {3.0, 1.0, 2.5}, {1.8, 4.3, 2.8}, {3.2, 7.1, 4.3}},
+                            {64, 64, {3.5, 3.5, 3.5}, {1.0, 1.5, 0.9}, {2.1, 4.5, 3.1}}};
 
-// The kernel of the least time.  Few rows: mx_gemv.hip (2048 -> 5120, 64 rows 7.6
-// us, on 64 x 64 tiles 6.9, 48 rows 6.1 and 6.8; gate/up 2048 -> 6144, 48 rows 9.4,
-// on 128 x 64 9.2), and 32 rows always: there reading the weights is more of the
-// time than the fit knows (2048 -> 151936 of 16 rows 42 us, on 256 x 128 49; gate/up
-// 2912 -> 14240 of 27 rows 13.2 and 17.4).
+// The kernel of the least time.  Few rows: mx_gemv.hip (2048 -> 5120 of 128 rows
+// 11.2 us, on 64 x 64 tiles 10.2, 64 rows 9.1 and 9.6), and 32 rows always: there
+// reading the weights is more of the time than the fit knows (in short sums 2048 ->
+// 151936 of 16 rows 42 us, on 256 x 128 49; gate/up 2912 -> 14240 of 27 rows 13.2
+// and 17.4).
 static hipError_t launch_mx_product(int format, bool dual, int out_format, const MxMatmulArgs &a,
                                     hipStream_t st) {
   const int64_t columns = (int64_t)a.K * (dual ? 2 : 1), cus = cu_count() / 8 * 8;
@@ -76,6 +88,11 @@ static hipError_t launch_mx_product(int format, bool dual, int out_format, const
   return launch_mx_gemm_pipe(format, best->bn, best->bm, dual, out_format, a, st);
 }
 
+// What the kernels take for an entry's a_format.
+static int mx_activations(int a_format) {
+  return a_format == (NVM_MX_FP8 | NVM_MX_SHORT_SUMS) ? kMxShort : a_format & ~NVM_MX_SHORT_SUMS;
+}
+
 }  // namespace nvm
 
 extern "C" {
@@ -87,7 +104,7 @@ int nvm_mx_matmul(const void *a_codes, const uint8_t *a_scales, int64_t a_scale_
   const char *op = "mx_matmul";
   if (out_dtype != NVM_MX_F16 && out_dtype != NVM_MX_BF16 && out_dtype != NVM_MX_F32)
     return set_error(NVM_ERR_INVALID, "%s: out_dtype must be f16, bf16 or f32", op);
-  if (int rc = mx_check_rows(op, M, N, a_format, "a")) return rc;
+  if (int rc = mx_check_rows(op, M, N, a_format & ~NVM_MX_SHORT_SUMS, "a")) return rc;
   if (int rc = mx_check_rows(op, K, N, NVM_MX_FP4, "w")) return rc;
   if (M == 0 || K == 0) return NVM_OK;
   if (int rc = mx_check_tensor(op, a_codes, a_scales, a_scale_ld, N, "a")) return rc;
@@ -106,7 +123,7 @@ int nvm_mx_matmul(const void *a_codes, const uint8_t *a_scales, int64_t a_scale_
   a.K = (int)K;
   a.out_dtype = out_dtype;
   a.out = out;
-  const hipError_t e = launch_mx_product(a_format, false, NVM_MX_FP8, a, (hipStream_t)stream);
+  const hipError_t e = launch_mx_product(mx_activations(a_format), false, NVM_MX_FP8, a, (hipStream_t)stream);
   if (e == hipErrorInvalidConfiguration)
     return set_error(NVM_ERR_UNSUPPORTED, "%s: too many output tiles", op);
   if (e != hipSuccess) return set_error(NVM_ERR_HIP, "%s: %s", op, hipGetErrorString(e));
@@ -120,7 +137,7 @@ int nvm_mx_swiglu(const void *a_codes, const uint8_t *a_scales, int64_t a_scale_
                   int64_t out_scale_ld, nvm_stream_t stream) {
   using namespace nvm;
   const char *op = "mx_swiglu";
-  if (int rc = mx_check_rows(op, M, N, a_format, "a")) return rc;
+  if (int rc = mx_check_rows(op, M, N, a_format & ~NVM_MX_SHORT_SUMS, "a")) return rc;
   if (int rc = mx_check_rows(op, K, N, NVM_MX_FP4, "gate and up")) return rc;
   if (int rc = mx_check_rows(op, M, K, out_format, "output")) return rc;
   if (M == 0) return NVM_OK;
@@ -144,7 +161,7 @@ int nvm_mx_swiglu(const void *a_codes, const uint8_t *a_scales, int64_t a_scale_
   a.out = out_codes;
   a.out_s = out_scales;
   a.out_sld = out_scale_ld;
-  const hipError_t e = launch_mx_product(a_format, true, out_format, a, (hipStream_t)stream);
+  const hipError_t e = launch_mx_product(mx_activations(a_format), true, out_format, a, (hipStream_t)stream);
   if (e == hipErrorInvalidConfiguration)
     return set_error(NVM_ERR_UNSUPPORTED, "%s: too many output tiles", op);
   if (e != hipSuccess) return set_error(NVM_ERR_HIP, "%s: %s", op, hipGetErrorString(e));

@@ -73,6 +73,18 @@ struct MxTile {
   static __device__ __forceinline__ int piece_at(int piece, int lane) {
     return 16 * (lane % (W / 16) ^ turned<W>(piece_row<W>(piece, lane)));
   }
+  // The same of activation rows.  (E4M3 that is converted to bf16: a lane group's
+  // chunks are 2 G and 2 G + 1, the neighbour's k ^ 2, so the places of rows 0-3
+  // and 12-15, turned by even numbers, and those of rows 4-11, by odd ones, are
+  // closed under that.)
+  static __device__ __forceinline__ int turned_act(int r) {
+    if constexpr (FMT != NVM_MX_FP8) return turned<XR>(r);
+    const int i = r >> 1;
+    return (i & 4) | ((i & 1) << 1) | ((i >> 1 ^ i >> 2) & 1);
+  }
+  static __device__ __forceinline__ int act_piece_at(int piece, int lane) {
+    return 16 * (lane % (XR / 16) ^ turned_act(piece_row<XR>(piece, lane)));
+  }
 
   // Where the loads of an output tile read.  Weight row r of a stage is column
   // r % BK of matrix r / BK; rows past an operand repeat its last row, whose
@@ -115,7 +127,7 @@ struct MxTile {
 #pragma unroll
       for (int j = 0; j < LX; ++j) {
         const int i = wv + j * NW % PX;
-        vx[j] = min(piece_row<XR>(i, lane), q.nm - 1) * XB + piece_at<XR>(i, lane) +
+        vx[j] = min(piece_row<XR>(i, lane), q.nm - 1) * XB + act_piece_at(i, lane) +
                 128 * (j * NW / PX);
       }
     }
@@ -171,11 +183,12 @@ struct MxTile {
       const int g = KG == 2 ? 4 * kg + G : G;  // chunk of the two steps in a row
       w = wrow * WR + 16 * (g ^ turned<WR>(wrow));
       if constexpr (FMT == NVM_MX_FP4) {
-        x[0] = kW + xrow * XR + 16 * (g ^ turned<XR>(xrow));
+        x[0] = kW + xrow * XR + 16 * (g ^ turned_act(xrow));
       } else {
 #pragma unroll
         for (int c = 0; c < 2; ++c)
-          x[c] = kW + kg * kX + xrow * XR + 16 * ((4 * c + G) ^ turned<XR>(xrow));
+          x[c] = kW + kg * kX + xrow * XR +
+                 16 * ((mx_act_at<FMT>(G, c) / 16) ^ turned_act(xrow));
       }
       auto scale_at = [](int tile) { return tile / 4 * 1024 + 4 * (tile % 4); };
       ws = kScales + scale_at(wf * FM) + 256 * G + 16 * col;

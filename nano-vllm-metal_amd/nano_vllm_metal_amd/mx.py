@@ -4,7 +4,7 @@ An ``MxTensor`` holds rows of block-scaled floating point: 32 consecutive
 values share one power-of-two scale (E8M0), the values are E2M1 (``mxfp4``) or
 E4M3 (``mxfp8``), as in the OCP Microscaling formats and in MLX's ``mxfp4``
 weights.  ``mx_linear`` multiplies MX activations with MXFP4 weights on the
-scaled matrix instructions; it stands beside ``quantized_linear``
+matrix cores; it stands beside ``quantized_linear``
 (``layers/linear.py:92-126``), ``mx_swiglu`` beside ``quantized_swiglu`` and
 ``residual_rms_norm_mx`` beside ``residual_rms_norm``, with activations of
 eight (or four) bits between them.  No CPU fallback.
@@ -22,6 +22,7 @@ MX_BLOCK = 32
 # nvm_mx_format and nvm_mx_dtype of include/nvm_mx.h
 MX_FORMATS = {"mxfp4": 0, "mxfp8": 1}
 MX_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_SHORT_SUMS = 16  # NVM_MX_SHORT_SUMS
 _PER_BYTE = {"mxfp4": 2, "mxfp8": 1}
 _MAX_PITCH = 1 << 20
 
@@ -338,12 +339,13 @@ def _check_weight(op: str, name: str, w: MxTensor, a: MxTensor) -> None:
 
 def mx_linear(x: Union[MxTensor, torch.Tensor], w: MxTensor,
               dtype: Optional[torch.dtype] = None,
-              bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+              bias: Optional[torch.Tensor] = None, short_sums: bool = False) -> torch.Tensor:
     """``x . w^T (+ bias)``: ``x [..., N]`` in MX (16-bit activations are
-    quantised to mxfp8 first), ``w [K, N]`` in mxfp4.  Float32 sums
-    (include/nvm_mx.h says what mxfp8 activations lose in them), one rounding
-    to ``dtype`` (float16, bfloat16 or float32; by default that of 16-bit
-    activations, else bfloat16)."""
+    quantised to mxfp8 first), ``w [K, N]`` in mxfp4.  Float32 sums, one rounding to ``dtype``
+    (float16, bfloat16 or float32; by default that of 16-bit activations, else
+    bfloat16).  ``short_sums``: mxfp8 activations are summed by the scaled matrix
+    instruction itself, at about twice the rate for many rows, and some 2^-15 of
+    a sum is lost (include/nvm_mx.h)."""
     lib = _lib.load()
     if type(x) is MxTensor:
         a = x
@@ -358,24 +360,25 @@ def mx_linear(x: Union[MxTensor, torch.Tensor], w: MxTensor,
     index = _index(a._base, w._base)
     if index != _current_device():
         with torch.cuda.device(index):
-            return mx_linear(a, w, dtype, bias)
+            return mx_linear(a, w, dtype, bias, short_sums)
     K, N = w.shape
     lead = a.shape
     out = torch.empty((lead[0], K) if len(lead) == 2 else (*lead[:-1], K), dtype=dtype,
                       device=a._base.device)
     ac, asc = a._pointers()
     wc, wsc = w._pointers()
-    _lib.check(lib.nvm_mx_matmul(ac, asc, a.pitch, MX_FORMATS[a.fmt], wc, wsc, w.pitch, a.rows, N,
-                                 K, code, out.data_ptr(), _raw_stream(index)))
+    sums = _SHORT_SUMS if short_sums else 0
+    _lib.check(lib.nvm_mx_matmul(ac, asc, a.pitch, MX_FORMATS[a.fmt] | sums, wc, wsc, w.pitch,
+                                 a.rows, N, K, code, out.data_ptr(), _raw_stream(index)))
     return out if bias is None else out + bias
 
 
 def mx_swiglu(x: Union[MxTensor, torch.Tensor], w_gate: MxTensor, w_up: MxTensor,
-              fmt: str = "mxfp8") -> MxTensor:
+              fmt: str = "mxfp8", short_sums: bool = False) -> MxTensor:
     """``silu(x . gate^T) * (x . up^T)`` in MX, the input of a down projection
     (models/qwen3.py:176-184): ``x`` as for ``mx_linear``, both weights ``[K,
     N]`` in mxfp4, K a multiple of 32.  Everything up to the quantisation is
-    float32."""
+    float32, unless ``short_sums`` asks for sums as ``mx_linear`` says."""
     lib = _lib.load()
     code = _format(fmt)
     a = x if type(x) is MxTensor else _activations(x, "mx_swiglu")
@@ -390,13 +393,14 @@ def mx_swiglu(x: Union[MxTensor, torch.Tensor], w_gate: MxTensor, w_up: MxTensor
         _lib.require_device(a._base, w_up._base)
     if index != _current_device():
         with torch.cuda.device(index):
-            return mx_swiglu(a, w_gate, w_up, fmt)
+            return mx_swiglu(a, w_gate, w_up, fmt, short_sums)
     out = MxTensor._empty(a.shape[:-1], a.rows, K, fmt, a._base.device)
     ac, asc = a._pointers()
     gc, gsc = w_gate._pointers()
     uc, usc = w_up._pointers()
     oc, osc = out._pointers()
-    _lib.check(lib.nvm_mx_swiglu(ac, asc, a.pitch, MX_FORMATS[a.fmt], gc, gsc, w_gate.pitch, uc,
-                                 usc, w_up.pitch, a.rows, N, K, code, oc, osc, out.pitch,
+    sums = _SHORT_SUMS if short_sums else 0
+    _lib.check(lib.nvm_mx_swiglu(ac, asc, a.pitch, MX_FORMATS[a.fmt] | sums, gc, gsc, w_gate.pitch,
+                                 uc, usc, w_up.pitch, a.rows, N, K, code, oc, osc, out.pitch,
                                  _raw_stream(index)))
     return out

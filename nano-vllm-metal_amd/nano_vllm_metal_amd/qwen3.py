@@ -27,6 +27,8 @@ Projections, dense MLPs, the embedding and the lm head may instead be
 output goes into such weights only, it is computed in MX (``mxfp8``) and never
 stored in 16 bits: norm -> q/k/v product, and norm -> gate/up -> down product;
 the attention's output and the lm head's input are quantised by ``mx_linear``.
+So every product with such weights has activations of eight bits (E4M3, four
+significant ones); q, k and v are of one kind, and so are gate, up and down.
 """
 
 from __future__ import annotations
@@ -100,10 +102,13 @@ class RoPE:
         self.sin = torch.sin(freqs).to(device).contiguous()
 
 
-def linear(x, w: Weights, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+def linear(x, w: Weights, dtype: Optional[torch.dtype] = None,
+           short_sums: bool = False) -> torch.Tensor:
     """``x . w^T`` by the weight's kind; ``dtype``: of the output of an ``x`` in
-    MX."""
-    return mx_linear(x, w, dtype) if isinstance(w, MxTensor) else quantized_linear(x, w)
+    MX; ``short_sums`` as for ``mx_linear``."""
+    if isinstance(w, MxTensor):
+        return mx_linear(x, w, dtype, short_sums=short_sums)
+    return quantized_linear(x, w)
 
 
 def norm_for(consumer: object, h: torch.Tensor, r: Optional[torch.Tensor], weight: torch.Tensor,
@@ -126,10 +131,12 @@ class DenseMLP:
             raise ValueError("DenseMLP: gate, up and down must all be MxTensors, or none")
         self.mx = all(mx)
 
-    def __call__(self, x, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    def __call__(self, x, dtype: Optional[torch.dtype] = None,
+                 short_sums: bool = False) -> torch.Tensor:
         if self.mx:
             out = dtype if isinstance(x, MxTensor) else x.dtype
-            return mx_linear(mx_swiglu(x, self.w_gate, self.w_up), self.w_down, out)
+            h = mx_swiglu(x, self.w_gate, self.w_up, short_sums=short_sums)
+            return mx_linear(h, self.w_down, out, short_sums=short_sums)
         if swiglu_supports(x, self.w_gate, self.w_up):
             h = quantized_swiglu(x, self.w_gate, self.w_up)
         else:
@@ -196,6 +203,9 @@ class Qwen3Model:
         self.norm = norm
         self.lm_head = lm_head
         self.dtype = dtype
+        # products of MX weights in the matrix instruction's own sums (``mx_linear``):
+        # prefill in less time, for some 2^-15 of each sum
+        self.short_sums = False
         self.device = embed.device if isinstance(embed, MxTensor) else embed.weight.device
         self.rope = RoPE(config.head_dim, config.max_position_embeddings, config.rope_theta,
                          self.device)
@@ -225,7 +235,7 @@ class Qwen3Model:
         c = self.config
         B, L, _ = x.shape
         Hq, Hkv, D = c.num_attention_heads, c.num_key_value_heads, c.head_dim
-        qkv = linear(x, layer.wqkv, self.dtype)
+        qkv = linear(x, layer.wqkv, self.dtype, self.short_sums)
         q, k, v = qk_norm_rope_store(qkv, Hq, Hkv, D, layer.q_norm, layer.k_norm, c.rms_norm_eps,
                                      step.positions, self.rope.cos, self.rope.sin, step.page_ids,
                                      step.slots, cache.key_pages[li], cache.value_pages[li],
@@ -244,7 +254,7 @@ class Qwen3Model:
                                 cache.value_pages[li], step.block_table, step.lens,
                                 cache.page_size, scale=scale, mask="causal", out_dtype=qkv.dtype)
             o = o.transpose(1, 2).reshape(B, L, Hq * D)
-        return linear(o, layer.wo)
+        return linear(o, layer.wo, short_sums=self.short_sums)
 
     # ---------------------------------------------------------------- forward
 
@@ -280,11 +290,13 @@ class Qwen3Model:
                 # the MoE combine fused into this residual add and norm
                 h, x = moe_residual_rms_norm(layer.mlp, x, h, nxt, eps)
             else:
-                y = layer.mlp(x, self.dtype) if isinstance(x, MxTensor) else layer.mlp(x)
+                mx = isinstance(x, MxTensor)
+                y = layer.mlp(x, self.dtype, self.short_sums) if mx else layer.mlp(x)
                 h, x = norm_for(follow.wqkv if follow else None, h, y, nxt, eps)
         if last_only:
             x = x[:, -1]
-        return linear(x, self.lm_head if self.lm_head is not None else self.embed_w)
+        return linear(x, self.lm_head if self.lm_head is not None else self.embed_w,
+                      short_sums=self.short_sums)
 
     def forward(self, tokens: torch.Tensor, cache: PagedKVCache, seq_ids: Sequence[int],
                 last_only: bool = True) -> torch.Tensor:
@@ -307,7 +319,8 @@ class Qwen3Model:
     def from_checkpoint(cls, path, device="cuda", dtype: torch.dtype = torch.bfloat16):
         """Load an MLX 4-bit Qwen3 / Qwen3-MoE checkpoint from a local directory
         (``config.json`` plus safetensors, sharded or not); modules in ``mxfp4``
-        mode as ``MxTensor`` weights (the sparse blocks have to be affine)."""
+        mode as ``MxTensor`` weights, whose activations are rounded to ``mxfp8`` (the
+        sparse blocks have to be affine)."""
         from .loader import _Tensors, _weights, load_moe_block, read_config
 
         path = Path(path)
