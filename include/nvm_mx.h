@@ -91,6 +91,13 @@ int nvm_mx_swiglu(const void *a_codes, const uint8_t *a_scales, int64_t a_scale_
                   int64_t N, int64_t K, int out_format, void *out_codes, uint8_t *out_scales,
                   int64_t out_scale_ld, nvm_stream_t stream);
 
+/* The kernel that nvm_mx_matmul (gate_up 0) or nvm_mx_swiglu (1) runs for these
+ * sizes on the current device.  plan[0]: 0 for few rows, 1 for some hundred, 2 for
+ * many, -1 if there is nothing to compute; plan[1], plan[2]: a block's outputs (of
+ * both matrices for gate_up) and rows; plan[3]: the parts that the tiles past whole
+ * rounds are computed in, 2 or 4, or 0. */
+int nvm_mx_product_plan(int gate_up, int64_t M, int64_t N, int64_t K, int a_format, int plan[4]);
+
 #ifdef __cplusplus
 }
 #endif

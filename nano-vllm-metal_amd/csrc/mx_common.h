@@ -212,13 +212,17 @@ struct MxMatmulArgs {
   int64_t out_sld;
 };
 // The products for few rows (mx_gemv.hip, with the block's `tile` that
-// mx_gemv_time names: the one of the least time, which it returns in us), for some
-// (mx_gemm_pipe.hip, in tiles of bn outputs by bm rows) and for many (mx_gemm.hip:
-// 256 by 256, those past whole rounds in `parts`: 0, 2 or 4, a part a block).
-// hipErrorInvalidConfiguration: more blocks than a launch has, more than
-// kMxMaxTiles output tiles.
+// mx_gemv_time names: of those that a launch takes the one of the least time, which
+// it returns in us, infinity if there is none; columns and rows: its outputs, for
+// gate/up of both matrices, and rows), for some (mx_gemm_pipe.hip, in tiles of bn
+// outputs by bm rows) and for many (mx_gemm.hip: 256 by 256, those past whole
+// rounds in `parts`: 0, 2 or 4, a part a block), of at most kMxMaxTiles output
+// tiles.  hipErrorInvalidConfiguration: more than a launch takes.
 constexpr int64_t kMxMaxTiles = 1 << 22;
-double mx_gemv_time(int format, bool dual, const MxMatmulArgs &a, int *tile);
+struct MxBlock {
+  int tile, columns, rows;
+};
+double mx_gemv_time(int format, bool dual, int64_t M, int N, int K, MxBlock *block);
 hipError_t launch_mx_gemv(int format, int tile, bool dual, int out_format, const MxMatmulArgs &a,
                           hipStream_t st);
 hipError_t launch_mx_gemm_pipe(int format, int bn, int bm, bool dual, int out_format,

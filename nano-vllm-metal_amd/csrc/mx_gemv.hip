@@ -171,12 +171,19 @@ __global__ __launch_bounds__(64 * NW) void mx_gemv_kernel(const MxMatmulArgs p) 
   }
 }
 
+// Blocks of a launch (DUAL: RT / 2 tiles of either matrix); false: more than it
+// takes, 2^32 - 1 threads and 65535 rows of blocks.
+bool grid_of(bool dual, int rt, int mt, int64_t M, int64_t K, int64_t &x, int64_t &y) {
+  const int64_t columns = 16 * (dual ? rt / 2 : rt), rows = 16 * mt;
+  x = (K + columns - 1) / columns;
+  y = (M + rows - 1) / rows;
+  return x * (64 * NW) <= (int64_t)UINT32_MAX && y <= 65535;
+}
+
 template <int FMT, int OFMT, bool DUAL, int RT, int MT>
 hipError_t go(const MxMatmulArgs &a, hipStream_t st) {
-  constexpr int RF = DUAL ? RT / 2 : RT;
-  const int64_t x = ((int64_t)a.K + 16 * RF - 1) / (16 * RF), y = (a.M + 16 * MT - 1) / (16 * MT);
-  // (threads of a launch's dimension: below 2^32)
-  if (x * (64 * NW) > (int64_t)UINT32_MAX || y > 65535) return hipErrorInvalidConfiguration;
+  int64_t x, y;
+  if (!grid_of(DUAL, RT, MT, a.M, a.K, x, y)) return hipErrorInvalidConfiguration;
   hipLaunchKernelGGL((mx_gemv_kernel<FMT, OFMT, DUAL, RT, MT>),
                      dim3((unsigned)x, (unsigned)y), dim3(64 * NW), 0, st, a);
   return hipGetLastError();
@@ -227,19 +234,20 @@ hipError_t launch_fmt(int tile, bool dual, int out_format, const MxMatmulArgs &a
                                   : launch_tile<FMT, NVM_MX_FP8, true, ns - 1>(tile, a, st);
 }
 
-template <int N>
-double best_of(const Blocks (&blocks)[N], int format, bool dual, const MxMatmulArgs &a, int *tile) {
+template <int COUNT>
+double best_of(const Blocks (&blocks)[COUNT], int format, bool dual, int64_t M, int N, int K,
+               MxBlock *block) {
   const int64_t cus = cu_count();
   double best = INFINITY;
-  for (int i = 0; i < N; ++i) {
+  for (int i = 0; i < COUNT; ++i) {
     const Blocks &b = blocks[i];
-    const int64_t columns = 16 * (dual ? b.rt / 2 : b.rt), rows = 16 * b.mt;
-    const int64_t n = (a.K + columns - 1) / columns * ((a.M + rows - 1) / rows);
-    const double round = b.round[format] * (a.N / 2048.0);
-    const double t = b.fixed[format] + round + ((n - 1) / cus) * fmax(round, kLeastRound);
+    int64_t x, y;
+    if (!grid_of(dual, b.rt, b.mt, M, K, x, y)) continue;
+    const double round = b.round[format] * (N / 2048.0);
+    const double t = b.fixed[format] + round + ((x * y - 1) / cus) * fmax(round, kLeastRound);
     if (t < best) {
       best = t;
-      *tile = i;
+      *block = {i, 16 * b.rt, 16 * b.mt};
     }
   }
   return best;
@@ -247,8 +255,9 @@ double best_of(const Blocks (&blocks)[N], int format, bool dual, const MxMatmulA
 
 }  // namespace
 
-double mx_gemv_time(int format, bool dual, const MxMatmulArgs &a, int *tile) {
-  return dual ? best_of(kSwiglu, format, dual, a, tile) : best_of(kLinear, format, dual, a, tile);
+double mx_gemv_time(int format, bool dual, int64_t M, int N, int K, MxBlock *block) {
+  return dual ? best_of(kSwiglu, format, dual, M, N, K, block)
+              : best_of(kLinear, format, dual, M, N, K, block);
 }
 
 hipError_t launch_mx_gemv(int format, int tile, bool dual, int out_format, const MxMatmulArgs &a,

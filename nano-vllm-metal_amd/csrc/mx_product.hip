@@ -1,5 +1,7 @@
 // Products of MX rows with MXFP4 weights: which kernel, and the entry points
 // (include/nvm_mx.h).
+#include <math.h>
+
 #include "internal.h"
 #include "mx_common.h"
 
@@ -54,38 +56,56 @@ constexpr Tiles kTiles[] = {{256, 128, {2.5, 1.0, 3.5}, {4.0, 5.6, 3.5}, {7.0, 2
                             {128, 64, {3.0, 1.0, 2.5}, {1.8, 4.3, 2.8}, {3.2, 7.1, 4.3}},
                             {64, 64, {3.5, 3.5, 3.5}, {1.0, 1.5, 0.9}, {2.1, 4.5, 3.1}}};
 
-// The kernel of the least time.  Few rows: mx_gemv.hip (2048 -> 5120 of 128 rows
+// The kernel of the least time, of those that take so many outputs.  Few rows: mx_gemv.hip (2048 -> 5120 of 128 rows
 // 11.2 us, on 64 x 64 tiles 10.2, 64 rows 9.1 and 9.6), and 32 rows always: there
 // reading the weights is more of the time than the fit knows (in short sums 2048 ->
 // 151936 of 16 rows 42 us, on 256 x 128 49; gate/up 2912 -> 14240 of 27 rows 13.2
 // and 17.4).
-static hipError_t launch_mx_product(int format, bool dual, int out_format, const MxMatmulArgs &a,
-                                    hipStream_t st) {
-  const int64_t columns = (int64_t)a.K * (dual ? 2 : 1), cus = cu_count() / 8 * 8;
+struct Choice {
+  int kernel = -1;  // 0 mx_gemv.hip, 1 mx_gemm_pipe.hip, 2 mx_gemm.hip; -1: more outputs than any takes
+  MxBlock block{};
+  int parts = 0;
+};
+static Choice choose(int format, bool dual, int64_t M, int N, int K) {
+  const int64_t columns = (int64_t)K * (dual ? 2 : 1), cus = cu_count() / 8 * 8;
   auto count = [&](const Tiles &t) {
-    return (columns + t.bn - 1) / t.bn * ((a.M + t.bm - 1) / t.bm);
+    return (columns + t.bn - 1) / t.bn * ((M + t.bm - 1) / t.bm);
   };
+  Choice c;
+  const double few = mx_gemv_time(format, dual, M, N, K, &c.block);
+  double least = few;
+  if (few < INFINITY) {
+    c.kernel = 0;
+    if (M <= 32) return c;
+  }
+  auto take = [&](const Tiles &t, double time, int kernel, int parts) {
+    if (time < least && count(t) <= kMxMaxTiles) {
+      least = time;
+      c = {kernel, {0, t.bn, t.bm}, parts};
+    }
+  };
+  for (const Tiles &t : kTiles)
+    if (!dual || t.bn != 64)
+      take(t, t.fixed[format] + (count(t) + cus - 1) / cus * t.round(format, N), 1, 0);
   // A last round of 256 x 256 that no more than a quarter (half) of the CUs would
   // have is computed in parts, of 128 x 128 (256 x 128), by all of them.
   const int64_t n = count(kBig), rest = n % cus;
   const int parts = n < cus || rest == 0 || 2 * rest > cus ? 0 : 4 * rest > cus ? 2 : 4;
-  double least = kBig.fixed[format] +
-                 (parts ? n / cus : (n + cus - 1) / cus) * kBig.round(format, a.N) +
-                 (parts ? kTiles[parts == 4].round(format, a.N) : 0.0);
-  const Tiles *best = &kBig;
-  for (const Tiles &t : kTiles) {
-    if (dual && t.bn == 64) continue;
-    const double time = t.fixed[format] + (count(t) + cus - 1) / cus * t.round(format, a.N);
-    if (time < least) {
-      least = time;
-      best = &t;
-    }
-  }
-  int tile = 0;
-  if (mx_gemv_time(format, dual, a, &tile) <= least || a.M <= 32)
-    return launch_mx_gemv(format, tile, dual, out_format, a, st);
-  if (best == &kBig) return launch_mx_gemm(format, parts, dual, out_format, a, st);
-  return launch_mx_gemm_pipe(format, best->bn, best->bm, dual, out_format, a, st);
+  take(kBig,
+       kBig.fixed[format] + (parts ? n / cus : (n + cus - 1) / cus) * kBig.round(format, N) +
+           (parts ? kTiles[parts == 4].round(format, N) : 0.0),
+       2, parts);
+  return c;
+}
+
+static hipError_t launch_mx_product(int format, bool dual, int out_format, const MxMatmulArgs &a,
+                                    hipStream_t st) {
+  const Choice c = choose(format, dual, a.M, a.N, a.K);
+  if (c.kernel == 0) return launch_mx_gemv(format, c.block.tile, dual, out_format, a, st);
+  if (c.kernel == 1)
+    return launch_mx_gemm_pipe(format, c.block.columns, c.block.rows, dual, out_format, a, st);
+  if (c.kernel == 2) return launch_mx_gemm(format, c.parts, dual, out_format, a, st);
+  return hipErrorInvalidConfiguration;
 }
 
 // What the kernels take for an entry's a_format.
@@ -165,6 +185,26 @@ int nvm_mx_swiglu(const void *a_codes, const uint8_t *a_scales, int64_t a_scale_
   if (e == hipErrorInvalidConfiguration)
     return set_error(NVM_ERR_UNSUPPORTED, "%s: too many output tiles", op);
   if (e != hipSuccess) return set_error(NVM_ERR_HIP, "%s: %s", op, hipGetErrorString(e));
+  return NVM_OK;
+}
+
+int nvm_mx_product_plan(int gate_up, int64_t M, int64_t N, int64_t K, int a_format, int *plan) {
+  using namespace nvm;
+  const char *op = "mx_product_plan";
+  if (!plan) return set_error(NVM_ERR_INVALID, "%s: null pointer", op);
+  if (int rc = mx_check_rows(op, M, N, a_format & ~NVM_MX_SHORT_SUMS, "a")) return rc;
+  if (int rc = mx_check_rows(op, K, N, NVM_MX_FP4, "w")) return rc;
+  if (gate_up)
+    if (int rc = mx_check_rows(op, M, K, NVM_MX_FP4, "output")) return rc;
+  Choice c;
+  if (M > 0 && K > 0) {
+    c = choose(mx_activations(a_format), gate_up != 0, M, (int)N, (int)K);
+    if (c.kernel < 0) return set_error(NVM_ERR_UNSUPPORTED, "%s: too many output tiles", op);
+  }
+  plan[0] = c.kernel;
+  plan[1] = c.block.columns;
+  plan[2] = c.block.rows;
+  plan[3] = c.parts;
   return NVM_OK;
 }
 

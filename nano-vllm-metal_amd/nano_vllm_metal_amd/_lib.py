@@ -70,6 +70,7 @@ SIGNATURES = {
     "nvm_mx_matmul": [_P, _P, _I64, _I, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P],
     "nvm_mx_swiglu": [_P, _P, _I64, _I, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P,
                       _I64, _P],
+    "nvm_mx_product_plan": [_I, _I64, _I64, _I64, _I, ctypes.POINTER(_I)],
     "nvm_moe_forward_residual_norm": [_P, _I64, _I64, _I64, _I64, _I, _I, _I, _I, _I,
                                       _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                       _P, _P, ctypes.c_float, _P, _P, _I, _P, _SZ, _P],
