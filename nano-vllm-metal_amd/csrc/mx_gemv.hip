@@ -196,8 +196,7 @@ hipError_t go(const MxMatmulArgs &a, hipStream_t st) {
 // takes kLeastRound, however short the rows (in short sums 32 -> 2048 of 2048 rows,
 // 11 rounds of 3 x 2 tiles: 17.3 us).  Larger blocks read the activations, and a
 // column of them the weights, less often, but a round of them is longer: 4096 ->
-// 4096 of 128 rows 14.3 us on 256 blocks of 4 x 2 tiles, 16.9 on 192 of 4 x 3, 16.5
-// on 512 of 2 x 2, 20.1 on 1024 of 2 x 1; 2048 -> 2048 of 32 rows 4.2 on 256 of 1 x
+// 4096 of 128 rows 14.3 us on 256 blocks of 4 x 2 tiles, 16.5 on 512 of 2 x 2, 20.1 on 1024 of 2 x 1; 2048 -> 2048 of 32 rows 4.2 on 256 of 1 x
 // 1, 4.7 on 128 of 2 x 1, 6.5 on 64 of 2 x 2.
 constexpr double kLeastRound = 1.8;
 struct Blocks {
@@ -208,7 +207,11 @@ constexpr Blocks kLinear[] = {
     {1, 1, {2, 1.9, 2.2}, {1.15, 1.8, 1.5}}, {2, 1, {2.1, 2.6, 2.3}, {1.8, 2.2, 2.05}},
     {4, 1, {2.3, 3.5, 2.6}, {3, 3.2, 3.25}}, {2, 2, {2.4, 3.4, 2.6}, {2.4, 3.1, 3.3}},
     {2, 3, {2.7, 3.9, 2.7}, {2.9, 3.6, 4.5}}, {4, 2, {3, 4.6, 3.3}, {3.6, 4.3, 4.5}},
-    {4, 3, {3.5, 5.3, 3.6}, {4.1, 5, 6}}};
+    {4, 3, {3.5, 0, 3.6}, {4.1, 0, 6}}};
+// (4 x 3 of E4M3, 5.3 and 5, takes longer than 64 x 64 tiles whatever the sizes.)
+constexpr int linear_blocks(int format) {
+  return sizeof(kLinear) / sizeof(Blocks) - (format == NVM_MX_FP8);
+}
 // (SwiGLU: 32 outputs a block, which its scale needs: two tiles of each matrix.
 // 2048 -> 6144 of 32 rows 9.3 us on 192 blocks of 2 tiles of rows, 10.4 on 384 of
 // 1; 2048 -> 768 of 64 rows 6.5 on 96 of 1, 11.6 on 24 of 4)
@@ -228,18 +231,17 @@ hipError_t launch_tile(int tile, const MxMatmulArgs &a, hipStream_t st) {
 template <int FMT>
 hipError_t launch_fmt(int tile, bool dual, int out_format, const MxMatmulArgs &a,
                       hipStream_t st) {
-  constexpr int nl = sizeof(kLinear) / sizeof(Blocks), ns = sizeof(kSwiglu) / sizeof(Blocks);
+  constexpr int nl = linear_blocks(FMT), ns = sizeof(kSwiglu) / sizeof(Blocks);
   if (!dual) return launch_tile<FMT, NVM_MX_FP8, false, nl - 1>(tile, a, st);
   return out_format == NVM_MX_FP4 ? launch_tile<FMT, NVM_MX_FP4, true, ns - 1>(tile, a, st)
                                   : launch_tile<FMT, NVM_MX_FP8, true, ns - 1>(tile, a, st);
 }
 
-template <int COUNT>
-double best_of(const Blocks (&blocks)[COUNT], int format, bool dual, int64_t M, int N, int K,
+double best_of(const Blocks *blocks, int count, int format, bool dual, int64_t M, int N, int K,
                MxBlock *block) {
   const int64_t cus = cu_count();
   double best = INFINITY;
-  for (int i = 0; i < COUNT; ++i) {
+  for (int i = 0; i < count; ++i) {
     const Blocks &b = blocks[i];
     int64_t x, y;
     if (!grid_of(dual, b.rt, b.mt, M, K, x, y)) continue;
@@ -256,8 +258,9 @@ double best_of(const Blocks (&blocks)[COUNT], int format, bool dual, int64_t M, 
 }  // namespace
 
 double mx_gemv_time(int format, bool dual, int64_t M, int N, int K, MxBlock *block) {
-  return dual ? best_of(kSwiglu, format, dual, M, N, K, block)
-              : best_of(kLinear, format, dual, M, N, K, block);
+  constexpr int ns = sizeof(kSwiglu) / sizeof(Blocks);
+  return dual ? best_of(kSwiglu, ns, format, dual, M, N, K, block)
+              : best_of(kLinear, linear_blocks(format), format, dual, M, N, K, block);
 }
 
 hipError_t launch_mx_gemv(int format, int tile, bool dual, int out_format, const MxMatmulArgs &a,

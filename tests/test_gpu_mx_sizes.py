@@ -10,6 +10,7 @@ import ctypes
 import pytest
 import torch
 
+from mx_sizes import REACH
 from oracle import mx_oracle as O
 
 pytestmark = pytest.mark.gpu
@@ -103,3 +104,95 @@ def test_product_of_four_million_rows_of_few_columns(fmt):
     want, bound = _sums(va, _val(w), False)
     assert ((y[:part].double() - want).abs() <= bound).all()
     assert torch.equal(y.view(42, part, K), y[:part].expand(42, part, K))
+
+
+# ------------------------------------------------- every tile, every length of a row
+
+
+def _hostile(t):
+    """The tensor with NaN codes in the rows behind it, and NaN scales there and in
+    the padding of its rows."""
+    from nano_vllm_metal_amd import MxTensor
+
+    rows, blocks = t.scales.shape
+    codes = torch.full((rows + 3, t.codes.shape[1]), 0xFF, dtype=torch.uint8, device=DEV)
+    scales = torch.full((rows + 3, t.pitch + 16), 255, dtype=torch.uint8, device=DEV)
+    codes[:rows], scales[:rows, :blocks] = t.codes, t.scales
+    return MxTensor(codes[:rows], scales[:rows, :blocks], t.fmt)
+
+
+def _id(case):
+    gate_up, plan, fmt, _ = case
+    return f"{'gate_up' if gate_up else 'linear'}-{plan[0]}-{plan[1]}x{plan[2]}-{plan[3]}-{fmt}"
+
+
+@pytest.mark.parametrize("case", [c for c in REACH if not c[0]], ids=_id)
+def test_linear_on_every_tile(case):
+    from nano_vllm_metal_amd import _lib
+
+    _, plan, code, sizes = case
+    fmt, short = FMTS[code & 1], code > SHORT
+    for M, N, K in sizes:
+        print("size", M, N, K, flush=True)
+        assert _plan(0, M, N, K, fmt, short) == plan
+        g = _gen(M + N + K)
+        a, w = _random(g, M, N, fmt), _random(g, K, N, "mxfp4")
+        want, bound = _sums(_val(a), _val(w), short)
+        ah, wh = _hostile(a), _hostile(w)
+        for dtype, dt in ((2, torch.float32), (M % 2, (torch.float16, torch.bfloat16)[M % 2])):
+            out = torch.full((M + 2, K), 7.0, dtype=dt, device=DEV)
+            _lib.check(_lib.load().nvm_mx_matmul(
+                ah.codes.data_ptr(), ah.scales.data_ptr(), ah.pitch, code, wh.codes.data_ptr(),
+                wh.scales.data_ptr(), wh.pitch, M, N, K, dtype, out.data_ptr(),
+                _lib.stream_of(out.device)))
+            tol = bound + torch.finfo(dt).eps / 2 * (want.abs() + bound) + torch.finfo(dt).tiny
+            if dt == torch.float16:
+                big = want.abs() + bound > 65504
+                tol = torch.where(big, torch.full_like(tol, float("inf")), tol)
+            off = (out[:M].double() - want).abs()
+            assert (torch.nan_to_num(off, nan=float("inf"), posinf=1e300) <= tol).all()
+            assert (out[M:] == 7).all()
+
+
+@pytest.mark.parametrize("case", [c for c in REACH if c[0]], ids=_id)
+def test_gate_and_up_on_every_tile(case):
+    from nano_vllm_metal_amd import mx_swiglu
+
+    _, plan, code, sizes = case
+    fmt, short = FMTS[code & 1], code > SHORT
+    for M, N, K in sizes:
+        print("size", M, N, K, flush=True)
+        assert _plan(1, M, N, K, fmt, short) == plan
+        g = _gen(M + N + K)
+        a = _random(g, M, N, fmt, 117, 121)
+        wg, wu = _random(g, K, N, "mxfp4", 117, 121), _random(g, K, N, "mxfp4", 117, 121)
+        ofmt = FMTS[N // 32 % 2]
+        y = mx_swiglu(_hostile(a), _hostile(wg), _hostile(wu), ofmt, short)
+        (gate, eg), (up, eu) = _sums(_val(a), _val(wg), short), _sums(_val(a), _val(wu), short)
+        O.check_quantized(y.codes, y.scales, ofmt, *_silu_bound(gate, eg, up, eu))
+
+
+@pytest.mark.parametrize("M", [3, 70, 300])
+@pytest.mark.parametrize("fmt", FMTS)
+def test_blocks_of_different_scales_add_up(M, fmt):
+    """Bit for bit: a row has one value in each of four neighbouring blocks, whose
+    scales are 2^0, 2^5, 2^10 and 2^15.  E2M1 by E2M1, and E4M3 elements of 1 to 7 in
+    halves, are multiples of 1/4 up to 42: with the scales below 2^21 together."""
+    from nano_vllm_metal_amd import MxTensor, mx_linear
+
+    N, K = 672, 200
+    g = _gen(M)
+    w = _random(g, K, N, "mxfp4", 127, 128)
+    m = torch.arange(M, device=DEV)
+    grid = O.elements(fmt, DEV)
+    ok = ((grid * 2 == (grid * 2).round()) & (grid <= 7)).nonzero()[:, 0]
+    codes = torch.zeros(M, N, dtype=torch.int64, device=DEV)
+    scales = torch.full((M, N // 32), 127, dtype=torch.uint8, device=DEV)
+    for j in range(4):
+        block = (4 * (m % 5) + j) % (N // 32)
+        at = 32 * block + torch.randint(0, 32, (M,), device=DEV, generator=g)
+        sign = torch.randint(0, 2, (M,), device=DEV, generator=g) * O.SIGN[fmt]
+        codes[m, at] = ok[torch.randint(0, len(ok), (M,), device=DEV, generator=g)] + sign
+        scales[m, block] = 127 + 5 * ((j + m) % 4).to(torch.uint8)
+    a = MxTensor(O.pack(codes, fmt), scales, fmt)
+    assert torch.equal(mx_linear(a, w, torch.float32).double(), _val(a) @ _val(w).t())

@@ -99,3 +99,32 @@ def test_the_plan_refuses_what_the_products_refuse():
                           ((0, 4, 64, 8, 2, plan), -1, b"a format"), ((1, 4, 64, 8, 1, plan), -1, b"output"),
                           ((0, 2 ** 31, 64, 8, 1, plan), -2, b"large")]:
         assert lib.nvm_mx_product_plan(*args) == rc and msg in lib.nvm_last_error()
+
+
+def test_listed_sizes_reach_their_kernels():
+    """(tests/mx_sizes.py, which the GPU tests go through: a new fit that sends them
+    elsewhere shows here)"""
+    from mx_sizes import REACH
+
+    for gate_up, plan, fmt, sizes in REACH:
+        for M, N, K in sizes:
+            assert _plan(gate_up, M, N, K, fmt) == plan, (gate_up, M, N, K, fmt)
+    assert len({(g, p, f) for g, p, f, _ in REACH}) == len(REACH) == REACHED
+
+
+# every tile of every kernel for each of E2M1, E4M3 and E4M3 in short sums: seven
+# blocks (E4M3 six) and four for gate/up, four tiles and three, 256 x 256 in whole
+# tiles, halves and quarters
+REACHED = 3 * (7 + 4 + 4 + 3 + 3 + 3) - 1
+
+
+@pytest.mark.parametrize("fmt", [0, 1, SHORT | 1])
+def test_no_other_kernel_is_chosen(fmt):
+    from mx_sizes import REACH
+
+    known = {(g, p, f) for g, p, f, _ in REACH}
+    rng = random.Random(fmt + 1)
+    for _ in range(20000):
+        gate_up, M = rng.randint(0, 1), int(2 ** rng.uniform(0, 14))
+        N, K = 32 * int(2 ** rng.uniform(0, 9)), 32 * int(2 ** rng.uniform(0, 10))
+        assert (gate_up, _plan(gate_up, M, N, K, fmt), fmt) in known, (gate_up, M, N, K)
