@@ -188,15 +188,20 @@ __device__ __forceinline__ void mx_products(const MxFrag<NVM_MX_FP4> (&w)[TF],
   }
 }
 
-// g / (1 + exp(-g)) * u.  exp(-g) = 2^t 2^d with t = -g log2(e) rounded and d
-// what the rounding left (2^t is v_exp_f32, 1 ulp), the quotient by v_rcp_f32
-// (1 ulp): some 2^-21 in all, in 9 instructions for the 30 of the library's
-// exp and division.  Where exp overflows the result is zero; NaNs go through.
+// g / (1 + exp(-g)) * u.  exp(-g) = 2^t (1 + d ln 2) with t = -g log2(e) rounded
+// and d what was left of it, the rest of log2(e) beyond a float32 included (without
+// that the error grows with g, to 2^-19.7 at -87).  2^t is v_exp_f32 and the quotient
+// v_rcp_f32, 1 ulp each, so 2^-20.8 in all, in 12 instructions for the 30 of the
+// library's exp and division.  The quotient is taken of a quarter of the sum: of more
+// than 2^126 v_rcp_f32 gives zero.  Where exp overflows (g below -88.7) so does the
+// result.  Gates beyond 200 count as 200 in t, where 2^t is 0 or infinity already:
+// g log2(e) itself may leave float32's range.  NaNs go through.
 __device__ __forceinline__ float mx_swiglu(float g, float u) {
-  constexpr float kL = -1.44269504088896f, kLn2 = 0.69314718056f;
-  const float t = g * kL, d = __builtin_fmaf(g, kL, -t);
+  constexpr float kL = -0x1.715476p+0f, kLow = -0x1.4ae0cp-26f, kLn2 = 0.69314718056f;
+  const float c = __builtin_amdgcn_fmed3f(g, -200.f, 200.f);
+  const float t = c * kL, d = __builtin_fmaf(c, kLow, __builtin_fmaf(c, kL, -t));
   const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(d, kLn2, 1.f);
-  return g * __builtin_amdgcn_rcpf(1.f + e) * u;
+  return 0.25f * g * __builtin_amdgcn_rcpf(__builtin_fmaf(0.25f, e, 0.25f)) * u;
 }
 
 // Arguments of the products (gate/up: two weights, MX output).
