@@ -343,7 +343,8 @@ def mx_linear(x: Union[MxTensor, torch.Tensor], w: MxTensor,
     """``x . w^T (+ bias)``: ``x [..., N]`` in MX (16-bit activations are
     quantised to mxfp8 first), ``w [K, N]`` in mxfp4.  Float32 sums, one rounding to ``dtype``
     (float16, bfloat16 or float32; by default that of 16-bit activations, else
-    bfloat16).  ``short_sums``: mxfp8 activations are summed by the scaled matrix
+    bfloat16); ``bias [K]`` of any of these types is added to that, as by
+    ``quantized_linear``, and the sum rounded again.  ``short_sums``: mxfp8 activations are summed by the scaled matrix
     instruction itself, at about twice the rate for many rows, and some 2^-15 of
     a sum is lost (include/nvm_mx.h)."""
     lib = _lib.load()
@@ -357,7 +358,12 @@ def mx_linear(x: Union[MxTensor, torch.Tensor], w: MxTensor,
     if code is None:
         raise ValueError(f"mx_linear: dtype must be float16, bfloat16 or float32, got {dtype}")
     _check_weight("mx_linear", "w", w, a)
+    if bias is not None and (bias.shape != w.shape[:1] or bias.dtype not in MX_DTYPES):
+        raise ValueError(f"mx_linear: bias must be [{w.shape[0]}] of float16, bfloat16 or float32, "
+                         f"got {tuple(bias.shape)} of {bias.dtype}")
     index = _index(a._base, w._base)
+    if bias is not None and bias.get_device() != index:
+        _lib.require_device(a._base, bias)
     if index != _current_device():
         with torch.cuda.device(index):
             return mx_linear(a, w, dtype, bias, short_sums)
@@ -370,7 +376,7 @@ def mx_linear(x: Union[MxTensor, torch.Tensor], w: MxTensor,
     sums = _SHORT_SUMS if short_sums else 0
     _lib.check(lib.nvm_mx_matmul(ac, asc, a.pitch, MX_FORMATS[a.fmt] | sums, wc, wsc, w.pitch,
                                  a.rows, N, K, code, out.data_ptr(), _raw_stream(index)))
-    return out if bias is None else out + bias
+    return out if bias is None else (out + bias).to(dtype)
 
 
 def mx_swiglu(x: Union[MxTensor, torch.Tensor], w_gate: MxTensor, w_up: MxTensor,

@@ -234,3 +234,25 @@ def test_a_model_in_short_sums():
         _, x = residual_rms_norm(h, y, m.norm, eps)
         assert torch.equal(got[short], mx_linear(x, m.lm_head, **kw))
     assert not torch.equal(got[False], got[True])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("bias_dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("M", [1, 70])
+def test_bias_of_any_type_leaves_the_output_type(M, dtype, bias_dtype):
+    """The product's rounding and the sum's: eps / 2 of each, and of the bias, which the
+    sum takes as it is, none."""
+    from nano_vllm_metal_amd import mx_linear
+
+    g = _gen(M)
+    a, w = _tensor(_codes(g, M, 96, "mxfp8"), 122, "mxfp8"), _tensor(_codes(g, 40, 96, "mxfp4"), 124,
+                                                                    "mxfp4")
+    b = (100 * torch.randn(40, device=DEV, generator=g)).to(bias_dtype)
+    plain, y = mx_linear(a, w, dtype), mx_linear(a, w, dtype, b)
+    assert y.dtype == dtype and y.shape == (M, 40)
+    want = plain.double() + b.double()
+    # (float32's own rounding of the sum comes first)
+    tol = (torch.finfo(dtype).eps / 2 + 2.0 ** -24) * want.abs() * (1 + 2.0 ** -7)
+    assert ((y.double() - want).abs() <= tol + torch.finfo(dtype).tiny).all()
+    row = mx_linear(type(a)(a.codes[0], a.scales[0], "mxfp8"), w, dtype, b)
+    assert row.shape == (40,) and row.dtype == dtype

@@ -7,6 +7,7 @@ import ctypes
 import random
 
 import pytest
+import torch
 
 P = 1 << 20  # a 16-byte aligned address
 SHORT = 16   # NVM_MX_SHORT_SUMS
@@ -128,3 +129,20 @@ def test_no_other_kernel_is_chosen(fmt):
         gate_up, M = rng.randint(0, 1), int(2 ** rng.uniform(0, 14))
         N, K = 32 * int(2 ** rng.uniform(0, 9)), 32 * int(2 ** rng.uniform(0, 10))
         assert (gate_up, _plan(gate_up, M, N, K, fmt), fmt) in known, (gate_up, M, N, K)
+
+
+@pytest.mark.parametrize("shape,dtype", [((31,), torch.bfloat16), ((1, 32), torch.bfloat16),
+                                         ((3, 32), torch.float32), ((3, 1), torch.float32),
+                                         ((), torch.float32), ((1,), torch.float16),
+                                         ((32,), torch.int32), ((32,), torch.float64)])
+def test_linear_refuses_what_is_no_bias(shape, dtype):
+    from nano_vllm_metal_amd import MxTensor, mx_linear
+
+    def mx(rows, fmt):
+        codes = torch.zeros(rows, 64 if fmt == "mxfp8" else 32, dtype=torch.uint8)
+        return MxTensor(codes, torch.full((rows, 2), 127, dtype=torch.uint8), fmt)
+
+    with pytest.raises(ValueError, match="bias must be"):
+        mx_linear(mx(3, "mxfp8"), mx(32, "mxfp4"), bias=torch.zeros(shape, dtype=dtype))
+    with pytest.raises(ValueError, match="GPU only"):  # (a good one: the next check)
+        mx_linear(mx(3, "mxfp8"), mx(32, "mxfp4"), bias=torch.zeros(32))
