@@ -1,7 +1,7 @@
 /*
  * C ABI of the microscaled (MX) path: quantisation to block-scaled 4- and
  * 8-bit floating point, products of MX activations with MXFP4 weights on the
- * scaled matrix instructions, and the layer steps that hand MX activations on
+ * matrix cores, and the layer steps that hand MX activations on
  * (RMSNorm, SwiGLU).  In the same library and with the same conventions as
  * nvm_moe.h: device pointers, work on `stream`, no host synchronisation, no
  * device allocation, no workspace, NVM_OK or a negative NVM_ERR_* status
