@@ -235,6 +235,8 @@ def mx_quantize(x: torch.Tensor, fmt: str = "mxfp8") -> MxTensor:
 def mx_dequantize(t: MxTensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """The values that ``t`` stands for, rounded once to ``dtype``."""
     lib = _lib.load()
+    if type(t) is not MxTensor:
+        raise ValueError("mx_dequantize: t must be an MxTensor")
     dev = _lib.require_device(t._base)
     code = MX_DTYPES.get(dtype)
     if code is None:

@@ -146,3 +146,11 @@ def test_linear_refuses_what_is_no_bias(shape, dtype):
         mx_linear(mx(3, "mxfp8"), mx(32, "mxfp4"), bias=torch.zeros(shape, dtype=dtype))
     with pytest.raises(ValueError, match="GPU only"):  # (a good one: the next check)
         mx_linear(mx(3, "mxfp8"), mx(32, "mxfp4"), bias=torch.zeros(32))
+
+
+def test_dequantize_refuses_what_is_no_mx_tensor():
+    from nano_vllm_metal_amd import mx_dequantize
+
+    for t in (torch.zeros(3, 64, dtype=torch.uint8), None):
+        with pytest.raises(ValueError, match="must be an MxTensor"):
+            mx_dequantize(t)
