@@ -26,8 +26,8 @@
 //    behind the row replaced by zeros and scales by one in registers, so what
 //    lies there does not matter (a weight code is finite whatever its bits).
 //
-// 8192 x 8192 x 8192: 743 us, 1.48 PFLOP/s, the rate of a bf16 library product
-// there (1.41); E2M1 293 us, 3.75; short sums 367 us, 3.0.  4096 rows of 2048
+// 8192 x 8192 x 8192: 729 us, 1.5 PFLOP/s, as a bf16 library product there (732);
+// E2M1 293 us, 3.75; short sums 367 us, 3.0.  4096 rows of 2048
 // through a gate/up pair of 6144: 153 us, 1.35 PFLOP/s; short sums 84 us, 2.5.
 #include "mx_pipe.h"
 

@@ -196,8 +196,9 @@ hipError_t go(const MxMatmulArgs &a, hipStream_t st) {
 // takes kLeastRound, however short the rows (in short sums 32 -> 2048 of 2048 rows,
 // 11 rounds of 3 x 2 tiles: 17.3 us).  Larger blocks read the activations, and a
 // column of them the weights, less often, but a round of them is longer: 4096 ->
-// 4096 of 128 rows 14.3 us on 256 blocks of 4 x 2 tiles, 16.5 on 512 of 2 x 2, 20.1 on 1024 of 2 x 1; 2048 -> 2048 of 32 rows 4.2 on 256 of 1 x
-// 1, 4.7 on 128 of 2 x 1, 6.5 on 64 of 2 x 2.
+// 4096 of 128 rows 14.3 us on 256 blocks of 4 x 2 tiles, 16.5 on 512 of 2 x 2, 20.1
+// on 1024 of 2 x 1; 2048 -> 2048 of 32 rows 4.2 on 256 of 1 x 1, 4.7 on 128 of 2 x
+// 1, 6.5 on 64 of 2 x 2.
 constexpr double kLeastRound = 1.8;
 struct Blocks {
   int rt, mt;

@@ -347,8 +347,8 @@ def mx_linear(x: Union[MxTensor, torch.Tensor], w: MxTensor,
     (float16, bfloat16 or float32; by default that of 16-bit activations, else
     bfloat16); ``bias [K]`` of any of these types is added to that, as by
     ``quantized_linear``, and the sum rounded again.  ``short_sums``: mxfp8 activations are summed by the scaled matrix
-    instruction itself, at about twice the rate for many rows, and some 2^-15 of
-    a sum is lost (include/nvm_mx.h)."""
+    instruction itself, at about twice the rate for many rows, and 2^-17 to
+    2^-15 of a sum is lost, in a float32 output too (include/nvm_mx.h)."""
     lib = _lib.load()
     if type(x) is MxTensor:
         a = x

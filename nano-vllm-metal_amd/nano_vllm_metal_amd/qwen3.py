@@ -204,7 +204,7 @@ class Qwen3Model:
         self.lm_head = lm_head
         self.dtype = dtype
         # products of MX weights in the matrix instruction's own sums (``mx_linear``):
-        # prefill in less time, for some 2^-15 of each sum (to be set before an LLM
+        # prefill in less time, for 2^-17 to 2^-15 of each sum (to be set before an LLM
         # captures its steps)
         self.short_sums = False
         self.device = embed.device if isinstance(embed, MxTensor) else embed.weight.device
