@@ -238,4 +238,10 @@ int mx_check_tensor(const char *op, const void *codes, const uint8_t *scales, in
 hipError_t launch_combine(int dtype, const void *down, const void *scores, int64_t T, int k,
                           int64_t H, void *y, hipStream_t st);
 
+// Pages of the 4-bit cache (mx_cache.hip): sizes, null pointers and alignment,
+// as a status with its message.
+int mx_check_pages(const char *op, int Hkv, int64_t D, int64_t P, int64_t page_size,
+                   const void *key_codes, const void *key_scales, const void *value_codes,
+                   const void *value_scales);
+
 }  // namespace nvm

@@ -74,6 +74,18 @@ __device__ __forceinline__ uint32_t absmax8(const float (&x)[8]) {
   return m;
 }
 
+// A float64 value as a float32 that rounds to an element as the float64 value
+// itself does: rounded to odd, so a value next to a tie stays off it.
+__device__ __forceinline__ float round_to_odd(double d) {
+  const float t = (float)d;
+  const double r = d - (double)t;
+  const uint32_t b = __float_as_uint(t);
+  // an even float32 beside the exact value: its neighbour on the value's side
+  if (r != 0.0 && !(b & 1u) && (b & 0x7F800000u) != 0x7F800000u)
+    return __uint_as_float((r > 0.0) == (d > 0.0) ? b + 1u : b - 1u);
+  return t;
+}
+
 // Operands of a 16 x 16 x 128 product, row or column lane % 16.  Lane group G =
 // lane / 16 passes the scale of k-values 32 G .. 32 G + 31, and holds these, 16
 // bytes of E2M1 or 32 of E4M3.  Only where E4M3 goes into the scaled matrix

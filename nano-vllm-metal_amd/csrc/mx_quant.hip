@@ -130,18 +130,6 @@ __global__ __launch_bounds__(kThreads) void mx_dequantize_kernel(
   }
 }
 
-// A float64 value as a float32 that rounds to an element as the float64 value
-// itself does: rounded to odd, so a value next to a tie stays off it.
-__device__ __forceinline__ float round_to_odd(double d) {
-  const float t = (float)d;
-  const double r = d - (double)t;
-  const uint32_t b = __float_as_uint(t);
-  // an even float32 beside the exact value: its neighbour on the value's side
-  if (r != 0.0 && !(b & 1u) && (b & 0x7F800000u) != 0x7F800000u)
-    return __uint_as_float((r > 0.0) == (d > 0.0) ? b + 1u : b - 1u);
-  return t;
-}
-
 // Residual add, RMSNorm and quantisation, a row per block of NT threads of NC
 // 8-value chunks; every load of the row, of the residual and of the weights
 // goes out before the first is used.  The sum of squares, its root and the

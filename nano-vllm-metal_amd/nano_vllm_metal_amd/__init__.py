@@ -7,7 +7,8 @@ Public names mirror the reference's package root for this path
 (``layers/attention.py:154``), the Qwen3 model with its paged KV cache and
 ``LLM``/``SamplingParams`` (``llm.py``).  Beyond the reference: the microscaled
 path (``mx.py``), ``MxTensor`` weights in ``mxfp4`` with activations in eight or
-four bits, on its own and in the model's dense layers.  All compute runs in HIP kernels on the GPU
+four bits, on its own and in the model's dense layers, and the KV cache in four
+bits (``mx_cache.py``).  All compute runs in HIP kernels on the GPU
 (libnvm_moe.so); nothing falls back to the CPU.
 """
 
@@ -17,6 +18,7 @@ from .loader import load_moe_block, load_moe_blocks, read_config, sparse_layers
 from .attention import paged_attention
 from .mx import (MxTensor, mx_dequantize, mx_embedding, mx_linear, mx_quantize, mx_swiglu,
                  residual_rms_norm_mx)
+from .mx_cache import MxPages, paged_attention_mx, paged_kv_read_mx, qk_norm_rope_store_mx
 from .kv_cache import PagedKVCache
 from .qwen3 import Qwen3Config, Qwen3Model, qwen3_30b_a3b_config
 from .llm import LLM, GenerationOutput, SamplingParams
@@ -44,6 +46,10 @@ __all__ = [
     "mx_linear",
     "mx_swiglu",
     "residual_rms_norm_mx",
+    "MxPages",
+    "qk_norm_rope_store_mx",
+    "paged_kv_read_mx",
+    "paged_attention_mx",
     "PagedKVCache",
     "Qwen3Config",
     "Qwen3Model",

@@ -71,6 +71,13 @@ SIGNATURES = {
     "nvm_mx_swiglu": [_P, _P, _I64, _I, _P, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _I, _P, _P,
                       _I64, _P],
     "nvm_mx_product_plan": [_I, _I64, _I64, _I64, _I, ctypes.POINTER(_I)],
+    "nvm_qk_norm_rope_store_mx": [_P, _I64, _I, _I, _I64, _P, _P, ctypes.c_float, _P, _P, _P, _I64,
+                                  _P, _P, _P, _P, _P, _P, _I64, _I64, _I, _I, _P, _P, _P, _P],
+    "nvm_paged_kv_read_mx": [_P, _P, _P, _P, _I64, _I, _I64, _I64, _P, _P, _I64, _I, _P, _P, _P],
+    "nvm_paged_attention_mx_workspace_size": [_I64, _I64, _I64, _I64, _I64, _I, _I,
+                                              ctypes.POINTER(_SZ)],
+    "nvm_paged_attention_mx": [_P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64,
+                               _I64, _P, _I64, _P, ctypes.c_float, _I, _I, _I, _I, _P, _P, _SZ, _P],
     "nvm_moe_forward_residual_norm": [_P, _I64, _I64, _I64, _I64, _I, _I, _I, _I, _I,
                                       _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                       _P, _P, ctypes.c_float, _P, _P, _I, _P, _SZ, _P],
