@@ -19,6 +19,7 @@ from .attention import paged_attention
 from .mx import (MxTensor, mx_dequantize, mx_embedding, mx_linear, mx_quantize, mx_swiglu,
                  residual_rms_norm_mx)
 from .mx_cache import MxPages, paged_attention_mx, paged_kv_read_mx, qk_norm_rope_store_mx
+from .logprobs import TokenLogprobs, token_logprobs
 from .kv_cache import PagedKVCache
 from .qwen3 import Qwen3Config, Qwen3Model, qwen3_30b_a3b_config
 from .llm import LLM, GenerationOutput, SamplingParams
@@ -50,6 +51,8 @@ __all__ = [
     "qk_norm_rope_store_mx",
     "paged_kv_read_mx",
     "paged_attention_mx",
+    "TokenLogprobs",
+    "token_logprobs",
     "PagedKVCache",
     "Qwen3Config",
     "Qwen3Model",

@@ -78,6 +78,8 @@ SIGNATURES = {
                                               ctypes.POINTER(_SZ)],
     "nvm_paged_attention_mx": [_P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64,
                                _I64, _P, _I64, _P, ctypes.c_float, _I, _I, _I, _I, _P, _P, _SZ, _P],
+    "nvm_token_logprobs_workspace_size": [_I64, _I64, _I, _I, ctypes.POINTER(_SZ)],
+    "nvm_token_logprobs": [_P, _I64, _I64, _I64, _I, _P, _I, _P, _P, _P, _P, _P, _SZ, _P],
     "nvm_moe_forward_residual_norm": [_P, _I64, _I64, _I64, _I64, _I, _I, _I, _I, _I,
                                       _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                       _P, _P, ctypes.c_float, _P, _P, _I, _P, _SZ, _P],
