@@ -22,7 +22,7 @@ from .mx_cache import MxPages, paged_attention_mx, paged_kv_read_mx, qk_norm_rop
 from .logprobs import TokenLogprobs, token_logprobs
 from .kv_cache import PagedKVCache
 from .qwen3 import Qwen3Config, Qwen3Model, qwen3_30b_a3b_config
-from .llm import LLM, GenerationOutput, SamplingParams
+from .llm import LLM, GenerationOutput, SamplingParams, TokenLogprob
 
 __all__ = [
     "QuantizedWeights",
@@ -60,4 +60,5 @@ __all__ = [
     "LLM",
     "SamplingParams",
     "GenerationOutput",
+    "TokenLogprob",
 ]

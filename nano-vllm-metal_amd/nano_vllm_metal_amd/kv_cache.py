@@ -7,37 +7,52 @@ a pool holds ``key_pages``/``value_pages [P, num_kv_heads, page_size, D]``;
 token ``j`` of a request lives in slot ``j % page_size`` of the request's page
 ``j // page_size``.  Here every pool is allocated once at its full size (HBM
 is large) instead of grown geometrically, and one free list serves all layers
-(a request holds the same page ids in every layer).  Prefix caching and int8
-pages are not built.
+(a request holds the same page ids in every layer).  ``kv_bits`` 4 holds pages
+in MXFP4 (``MxPages``, 4.25 bits a value; the reference's quantised cache has
+eight).  Prefix caching and int8 pages are not built.
 """
 
 from __future__ import annotations
 
-from typing import Dict, List, Sequence
+from typing import Dict, List, Sequence, Tuple
 
 import torch
+
+from .mx import mx_quantize
+from .mx_cache import MxPages, paged_kv_read_mx
 
 
 class PagedKVCache:
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int,
-                 page_size: int, dtype: torch.dtype = torch.bfloat16, device="cuda"):
+                 page_size: int, dtype: torch.dtype = torch.bfloat16, device="cuda",
+                 kv_bits: int = 16):
         if num_pages <= 0 or page_size <= 0:
             raise ValueError("PagedKVCache: num_pages and page_size must be positive")
+        if kv_bits not in (4, 16):
+            raise ValueError(f"PagedKVCache: kv_bits must be 4 or 16, got {kv_bits}")
+        if kv_bits == 4 and (head_dim % 32 or not 0 < head_dim <= 256):
+            raise ValueError(f"PagedKVCache: kv_bits=4 needs a head dim that is a multiple of 32, at "
+                             f"most 256, got {head_dim}")
         self.num_layers = num_layers
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
         self.num_pages = num_pages
         self.page_size = page_size
         self.dtype = dtype
+        self.kv_bits = kv_bits
         self.device = torch.device(device)
         # one page past the pool takes the writes of padding rows and of
         # graph warm-up/capture runs; it is never handed to a request
         self.scratch_page = num_pages
         shape = (num_pages + 1, num_kv_heads, page_size, head_dim)
-        self.key_pages = [torch.zeros(shape, dtype=dtype, device=self.device)
-                          for _ in range(num_layers)]
-        self.value_pages = [torch.zeros(shape, dtype=dtype, device=self.device)
-                            for _ in range(num_layers)]
+
+        def pool():
+            if kv_bits == 4:
+                return MxPages.zeros(*shape, device=self.device)
+            return torch.zeros(shape, dtype=dtype, device=self.device)
+
+        self.key_pages = [pool() for _ in range(num_layers)]
+        self.value_pages = [pool() for _ in range(num_layers)]
         self._free: List[int] = list(range(num_pages - 1, -1, -1))
         self.pages: Dict[int, List[int]] = {}
         self.lens: Dict[int, int] = {}
@@ -96,8 +111,23 @@ class PagedKVCache:
         kk = k.reshape(-1, self.num_kv_heads, self.head_dim).to(self.dtype)
         vv = v.reshape(-1, self.num_kv_heads, self.head_dim).to(self.dtype)
         page_ids, slots = page_ids.long(), slots.long()
-        self.key_pages[layer][page_ids, :, slots, :] = kk
-        self.value_pages[layer][page_ids, :, slots, :] = vv
+        for pages, x in ((self.key_pages[layer], kk), (self.value_pages[layer], vv)):
+            if self.kv_bits == 4:
+                t = mx_quantize(x, "mxfp4")
+                pages.codes[page_ids, :, slots] = t.codes
+                pages.scales[page_ids, :, slots] = t.scales
+            else:
+                pages[page_ids, :, slots, :] = x
+
+    def read(self, layer: int, page_ids: torch.Tensor, slots: torch.Tensor
+             ) -> Tuple[torch.Tensor, torch.Tensor]:
+        """What the mapped slots hold: ``k, v [T, num_kv_heads, D]`` of the
+        cache's dtype."""
+        kp, vp = self.key_pages[layer], self.value_pages[layer]
+        if self.kv_bits == 4:
+            return paged_kv_read_mx(kp, vp, page_ids, slots, self.dtype)
+        page_ids, slots = page_ids.long(), slots.long()
+        return kp[page_ids, :, slots, :], vp[page_ids, :, slots, :]
 
     def advance(self, seq_ids: Sequence[int], n_new: int) -> None:
         for s in seq_ids:

@@ -9,7 +9,9 @@ chunks of ``prefill_step``); then every running request decodes one
 token in a single batched step; a request that reaches ``max_tokens`` (or its
 end-of-sequence token) is retired and its pages freed.  Sampling follows
 ``layers/sampler.py``: greedy at temperature 0, else temperature with top-k
-and top-p filtering.
+and top-p filtering.  Beyond the reference: ``SamplingParams.logprobs`` and
+``LLM.score`` say how probable generated or given tokens were, and ``kv_bits``
+4 keeps the cache in MXFP4 (its quantised cache has eight bits).
 
 Prompts are token-id lists, or strings when a tokenizer is given (or found in
 the checkpoint directory; loaded with ``local_files_only``, no hub access).
@@ -20,23 +22,39 @@ from __future__ import annotations
 import time
 from collections import deque
 from dataclasses import dataclass, field
-from typing import List, Optional, Sequence, Union
+from typing import List, Optional, Sequence, Tuple, Union
 
 import torch
 
+from .logprobs import MAX_TOP_LOGPROBS, TokenLogprobs, token_logprobs
 from .moe import Moe
 from .qwen3 import Qwen3Model, StepInputs
 
 
 @dataclass
 class SamplingParams:
-    """Decoding controls (``sampling_params.py``): temperature 0 is greedy."""
+    """Decoding controls (``sampling_params.py``): temperature 0 is greedy.
+    ``logprobs``: report each generated token's log probability, with so many (0
+    to 64) of the most probable tokens; of the model's own distribution, before
+    temperature, top-k and top-p."""
 
     max_tokens: int = 64
     temperature: float = 0.0
     top_p: float = 0.0
     top_k: Optional[int] = None
     ignore_eos: bool = False
+    logprobs: Optional[int] = None
+
+
+@dataclass
+class TokenLogprob:
+    """One token: its log probability where the model put it, the entropy of the
+    distribution there (nats), and the most probable tokens."""
+
+    token_id: int
+    logprob: float
+    entropy: float
+    top: List[Tuple[int, float]] = field(default_factory=list)
 
 
 @dataclass
@@ -44,6 +62,7 @@ class GenerationOutput:
     prompt: Union[str, List[int]]
     text: str
     token_ids: List[int] = field(default_factory=list)
+    logprobs: Optional[List[TokenLogprob]] = None
 
 
 @dataclass
@@ -71,6 +90,28 @@ def sample(logits: torch.Tensor, sp: SamplingParams, generator=None) -> torch.Te
         lp = torch.full_like(lp, -float("inf")).scatter(-1, idx, srt)
     probs = torch.softmax(lp / sp.temperature, dim=-1)
     return torch.multinomial(probs, 1, generator=generator)[:, 0]
+
+
+def _records(tokens: List[int], r: TokenLogprobs) -> List[TokenLogprob]:
+    return [TokenLogprob(t, lp, ent, list(zip(ids, top)))
+            for t, lp, ent, ids, top in zip(tokens, r.logprobs.tolist(), r.entropy.tolist(),
+                                            r.top_ids.tolist(), r.top_logprobs.tolist())]
+
+
+def _pick(logits: torch.Tensor, sp: SamplingParams):
+    """Next token per row, and its record if ``sp`` asks for one (else None)."""
+    nxt = sample(logits, sp)
+    if sp.logprobs is None:
+        tokens = nxt.tolist()
+        return tokens, [None] * len(tokens)
+    r = token_logprobs(logits, nxt, sp.logprobs)
+    tokens = nxt.tolist()
+    return tokens, _records(tokens, r)
+
+
+def _check_top(name: str, n: Optional[int], vocab: int) -> None:
+    if n is not None and not 0 <= n <= min(MAX_TOP_LOGPROBS, vocab):
+        raise ValueError(f"{name} must be in [0, {min(MAX_TOP_LOGPROBS, vocab)}], got {n}")
 
 
 class _DecodeGraph:
@@ -112,18 +153,25 @@ class _Request:
         self.ids = list(ids)
         self.sp = sp
         self.out: List[int] = []
+        self.logprobs: List[TokenLogprob] = []
         self.done = False
+
+    def append(self, token: int, record: Optional[TokenLogprob]) -> None:
+        self.out.append(token)
+        if record is not None:
+            self.logprobs.append(record)
 
 
 class LLM:
-    """``LLM(model, max_num_seqs=8, max_model_len=4096, page_size=16)``.
+    """``LLM(model, max_num_seqs=8, max_model_len=4096, page_size=16, kv_bits=16)``.
 
-    ``model`` is a checkpoint directory or a ready ``Qwen3Model``."""
+    ``model`` is a checkpoint directory or a ready ``Qwen3Model``; ``kv_bits`` 4
+    keeps keys and values in MXFP4, in 4.25 bits a value."""
 
     def __init__(self, model: Union[str, Qwen3Model], max_num_seqs: int = 8,
                  max_model_len: int = 4096, page_size: int = 16, prefill_step: int = 2048,
                  tokenizer=None, device="cuda", dtype: torch.dtype = torch.bfloat16,
-                 eos_token_id: Optional[int] = None, use_graphs: bool = True):
+                 eos_token_id: Optional[int] = None, use_graphs: bool = True, kv_bits: int = 16):
         if isinstance(model, Qwen3Model):
             self.model = model
         else:
@@ -136,7 +184,8 @@ class LLM:
         self.prefill_step = prefill_step
         pages_per_seq = -(-max_model_len // page_size)
         self.pages_per_seq = pages_per_seq
-        self.cache = self.model.create_kv_cache(max_num_seqs * pages_per_seq, page_size)
+        self.cache = self.model.create_kv_cache(max_num_seqs * pages_per_seq, page_size,
+                                                kv_bits)
         # decode steps replay HIP graphs (one per batch size).  The MoE
         # workspaces are sized for the largest step first, so a captured graph
         # never refers to a buffer that a later, larger call reallocates.
@@ -183,10 +232,10 @@ class LLM:
         cache.advance(seq_ids, 1)
         return logits
 
-    def _prefill(self, batch: List[_Request]) -> List[int]:
+    def _prefill(self, batch: List[_Request]):
         """Prefill requests of one prompt length together (B x L tokens, at
         most ``prefill_step``), or one long prompt in chunks; returns the first
-        sampled token of each."""
+        sampled token of each, and their records."""
         m, cache = self.model, self.cache
         for r in batch:
             cache.add(r.rid)
@@ -201,7 +250,7 @@ class LLM:
                                      device=m.device)
                 logits = m.forward(chunk, cache, [r.rid])
         self.stats.prefill_tokens += L * len(batch)
-        return [int(t) for t in sample(logits, batch[0].sp).tolist()]
+        return _pick(logits, batch[0].sp)
 
     def _admit(self, waiting: deque, running: List[_Request]) -> None:
         """Admit waiting requests while a sequence slot is free, prefill them
@@ -223,11 +272,11 @@ class LLM:
                 batch = group[i:i + per]
                 torch.cuda.synchronize(self.model.device)
                 t0 = time.perf_counter()
-                toks = self._prefill(batch)
+                toks, records = self._prefill(batch)
                 torch.cuda.synchronize(self.model.device)
                 self.stats.prefill_s += time.perf_counter() - t0
-                for r, tok in zip(batch, toks):
-                    r.out.append(tok)
+                for r, tok, record in zip(batch, toks, records):
+                    r.append(tok, record)
                     if self._finished(r, tok):
                         r.done = True
                         cache.free(r.rid)
@@ -239,6 +288,7 @@ class LLM:
         if isinstance(prompts, (str,)) or (len(prompts) and isinstance(prompts[0], int)):
             prompts = [prompts]
         sp = sampling_params or SamplingParams()
+        _check_top("SamplingParams.logprobs", sp.logprobs, self.model.config.vocab_size)
         reqs = [_Request(i, p, self._encode(p), sp) for i, p in enumerate(prompts)]
         for r in reqs:
             if not r.ids:
@@ -256,20 +306,55 @@ class LLM:
             t0 = time.perf_counter()
             last = torch.tensor([[r.out[-1]] for r in running], dtype=torch.long, device=m.device)
             logits = self._decode_step(last, [r.rid for r in running])
-            nxt = sample(logits, sp).tolist()
+            nxt, records = _pick(logits, sp)
             self.stats.decode_s += time.perf_counter() - t0
             self.stats.decode_steps += 1
             self.stats.decode_tokens += len(running)
             still = []
-            for r, tok in zip(running, nxt):
-                r.out.append(int(tok))
-                if self._finished(r, int(tok)):
+            for r, tok, record in zip(running, nxt, records):
+                r.append(tok, record)
+                if self._finished(r, tok):
                     r.done = True
                     cache.free(r.rid)
                 else:
                     still.append(r)
             running = still
-        return [GenerationOutput(r.prompt, self._detok(r.out), r.out) for r in reqs]
+        return [GenerationOutput(r.prompt, self._detok(r.out), r.out,
+                                 None if sp.logprobs is None else r.logprobs) for r in reqs]
+
+    def score(self, prompts: Union[str, Sequence], top: int = 0) -> List[List[TokenLogprob]]:
+        """How probable the model finds each prompt's own tokens, from the second
+        on, given those before: their log probabilities, the entropies, and the
+        ``top`` (0 to 64) most probable tokens in each one's place.  The sum over a
+        prompt is its log likelihood.  Prompts go through the model one by one, in
+        steps of ``prefill_step`` tokens."""
+        if isinstance(prompts, (str,)) or (len(prompts) and isinstance(prompts[0], int)):
+            prompts = [prompts]
+        m, cache = self.model, self.cache
+        _check_top("score: top", top, m.config.vocab_size)
+        encoded = [self._encode(p) for p in prompts]
+        for ids in encoded:
+            if not ids:
+                raise ValueError("empty prompt")
+            if len(ids) > self.max_model_len:
+                raise ValueError(f"prompt of {len(ids)} tokens exceeds max_model_len")
+        out = []
+        for ids in encoded:
+            records: List[TokenLogprob] = []
+            rid = -1  # (generate counts its requests from zero)
+            cache.add(rid)
+            try:
+                for s in range(0, len(ids) - 1, self.prefill_step):
+                    given = ids[s:min(s + self.prefill_step, len(ids) - 1)]
+                    after = ids[s + 1:s + 1 + len(given)]
+                    logits = m.forward(torch.tensor([given], dtype=torch.long, device=m.device),
+                                       cache, [rid], last_only=False)[0]
+                    tokens = torch.tensor(after, dtype=torch.long, device=m.device)
+                    records += _records(after, token_logprobs(logits, tokens, top))
+            finally:
+                cache.free(rid)
+            out.append(records)
+        return out
 
 
 def _local_tokenizer(path):

@@ -29,6 +29,10 @@ stored in 16 bits: norm -> q/k/v product, and norm -> gate/up -> down product;
 the attention's output and the lm head's input are quantised by ``mx_linear``.
 So every product with such weights has activations of eight bits (E4M3, four
 significant ones); q, k and v are of one kind, and so are gate, up and down.
+
+A cache of ``kv_bits`` 4 (``create_kv_cache``) holds keys and values in MXFP4
+(``mx_cache.py``): every later step attends over what the pages stand for, the
+initial prefill over its own keys and values before they are quantised.
 """
 
 from __future__ import annotations
@@ -46,6 +50,7 @@ from .kv_cache import PagedKVCache
 from .linear import (QuantizedWeights, quantized_linear, quantized_swiglu,
                      swiglu_supports)
 from .moe import Moe
+from .mx_cache import MxPages, paged_attention_mx, qk_norm_rope_store_mx
 from .mx import (MxTensor, mx_embedding, mx_linear, mx_stack_outputs, mx_swiglu,
                  residual_rms_norm_mx)
 
@@ -216,10 +221,12 @@ class Qwen3Model:
 
     # ---------------------------------------------------------------- pieces
 
-    def create_kv_cache(self, num_pages: int, page_size: int = 16) -> PagedKVCache:
+    def create_kv_cache(self, num_pages: int, page_size: int = 16,
+                        kv_bits: int = 16) -> PagedKVCache:
+        """A page pool for each layer; ``kv_bits`` 16 (the model's dtype) or 4."""
         c = self.config
         return PagedKVCache(c.num_hidden_layers, c.num_key_value_heads, c.head_dim, num_pages,
-                            page_size, self.dtype, self.device)
+                            page_size, self.dtype, self.device, kv_bits)
 
     def embed(self, tokens: torch.Tensor) -> torch.Tensor:
         """``QuantizedEmbedding`` (layers/embed_head.py:21-36): dequantised rows
@@ -237,12 +244,19 @@ class Qwen3Model:
         B, L, _ = x.shape
         Hq, Hkv, D = c.num_attention_heads, c.num_key_value_heads, c.head_dim
         qkv = linear(x, layer.wqkv, self.dtype, self.short_sums)
-        q, k, v = qk_norm_rope_store(qkv, Hq, Hkv, D, layer.q_norm, layer.k_norm, c.rms_norm_eps,
-                                     step.positions, self.rope.cos, self.rope.sin, step.page_ids,
-                                     step.slots, cache.key_pages[li], cache.value_pages[li],
-                                     want_kv=step.initial)
+        kp, vp = cache.key_pages[li], cache.value_pages[li]
+        mx = isinstance(kp, MxPages)
+        dense = step.initial and causal_attention_supports(Hq, Hkv, D)
+        heads = (qkv, Hq, Hkv, D, layer.q_norm, layer.k_norm, c.rms_norm_eps, step.positions,
+                 self.rope.cos, self.rope.sin, step.page_ids, step.slots, kp, vp)
+        if mx:
+            # (causal_attention takes its operands in float32)
+            q, k, v = qk_norm_rope_store_mx(*heads, want_kv=dense,
+                                            out_dtype=torch.float32 if dense else None)
+        else:
+            q, k, v = qk_norm_rope_store(*heads, want_kv=step.initial)
         scale = D ** -0.5
-        if step.initial and causal_attention_supports(Hq, Hkv, D):
+        if dense:
             # every request starts from an empty cache: causal attention over
             # the new tokens only (models/qwen3.py:134-141); the grouped query
             # heads share each key/value read
@@ -251,9 +265,13 @@ class Qwen3Model:
             o = o.reshape(B, L, Hq * D)
         else:
             # (the k/v of an initial step are in the pages as well)
-            o = paged_attention(q.view(B, L, Hq, D).transpose(1, 2), cache.key_pages[li],
-                                cache.value_pages[li], step.block_table, step.lens,
-                                cache.page_size, scale=scale, mask="causal", out_dtype=qkv.dtype)
+            q = q.view(B, L, Hq, D).transpose(1, 2)
+            if mx:
+                o = paged_attention_mx(q, kp, vp, step.block_table, step.lens, scale=scale,
+                                       mask="causal")
+            else:
+                o = paged_attention(q, kp, vp, step.block_table, step.lens, cache.page_size,
+                                    scale=scale, mask="causal", out_dtype=qkv.dtype)
             o = o.transpose(1, 2).reshape(B, L, Hq * D)
         return linear(o, layer.wo, short_sums=self.short_sums)
 
