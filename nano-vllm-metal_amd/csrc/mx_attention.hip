@@ -1,5 +1,26 @@
 // Paged attention over the 4-bit cache (declared in include/nvm_mx_cache.h).
 //
+// mx_decode_kernel: one query row a request, D of 64 or 128.  A block owns a
+//   request, a kv head, a group of up to 16 of its query heads and a split of the
+//   context, which it shares out from the context's own length; its wavefronts
+//   take tiles of 64 positions in turn.
+//   * S^T = K . Q^T on v_mfma_f32_16x16x32_bf16.  E2M1 times a power of two is
+//     exact in bf16, two values an instruction, so codes go from memory into the
+//     operand: lane (c, G) loads position c's D/4 values from D/4 G on, its own
+//     part of a block, and takes them as its dims of the MFMA's D/32 steps; the
+//     query's operand is laid out in that order.  It is split into as many bf16
+//     parts as its type needs (bf16 one, f16 two, float32 three), so products
+//     are exact.
+//   * Softmax in base 2; the running maximum is looked at across lanes only where
+//     a score exceeds it.
+//   * O^T += V^T . P^T: the scores' layout is that of the operand P^T.  Value rows
+//     go to LDS as bf16 and come back transposed (ds_read_b64_tr_b16).  P is two
+//     bf16 parts (2^-17): with up to eight query heads the MFMA's other eight
+//     columns hold the second part, so both cost one product.
+//   * A masked position has a finite scale and any codes: its weight is zero, and
+//     zero times a finite value is zero.
+//   The next tile's keys are requested when this one's are converted, the next
+//   values when these are in LDS.
 // mx_rows_kernel: any head dim, one wavefront per query row.  A position's row
 //   of codes goes to a group of GL lanes (eight values, one dword, a lane), so
 //   64 / GL positions are in flight side by side, each group with a running
@@ -29,7 +50,17 @@ struct MxAttnArgs {
   int out_dt;
   int B, L, D, P, page_size, max_pages, Hkv, Hq, R, causal;
   float scale2;  // scale * log2(e): scores are kept in base 2
+  uint32_t ps_mul, ps_shift;  // position / page_size, see page_of
+  int HG, S;                  // groups of query heads, splits of a context
+  float *part_o, *part_ml;    // splits' outputs [row][S][D], maxima and sums [row][S][2]
 };
+
+// n / page_size of n below 2^31: with 2^(l-1) < page_size <= 2^l the factor is
+// ceil(2^(31 + l) / page_size), off by less than 2^-31 of n, which no quotient
+// notices (page_size 1: a factor of 0 stands for 2^32).
+__device__ __forceinline__ int page_of(int n, uint32_t mul, uint32_t shift) {
+  return mul ? (int)(__umulhi((uint32_t)n, mul) >> shift) : n;
+}
 
 __device__ __forceinline__ void store_out(void *out, int dt, int64_t i, float v) {
   if (dt == NVM_KV_F32)
@@ -140,7 +171,405 @@ hipError_t launch_rows(const MxAttnArgs &a, hipStream_t st) {
   return hipGetLastError();
 }
 
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// A 4 x 16 block of 16-bit values in LDS, transposed: of a group of 16 lanes,
+// lane i passes the address of values 4 (i % 4) .. + 3 of row i / 4 and gets
+// column i.
+__device__ __forceinline__ u32x2 lds_read_tr(const uint16_t *p) {
+  return __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p));
+}
+
+template <int QT>
+constexpr int kParts = QT == NVM_KV_F32 ? 3 : QT == NVM_KV_F16 ? 2 : 1;
+
+// Eight query values as bf16 parts whose sum they are.
+template <int QT>
+__device__ __forceinline__ void query8(const void *q, int64_t i, u32x4 (&p)[kParts<QT>]) {
+  using A = Act<DT_BF16>;
+  if constexpr (QT == NVM_KV_BF16) {
+    p[0] = ldg16((const uint16_t *)q + i);
+  } else {
+    float x[8];
+    if constexpr (QT == NVM_KV_F32) {
+      const f32x4 a = *(const f32x4 *)((const float *)q + i);
+      const f32x4 b = *(const f32x4 *)((const float *)q + i + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = a[j], x[4 + j] = b[j];
+    } else {
+      const u32x4 a = ldg16((const uint16_t *)q + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[2 * j] = Act<DT_F16>::lo(a[j]), x[2 * j + 1] = Act<DT_F16>::hi(a[j]);
+    }
+#pragma unroll
+    for (int k = 0; k < kParts<QT>; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[k][j] = A::pack2(x[2 * j], x[2 * j + 1]);
+        x[2 * j] -= A::lo(p[k][j]);
+        x[2 * j + 1] -= A::hi(p[k][j]);
+      }
+  }
+}
+
+// Eight codes times a scale (a float of that exponent), as an MFMA operand.
+__device__ __forceinline__ u32x4 codes_bf16(uint32_t d, float s) {
+  return u32x4{mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 0)),
+               mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 1)),
+               mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 2)),
+               mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 3))};
+}
+
+// N dwords from p, 4 N-byte aligned.
+template <int N>
+__device__ __forceinline__ void load_dwords(const uint8_t *p, uint32_t (&d)[N]) {
+  static_assert(N == 2 || N == 4, "a load");
+  if constexpr (N == 4) {
+    const u32x4 v = ldg16(p);
+    d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
+  } else {
+    const u32x2 v = ldg8(p);
+    d[0] = v.x, d[1] = v.y;
+  }
+}
+
+// The largest over a column's four lanes (lane groups 0..3).
+__device__ __forceinline__ float column_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+constexpr int kTile = 64;  // positions of a wavefront's step
+
+// DUP: at most eight query heads; columns 8..15 hold them again, for the second
+// part of P.
+template <int QT, int DH, bool DUP, int NW>
+__global__ __launch_bounds__(64 * NW) void mx_decode_kernel(MxAttnArgs a) {
+  using A = Act<DT_BF16>;
+  constexpr int NC = DH / 32;       // steps of a score MFMA; dwords of a lane's codes
+  constexpr int NT = DH / 16;       // tiles of the output
+  constexpr int NB = DH / 32;       // scales of a row
+  constexpr int VP = DH + 8;        // LDS pitch of a value row
+  constexpr int RP = DUP ? 8 : 16;  // query heads of a block
+  constexpr int QP = kParts<QT>;
+  constexpr int kVBytes = NW * 32 * VP * 2, kOBytes = NW * RP * DH * 4;
+  __shared__ __attribute__((aligned(16))) char s_buf[kVBytes > kOBytes ? kVBytes : kOBytes];
+  auto s_v = reinterpret_cast<uint16_t(*)[32][VP]>(s_buf);
+  auto s_o = reinterpret_cast<float(*)[RP][DH]>(s_buf);
+  __shared__ float s_m[NW][RP], s_l[NW][RP];
+
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int c16 = lane & 15, G = lane >> 4;
+  int blk = blockIdx.x;
+  const int s = blk % a.S;
+  blk /= a.S;
+  const int hg = blk % a.HG;
+  blk /= a.HG;
+  const int kvh = blk % a.Hkv;
+  const int b = blk / a.Hkv;
+  const int nh = min(RP, a.R - hg * RP);
+  const int h0 = kvh * a.R + hg * RP;
+  const int ctx = (int)max((int64_t)0, min((int64_t)a.lens[b], (int64_t)a.max_pages * a.page_size));
+  // this split's tiles
+  const int tiles = (ctx + kTile - 1) / kTile, per = (tiles + a.S - 1) / a.S;
+  const int t_end = min(tiles, (s + 1) * per);
+  const int32_t *bt = a.bt + (int64_t)b * a.max_pages;
+
+  u32x4 qop[NC][QP];
+  {
+    const int h = DUP ? c16 & 7 : c16;
+    const bool ok = h < nh;
+    const int64_t at = b * a.q_sb + (h0 + (ok ? h : 0)) * a.q_sh;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      query8<QT>(a.q, at + (DH / 4) * G + 8 * k, qop[k]);
+      if (!ok)
+#pragma unroll
+        for (int p = 0; p < QP; ++p) qop[k][p] = u32x4{0u, 0u, 0u, 0u};
+    }
+  }
+
+  // page ids of a tile's positions 16 u + c16, and their rows in the pool (row 0,
+  // and the bit not set, of those that are not there)
+  auto page_ids = [&](int t, int (&pg)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int pos = kTile * t + 16 * u + c16;
+      pg[u] = t < t_end && pos < ctx ? bt[page_of(pos, a.ps_mul, a.ps_shift)] : -1;
+    }
+  };
+  auto rows = [&](int t, const int (&pg)[4], int64_t (&row)[4], uint32_t (&there)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int pos = kTile * t + 16 * u + c16;
+      const int slot = pos - page_of(pos, a.ps_mul, a.ps_shift) * a.page_size;
+      const bool ok = pg[u] >= 0 && pg[u] < a.P;
+      row[u] = ok ? ((int64_t)pg[u] * a.Hkv + kvh) * a.page_size + slot : 0;
+      there[u] = (uint32_t)__builtin_amdgcn_ballot_w64(ok) & 0xFFFFu;
+    }
+  };
+  auto load = [&](const uint8_t *codes, const uint8_t *scales, const int64_t (&row)[4],
+                  uint32_t (&d)[4][NC], uint32_t (&sc)[4]) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) load_dwords<NC>(codes + row[u] * (DH / 2) + (DH / 8) * G, d[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sc[u] = scales[row[u] * NB + (DH / 4) * G / 32];
+  };
+  // a lane's scale of subtile u: a finite one for a position that is not there
+  auto scale_of = [&](uint32_t sc, uint32_t there) {
+    return __uint_as_float((there >> c16 & 1u) ? sc << 23 : 0u);
+  };
+
+  float m_run = -INFINITY, l_run = 0.f;  // column c16's; l_run this lane's share
+  f32x4 oacc[NT];                        // O^T: column c16, dims 16 t + 4 G + i
+#pragma unroll
+  for (int t = 0; t < NT; ++t) oacc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  int t = s * per + wv;
+  int pg[4];
+  int64_t row[4];
+  uint32_t there[4], kd[4][NC], ksc[4], vd[4][NC], vsc[4];
+  page_ids(t, pg);
+  if (t < t_end) {
+    rows(t, pg, row, there);
+    load(a.kc, a.ks, row, kd, ksc);
+    load(a.vc, a.vs, row, vd, vsc);
+  }
+  page_ids(t + NW, pg);
+  for (; t < t_end; t += NW) {
+    // S^T: column c16 at positions 16 u + 4 G + i
+    f32x4 acc[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const float f = scale_of(ksc[u], there[u]);
+#pragma unroll
+      for (int k = 0; k < NC; ++k) {
+        const u32x4 kb = codes_bf16(kd[u][k], f);
+#pragma unroll
+        for (int p = 0; p < QP; ++p) acc[u] = A::mfma16(kb, qop[k][p], acc[u]);
+      }
+    }
+    uint32_t now[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) now[u] = there[u];
+    const bool more = t + NW < t_end;  // uniform
+    if (more) {
+      rows(t + NW, pg, row, there);
+      load(a.kc, a.ks, row, kd, ksc);
+    }
+    page_ids(t + 2 * NW, pg);
+
+    float p[4][4];
+    float tmax = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[u][i] = acc[u][i] * a.scale2;
+    if ((now[0] & now[1] & now[2] & now[3]) != 0xFFFFu) {  // uniform
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!((now[u] >> (4 * G + i)) & 1u)) p[u][i] = -INFINITY;
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, p[u][i]);
+    if (__any(tmax > m_run)) {
+      const float m_new = fmaxf(m_run, column_max(tmax));
+      const float alpha = exp2_below(m_run, m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int k = 0; k < NT; ++k) oacc[k] *= alpha;
+      m_run = m_new;
+    }
+    const float m_sub = m_run == -INFINITY ? 0.f : m_run;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[u][i] = __builtin_amdgcn_exp2f(p[u][i] - m_sub);
+        l_run += p[u][i];
+      }
+
+    // O^T += V^T . P^T, 32 positions at a time: slot 8 G + j of the product is
+    // position 4 G + j, or 16 + 4 G + j - 4 from j = 4 on
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc) {
+#pragma unroll
+      for (int uu = 0; uu < 2; ++uu) {
+        const int u = 2 * kc + uu;
+        const float f = scale_of(vsc[u], now[u]);
+#pragma unroll
+        for (int k = 0; k < NC; ++k)
+          *(u32x4 *)&s_v[wv][16 * uu + c16][(DH / 4) * G + 8 * k] = codes_bf16(vd[u][k], f);
+      }
+      wave_lds_sync();
+      u32x4 hi, lo;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = p[2 * kc + (j >> 1)][2 * (j & 1)], y = p[2 * kc + (j >> 1)][2 * (j & 1) + 1];
+        hi[j] = A::pack2(x, y);
+        lo[j] = A::pack2(x - A::lo(hi[j]), y - A::hi(hi[j]));
+        if (DUP && c16 >= 8) hi[j] = lo[j];
+      }
+      const uint16_t *v0 = &s_v[wv][4 * G + (c16 >> 2)][4 * (c16 & 3)];
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        const u32x2 x = lds_read_tr(v0 + 16 * k), y = lds_read_tr(v0 + 16 * VP + 16 * k);
+        const u32x4 va = {x.x, x.y, y.x, y.y};
+        oacc[k] = A::mfma16(va, hi, oacc[k]);
+        if constexpr (!DUP) oacc[k] = A::mfma16(va, lo, oacc[k]);
+      }
+      wave_lds_sync();
+    }
+    if (more) load(a.vc, a.vs, row, vd, vsc);
+  }
+
+  l_run += __shfl_xor(l_run, 16);
+  l_run += __shfl_xor(l_run, 32);
+  __syncthreads();  // every wavefront is past its last use of s_v
+#pragma unroll
+  for (int k = 0; k < NT; ++k) {
+    f32x4 o = oacc[k];
+    if constexpr (DUP) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], 8);
+    }
+    if (c16 < RP) *(f32x4 *)&s_o[wv][c16][16 * k + 4 * G] = o;
+  }
+  if (G == 0 && c16 < RP) {
+    s_m[wv][c16] = m_run;
+    s_l[wv][c16] = l_run;
+  }
+  __syncthreads();
+
+  for (int e = threadIdx.x; e < RP * DH; e += 64 * NW) {
+    const int r = e / DH, d = e % DH;
+    if (r >= nh) break;
+    float M = s_m[0][r];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) M = fmaxf(M, s_m[w][r]);
+    float Ls = 0.f, Os = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float f = exp2_below(s_m[w][r], M);
+      Ls += f * s_l[w][r];
+      Os += f * s_o[w][r][d];
+    }
+    const int64_t n = (int64_t)b * a.Hq + h0 + r;
+    if (a.S == 1) {
+      store_out(a.out, a.out_dt, n * DH + d, Ls == 0.f ? 0.f : Os / Ls);
+    } else {
+      a.part_o[(n * a.S + s) * DH + d] = Os;
+      if (d == 0) {
+        a.part_ml[(n * a.S + s) * 2] = M;
+        a.part_ml[(n * a.S + s) * 2 + 1] = Ls;
+      }
+    }
+  }
+}
+
+// Splits of a row: sum_s 2^(M_s - M) O_s / sum_s 2^(M_s - M) L_s, a wavefront a
+// row: lane s takes split s's maximum and sum, then each lane D / 64 dims of all.
+constexpr int kMaxSplits = 64;
+template <int DH>
+__global__ __launch_bounds__(kRowThreads) void mx_combine_kernel(const float *__restrict__ part_o,
+                                                                 const float *__restrict__ part_ml,
+                                                                 int64_t rows, int S, void *out,
+                                                                 int out_dt) {
+  constexpr int PD = DH / 64;
+  const int64_t n = (int64_t)blockIdx.x * (kRowThreads / 64) + (threadIdx.x >> 6);
+  if (n >= rows) return;
+  const int lane = threadIdx.x & 63;
+  const float *po = part_o + n * S * DH + PD * lane;
+  float ms = -INFINITY, ls = 0.f;
+  if (lane < S) {
+    ms = part_ml[(n * S + lane) * 2];
+    ls = part_ml[(n * S + lane) * 2 + 1];
+  }
+  float M = ms;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
+  const float w = exp2_below(ms, M);
+  float L = w * ls;
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) L += __shfl_xor(L, x);
+  float acc[PD] = {};
+  constexpr int kAhead = 8;
+  for (int s0 = 0; s0 < S; s0 += kAhead) {
+    float v[kAhead][PD];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+      for (int d = 0; d < PD; ++d) v[j][d] = s0 + j < S ? po[(int64_t)(s0 + j) * DH + d] : 0.f;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), (s0 + j) & 63));
+#pragma unroll
+      for (int d = 0; d < PD; ++d) acc[d] += s0 + j < S ? f * v[j][d] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < PD; ++d)
+    store_out(out, out_dt, n * DH + PD * lane + d, L == 0.f ? 0.f : acc[d] / L);
+}
+
 constexpr int64_t kMaxRows = 0x3FFFFFF;  // query rows of a call: wavefronts of a launch
+
+// Splits: enough blocks of kDecodeWaves wavefronts for the CUs, none with less
+// than a tile a wavefront at the table's capacity.
+constexpr int kDecodeWaves = 4;
+struct MxPlan {
+  bool decode;
+  int HG, S;
+};
+MxPlan mx_plan(int64_t B, int64_t L, int64_t D, int64_t max_pages, int64_t page_size, int Hkv,
+               int Hq) {
+  MxPlan p{false, 1, 1};
+  p.decode = L == 1 && (D == 64 || D == 128);
+  if (!p.decode || B == 0) return p;
+  const int R = Hq / Hkv;
+  p.HG = R <= 8 ? 1 : (R + 15) / 16;
+  const int64_t tiles = (max_pages * page_size + kTile - 1) / kTile;
+  const int64_t base = B * Hkv * p.HG, want = 4 * (int64_t)cu_count();
+  if (base > kMaxRows / kDecodeWaves) return MxPlan{false, 1, 1};  // more than a launch takes
+  p.S = (int)std::max<int64_t>(1, std::min<int64_t>({(want + base - 1) / base,
+                                                     (tiles + kDecodeWaves - 1) / kDecodeWaves,
+                                                     (int64_t)kMaxSplits}));
+  return p;
+}
+size_t mx_workspace(const MxPlan &p, int64_t rows, int64_t D) {
+  if (p.S == 1) return 0;
+  const size_t o = ((size_t)rows * p.S * D * sizeof(float) + 255) & ~(size_t)255;
+  return o + (size_t)rows * p.S * 2 * sizeof(float) + 256;
+}
+
+template <int QT>
+hipError_t launch_decode(const MxAttnArgs &a, hipStream_t st) {
+  const unsigned grid = (unsigned)((int64_t)a.B * a.Hkv * a.HG * a.S);
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * kDecodeWaves), 0, st, a);
+  };
+  if (a.D == 128)
+    a.R <= 8 ? go(mx_decode_kernel<QT, 128, true, kDecodeWaves>)
+             : go(mx_decode_kernel<QT, 128, false, kDecodeWaves>);
+  else
+    a.R <= 8 ? go(mx_decode_kernel<QT, 64, true, kDecodeWaves>)
+             : go(mx_decode_kernel<QT, 64, false, kDecodeWaves>);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.S == 1) return e;
+  const int64_t rows = (int64_t)a.B * a.Hq;
+  const unsigned blocks = (unsigned)((rows + kRowThreads / 64 - 1) / (kRowThreads / 64));
+  hipLaunchKernelGGL(a.D == 128 ? mx_combine_kernel<128> : mx_combine_kernel<64>, dim3(blocks),
+                     dim3(kRowThreads), 0, st, a.part_o, a.part_ml, rows, a.S, a.out, a.out_dt);
+  return hipGetLastError();
+}
 
 int check_shape(const char *op, int64_t B, int64_t L, int64_t D, int64_t max_pages,
                 int64_t page_size, int Hkv, int Hq) {
@@ -174,7 +603,8 @@ int nvm_paged_attention_mx_workspace_size(int64_t B, int64_t L, int64_t D, int64
   constexpr const char *op = "paged_attention_mx";
   if (int rc = check_shape(op, B, L, D, max_pages, page_size, num_kv_heads, num_heads)) return rc;
   if (!bytes) return set_error(NVM_ERR_INVALID, "%s: null bytes", op);
-  *bytes = 0;
+  *bytes = mx_workspace(mx_plan(B, L, D, max_pages, page_size, num_kv_heads, num_heads),
+                        B * L * num_heads, D);
   return NVM_OK;
 }
 
@@ -226,11 +656,29 @@ int nvm_paged_attention_mx(const void *q, int q_dtype, int64_t q_stride_b, int64
   a.causal = is_causal ? 1 : 0;
   a.scale2 = scale * kLog2e;
   hipStream_t st = (hipStream_t)stream;
-  (void)workspace;
-  (void)workspace_bytes;
-  const hipError_t e = q_dtype == NVM_KV_F32    ? launch_rows<NVM_KV_F32>(a, st)
-                       : q_dtype == NVM_KV_BF16 ? launch_rows<NVM_KV_BF16>(a, st)
-                                                : launch_rows<NVM_KV_F16>(a, st);
+  uint32_t l = 0;
+  while (((int64_t)1 << l) < page_size) ++l;
+  a.ps_mul = l ? (uint32_t)((((uint64_t)1 << (31 + l)) + page_size - 1) / page_size) : 0;
+  a.ps_shift = l ? l - 1 : 0;
+  const MxPlan plan = mx_plan(B, L, D, max_pages, page_size, num_kv_heads, num_heads);
+  const size_t need = mx_workspace(plan, B * L * num_heads, D);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(NVM_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", op, need);
+  a.HG = plan.HG;
+  a.S = plan.S;
+  if (plan.S > 1) {
+    a.part_o = (float *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
+    a.part_ml = (float *)((char *)a.part_o +
+                          (((size_t)(B * L * num_heads) * plan.S * D * sizeof(float) + 255) &
+                           ~(size_t)255));
+  }
+  auto go = [&](auto qt) {
+    constexpr int QT = decltype(qt)::value;
+    return plan.decode ? launch_decode<QT>(a, st) : launch_rows<QT>(a, st);
+  };
+  const hipError_t e = q_dtype == NVM_KV_F32    ? go(MxInt<NVM_KV_F32>{})
+                       : q_dtype == NVM_KV_BF16 ? go(MxInt<NVM_KV_BF16>{})
+                                                : go(MxInt<NVM_KV_F16>{});
   if (e != hipSuccess) return set_error(NVM_ERR_HIP, "%s: %s", op, hipGetErrorString(e));
   return NVM_OK;
 }
