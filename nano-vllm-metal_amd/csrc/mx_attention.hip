@@ -49,9 +49,11 @@ struct MxAttnArgs {
   void *out;
   int out_dt;
   int B, L, D, P, page_size, max_pages, Hkv, Hq, R, causal;
-  float scale2;  // scale * log2(e): scores are kept in base 2
+  float scale2;  // |scale| * log2(e): scores are kept in base 2
+  uint32_t q_sign;  // the sign bits to flip in two 16-bit query parts, for a negative scale
   uint32_t ps_mul, ps_shift;  // position / page_size, see page_of
   int HG, S;                  // groups of query heads, splits of a context
+  int dpage, dslot;           // from a wavefront's tile to its next, in pages and slots
   float *part_o, *part_ml;    // splits' outputs [row][S][D], maxima and sums [row][S][2]
 };
 
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(kRowThreads) void mx_rows_kernel(MxAttnArgs a, int6
     for (int e = 0; e < 8; ++e) dot = fmaf(qv[e], k[e], dot);
 #pragma unroll
     for (int x = 1; x < GL; x <<= 1) dot += __shfl_xor(dot, x);
-    const float sc = dot * a.scale2, m_new = fmaxf(m, sc);
+    const float sc = (a.q_sign ? -dot : dot) * a.scale2, m_new = fmaxf(m, sc);
     const float alpha = exp2_below(m, m_new), p = exp2_below(sc, m_new);
     l = fmaf(l, alpha, p);
 #pragma unroll
@@ -226,10 +228,10 @@ template <int N>
 __device__ __forceinline__ void load_dwords(const uint8_t *p, uint32_t (&d)[N]) {
   static_assert(N == 2 || N == 4, "a load");
   if constexpr (N == 4) {
-    const u32x4 v = ldg16(p);
+    const u32x4 v = ldg16_once(p);
     d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
   } else {
-    const u32x2 v = ldg8(p);
+    const u32x2 v = __builtin_nontemporal_load((const u32x2 *)p);
     d[0] = v.x, d[1] = v.y;
   }
 }
@@ -242,205 +244,227 @@ __device__ __forceinline__ float column_max(float v) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-constexpr int kTile = 64;  // positions of a wavefront's step
+constexpr int kTile = 32;  // positions of a wavefront's step: two of the MFMA's 16 rows
+
+// Four consecutive outputs, from element i on.
+__device__ __forceinline__ void store_out4(void *out, int dt, int64_t i, f32x4 v) {
+  if (dt == NVM_KV_F32)
+    *(f32x4 *)((float *)out + i) = v;
+  else if (dt == NVM_KV_BF16)
+    *(u32x2 *)((uint16_t *)out + i) =
+        u32x2{Act<DT_BF16>::pack2(v[0], v[1]), Act<DT_BF16>::pack2(v[2], v[3])};
+  else
+    *(u32x2 *)((uint16_t *)out + i) =
+        u32x2{Act<DT_F16>::pack2(v[0], v[1]), Act<DT_F16>::pack2(v[2], v[3])};
+}
 
 // DUP: at most eight query heads; columns 8..15 hold them again, for the second
-// part of P.
+// part of P.  Grid: requests, splits, kv heads x groups of query heads.
+//
+// A tile is 32 positions and not 64: its code runs cold in each launch (from L2
+// into the instruction cache some 50 cycles a line), and a short context is little
+// else.
 template <int QT, int DH, bool DUP, int NW>
-__global__ __launch_bounds__(64 * NW) void mx_decode_kernel(MxAttnArgs a) {
+__global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
   using A = Act<DT_BF16>;
   constexpr int NC = DH / 32;       // steps of a score MFMA; dwords of a lane's codes
   constexpr int NT = DH / 16;       // tiles of the output
   constexpr int NB = DH / 32;       // scales of a row
+  constexpr int NU = kTile / 16;    // 16-row parts of a tile
   constexpr int VP = DH + 8;        // LDS pitch of a value row
   constexpr int RP = DUP ? 8 : 16;  // query heads of a block
   constexpr int QP = kParts<QT>;
-  constexpr int kVBytes = NW * 32 * VP * 2, kOBytes = NW * RP * DH * 4;
+  constexpr int kVBytes = NW * kTile * VP * 2, kOBytes = NW * RP * DH * 4;
   __shared__ __attribute__((aligned(16))) char s_buf[kVBytes > kOBytes ? kVBytes : kOBytes];
-  auto s_v = reinterpret_cast<uint16_t(*)[32][VP]>(s_buf);
+  auto s_v = reinterpret_cast<uint16_t(*)[kTile][VP]>(s_buf);
   auto s_o = reinterpret_cast<float(*)[RP][DH]>(s_buf);
   __shared__ float s_m[NW][RP], s_l[NW][RP];
+  __shared__ u32x4 s_q[NC][QP][64];  // the score MFMAs' query operand, by lane
 
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   const int c16 = lane & 15, G = lane >> 4;
-  int blk = blockIdx.x;
-  const int s = blk % a.S;
-  blk /= a.S;
-  const int hg = blk % a.HG;
-  blk /= a.HG;
-  const int kvh = blk % a.Hkv;
-  const int b = blk / a.Hkv;
+  const int b = blockIdx.x, s = blockIdx.y;
+  int kvh = blockIdx.z, hg = 0;
+  if (a.HG > 1) {
+    kvh = blockIdx.z / a.HG;
+    hg = blockIdx.z - kvh * a.HG;
+  }
   const int nh = min(RP, a.R - hg * RP);
   const int h0 = kvh * a.R + hg * RP;
-  const int ctx = (int)max((int64_t)0, min((int64_t)a.lens[b], (int64_t)a.max_pages * a.page_size));
-  // this split's tiles
-  const int tiles = (ctx + kTile - 1) / kTile, per = (tiles + a.S - 1) / a.S;
-  const int t_end = min(tiles, (s + 1) * per);
   const int32_t *bt = a.bt + (int64_t)b * a.max_pages;
 
-  u32x4 qop[NC][QP];
-  {
+  // The block's wavefronts take tiles first, first + step, ... of the context,
+  // whose length they need not know for that: the first page ids are requested
+  // beside it.  pidx, slot: of position kTile t + 16 u + c16 of the tile whose
+  // page ids are requested next.
+  const int first = s * NW + wv, step = a.S * NW;
+  int pidx[NU], slot[NU], pg[NU];
+#pragma unroll
+  for (int u = 0; u < NU; ++u) {
+    const int pos = kTile * first + 16 * u + c16;
+    pidx[u] = page_of(pos, a.ps_mul, a.ps_shift);
+    slot[u] = pos - pidx[u] * a.page_size;
+  }
+  auto page_ids = [&]() {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) pg[u] = pidx[u] < a.max_pages ? bt[pidx[u]] : -1;
+  };
+  page_ids();
+  const int ctx = (int)max((int64_t)0, min((int64_t)a.lens[b], (int64_t)a.max_pages * a.page_size));
+
+  for (int k = wv; k < NC; k += NW) {
     const int h = DUP ? c16 & 7 : c16;
     const bool ok = h < nh;
     const int64_t at = b * a.q_sb + (h0 + (ok ? h : 0)) * a.q_sh;
+    u32x4 q[QP];
+    query8<QT>(a.q, at + (DH / 4) * G + 8 * k, q);
 #pragma unroll
-    for (int k = 0; k < NC; ++k) {
-      query8<QT>(a.q, at + (DH / 4) * G + 8 * k, qop[k]);
-      if (!ok)
-#pragma unroll
-        for (int p = 0; p < QP; ++p) qop[k][p] = u32x4{0u, 0u, 0u, 0u};
-    }
+    for (int p = 0; p < QP; ++p) s_q[k][p][lane] = ok ? q[p] ^ a.q_sign : u32x4{0u, 0u, 0u, 0u};
   }
 
-  // page ids of a tile's positions 16 u + c16, and their rows in the pool (row 0,
-  // and the bit not set, of those that are not there)
-  auto page_ids = [&](int t, int (&pg)[4]) {
+  // rows in the pool of tile t's positions, whose page ids are there, and which
+  // lanes' positions exist (row 0 for others); then on to the next tile's ids
+  auto rows = [&](int t, uint32_t (&row)[NU], uint64_t (&there)[NU]) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int pos = kTile * t + 16 * u + c16;
-      pg[u] = t < t_end && pos < ctx ? bt[page_of(pos, a.ps_mul, a.ps_shift)] : -1;
+    for (int u = 0; u < NU; ++u) {
+      const bool ok = c16 < ctx - kTile * t - 16 * u && pg[u] >= 0 && pg[u] < a.P;
+      row[u] = ok ? ((uint32_t)pg[u] * a.Hkv + kvh) * a.page_size + slot[u] : 0;
+      there[u] = __builtin_amdgcn_ballot_w64(ok);
+      slot[u] += a.dslot;
+      const bool over = slot[u] >= a.page_size;
+      pidx[u] += a.dpage + over;
+      slot[u] -= over ? a.page_size : 0;
     }
+    page_ids();
   };
-  auto rows = [&](int t, const int (&pg)[4], int64_t (&row)[4], uint32_t (&there)[4]) {
+  auto load = [&](const uint8_t *codes, const uint8_t *scales, const uint32_t (&row)[NU],
+                  uint32_t (&d)[NU][NC], uint32_t (&sc)[NU]) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int pos = kTile * t + 16 * u + c16;
-      const int slot = pos - page_of(pos, a.ps_mul, a.ps_shift) * a.page_size;
-      const bool ok = pg[u] >= 0 && pg[u] < a.P;
-      row[u] = ok ? ((int64_t)pg[u] * a.Hkv + kvh) * a.page_size + slot : 0;
-      there[u] = (uint32_t)__builtin_amdgcn_ballot_w64(ok) & 0xFFFFu;
-    }
+    for (int u = 0; u < NU; ++u)
+      load_dwords<NC>(codes + (uint64_t)row[u] * (DH / 2) + (DH / 8) * G, d[u]);
+#pragma unroll
+    for (int u = 0; u < NU; ++u) sc[u] = scales[(uint64_t)row[u] * NB + (DH / 4) * G / 32];
   };
-  auto load = [&](const uint8_t *codes, const uint8_t *scales, const int64_t (&row)[4],
-                  uint32_t (&d)[4][NC], uint32_t (&sc)[4]) {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) load_dwords<NC>(codes + row[u] * (DH / 2) + (DH / 8) * G, d[u]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) sc[u] = scales[row[u] * NB + (DH / 4) * G / 32];
-  };
-  // a lane's scale of subtile u: a finite one for a position that is not there
-  auto scale_of = [&](uint32_t sc, uint32_t there) {
-    return __uint_as_float((there >> c16 & 1u) ? sc << 23 : 0u);
+  // a lane's scale of a part: a finite one for a position that is not there
+  auto scale_of = [&](uint32_t sc, uint64_t there) {
+    return __uint_as_float(__builtin_amdgcn_inverse_ballot_w64(there) ? sc << 23 : 0u);
   };
 
-  float m_run = -INFINITY, l_run = 0.f;  // column c16's; l_run this lane's share
-  f32x4 oacc[NT];                        // O^T: column c16, dims 16 t + 4 G + i
+  float m_run = -INFINITY;  // column c16's
+  f32x4 oacc[NT], lacc = {0.f, 0.f, 0.f, 0.f};  // O^T: column c16, dims 16 t + 4 G + i; sums of P
 #pragma unroll
   for (int t = 0; t < NT; ++t) oacc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // with DUP columns 8..15 hold P less its first part: (-1, 0) and (0, -1) pick
+  // that part out of a pair
+  // (in registers: as a constant the second is taken for the inline constant -1.0,
+  // whose value the instruction puts into the other half)
+  uint32_t pick0 = DUP && c16 < 8 ? 0u : 0x0000BF80u, pick1 = pick0 << 16;
+  asm volatile("" : "+v"(pick0), "+v"(pick1));
+  const u32x4 ones = {A::kOne2, A::kOne2, A::kOne2, A::kOne2};
 
-  int t = s * per + wv;
-  int pg[4];
-  int64_t row[4];
-  uint32_t there[4], kd[4][NC], ksc[4], vd[4][NC], vsc[4];
-  page_ids(t, pg);
+  uint32_t row[NU], kd[NU][NC], ksc[NU], vd[NU][NC], vsc[NU];
+  uint64_t there[NU];
+  int t = first;
+  const int t_end = (ctx + kTile - 1) / kTile;
   if (t < t_end) {
-    rows(t, pg, row, there);
+    rows(t, row, there);
     load(a.kc, a.ks, row, kd, ksc);
     load(a.vc, a.vs, row, vd, vsc);
   }
-  page_ids(t + NW, pg);
-  for (; t < t_end; t += NW) {
+  __syncthreads();  // the query is there
+  for (; t < t_end; t += step) {
     // S^T: column c16 at positions 16 u + 4 G + i
-    f32x4 acc[4];
+    f32x4 acc[NU];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < NU; ++u) {
       acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
       const float f = scale_of(ksc[u], there[u]);
 #pragma unroll
       for (int k = 0; k < NC; ++k) {
         const u32x4 kb = codes_bf16(kd[u][k], f);
 #pragma unroll
-        for (int p = 0; p < QP; ++p) acc[u] = A::mfma16(kb, qop[k][p], acc[u]);
+        for (int p = 0; p < QP; ++p) acc[u] = A::mfma16(kb, s_q[k][p][lane], acc[u]);
       }
     }
-    uint32_t now[4];
+    uint64_t now[NU];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) now[u] = there[u];
-    const bool more = t + NW < t_end;  // uniform
+    for (int u = 0; u < NU; ++u) now[u] = there[u];
+    const bool more = t + step < t_end;  // uniform
     if (more) {
-      rows(t + NW, pg, row, there);
+      rows(t + step, row, there);
       load(a.kc, a.ks, row, kd, ksc);
     }
-    page_ids(t + 2 * NW, pg);
 
-    float p[4][4];
-    float tmax = -INFINITY;
+    if ((now[0] & now[1]) != ~0ull) {  // uniform
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[u][i] = acc[u][i] * a.scale2;
-    if ((now[0] & now[1] & now[2] & now[3]) != 0xFFFFu) {  // uniform
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (!((now[u] >> (4 * G + i)) & 1u)) p[u][i] = -INFINITY;
+          if (!(((uint32_t)now[u] >> (4 * G + i)) & 1u)) acc[u][i] = -INFINITY;
     }
+    float tmax = acc[0][0];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, p[u][i]);
+      for (int i = 0; i < 4; ++i) tmax = fmaxf(tmax, acc[u][i]);
+    tmax *= a.scale2;
     if (__any(tmax > m_run)) {
       const float m_new = fmaxf(m_run, column_max(tmax));
       const float alpha = exp2_below(m_run, m_new);
-      l_run *= alpha;
+      lacc *= alpha;
 #pragma unroll
       for (int k = 0; k < NT; ++k) oacc[k] *= alpha;
       m_run = m_new;
     }
     const float m_sub = m_run == -INFINITY ? 0.f : m_run;
+    // P^T, which lies as the product's operand wants it: slot 8 G + j is position
+    // 4 G + j, or 16 + 4 G + j - 4 from j = 4 on
+    u32x4 hi, lo;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[u][i] = __builtin_amdgcn_exp2f(p[u][i] - m_sub);
-        l_run += p[u][i];
-      }
-
-    // O^T += V^T . P^T, 32 positions at a time: slot 8 G + j of the product is
-    // position 4 G + j, or 16 + 4 G + j - 4 from j = 4 on
-#pragma unroll
-    for (int kc = 0; kc < 2; ++kc) {
-#pragma unroll
-      for (int uu = 0; uu < 2; ++uu) {
-        const int u = 2 * kc + uu;
-        const float f = scale_of(vsc[u], now[u]);
-#pragma unroll
-        for (int k = 0; k < NC; ++k)
-          *(u32x4 *)&s_v[wv][16 * uu + c16][(DH / 4) * G + 8 * k] = codes_bf16(vd[u][k], f);
-      }
-      wave_lds_sync();
-      u32x4 hi, lo;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x = p[2 * kc + (j >> 1)][2 * (j & 1)], y = p[2 * kc + (j >> 1)][2 * (j & 1) + 1];
-        hi[j] = A::pack2(x, y);
-        lo[j] = A::pack2(x - A::lo(hi[j]), y - A::hi(hi[j]));
-        if (DUP && c16 >= 8) hi[j] = lo[j];
-      }
-      const uint16_t *v0 = &s_v[wv][4 * G + (c16 >> 2)][4 * (c16 & 3)];
-#pragma unroll
-      for (int k = 0; k < NT; ++k) {
-        const u32x2 x = lds_read_tr(v0 + 16 * k), y = lds_read_tr(v0 + 16 * VP + 16 * k);
-        const u32x4 va = {x.x, x.y, y.x, y.y};
-        oacc[k] = A::mfma16(va, hi, oacc[k]);
-        if constexpr (!DUP) oacc[k] = A::mfma16(va, lo, oacc[k]);
-      }
-      wave_lds_sync();
+    for (int j = 0; j < 4; ++j) {
+      const float x = __builtin_amdgcn_exp2f(fmaf(acc[j >> 1][2 * (j & 1)], a.scale2, -m_sub));
+      const float y = __builtin_amdgcn_exp2f(fmaf(acc[j >> 1][2 * (j & 1) + 1], a.scale2, -m_sub));
+      hi[j] = A::pack2(x, y);
+      lo[j] = A::pack2(A::dot2(hi[j], pick0, x), A::dot2(hi[j], pick1, y));
     }
+    const u32x4 pb = DUP ? lo : hi;
+
+    // O^T += V^T . P^T
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const float f = scale_of(vsc[u], now[u]);
+#pragma unroll
+      for (int k = 0; k < NC; ++k)
+        *(u32x4 *)&s_v[wv][16 * u + c16][(DH / 4) * G + 8 * k] = codes_bf16(vd[u][k], f);
+    }
+    wave_lds_sync();
     if (more) load(a.vc, a.vs, row, vd, vsc);
+    const uint16_t *v0 = &s_v[wv][4 * G + (c16 >> 2)][4 * (c16 & 3)];
+#pragma unroll
+    for (int k = 0; k < NT; ++k) {
+      const u32x2 x = lds_read_tr(v0 + 16 * k), y = lds_read_tr(v0 + 16 * VP + 16 * k);
+      const u32x4 va = {x.x, x.y, y.x, y.y};
+      oacc[k] = A::mfma16(va, pb, oacc[k]);
+      if constexpr (!DUP) oacc[k] = A::mfma16(va, lo, oacc[k]);
+    }
+    lacc = A::mfma16(ones, pb, lacc);
+    if constexpr (!DUP) lacc = A::mfma16(ones, lo, lacc);
+    wave_lds_sync();
   }
 
-  l_run += __shfl_xor(l_run, 16);
-  l_run += __shfl_xor(l_run, 32);
-  __syncthreads();  // every wavefront is past its last use of s_v
+  // the wavefronts' outputs meet (with DUP columns h and h + 8 are one: lanes 8
+  // apart in a row of 16)
+  auto both = [&](float v) {
+    if constexpr (DUP) v += __uint_as_float(dpp_u32<0x128>(__float_as_uint(v)));
+    return v;
+  };
+  const float l_run = both(lacc[0]);  // (all of its rows are alike)
+  __syncthreads();                    // every wavefront is past its last use of s_v
 #pragma unroll
   for (int k = 0; k < NT; ++k) {
     f32x4 o = oacc[k];
-    if constexpr (DUP) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], 8);
-    }
+    for (int i = 0; i < 4; ++i) o[i] = both(o[i]);
     if (c16 < RP) *(f32x4 *)&s_o[wv][c16][16 * k + 4 * G] = o;
   }
   if (G == 0 && c16 < RP) {
@@ -449,24 +473,26 @@ __global__ __launch_bounds__(64 * NW) void mx_decode_kernel(MxAttnArgs a) {
   }
   __syncthreads();
 
-  for (int e = threadIdx.x; e < RP * DH; e += 64 * NW) {
-    const int r = e / DH, d = e % DH;
+  for (int e = threadIdx.x; e < RP * DH / 4; e += 64 * NW) {
+    const int r = e / (DH / 4), d = 4 * (e % (DH / 4));
     if (r >= nh) break;
     float M = s_m[0][r];
 #pragma unroll
     for (int w = 1; w < NW; ++w) M = fmaxf(M, s_m[w][r]);
-    float Ls = 0.f, Os = 0.f;
+    float Ls = 0.f;
+    f32x4 Os = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float f = exp2_below(s_m[w][r], M);
       Ls += f * s_l[w][r];
-      Os += f * s_o[w][r][d];
+      Os += f * *(const f32x4 *)&s_o[w][r][d];
     }
     const int64_t n = (int64_t)b * a.Hq + h0 + r;
     if (a.S == 1) {
-      store_out(a.out, a.out_dt, n * DH + d, Ls == 0.f ? 0.f : Os / Ls);
+      const float inv = 1.f / Ls;
+      store_out4(a.out, a.out_dt, n * DH + d, Ls == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : Os * inv);
     } else {
-      a.part_o[(n * a.S + s) * DH + d] = Os;
+      *(f32x4 *)(a.part_o + (n * a.S + s) * DH + d) = Os;
       if (d == 0) {
         a.part_ml[(n * a.S + s) * 2] = M;
         a.part_ml[(n * a.S + s) * 2 + 1] = Ls;
@@ -538,7 +564,8 @@ MxPlan mx_plan(int64_t B, int64_t L, int64_t D, int64_t max_pages, int64_t page_
   p.HG = R <= 8 ? 1 : (R + 15) / 16;
   const int64_t tiles = (max_pages * page_size + kTile - 1) / kTile;
   const int64_t base = B * Hkv * p.HG, want = 4 * (int64_t)cu_count();
-  if (base > kMaxRows / kDecodeWaves) return MxPlan{false, 1, 1};  // more than a launch takes
+  // (a launch has below 2^32 threads, and below 2^16 blocks but for the first dimension)
+  if (B > kMaxRows / kDecodeWaves || (int64_t)Hkv * p.HG > 0xFFFF) return MxPlan{false, 1, 1};
   p.S = (int)std::max<int64_t>(1, std::min<int64_t>({(want + base - 1) / base,
                                                      (tiles + kDecodeWaves - 1) / kDecodeWaves,
                                                      (int64_t)kMaxSplits}));
@@ -552,9 +579,9 @@ size_t mx_workspace(const MxPlan &p, int64_t rows, int64_t D) {
 
 template <int QT>
 hipError_t launch_decode(const MxAttnArgs &a, hipStream_t st) {
-  const unsigned grid = (unsigned)((int64_t)a.B * a.Hkv * a.HG * a.S);
+  const dim3 grid(a.B, a.S, a.Hkv * a.HG);
   auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * kDecodeWaves), 0, st, a);
+    hipLaunchKernelGGL(kern, grid, dim3(64 * kDecodeWaves), 0, st, a);
   };
   if (a.D == 128)
     a.R <= 8 ? go(mx_decode_kernel<QT, 128, true, kDecodeWaves>)
@@ -654,7 +681,11 @@ int nvm_paged_attention_mx(const void *q, int q_dtype, int64_t q_stride_b, int64
   a.Hq = num_heads;
   a.R = num_heads / num_kv_heads;
   a.causal = is_causal ? 1 : 0;
-  a.scale2 = scale * kLog2e;
+  // (the largest score is the largest product then; a scale of zero as one that
+  // takes any product to zero, but not -infinity to a NaN)
+  a.scale2 = std::max(fabsf(scale) * kLog2e, 1.17549435e-38f);
+  if (scale != scale) a.scale2 = scale;
+  a.q_sign = scale < 0.f ? 0x80008000u : 0u;
   hipStream_t st = (hipStream_t)stream;
   uint32_t l = 0;
   while (((int64_t)1 << l) < page_size) ++l;
@@ -666,6 +697,9 @@ int nvm_paged_attention_mx(const void *q, int q_dtype, int64_t q_stride_b, int64
     return set_error(NVM_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", op, need);
   a.HG = plan.HG;
   a.S = plan.S;
+  const int64_t ahead = (int64_t)kTile * plan.S * kDecodeWaves;
+  a.dpage = (int)(ahead / page_size);
+  a.dslot = (int)(ahead % page_size);
   if (plan.S > 1) {
     a.part_o = (float *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
     a.part_ml = (float *)((char *)a.part_o +

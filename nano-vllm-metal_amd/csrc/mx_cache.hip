@@ -233,7 +233,9 @@ int mx_check_pages(const char *op, int Hkv, int64_t D, int64_t P, int64_t page_s
   if (D % 32 || D > kMaxD)
     return set_error(NVM_ERR_UNSUPPORTED, "%s: head dim %lld must be a multiple of 32, at most %d",
                      op, (long long)D, kMaxD);
-  if (P > INT32_MAX || page_size > INT32_MAX || P > (INT64_MAX / kMaxD) / Hkv / page_size)
+  // (rows have 32-bit numbers, their bytes 64-bit addresses: at D = 128 2^31 rows
+  // are 128 GiB of codes)
+  if (page_size > INT32_MAX || P > INT32_MAX / Hkv / page_size)
     return set_error(NVM_ERR_UNSUPPORTED, "%s: pool too large", op);
   if (!kc || !ks || !vc || !vs) return set_error(NVM_ERR_INVALID, "%s: null page pointer", op);
   if (!aligned16(kc) || !aligned16(ks) || !aligned16(vc) || !aligned16(vs))
