@@ -395,6 +395,17 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
       load(a.kc, a.ks, row, kd, ksc);
     }
 
+    // (before the softmax, so that the next values are requested before it too)
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const float f = scale_of(vsc[u], now[u]);
+#pragma unroll
+      for (int k = 0; k < NC; ++k)
+        *(u32x4 *)&s_v[wv][16 * u + c16][(DH / 4) * G + 8 * k] = codes_bf16(vd[u][k], f);
+    }
+    wave_lds_sync();
+    if (more) load(a.vc, a.vs, row, vd, vsc);
+
     if ((now[0] & now[1]) != ~0ull) {  // uniform
 #pragma unroll
       for (int u = 0; u < NU; ++u)
@@ -430,15 +441,6 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
     const u32x4 pb = DUP ? lo : hi;
 
     // O^T += V^T . P^T
-#pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const float f = scale_of(vsc[u], now[u]);
-#pragma unroll
-      for (int k = 0; k < NC; ++k)
-        *(u32x4 *)&s_v[wv][16 * u + c16][(DH / 4) * G + 8 * k] = codes_bf16(vd[u][k], f);
-    }
-    wave_lds_sync();
-    if (more) load(a.vc, a.vs, row, vd, vsc);
     const uint16_t *v0 = &s_v[wv][4 * G + (c16 >> 2)][4 * (c16 & 3)];
 #pragma unroll
     for (int k = 0; k < NT; ++k) {
