@@ -281,7 +281,7 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
   __shared__ float s_m[NW][RP], s_l[NW][RP];
   __shared__ u32x4 s_q[NC][QP][64];  // the score MFMAs' query operand, by lane
 
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, G = lane >> 4;
   const int b = blockIdx.x, s = blockIdx.y;
   int kvh = blockIdx.z, hg = 0;
@@ -305,9 +305,12 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
     pidx[u] = page_of(pos, a.ps_mul, a.ps_shift);
     slot[u] = pos - pidx[u] * a.page_size;
   }
+  // (No load stands behind a branch: at a branch's end the compiler waits for all
+  // loads, the values of this tile among them, and a step took twice as long.  So
+  // ids past the table are its last, and a tile past the context is row 0.)
   auto page_ids = [&]() {
 #pragma unroll
-    for (int u = 0; u < NU; ++u) pg[u] = pidx[u] < a.max_pages ? bt[pidx[u]] : -1;
+    for (int u = 0; u < NU; ++u) pg[u] = bt[max(min(pidx[u], a.max_pages - 1), 0)];
   };
   page_ids();
   const int ctx = (int)max((int64_t)0, min((int64_t)a.lens[b], (int64_t)a.max_pages * a.page_size));
@@ -327,12 +330,12 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
   auto rows = [&](int t, uint32_t (&row)[NU], uint64_t (&there)[NU]) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-      const bool ok = c16 < ctx - kTile * t - 16 * u && pg[u] >= 0 && pg[u] < a.P;
-      row[u] = ok ? ((uint32_t)pg[u] * a.Hkv + kvh) * a.page_size + slot[u] : 0;
+      const bool ok = (c16 < ctx - kTile * t - 16 * u) & ((uint32_t)pg[u] < (uint32_t)a.P);
+      row[u] = (((uint32_t)pg[u] * a.Hkv + kvh) * a.page_size + slot[u]) & (ok ? ~0u : 0u);
       there[u] = __builtin_amdgcn_ballot_w64(ok);
       slot[u] += a.dslot;
       const bool over = slot[u] >= a.page_size;
-      pidx[u] += a.dpage + over;
+      pidx[u] += a.dpage + (over ? 1 : 0);
       slot[u] -= over ? a.page_size : 0;
     }
     page_ids();
@@ -366,11 +369,9 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
   uint64_t there[NU];
   int t = first;
   const int t_end = (ctx + kTile - 1) / kTile;
-  if (t < t_end) {
-    rows(t, row, there);
-    load(a.kc, a.ks, row, kd, ksc);
-    load(a.vc, a.vs, row, vd, vsc);
-  }
+  rows(t, row, there);
+  load(a.kc, a.ks, row, kd, ksc);
+  load(a.vc, a.vs, row, vd, vsc);
   __syncthreads();  // the query is there
   for (; t < t_end; t += step) {
     // S^T: column c16 at positions 16 u + 4 G + i
@@ -389,11 +390,9 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
     uint64_t now[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) now[u] = there[u];
-    const bool more = t + step < t_end;  // uniform
-    if (more) {
-      rows(t + step, row, there);
-      load(a.kc, a.ks, row, kd, ksc);
-    }
+    rows(t + step, row, there);
+    load(a.kc, a.ks, row, kd, ksc);
+    __builtin_amdgcn_sched_barrier(0);  // (requested before this tile's values are waited for)
 
     // (before the softmax, so that the next values are requested before it too)
 #pragma unroll
@@ -404,7 +403,7 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
         *(u32x4 *)&s_v[wv][16 * u + c16][(DH / 4) * G + 8 * k] = codes_bf16(vd[u][k], f);
     }
     wave_lds_sync();
-    if (more) load(a.vc, a.vs, row, vd, vsc);
+    load(a.vc, a.vs, row, vd, vsc);
 
     if ((now[0] & now[1]) != ~0ull) {  // uniform
 #pragma unroll
@@ -550,26 +549,24 @@ __global__ __launch_bounds__(kRowThreads) void mx_combine_kernel(const float *__
 
 constexpr int64_t kMaxRows = 0x3FFFFFF;  // query rows of a call: wavefronts of a launch
 
-// Splits: enough blocks of kDecodeWaves wavefronts for the CUs, none with less
-// than a tile a wavefront at the table's capacity.
-constexpr int kDecodeWaves = 4;
+// Wavefronts a block and splits of a context.
 struct MxPlan {
   bool decode;
-  int HG, S;
+  int HG, S, NW;
 };
 MxPlan mx_plan(int64_t B, int64_t L, int64_t D, int64_t max_pages, int64_t page_size, int Hkv,
                int Hq) {
-  MxPlan p{false, 1, 1};
-  p.decode = L == 1 && (D == 64 || D == 128);
-  if (!p.decode || B == 0) return p;
+  MxPlan p{false, 1, 1, 4};
+  if (L > 1 || (D != 64 && D != 128) || B == 0) return p;
   const int R = Hq / Hkv;
   p.HG = R <= 8 ? 1 : (R + 15) / 16;
+  // (a launch has below 2^32 threads, and below 2^16 blocks but for the first dimension)
+  if (B > kMaxRows / 8 || (int64_t)Hkv * p.HG > 0xFFFF) return p;
+  p.decode = true;
   const int64_t tiles = (max_pages * page_size + kTile - 1) / kTile;
   const int64_t base = B * Hkv * p.HG, want = 4 * (int64_t)cu_count();
-  // (a launch has below 2^32 threads, and below 2^16 blocks but for the first dimension)
-  if (B > kMaxRows / kDecodeWaves || (int64_t)Hkv * p.HG > 0xFFFF) return MxPlan{false, 1, 1};
   p.S = (int)std::max<int64_t>(1, std::min<int64_t>({(want + base - 1) / base,
-                                                     (tiles + kDecodeWaves - 1) / kDecodeWaves,
+                                                     (tiles + p.NW - 1) / p.NW,
                                                      (int64_t)kMaxSplits}));
   return p;
 }
@@ -579,18 +576,23 @@ size_t mx_workspace(const MxPlan &p, int64_t rows, int64_t D) {
   return o + (size_t)rows * p.S * 2 * sizeof(float) + 256;
 }
 
-template <int QT>
-hipError_t launch_decode(const MxAttnArgs &a, hipStream_t st) {
+template <int QT, int DH, bool DUP>
+void launch_decode_nw(const MxAttnArgs &a, int NW, hipStream_t st) {
   const dim3 grid(a.B, a.S, a.Hkv * a.HG);
-  auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, grid, dim3(64 * kDecodeWaves), 0, st, a);
-  };
-  if (a.D == 128)
-    a.R <= 8 ? go(mx_decode_kernel<QT, 128, true, kDecodeWaves>)
-             : go(mx_decode_kernel<QT, 128, false, kDecodeWaves>);
+  if (NW == 8)
+    hipLaunchKernelGGL((mx_decode_kernel<QT, DH, DUP, 8>), grid, dim3(512), 0, st, a);
   else
-    a.R <= 8 ? go(mx_decode_kernel<QT, 64, true, kDecodeWaves>)
-             : go(mx_decode_kernel<QT, 64, false, kDecodeWaves>);
+    hipLaunchKernelGGL((mx_decode_kernel<QT, DH, DUP, 4>), grid, dim3(256), 0, st, a);
+}
+
+template <int QT>
+hipError_t launch_decode(const MxAttnArgs &a, int NW, hipStream_t st) {
+  if (a.D == 128)
+    a.R <= 8 ? launch_decode_nw<QT, 128, true>(a, NW, st)
+             : launch_decode_nw<QT, 128, false>(a, NW, st);
+  else
+    a.R <= 8 ? launch_decode_nw<QT, 64, true>(a, NW, st)
+             : launch_decode_nw<QT, 64, false>(a, NW, st);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.S == 1) return e;
   const int64_t rows = (int64_t)a.B * a.Hq;
@@ -669,7 +671,7 @@ int nvm_paged_attention_mx(const void *q, int q_dtype, int64_t q_stride_b, int64
   a.ks = key_scales;
   a.vc = (const uint8_t *)value_codes;
   a.vs = value_scales;
-  a.bt = block_table;
+  a.bt = max_pages ? block_table : context_lens;  // (ids are read before they are known to count)
   a.lens = context_lens;
   a.out = out;
   a.out_dt = out_dtype;
@@ -699,7 +701,7 @@ int nvm_paged_attention_mx(const void *q, int q_dtype, int64_t q_stride_b, int64
     return set_error(NVM_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", op, need);
   a.HG = plan.HG;
   a.S = plan.S;
-  const int64_t ahead = (int64_t)kTile * plan.S * kDecodeWaves;
+  const int64_t ahead = (int64_t)kTile * plan.S * plan.NW;
   a.dpage = (int)(ahead / page_size);
   a.dslot = (int)(ahead % page_size);
   if (plan.S > 1) {
@@ -710,7 +712,7 @@ int nvm_paged_attention_mx(const void *q, int q_dtype, int64_t q_stride_b, int64
   }
   auto go = [&](auto qt) {
     constexpr int QT = decltype(qt)::value;
-    return plan.decode ? launch_decode<QT>(a, st) : launch_rows<QT>(a, st);
+    return plan.decode ? launch_decode<QT>(a, plan.NW, st) : launch_rows<QT>(a, st);
   };
   const hipError_t e = q_dtype == NVM_KV_F32    ? go(MxInt<NVM_KV_F32>{})
                        : q_dtype == NVM_KV_BF16 ? go(MxInt<NVM_KV_BF16>{})
