@@ -52,8 +52,8 @@ struct MxAttnArgs {
   float scale2;  // |scale| * log2(e): scores are kept in base 2
   uint32_t q_sign;  // the sign bits to flip in two 16-bit query parts, for a negative scale
   uint32_t ps_mul, ps_shift;  // position / page_size, see page_of
-  int HG, S;                  // groups of query heads, splits of a context
-  int dpage, dslot;           // from a wavefront's tile to its next, in pages and slots
+  int HG, S;                  // groups of query heads, most splits of a context
+  float slots;                // blocks to be had for the splits, a kv head's group of query heads
   float *part_o, *part_ml;    // splits' outputs [row][S][D], maxima and sums [row][S][2]
 };
 
@@ -258,8 +258,41 @@ __device__ __forceinline__ void store_out4(void *out, int dt, int64_t i, f32x4 v
         u32x2{Act<DT_F16>::pack2(v[0], v[1]), Act<DT_F16>::pack2(v[2], v[3])};
 }
 
+// Sum over the wavefront, in an order of its own: the same in every lane and block.
+__device__ __forceinline__ float wave_sum(float v) {
+  auto step = [&](uint32_t o) { v += __uint_as_float(o); };
+  step(dpp_u32<0xB1>(__float_as_uint(v)));
+  step(dpp_u32<0x4E>(__float_as_uint(v)));
+  step(dpp_u32<0x141>(__float_as_uint(v)));
+  step(dpp_u32<0x140>(__float_as_uint(v)));
+  float r = 0.f;
+#pragma unroll
+  for (int i = 0; i < 64; i += 16)
+    r += __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), i));
+  return r;
+}
+
+__device__ __forceinline__ int context_of(const MxAttnArgs &a, int len) {
+  return (int)max((int64_t)0, min((int64_t)len, (int64_t)a.max_pages * a.page_size));
+}
+
+// Splits of a context of `tiles` tiles: its share of the slots by length (the host
+// does not know the lengths), and no more than sqrt(2 tiles), past which the merge
+// takes longer than the steps it saves (one request of 1024, 4096 and 16384
+// positions: 8, 16 and 32 splits of four wavefronts 7.2, 9.1 and 12.4 us; half and
+// twice as many 7.8 and 7.2, 10 and 9.8, 14.0 and 13.9).
+__device__ __forceinline__ int splits_of(const MxAttnArgs &a, int tiles, int lane, int tile) {
+  float total = 0.f;
+  for (int i = lane; i < a.B; i += 64)
+    total += (float)((context_of(a, a.lens[i]) + tile - 1) / tile);
+  total = wave_sum(total);
+  const float share = (float)tiles * a.slots / fmaxf(total, 1.f);
+  return max(1, min(a.S, (int)ceilf(fminf(share, sqrtf(2.f * (float)tiles)))));
+}
+
 // DUP: at most eight query heads; columns 8..15 hold them again, for the second
-// part of P.  Grid: requests, splits, kv heads x groups of query heads.
+// part of P.  Grid: requests, kv heads x groups of query heads, splits (last, so
+// that those that a context does not use come behind all others).
 //
 // A tile is 32 positions and not 64: its code runs cold in each launch (from L2
 // into the instruction cache some 50 cycles a line), and a short context is little
@@ -283,21 +316,21 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
 
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c16 = lane & 15, G = lane >> 4;
-  const int b = blockIdx.x, s = blockIdx.y;
-  int kvh = blockIdx.z, hg = 0;
+  const int b = blockIdx.x, s = blockIdx.z;
+  int kvh = blockIdx.y, hg = 0;
   if (a.HG > 1) {
-    kvh = blockIdx.z / a.HG;
-    hg = blockIdx.z - kvh * a.HG;
+    kvh = blockIdx.y / a.HG;
+    hg = blockIdx.y - kvh * a.HG;
   }
   const int nh = min(RP, a.R - hg * RP);
   const int h0 = kvh * a.R + hg * RP;
   const int32_t *bt = a.bt + (int64_t)b * a.max_pages;
 
   // The block's wavefronts take tiles first, first + step, ... of the context,
-  // whose length they need not know for that: the first page ids are requested
+  // whose length they need not know for the first: its page ids are requested
   // beside it.  pidx, slot: of position kTile t + 16 u + c16 of the tile whose
   // page ids are requested next.
-  const int first = s * NW + wv, step = a.S * NW;
+  const int first = s * NW + wv;
   int pidx[NU], slot[NU], pg[NU];
 #pragma unroll
   for (int u = 0; u < NU; ++u) {
@@ -313,7 +346,8 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
     for (int u = 0; u < NU; ++u) pg[u] = bt[max(min(pidx[u], a.max_pages - 1), 0)];
   };
   page_ids();
-  const int ctx = (int)max((int64_t)0, min((int64_t)a.lens[b], (int64_t)a.max_pages * a.page_size));
+  const int ctx = context_of(a, a.lens[b]);
+  const int t_end = (ctx + kTile - 1) / kTile;
 
   for (int k = wv; k < NC; k += NW) {
     const int h = DUP ? c16 & 7 : c16;
@@ -326,16 +360,23 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
   }
 
   // rows in the pool of tile t's positions, whose page ids are there, and which
-  // lanes' positions exist (row 0 for others); then on to the next tile's ids
+  // lanes' positions exist (row 0 for others)
   auto rows = [&](int t, uint32_t (&row)[NU], uint64_t (&there)[NU]) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const bool ok = (c16 < ctx - kTile * t - 16 * u) & ((uint32_t)pg[u] < (uint32_t)a.P);
       row[u] = (((uint32_t)pg[u] * a.Hkv + kvh) * a.page_size + slot[u]) & (ok ? ~0u : 0u);
       there[u] = __builtin_amdgcn_ballot_w64(ok);
-      slot[u] += a.dslot;
+    }
+  };
+  // on to the next tile's ids
+  int dpage, dslot;
+  auto advance = [&]() {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      slot[u] += dslot;
       const bool over = slot[u] >= a.page_size;
-      pidx[u] += a.dpage + (over ? 1 : 0);
+      pidx[u] += dpage + (over ? 1 : 0);
       slot[u] -= over ? a.page_size : 0;
     }
     page_ids();
@@ -368,8 +409,20 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
   uint32_t row[NU], kd[NU][NC], ksc[NU], vd[NU][NC], vsc[NU];
   uint64_t there[NU];
   int t = first;
-  const int t_end = (ctx + kTile - 1) / kTile;
+  const int S = __builtin_amdgcn_readfirstlane(a.S > 1 ? splits_of(a, t_end, lane, kTile) : 1);
+  const int step = S * NW;
+  if (s >= S) {
+    if (threadIdx.x < nh) {
+      const int64_t n = (int64_t)b * a.Hq + h0 + threadIdx.x;
+      a.part_ml[(n * a.S + s) * 2] = -INFINITY;
+      a.part_ml[(n * a.S + s) * 2 + 1] = 0.f;
+    }
+    return;
+  }
+  dpage = page_of(kTile * step, a.ps_mul, a.ps_shift);
+  dslot = kTile * step - dpage * a.page_size;
   rows(t, row, there);
+  advance();  // (before the keys, in the loop's order)
   load(a.kc, a.ks, row, kd, ksc);
   load(a.vc, a.vs, row, vd, vsc);
   __syncthreads();  // the query is there
@@ -391,6 +444,7 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
 #pragma unroll
     for (int u = 0; u < NU; ++u) now[u] = there[u];
     rows(t + step, row, there);
+    advance();
     load(a.kc, a.ks, row, kd, ksc);
     __builtin_amdgcn_sched_barrier(0);  // (requested before this tile's values are waited for)
 
@@ -503,7 +557,8 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
 }
 
 // Splits of a row: sum_s 2^(M_s - M) O_s / sum_s 2^(M_s - M) L_s, a wavefront a
-// row: lane s takes split s's maximum and sum, then each lane D / 64 dims of all.
+// row: lane s takes split s's maximum and sum, then each lane D / 64 dims of those
+// with a weight (others were perhaps not written).
 constexpr int kMaxSplits = 64;
 template <int DH>
 __global__ __launch_bounds__(kRowThreads) void mx_combine_kernel(const float *__restrict__ part_o,
@@ -524,22 +579,22 @@ __global__ __launch_bounds__(kRowThreads) void mx_combine_kernel(const float *__
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
   const float w = exp2_below(ms, M);
-  float L = w * ls;
-#pragma unroll
-  for (int x = 32; x > 0; x >>= 1) L += __shfl_xor(L, x);
+  const float L = wave_sum(w * ls);
+  const uint64_t on = __builtin_amdgcn_ballot_w64(w != 0.f);
+  const int last = on ? 64 - __builtin_clzll(on) : 0;
   float acc[PD] = {};
   constexpr int kAhead = 8;
-  for (int s0 = 0; s0 < S; s0 += kAhead) {
+  for (int s0 = 0; s0 < last; s0 += kAhead) {
     float v[kAhead][PD];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
 #pragma unroll
-      for (int d = 0; d < PD; ++d) v[j][d] = s0 + j < S ? po[(int64_t)(s0 + j) * DH + d] : 0.f;
+      for (int d = 0; d < PD; ++d) v[j][d] = po[(int64_t)min(s0 + j, last - 1) * DH + d];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), (s0 + j) & 63));
 #pragma unroll
-      for (int d = 0; d < PD; ++d) acc[d] += s0 + j < S ? f * v[j][d] : 0.f;
+      for (int d = 0; d < PD; ++d) acc[d] += s0 + j < last && f != 0.f ? f * v[j][d] : 0.f;
     }
   }
 #pragma unroll
@@ -549,25 +604,37 @@ __global__ __launch_bounds__(kRowThreads) void mx_combine_kernel(const float *__
 
 constexpr int64_t kMaxRows = 0x3FFFFFF;  // query rows of a call: wavefronts of a launch
 
-// Wavefronts a block and splits of a context.
+// Wavefronts a block and most splits of a context (which the kernel shares out by
+// length).  us, 32/4 heads of 128: 64 requests of 4096 positions in blocks of 8 x 1
+// wavefronts x splits 27, 4 x 1 36, 8 x 2 32; 16 of 4096 8 x 4 13.4, 4 x 4 and 4 x 8
+// 14.4, 8 x 8 16; 16/16 heads of 64, 64 requests of 1024: 4 x 1 21.6, 8 x 1 23.6.
+// (A long context among short ones has no more than an equal share: twice as many
+// splits, half of them without work, 32 requests of 500 to 4096 positions 21.2 us
+// for 19.6, and 16 of 38000 to 40960 81 for 62, since some CUs get two blocks.)
 struct MxPlan {
   bool decode;
   int HG, S, NW;
+  float slots;  // blocks for a kv head's group of query heads: one of 8 wavefronts or
+                // two of 4 a CU
 };
 MxPlan mx_plan(int64_t B, int64_t L, int64_t D, int64_t max_pages, int64_t page_size, int Hkv,
                int Hq) {
-  MxPlan p{false, 1, 1, 4};
+  MxPlan p{false, 1, 1, 4, 1.f};
   if (L > 1 || (D != 64 && D != 128) || B == 0) return p;
   const int R = Hq / Hkv;
   p.HG = R <= 8 ? 1 : (R + 15) / 16;
   // (a launch has below 2^32 threads, and below 2^16 blocks but for the first dimension)
-  if (B > kMaxRows / 8 || (int64_t)Hkv * p.HG > 0xFFFF) return p;
+  const int64_t heads = (int64_t)Hkv * p.HG;
+  if (B > kMaxRows / 8 || heads > 0xFFFF) return p;
   p.decode = true;
-  const int64_t tiles = (max_pages * page_size + kTile - 1) / kTile;
-  const int64_t base = B * Hkv * p.HG, want = 4 * (int64_t)cu_count();
-  p.S = (int)std::max<int64_t>(1, std::min<int64_t>({(want + base - 1) / base,
-                                                     (tiles + p.NW - 1) / p.NW,
-                                                     (int64_t)kMaxSplits}));
+  const int64_t tiles = (max_pages * page_size + kTile - 1) / kTile, cu = cu_count();
+  p.NW = B * heads >= 2 * cu || B * heads * 8 < cu ? 4 : 8;
+  p.slots = (float)(8 / p.NW * cu) / (float)heads;
+  if (B * heads < cu)
+    p.S = (int)std::max<int64_t>(1, std::min<int64_t>({(int64_t)ceil(sqrt(2. * (double)tiles)),
+                                                       (tiles + p.NW - 1) / p.NW,
+                                                       8 / p.NW * cu / heads / B,
+                                                       (int64_t)kMaxSplits}));
   return p;
 }
 size_t mx_workspace(const MxPlan &p, int64_t rows, int64_t D) {
@@ -578,7 +645,7 @@ size_t mx_workspace(const MxPlan &p, int64_t rows, int64_t D) {
 
 template <int QT, int DH, bool DUP>
 void launch_decode_nw(const MxAttnArgs &a, int NW, hipStream_t st) {
-  const dim3 grid(a.B, a.S, a.Hkv * a.HG);
+  const dim3 grid(a.B, a.Hkv * a.HG, a.S);
   if (NW == 8)
     hipLaunchKernelGGL((mx_decode_kernel<QT, DH, DUP, 8>), grid, dim3(512), 0, st, a);
   else
@@ -701,9 +768,7 @@ int nvm_paged_attention_mx(const void *q, int q_dtype, int64_t q_stride_b, int64
     return set_error(NVM_ERR_WORKSPACE, "%s: workspace of %zu bytes needed", op, need);
   a.HG = plan.HG;
   a.S = plan.S;
-  const int64_t ahead = (int64_t)kTile * plan.S * plan.NW;
-  a.dpage = (int)(ahead / page_size);
-  a.dslot = (int)(ahead % page_size);
+  a.slots = plan.slots;
   if (plan.S > 1) {
     a.part_o = (float *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
     a.part_ml = (float *)((char *)a.part_o +
