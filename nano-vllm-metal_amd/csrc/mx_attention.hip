@@ -31,6 +31,7 @@
 
 #include "common.h"
 #include "internal.h"
+#include "mx_attention.h"
 #include "mx_common.h"
 #include "nvm_mx_cache.h"
 
@@ -41,49 +42,11 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRowThreads = 256;
 
-struct MxAttnArgs {
-  const void *q;
-  int64_t q_sb, q_sh, q_sl;
-  const uint8_t *kc, *ks, *vc, *vs;
-  const int32_t *bt, *lens;
-  void *out;
-  int out_dt;
-  int B, L, D, P, page_size, max_pages, Hkv, Hq, R, causal;
-  float scale2;  // |scale| * log2(e): scores are kept in base 2
-  uint32_t q_sign;  // the sign bits to flip in two 16-bit query parts, for a negative scale
-  uint32_t ps_mul, ps_shift;  // position / page_size, see page_of
-  int HG, S;                  // groups of query heads, most splits of a context
-  float slots;                // blocks to be had for the splits, a kv head's group of query heads
-  float *part_o, *part_ml;    // splits' outputs [row][S][D], maxima and sums [row][S][2]
-};
-
-// n / page_size of n below 2^31: with 2^(l-1) < page_size <= 2^l the factor is
-// ceil(2^(31 + l) / page_size), off by less than 2^-31 of n, which no quotient
-// notices (page_size 1: a factor of 0 stands for 2^32).
-__device__ __forceinline__ int page_of(int n, uint32_t mul, uint32_t shift) {
-  return mul ? (int)(__umulhi((uint32_t)n, mul) >> shift) : n;
-}
-
-__device__ __forceinline__ void store_out(void *out, int dt, int64_t i, float v) {
-  if (dt == NVM_KV_F32)
-    ((float *)out)[i] = v;
-  else if (dt == NVM_KV_BF16)
-    ((uint16_t *)out)[i] = Act<DT_BF16>::from_f32(v);
-  else
-    ((uint16_t *)out)[i] = Act<DT_F16>::from_f32(v);
-}
-
 template <int QT>
 __device__ __forceinline__ float q_at(const void *q, int64_t i) {
   if constexpr (QT == NVM_KV_F32) return ((const float *)q)[i];
   if constexpr (QT == NVM_KV_BF16) return Act<DT_BF16>::to_f32(((const uint16_t *)q)[i]);
   return Act<DT_F16>::to_f32(((const uint16_t *)q)[i]);
-}
-
-// 2^(x - m) with m the running maximum: nothing seen so far (m = -inf) counts as
-// zero, so that a masked score gives 0 and a NaN stays one.
-__device__ __forceinline__ float exp2_below(float x, float m) {
-  return __builtin_amdgcn_exp2f(x - (m == -INFINITY ? 0.f : m));
 }
 
 __device__ __forceinline__ void values8(uint32_t d, float s, float (&v)[8]) {
@@ -173,56 +136,6 @@ hipError_t launch_rows(const MxAttnArgs &a, hipStream_t st) {
   return hipGetLastError();
 }
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-// A 4 x 16 block of 16-bit values in LDS, transposed: of a group of 16 lanes,
-// lane i passes the address of values 4 (i % 4) .. + 3 of row i / 4 and gets
-// column i.
-__device__ __forceinline__ u32x2 lds_read_tr(const uint16_t *p) {
-  return __builtin_bit_cast(
-      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p));
-}
-
-template <int QT>
-constexpr int kParts = QT == NVM_KV_F32 ? 3 : QT == NVM_KV_F16 ? 2 : 1;
-
-// Eight query values as bf16 parts whose sum they are.
-template <int QT>
-__device__ __forceinline__ void query8(const void *q, int64_t i, u32x4 (&p)[kParts<QT>]) {
-  using A = Act<DT_BF16>;
-  if constexpr (QT == NVM_KV_BF16) {
-    p[0] = ldg16((const uint16_t *)q + i);
-  } else {
-    float x[8];
-    if constexpr (QT == NVM_KV_F32) {
-      const f32x4 a = *(const f32x4 *)((const float *)q + i);
-      const f32x4 b = *(const f32x4 *)((const float *)q + i + 4);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = a[j], x[4 + j] = b[j];
-    } else {
-      const u32x4 a = ldg16((const uint16_t *)q + i);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) x[2 * j] = Act<DT_F16>::lo(a[j]), x[2 * j + 1] = Act<DT_F16>::hi(a[j]);
-    }
-#pragma unroll
-    for (int k = 0; k < kParts<QT>; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        p[k][j] = A::pack2(x[2 * j], x[2 * j + 1]);
-        x[2 * j] -= A::lo(p[k][j]);
-        x[2 * j + 1] -= A::hi(p[k][j]);
-      }
-  }
-}
-
-// Eight codes times a scale (a float of that exponent), as an MFMA operand.
-__device__ __forceinline__ u32x4 codes_bf16(uint32_t d, float s) {
-  return u32x4{mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 0)),
-               mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 1)),
-               mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 2)),
-               mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 3))};
-}
-
 // N dwords from p, 4 N-byte aligned.
 template <int N>
 __device__ __forceinline__ void load_dwords(const uint8_t *p, uint32_t (&d)[N]) {
@@ -246,18 +159,6 @@ __device__ __forceinline__ float column_max(float v) {
 
 constexpr int kTile = 32;  // positions of a wavefront's step: two of the MFMA's 16 rows
 
-// Four consecutive outputs, from element i on.
-__device__ __forceinline__ void store_out4(void *out, int dt, int64_t i, f32x4 v) {
-  if (dt == NVM_KV_F32)
-    *(f32x4 *)((float *)out + i) = v;
-  else if (dt == NVM_KV_BF16)
-    *(u32x2 *)((uint16_t *)out + i) =
-        u32x2{Act<DT_BF16>::pack2(v[0], v[1]), Act<DT_BF16>::pack2(v[2], v[3])};
-  else
-    *(u32x2 *)((uint16_t *)out + i) =
-        u32x2{Act<DT_F16>::pack2(v[0], v[1]), Act<DT_F16>::pack2(v[2], v[3])};
-}
-
 // Sum over the wavefront, in an order of its own: the same in every lane and block.
 __device__ __forceinline__ float wave_sum(float v) {
   auto step = [&](uint32_t o) { v += __uint_as_float(o); };
@@ -270,10 +171,6 @@ __device__ __forceinline__ float wave_sum(float v) {
   for (int i = 0; i < 64; i += 16)
     r += __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), i));
   return r;
-}
-
-__device__ __forceinline__ int context_of(const MxAttnArgs &a, int len) {
-  return (int)max((int64_t)0, min((int64_t)len, (int64_t)a.max_pages * a.page_size));
 }
 
 // Splits of a context of `tiles` tiles: its share of the slots by length (the host
@@ -612,16 +509,26 @@ constexpr int64_t kMaxRows = 0x3FFFFFF;  // query rows of a call: wavefronts of 
 // splits, half of them without work, 32 requests of 500 to 4096 positions 21.2 us
 // for 19.6, and 16 of 38000 to 40960 81 for 62, since some CUs get two blocks.)
 struct MxPlan {
-  bool decode;
+  bool decode, prefill;
   int HG, S, NW;
   float slots;  // blocks for a kv head's group of query heads: one of 8 wavefronts or
                 // two of 4 a CU
 };
 MxPlan mx_plan(int64_t B, int64_t L, int64_t D, int64_t max_pages, int64_t page_size, int Hkv,
                int Hq) {
-  MxPlan p{false, 1, 1, 4, 1.f};
-  if (L > 1 || (D != 64 && D != 128) || B == 0) return p;
+  MxPlan p{false, false, 1, 1, 4, 1.f};
+  if ((D != 64 && D != 128) || B == 0) return p;
   const int R = Hq / Hkv;
+  if (L > 1) {
+    // a block a CU and as many splits as that takes, none of fewer than four tiles
+    // of 64 positions
+    const int64_t blocks = mx_prefill_blocks(L, R), cu = cu_count();
+    if (B > 0xFFFF || blocks * Hkv > 0x7FFFFF) return p;
+    p.prefill = true;
+    const int64_t base = blocks * Hkv * B, tiles = (max_pages * page_size + 63) / 64;
+    p.S = (int)std::max<int64_t>(1, std::min<int64_t>({cu / base, tiles / 4, (int64_t)kMaxSplits}));
+    return p;
+  }
   p.HG = R <= 8 ? 1 : (R + 15) / 16;
   // (a launch has below 2^32 threads, and below 2^16 blocks but for the first dimension)
   const int64_t heads = (int64_t)Hkv * p.HG;
@@ -660,9 +567,13 @@ hipError_t launch_decode(const MxAttnArgs &a, int NW, hipStream_t st) {
   else
     a.R <= 8 ? launch_decode_nw<QT, 64, true>(a, NW, st)
              : launch_decode_nw<QT, 64, false>(a, NW, st);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.S == 1) return e;
-  const int64_t rows = (int64_t)a.B * a.Hq;
+  return hipGetLastError();
+}
+
+// The splits' outputs together, if there are any.
+hipError_t launch_combine(const MxAttnArgs &a, hipStream_t st) {
+  if (a.S == 1) return hipSuccess;
+  const int64_t rows = (int64_t)a.B * a.L * a.Hq;
   const unsigned blocks = (unsigned)((rows + kRowThreads / 64 - 1) / (kRowThreads / 64));
   hipLaunchKernelGGL(a.D == 128 ? mx_combine_kernel<128> : mx_combine_kernel<64>, dim3(blocks),
                      dim3(kRowThreads), 0, st, a.part_o, a.part_ml, rows, a.S, a.out, a.out_dt);
@@ -779,9 +690,11 @@ int nvm_paged_attention_mx(const void *q, int q_dtype, int64_t q_stride_b, int64
     constexpr int QT = decltype(qt)::value;
     return plan.decode ? launch_decode<QT>(a, plan.NW, st) : launch_rows<QT>(a, st);
   };
-  const hipError_t e = q_dtype == NVM_KV_F32    ? go(MxInt<NVM_KV_F32>{})
-                       : q_dtype == NVM_KV_BF16 ? go(MxInt<NVM_KV_BF16>{})
-                                                : go(MxInt<NVM_KV_F16>{});
+  hipError_t e = plan.prefill             ? launch_mx_prefill(q_dtype, a, st)
+                 : q_dtype == NVM_KV_F32  ? go(MxInt<NVM_KV_F32>{})
+                 : q_dtype == NVM_KV_BF16 ? go(MxInt<NVM_KV_BF16>{})
+                                          : go(MxInt<NVM_KV_F16>{});
+  if (e == hipSuccess) e = launch_combine(a, st);
   if (e != hipSuccess) return set_error(NVM_ERR_HIP, "%s: %s", op, hipGetErrorString(e));
   return NVM_OK;
 }
