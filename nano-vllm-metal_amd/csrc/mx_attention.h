@@ -40,15 +40,13 @@ __device__ __forceinline__ void store_out(void *out, int dt, int64_t i, float v)
 }
 
 // Four consecutive outputs, from element i on.
-__device__ __forceinline__ void store_out4(void *out, int dt, int64_t i, f32x4 v) {
-  if (dt == NVM_KV_F32)
+template <int DT>
+__device__ __forceinline__ void store_out4(void *out, int64_t i, f32x4 v) {
+  if constexpr (DT == NVM_KV_F32)
     *(f32x4 *)((float *)out + i) = v;
-  else if (dt == NVM_KV_BF16)
-    *(u32x2 *)((uint16_t *)out + i) =
-        u32x2{Act<DT_BF16>::pack2(v[0], v[1]), Act<DT_BF16>::pack2(v[2], v[3])};
   else
     *(u32x2 *)((uint16_t *)out + i) =
-        u32x2{Act<DT_F16>::pack2(v[0], v[1]), Act<DT_F16>::pack2(v[2], v[3])};
+        u32x2{Act<DT>::pack2(v[0], v[1]), Act<DT>::pack2(v[2], v[3])};
 }
 
 // 2^(x - m) with m the running maximum: nothing seen so far (m = -inf) counts as
@@ -105,6 +103,19 @@ __device__ __forceinline__ u32x4 codes_bf16(uint32_t d, float s) {
                mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 1)),
                mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 2)),
                mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(d, s, 3))};
+}
+
+// N dwords from p, 4 N-byte aligned.
+template <int N>
+__device__ __forceinline__ void load_dwords(const uint8_t *p, uint32_t (&d)[N]) {
+  static_assert(N == 2 || N == 4, "a load");
+  if constexpr (N == 4) {
+    const u32x4 v = ldg16_once(p);
+    d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
+  } else {
+    const u32x2 v = __builtin_nontemporal_load((const u32x2 *)p);
+    d[0] = v.x, d[1] = v.y;
+  }
 }
 
 __device__ __forceinline__ int context_of(const MxAttnArgs &a, int len) {

@@ -136,19 +136,6 @@ hipError_t launch_rows(const MxAttnArgs &a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// N dwords from p, 4 N-byte aligned.
-template <int N>
-__device__ __forceinline__ void load_dwords(const uint8_t *p, uint32_t (&d)[N]) {
-  static_assert(N == 2 || N == 4, "a load");
-  if constexpr (N == 4) {
-    const u32x4 v = ldg16_once(p);
-    d[0] = v.x, d[1] = v.y, d[2] = v.z, d[3] = v.w;
-  } else {
-    const u32x2 v = __builtin_nontemporal_load((const u32x2 *)p);
-    d[0] = v.x, d[1] = v.y;
-  }
-}
-
 // The largest over a column's four lanes (lane groups 0..3).
 __device__ __forceinline__ float column_max(float v) {
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -442,7 +429,8 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
     const int64_t n = (int64_t)b * a.Hq + h0 + r;
     if (a.S == 1) {
       const float inv = 1.f / Ls;
-      store_out4(a.out, a.out_dt, n * DH + d, Ls == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : Os * inv);
+      const f32x4 o = Ls == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : Os * inv;
+      mx_by_dtype(a.out_dt, [&](auto dt) { store_out4<decltype(dt)::value>(a.out, n * DH + d, o); });
     } else {
       *(f32x4 *)(a.part_o + (n * a.S + s) * DH + d) = Os;
       if (d == 0) {
@@ -520,13 +508,13 @@ MxPlan mx_plan(int64_t B, int64_t L, int64_t D, int64_t max_pages, int64_t page_
   if ((D != 64 && D != 128) || B == 0) return p;
   const int R = Hq / Hkv;
   if (L > 1) {
-    // a block a CU and as many splits as that takes, none of fewer than four tiles
-    // of 64 positions
+    // two blocks a CU and as many splits as that takes, none of fewer than four
+    // tiles of 64 positions
     const int64_t blocks = mx_prefill_blocks(L, R), cu = cu_count();
     if (B > 0xFFFF || blocks * Hkv > 0x7FFFFF) return p;
     p.prefill = true;
     const int64_t base = blocks * Hkv * B, tiles = (max_pages * page_size + 63) / 64;
-    p.S = (int)std::max<int64_t>(1, std::min<int64_t>({cu / base, tiles / 4, (int64_t)kMaxSplits}));
+    p.S = (int)std::max<int64_t>(1, std::min<int64_t>({2 * cu / base, tiles / 4, (int64_t)kMaxSplits}));
     return p;
   }
   p.HG = R <= 8 ? 1 : (R + 15) / 16;

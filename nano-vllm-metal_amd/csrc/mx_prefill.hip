@@ -2,7 +2,7 @@
 // prefill and prefill after a prefix (a launch of nvm_paged_attention_mx, declared
 // in include/nvm_mx_cache.h; D of 64 or 128).
 //
-// A block owns (request, kv head, 256 columns, a split of the context), a column
+// A block owns (request, kv head, 128 columns, a split of the context), a column
 // being one (query row, query head) of the heads that share the kv head, 32 of them
 // a wavefront.  Per 64 positions the codes of keys and values are converted to bf16
 // once for the block (exactly: E2M1 times a power of two) and put into LDS, two
@@ -30,7 +30,7 @@ namespace nvm {
 
 namespace {
 
-constexpr int kCW = 8;             // wavefronts of a block
+constexpr int kCW = 4;             // wavefronts of a block (two blocks a CU)
 constexpr int kCols = 32 * kCW;    // its columns
 constexpr int kKeys = 64;          // positions of a tile
 constexpr float kSlack = 6.f;
@@ -42,15 +42,14 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
   constexpr int NC = DH / 16;  // steps of a score MFMA
   constexpr int NT = DH / 32;  // tiles of the output
   constexpr int VP = DH + 8;   // LDS pitch of a row
-  constexpr int IT = DH / 16;  // threads of a row in staging: 16 values, 8 bytes of codes each
-  constexpr int NB = DH / 32;  // scales of a row
-  // (D of 128: every thread stages keys and values; 64: half of them each)
-  constexpr bool kBoth = kKeys * IT == 64 * kCW;
-  static_assert(kBoth || 2 * kKeys * IT == 64 * kCW, "one item a thread");
+  constexpr int NB = DH / 32;  // scales of a row; dwords of codes of a quarter of it
+  static_assert(4 * kKeys == 64 * kCW, "a quarter of a row a thread");
   __shared__ __attribute__((aligned(16))) uint16_t s_k[2][kKeys][VP], s_v[2][kKeys][VP];
-  __shared__ uint8_t s_ok[2][kKeys], s_nan[2][kKeys];  // there?  its value blocks of NaNs
-  // of each wavefront's positions: bit 0 all there, bit 1 NaNs among the values
-  __shared__ __attribute__((aligned(8))) uint8_t s_all[2][kCW];
+  // of each wavefront's 16 positions: which are there; NaNs among their values?  of a
+  // position: its value blocks of NaNs
+  __shared__ __attribute__((aligned(8))) uint16_t s_ok[2][kCW];
+  __shared__ int s_any[2][kCW];
+  __shared__ uint8_t s_nan[2][kKeys];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -84,64 +83,59 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
     }
   }
 
-  // staging: this thread's position of a tile and part of its row
-  const int item = kBoth ? tid : tid & (64 * kCW / 2 - 1);
-  const int key = item / IT, part = item % IT;
-  const bool vals = !kBoth && tid >= 64 * kCW / 2;
-  const uint8_t *codes0 = vals ? a.vc : a.kc, *scales0 = vals ? a.vs : a.ks;
+  // staging: this thread's position of a tile and quarter of its row
+  const int key = tid >> 2, part = tid & 3;
   int pg;
   auto page_id = [&](int t) {
     const int pos = kKeys * t + key;
     pg = bt[max(min(page_of(pos, a.ps_mul, a.ps_shift), a.max_pages - 1), 0)];
   };
-  u32x2 d0, d1;
-  uint32_t sc0, sc1;
+  uint32_t kd[NB], vd[NB], ksc, vsc;
   bool ok;
   auto stage_load = [&](int t) {
     const int pos = kKeys * t + key;
     const int slot = pos - page_of(pos, a.ps_mul, a.ps_shift) * a.page_size;
     ok = (pos < ctx) & ((uint32_t)pg < (uint32_t)a.P);
     const uint32_t row = (((uint32_t)pg * a.Hkv + kvh) * a.page_size + slot) & (ok ? ~0u : 0u);
-    d0 = ldg8(codes0 + (uint64_t)row * (DH / 2) + 8 * part);
-    sc0 = scales0[(uint64_t)row * NB + part / 2];
-    if constexpr (kBoth) {
-      d1 = ldg8(a.vc + (uint64_t)row * (DH / 2) + 8 * part);
-      sc1 = a.vs[(uint64_t)row * NB + part / 2];
-    }
+    load_dwords<NB>(a.kc + (uint64_t)row * (DH / 2) + (DH / 8) * part, kd);
+    load_dwords<NB>(a.vc + (uint64_t)row * (DH / 2) + (DH / 8) * part, vd);
+    ksc = a.ks[(uint64_t)row * NB + (DH / 4) * part / 32];
+    vsc = a.vs[(uint64_t)row * NB + (DH / 4) * part / 32];
   };
   auto stage_store = [&](int buf) {
-    // (the values' scales are sc1, or with half of the threads sc0 of the other half)
-    const bool nan = ok & (kBoth ? sc1 == 255u : vals & (sc0 == 255u));
+    const bool nan = ok & (vsc == 255u);
+    const float f = __uint_as_float(ok ? ksc << 23 : 0u);
+    const float g = __uint_as_float(ok & !nan ? vsc << 23 : 0u);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      *(u32x4 *)&s_k[buf][key][(DH / 4) * part + 8 * j] = codes_bf16(kd[j], f);
+      *(u32x4 *)&s_v[buf][key][(DH / 4) * part + 8 * j] = codes_bf16(vd[j], g);
+    }
+    // (lane i of the first sixteen: position i of the wavefront's)
+    const uint64_t there = __builtin_amdgcn_ballot_w64(__shfl((int)ok, 4 * lane & 63) != 0);
     const uint64_t nans = __builtin_amdgcn_ballot_w64(nan);
-    const float f = __uint_as_float(ok & !(vals & nan) ? sc0 << 23 : 0u);
-    uint16_t *p = vals ? &s_v[buf][key][16 * part] : &s_k[buf][key][16 * part];
-    *(u32x4 *)p = codes_bf16(d0.x, f);
-    *(u32x4 *)(p + 8) = codes_bf16(d0.y, f);
-    if constexpr (kBoth) {
-      const float g = __uint_as_float(ok & !nan ? sc1 << 23 : 0u);
-      *(u32x4 *)&s_v[buf][key][16 * part] = codes_bf16(d1.x, g);
-      *(u32x4 *)&s_v[buf][key][16 * part + 8] = codes_bf16(d1.y, g);
+    if (lane == 0) {
+      s_ok[buf][wv] = (uint16_t)there;
+      s_any[buf][wv] = nans != 0;
     }
     if (part == 0) {
-      if (kBoth || !vals) s_ok[buf][key] = ok;
-      if (kBoth || vals) {  // bit 2 j of the row's lanes is block j
-        const uint32_t m = (uint32_t)(nans >> lane);
-        s_nan[buf][key] = (uint8_t)((m & 1) | (m >> 1 & 2) |
-                                    (NB > 2 ? (m >> 2 & 4) | (m >> 3 & 8) : 0u));
-      }
+      const uint32_t m = (uint32_t)(nans >> lane) & 15u;  // by quarters
+      s_nan[buf][key] = (uint8_t)(NB == 4 ? m : (m & 1) | (m >> 1 & 2));
     }
-    if (lane == 0)
-      s_all[buf][wv] = (__builtin_amdgcn_ballot_w64(ok) == ~0ull ? 1 : 0) | (nans ? 2 : 0);
   };
 
   float m_run = -INFINITY, l_run = 0.f;  // column c32's; l_run this lane's share
-  uint32_t seen_nan = 0;                 // value blocks of NaNs that this lane's positions have
+  uint32_t seen_nan = 0;                 // value blocks of NaNs that the column sees
   f32x16 oacc[NT];                       // O^T: column c32, dims 32 t + 8 j + 4 h + i
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) oacc[t][i] = 0.f;
 
+  // (-1, 0) and (0, -1), which pick out of a pair (in registers: as a constant the
+  // second is taken for the inline constant -1.0, in the other half)
+  uint32_t pick0 = 0x0000BF80u, pick1 = 0xBF800000u;
+  asm volatile("" : "+v"(pick0), "+v"(pick1));
   page_id(t0);
   stage_load(t0);
   page_id(t0 + 1);
@@ -164,20 +158,25 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
         for (int p = 0; p < QP; ++p) acc[u] = A::mfma32(kb, qop[k][p], acc[u]);
       }
     }
-    const uint64_t all = *(const uint64_t *)s_all[buf];
-    if (all != 0x0101010101010101ull || kKeys * (t + 1) > all_see) {  // uniform
+    const uint64_t there = *(const uint64_t *)s_ok[buf];
+    if (there != ~0ull || kKeys * (t + 1) > all_see) {  // uniform
+      // bits of what this column sees; those of this lane's element i of part u are
+      // 8 (i / 4) + i % 4 of the word
+      const int n = bound - kKeys * t + 1;
+      const uint64_t seen = n >= 64 ? there : n <= 0 ? 0 : there & ((1ull << n) - 1);
+      const uint32_t w[2] = {(uint32_t)seen >> (4 * h), (uint32_t)(seen >> 32) >> (4 * h)};
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int kl = 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-          if (!s_ok[buf][kl] || kKeys * t + kl > bound) acc[u][i] = -INFINITY;
+          const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)w[u], 8 * (i >> 2) + (i & 3), 1);
+          acc[u][i] = __uint_as_float((__float_as_uint(acc[u][i]) & m) | (~m & 0xFF800000u));
         }
-      if (all & 0x0202020202020202ull)  // uniform
-        for (int j = 0; j < 32; ++j) {
-          const int kl = 8 * (j >> 2) + 4 * h + (j & 3);
-          if (kKeys * t + kl <= bound) seen_nan |= s_nan[buf][kl];
-        }
+    }
+    if (s_any[buf][0] | s_any[buf][1] | s_any[buf][2] | s_any[buf][3]) {  // uniform
+#pragma unroll 1
+      for (int kl = 0; kl < kKeys; ++kl)
+        if (kKeys * t + kl <= bound) seen_nan |= s_nan[buf][kl];
     }
     float tmax = acc[0][0];
 #pragma unroll
@@ -209,7 +208,7 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
         const float y = __builtin_amdgcn_exp2f(fmaf(acc[c >> 1][i + 1], a.scale2, -m_sub));
         l_run += x + y;
         hi[c][j] = A::pack2(x, y);
-        lo[c][j] = A::pack2(x - A::lo(hi[c][j]), y - A::hi(hi[c][j]));
+        lo[c][j] = A::pack2(A::dot2(hi[c][j], pick0, x), A::dot2(hi[c][j], pick1, y));
       }
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -228,27 +227,28 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
   }
 
   l_run += __shfl_xor(l_run, 32);
-  seen_nan |= __shfl_xor(seen_nan, 32);
   if (!col_ok) return;
   const int64_t n = ((int64_t)b * a.L + qrow) * a.Hq + head;
   const bool whole = a.S == 1;
   const float inv = whole ? (l_run == 0.f ? 0.f : 1.f / l_run) : 1.f;
+  auto store = [&](void *out, int64_t row, auto dt) {
 #pragma unroll
-  for (int k = 0; k < NT; ++k)
+    for (int k = 0; k < NT; ++k)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f32x4 o;
+      for (int j = 0; j < 4; ++j) {
+        f32x4 o;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        o[i] = seen_nan >> k & 1   ? __builtin_nanf("")
-               : l_run == 0.f ? 0.f
-                              : oacc[k][4 * j + i] * inv;
-      const int d = 32 * k + 8 * j + 4 * h;
-      if (whole)
-        store_out4(a.out, a.out_dt, n * DH + d, o);
-      else
-        *(f32x4 *)(a.part_o + (n * a.S + s) * DH + d) = o;
-    }
+        for (int i = 0; i < 4; ++i)
+          o[i] = seen_nan >> k & 1 ? __builtin_nanf("")
+                 : l_run == 0.f    ? 0.f
+                                   : oacc[k][4 * j + i] * inv;
+        store_out4<decltype(dt)::value>(out, row * DH + 32 * k + 8 * j + 4 * h, o);
+      }
+  };
+  if (whole)
+    mx_by_dtype(a.out_dt, [&](auto dt) { store(a.out, n, dt); });
+  else
+    store(a.part_o, n * a.S + s, MxInt<NVM_KV_F32>{});
   if (!whole && h == 0) {
     a.part_ml[(n * a.S + s) * 2] = m_run;
     a.part_ml[(n * a.S + s) * 2 + 1] = l_run;
