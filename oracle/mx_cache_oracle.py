@@ -27,14 +27,20 @@ def norm_rope(x, w, cos, sin, eps):
     return out, size
 
 
-def attention(q, keys, values, table, lens, scale, causal):
+def weight_error(L, D, out_dtype):
+    """What the weights are rounded by: 2^-11 (f16) where several rows on the matrix
+    cores have a bf16 output, else two bf16 parts."""
+    return 2.0 ** -11 if L > 1 and D in (64, 128) and out_dtype == torch.bfloat16 else 2.0 ** -16
+
+
+def attention(q, keys, values, table, lens, scale, causal, weights=2.0 ** -16):
     """``q [B, Hq, L, D]``, pages as (codes, scales) -> (float64 ``[B, Hq, L,
     D]``, bound): with n visible positions, scores s_j, largest value V of a
     column, and u = 2^-23 for a float32 addition in any order,
     a score is off by (D + 4) u sum |q k| scale and the exponent it goes into by
     u (|s_j| + |m|) log2 e more, so each weight by d of itself, twice exp's u among
-    it; the quotient by 2 d + (2 n + 8) u of V; weights go into the product in
-    parts that leave 2^-16."""
+    it; the quotient by 2 d + (2 n + 8) u of V; weights go into the product with
+    a rounding of ``weights``, beside their sum without it."""
     kd, vd = (MX.decode(c, s, "mxfp4") for c, s in (keys, values))
     P, Hkv, ps, D = kd.shape
     B, Hq, L, _ = q.shape
@@ -55,7 +61,7 @@ def attention(q, keys, values, table, lens, scale, causal):
             k, v = (t[page, h // (Hq // Hkv), j % ps] for t in (kd, vd))
             x = q[b, h].double()
             s = x @ k.T * scale
-            off = (D + 4) * u * scale * (x.abs() @ k.abs().T)
+            off = (D + 4) * u * abs(scale) * (x.abs() @ k.abs().T)
             seen = torch.ones_like(s, dtype=torch.bool)
             if causal:
                 seen = j[None] <= torch.arange(L)[:, None] + int(lens[b]) - L
@@ -69,7 +75,7 @@ def attention(q, keys, values, table, lens, scale, causal):
                 # (an error of a weight that hardly counts hardly counts)
                 d = float((p * torch.expm1(d)).sum() / p.sum())
                 out[b, h, i] = p @ vi / p.sum()
-                bound[b, h, i] = (2 * d + (2 * len(si) + 8) * u + 2.0 ** -16) * vi.abs().amax(0)
+                bound[b, h, i] = (2 * d + (2 * len(si) + 8) * u + weights) * vi.abs().amax(0)
     return out, bound
 
 

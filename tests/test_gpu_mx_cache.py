@@ -229,7 +229,7 @@ def _check_attention(q, k, v, bt, lens, causal, odt=None, scale=None):
     odt = odt or q.dtype
     assert got.dtype == odt and got.shape == q.shape
     want, bound = C.attention(q, k, v, bt, lens, q.shape[-1] ** -0.5 if scale is None else scale,
-                              causal)
+                              causal, C.weight_error(*q.shape[2:], odt))
     bound = bound + torch.finfo(odt).eps / 2 * want.abs() + torch.finfo(odt).tiny
     off = (got.cpu().double() - want).abs()
     assert (off <= bound).all(), (f"{int((off > bound).sum())} of {off.numel()} off, "
@@ -303,6 +303,14 @@ def test_rows_that_see_nothing():
     assert got.shape == (0, 8, 6, 64)
 
 
+def test_attention_scale_signs():
+    """A negative scale, and zero: all positions alike."""
+    for L, D in ((1, 128), (1, 96), (9, 64)):
+        q, k, v, bt, lens = _attention_case(13, 2, 8, 2, D, 16, [90, 33], L, torch.float16)
+        _check_attention(q, k, v, bt, lens, True, scale=-0.2)
+        _check_attention(q, k, v, bt, lens, True, scale=0.0)
+
+
 @pytest.mark.parametrize("L", [1, 20])
 @pytest.mark.parametrize("D", [64, 128, 96])
 def test_slots_behind_the_context_do_not_count(L, D):
@@ -358,10 +366,34 @@ def test_attention_query_strides():
                                want)
 
 
-def test_attention_extreme_scales():
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lo,hi", [(104, 104), (104, 140), (103, 103), (141, 141), (1, 1), (0, 0), (90, 127),
+                                   (200, 200)])
+def test_several_rows_value_scales(D, lo, hi):
+    """Value scales inside f16's range, at its ends, just beyond and far beyond."""
+    g = torch.Generator().manual_seed(lo + hi)
+    q, k, v, bt, lens = _attention_case(11, 2, 8, 2, D, 16, [150, 97], 40, torch.bfloat16)
+    v[1][:] = torch.where(torch.rand(v[1].shape, generator=g) < 0.5, lo, hi).to(torch.uint8)
+    _check_attention(q, k, v, bt, lens, True)
+
+
+def test_several_rows_many_small_weights():
+    """One position far above 3000 others, which weigh 2^-13 to 2^-27 of it."""
+    q, k, v, bt, lens = _attention_case(12, 1, 2, 1, 64, 16, [3000], 2, torch.bfloat16)
+    q[:] = 1
+    k[0][:], k[1][:] = 0x22, 127  # ones
+    at = bt[0].long()
+    for s, top in ((13.0, 100), (22.0, 2000), (27.0, 5)):
+        k[1][at[top // 16], 0, top % 16] = 128  # a score of 64 above the others
+        _check_attention(q, k, v, bt, lens, False, scale=s * 0.6931 / 64)
+        k[1][at[top // 16], 0, top % 16] = 127
+
+
+@pytest.mark.parametrize("L", [1, 3])
+def test_attention_extreme_scales(L):
     """Blocks at both ends of the scales' range: keys and values of 2^-127 to
     2^-120 and beside them 2^100, queries to match."""
-    q, k, v, bt, lens = _attention_case(10, 1, 4, 2, 128, 16, [100], 1, torch.float32)
+    q, k, v, bt, lens = _attention_case(10, 1, 4, 2, 128, 16, [100], L, torch.float32)
     k[1][:, :, :, 0], k[1][:, :, :, 1] = 3, 227
     q[..., :32] *= 2.0 ** 100
     q[..., 32:64] *= 2.0 ** -100

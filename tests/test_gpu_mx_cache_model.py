@@ -105,7 +105,8 @@ def test_steps_of_a_layer(dt):
         got = paged_attention_mx(q, kp, vp, bt, lens, mask="causal")
         cache.advance(who, L)
         held = [(p.codes.cpu(), p.scales.cpu()) for p in (kp, vp)]
-        want, bound = C.attention(q.cpu(), *held, bt.cpu(), lens.cpu(), D ** -0.5, True)
+        want, bound = C.attention(q.cpu(), *held, bt.cpu(), lens.cpu(), D ** -0.5, True,
+                                   C.weight_error(L, D, dt))
         bound = bound + torch.finfo(dt).eps / 2 * want.abs() + torch.finfo(dt).tiny
         assert ((got.cpu().double() - want).abs() <= bound).all(), (who, L)
         for i, s in enumerate(who):
