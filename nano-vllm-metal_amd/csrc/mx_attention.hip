@@ -508,13 +508,22 @@ MxPlan mx_plan(int64_t B, int64_t L, int64_t D, int64_t max_pages, int64_t page_
   if ((D != 64 && D != 128) || B == 0) return p;
   const int R = Hq / Hkv;
   if (L > 1) {
-    // two blocks a CU and as many splits as that takes, none of fewer than four
-    // tiles of 64 positions
+    // The splits of the least time: a tile of 64 positions takes a block 1.55 us, half
+    // as much more beside another block of its CU; a merge 3 us and its outputs'
+    // way there and back at 5 TB/s.  (us with 1, 2, 4, 8, 16, 32 splits, 32/4 heads of
+    // 128: 512 rows over 4096 positions 102, 69, 60, 70, 98, 161; 4 x 256 over 1280 42,
+    // 55, 64, 89, 158; 16 over 8192 193, 104, 57, 35, 25, 23.)
     const int64_t blocks = mx_prefill_blocks(L, R), cu = cu_count();
     if (B > 0xFFFF || blocks * Hkv > 0x7FFFFF) return p;
     p.prefill = true;
     const int64_t base = blocks * Hkv * B, tiles = (max_pages * page_size + 63) / 64;
-    p.S = (int)std::max<int64_t>(1, std::min<int64_t>({2 * cu / base, tiles / 4, (int64_t)kMaxSplits}));
+    const int64_t most = std::min<int64_t>({2 * cu / base, tiles, (int64_t)kMaxSplits});
+    double least = INFINITY;
+    for (int64_t s = 1; s <= std::max<int64_t>(1, most); ++s) {
+      const double t = (double)((tiles + s - 1) / s) * (base * s > cu ? 2.33 : 1.55) +
+                       (s > 1 ? 3. + (double)(s * B * L * Hq * D) * 8 / 5e6 : 0.);
+      if (t < least) least = t, p.S = (int)s;
+    }
     return p;
   }
   p.HG = R <= 8 ? 1 : (R + 15) / 16;
