@@ -33,7 +33,7 @@ struct StoreArgs {
   uint32_t *kc, *vc;
   uint8_t *ks, *vs;
   void *q_out, *k_out, *v_out;
-  uint32_t items;  // T * (Hq + 2 Hkv)
+  uint32_t items;  // T * (ceil(Hq / U) + 2 Hkv)
   int Hq, Hkv, D, max_pos, P, page_size;
   float eps;
 };
@@ -104,40 +104,35 @@ __device__ __forceinline__ void norm_rope(u32x4 x, u32x4 p, u32x4 wx, u32x4 wp, 
   }
 }
 
-// One launch's time: 1 token of 32/4 heads of 128 2 us or so (the launch), 4096
-// tokens at the rate that the read and the written bytes move.
-template <int DT, bool F32, int GL>
+// Items of a token: U query heads each (the last may be fewer), then a key or a
+// value head each.  Bound: for one token the launch and one load's latency, 2 us;
+// for 4096 of 32/4 heads of 128 the 80 MB read and written, 19 us, 4.2 TB/s.  (Loads
+// with the non-temporal hint: 25.4 -> 24.3 us with the read of the rows.)
+template <int DT, bool F32, int GL, int U>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_store_mx_kernel(StoreArgs a) {
   using A = Act<DT>;
   const uint32_t item = (blockIdx.x * kThreads + threadIdx.x) / GL;
   if (item >= a.items) return;
-  const int NH = a.Hq + 2 * a.Hkv, D = a.D;
+  const int QI = (a.Hq + U - 1) / U, NI = QI + 2 * a.Hkv, D = a.D;
   const int lane = threadIdx.x & (GL - 1), n8 = D / 8, half = D / 2, Q = n8 / 2;
-  const uint32_t t = item / (uint32_t)NH;
-  const int head = (int)(item - t * (uint32_t)NH);
+  const uint32_t t = item / (uint32_t)NI;
+  const int r = (int)(item - t * (uint32_t)NI);
   const bool on = lane < n8;
-  const bool is_q = head < a.Hq, is_v = head >= a.Hq + a.Hkv;
-  const int kvh = is_v ? head - a.Hq - a.Hkv : head - a.Hq;
+  const bool is_q = r < QI, is_v = r >= QI + a.Hkv;
+  const int head = is_q ? r * U : a.Hq + r - QI;
+  const int kvh = is_v ? r - QI - a.Hkv : r - QI;
   const u32x4 zero = {0u, 0u, 0u, 0u};
-  const u32x4 x = on ? ldg16(a.qkv + (int64_t)item * D + 8 * lane) : zero;
-  const int pg = a.pages[t], slot = a.slots[t];
-  const bool there = pg >= 0 && pg < a.P && slot >= 0 && slot < a.page_size;
-  const int64_t row = ((int64_t)pg * a.Hkv + kvh) * a.page_size + slot;
-  float out[8];
-  if (is_v) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      out[2 * j] = A::lo(x[j]);
-      out[2 * j + 1] = A::hi(x[j]);
-    }
-  } else {
-    const bool first = lane < Q;
-    const int mate = first ? lane + Q : lane - Q;
+  const uint16_t *src = a.qkv + ((int64_t)t * (a.Hq + 2 * a.Hkv) + head) * D + 8 * lane;
+  const bool first = lane < Q;
+  const int mate = first ? lane + Q : lane - Q;
+  // norm weights and angles of a lane's eight values
+  u32x4 wx = zero, wp = zero;
+  float c[8], s[8];
+  auto operands = [&]() {
     const uint16_t *w = is_q ? a.qw : a.kw;
-    const u32x4 wx = on ? ldg16(w + 8 * lane) : zero, wp = on ? ldg16(w + 8 * mate) : zero;
+    wx = on ? ldg16(w + 8 * lane) : zero, wp = on ? ldg16(w + 8 * mate) : zero;
     const int p = min(max(a.pos[t], 0), a.max_pos - 1);
     const int64_t at = (int64_t)p * half + 8 * (first ? lane : mate);
-    float c[8], s[8];
 #pragma unroll
     for (int j = 0; j < 8; j += 4) {
       const f32x4 z = {0.f, 0.f, 0.f, 0.f};
@@ -149,16 +144,42 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_store_mx_kernel(StoreAr
         s[j + i] = sv[i];
       }
     }
-    u32x4 xp;
+  };
+  auto partner = [&](u32x4 v) {
+    u32x4 o;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) xp[j] = (uint32_t)__shfl((int)x[j], on ? mate : lane, GL);
-    if (is_q) {
-      norm_rope<float, GL, DT>(x, xp, wx, wp, first, D, a.eps, c, s, out);
-      if (on) store8<DT, F32>(a.q_out, ((int64_t)t * a.Hq + head) * D + 8 * lane, out);
-      return;
+    for (int j = 0; j < 4; ++j) o[j] = (uint32_t)__shfl((int)v[j], on ? mate : lane, GL);
+    return o;
+  };
+  if (is_q) {
+    u32x4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = on && head + u < a.Hq ? ldg16_once(src + u * D) : zero;
+    operands();
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float out[8];
+      norm_rope<float, GL, DT>(x[u], partner(x[u]), wx, wp, first, D, a.eps, c, s, out);
+      if (on && head + u < a.Hq)
+        store8<DT, F32>(a.q_out, ((int64_t)t * a.Hq + head + u) * D + 8 * lane, out);
     }
+    return;
+  }
+  const u32x4 x = on ? ldg16(src) : zero;
+  const int pg = a.pages[t], slot = a.slots[t];
+  const bool there = pg >= 0 && pg < a.P && slot >= 0 && slot < a.page_size;
+  const int64_t row = ((int64_t)pg * a.Hkv + kvh) * a.page_size + slot;
+  float out[8];
+  if (is_v) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      out[2 * j] = A::lo(x[j]);
+      out[2 * j + 1] = A::hi(x[j]);
+    }
+  } else {
+    operands();
     double o[8];
-    norm_rope<double, GL, DT>(x, xp, wx, wp, first, D, a.eps, c, s, o);
+    norm_rope<double, GL, DT>(x, partner(x), wx, wp, first, D, a.eps, c, s, o);
 #pragma unroll
     for (int j = 0; j < 8; ++j) out[j] = round_to_odd(o[j]);
   }
@@ -297,7 +318,6 @@ int nvm_qk_norm_rope_store_mx(const void *qkv, int64_t T, int Hq, int Hkv, int64
   a.q_out = q_out;
   a.k_out = k_out;
   a.v_out = v_out;
-  a.items = (uint32_t)(T * NH);
   a.Hq = Hq;
   a.Hkv = Hkv;
   a.D = (int)D;
@@ -305,17 +325,27 @@ int nvm_qk_norm_rope_store_mx(const void *qkv, int64_t T, int Hq, int Hkv, int64
   a.P = (int)P;
   a.page_size = (int)page_size;
   a.eps = eps;
-  const unsigned grid = (unsigned)((T * NH * gl + kThreads - 1) / kThreads);
+  // four query heads a group from eight wavefronts a SIMD on (with the read of the
+  // rows: 4096 tokens of 32/4 heads of 128 28.4 us by one, 25.4 by four; 1024 11.7
+  // and 10.3; fewer leave CUs idle)
+  const int U = T * NH * gl >= (int64_t)8 * 64 * 4 * cu_count() ? 4 : 1;
+  a.items = (uint32_t)(T * ((Hq + U - 1) / U + 2 * Hkv));
+  const unsigned grid = (unsigned)(((int64_t)a.items * gl + kThreads - 1) / kThreads);
   hipStream_t st = (hipStream_t)stream;
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(grid), dim3(kThreads), 0, st, a); };
   auto by_gl = [&](auto dt, auto f32) {
     constexpr int DT = decltype(dt)::value;
     constexpr bool F32 = decltype(f32)::value;
+    auto by_u = [&](auto g) {
+      constexpr int GL = decltype(g)::value;
+      U == 4 ? go(qk_norm_rope_store_mx_kernel<DT, F32, GL, 4>)
+             : go(qk_norm_rope_store_mx_kernel<DT, F32, GL, 1>);
+    };
     switch (gl) {
-      case 4: return go(qk_norm_rope_store_mx_kernel<DT, F32, 4>);
-      case 8: return go(qk_norm_rope_store_mx_kernel<DT, F32, 8>);
-      case 16: return go(qk_norm_rope_store_mx_kernel<DT, F32, 16>);
-      default: return go(qk_norm_rope_store_mx_kernel<DT, F32, 32>);
+      case 4: return by_u(MxInt<4>{});
+      case 8: return by_u(MxInt<8>{});
+      case 16: return by_u(MxInt<16>{});
+      default: return by_u(MxInt<32>{});
     }
   };
   const bool f32 = out_dtype == NVM_KV_F32;
