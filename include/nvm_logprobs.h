@@ -32,7 +32,9 @@ enum { NVM_MAX_TOP_LOGPROBS = 64 };
  * smaller of V and NVM_MAX_TOP_LOGPROBS.  Sums are float32 of few terms and
  * float64 beyond, rounded to float32 once.  A row with a NaN or +infinity, or
  * of -infinities only, has NaN log probabilities (but for tokens outside) and
- * entropy; among the largest logits a NaN is the first.  V below 2^31.
+ * entropy; among the largest logits a NaN is the first.  V below 2^31 - 64, N below
+ * 2^24.  Rows are read in aligned pieces of 16 bytes, so up to 15 bytes around one
+ * are, too.
  * Workspace: nvm_token_logprobs_workspace_size, on the device that the call
  * runs on (zero bytes if no row is split; workspace may then be NULL).
  */

@@ -13,7 +13,7 @@
  *   scales  [P, num_kv_heads, page_size, D / 32]  E8M0 bytes, 255 for NaN
  * both contiguous and 16-byte aligned, for keys and for values: 4.25 bits a
  * value.  D is a multiple of 32, at most 256.  A pool may be larger than 4
- * GiB.
+ * GiB, with P * num_kv_heads * page_size below 2^31.
  */
 #ifndef NVM_MX_CACHE_H
 #define NVM_MX_CACHE_H
@@ -71,7 +71,9 @@ int nvm_paged_kv_read_mx(const void *key_codes, const uint8_t *key_scales,
  *        aligned)
  *   out  [B, L, num_heads, D] of out_dtype (the same three)
  * Codes times scales are exact, so are the products with q, and sums are
- * float32.  Workspace: nvm_paged_attention_mx_workspace_size, on the device
+ * float32.  For D of 64 or 128 the softmax weights go into the product with the
+ * values as two bf16 parts (2^-17 of each weight), with several rows and a bf16
+ * output as one f16 (2^-11).  Workspace: nvm_paged_attention_mx_workspace_size, on the device
  * that the call runs on (zero bytes if no context is split; workspace may
  * then be NULL).
  */

@@ -3,14 +3,14 @@
 // mx_decode_kernel: one query row a request, D of 64 or 128.  A block owns a
 //   request, a kv head, a group of up to 16 of its query heads and a split of the
 //   context, which it shares out from the context's own length; its wavefronts
-//   take tiles of 64 positions in turn.
+//   take tiles of 32 positions in turn.
 //   * S^T = K . Q^T on v_mfma_f32_16x16x32_bf16.  E2M1 times a power of two is
 //     exact in bf16, two values an instruction, so codes go from memory into the
 //     operand: lane (c, G) loads position c's D/4 values from D/4 G on, its own
 //     part of a block, and takes them as its dims of the MFMA's D/32 steps; the
 //     query's operand is laid out in that order.  It is split into as many bf16
 //     parts as its type needs (bf16 one, f16 two, float32 three), so products
-//     are exact.
+//     are exact, each part's sum float32.
 //   * Softmax in base 2; the running maximum is looked at across lanes only where
 //     a score exceeds it.
 //   * O^T += V^T . P^T: the scores' layout is that of the operand P^T.  Value rows
@@ -20,7 +20,10 @@
 //   * A masked position has a finite scale and any codes: its weight is zero, and
 //     zero times a finite value is zero.
 //   The next tile's keys are requested when this one's are converted, the next
-//   values when these are in LDS.
+//   values when these are in LDS.  Bound: for long contexts HBM (16 requests of 40000
+//   positions, 32/4 heads of 128: 62 us, 5.5 TB/s of codes and scales); for short ones
+//   the chain of trips to memory, code among them: one request of 700 positions 7.3 us
+//   with the merge, of 100 4.1 without.
 // mx_rows_kernel: any head dim, one wavefront per query row.  A position's row
 //   of codes goes to a group of GL lanes (eight values, one dword, a lane), so
 //   64 / GL positions are in flight side by side, each group with a running

@@ -7,8 +7,8 @@ Public names mirror the reference's package root for this path
 (``layers/attention.py:154``), the Qwen3 model with its paged KV cache and
 ``LLM``/``SamplingParams`` (``llm.py``).  Beyond the reference: the microscaled
 path (``mx.py``), ``MxTensor`` weights in ``mxfp4`` with activations in eight or
-four bits, on its own and in the model's dense layers, and the KV cache in four
-bits (``mx_cache.py``).  All compute runs in HIP kernels on the GPU
+four bits, on its own and in the model's dense layers, the KV cache in four bits
+(``mx_cache.py``), and log probabilities of tokens (``logprobs.py``).  All compute runs in HIP kernels on the GPU
 (libnvm_moe.so); nothing falls back to the CPU.
 """
 

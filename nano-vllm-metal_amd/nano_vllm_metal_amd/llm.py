@@ -338,6 +338,8 @@ class LLM:
                 raise ValueError("empty prompt")
             if len(ids) > self.max_model_len:
                 raise ValueError(f"prompt of {len(ids)} tokens exceeds max_model_len")
+            if min(ids) < 0 or max(ids) >= m.config.vocab_size:
+                raise ValueError(f"score: token ids must be in [0, {m.config.vocab_size})")
         out = []
         for ids in encoded:
             records: List[TokenLogprob] = []

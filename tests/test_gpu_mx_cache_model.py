@@ -243,3 +243,16 @@ def test_score(bits):
             llm.score(bad)
     with pytest.raises(ValueError, match="top"):
         llm.score(prompts, top=-1)
+
+
+@pytest.mark.gpu
+def test_score_refuses_ids_outside_the_vocabulary():
+    """(Their log probability would count as zero.)"""
+    from nano_vllm_metal_amd import LLM
+
+    m = _model(8)
+    llm = LLM(m, max_num_seqs=1, max_model_len=64, page_size=4)
+    for bad in (-1, m.config.vocab_size):
+        with pytest.raises(ValueError, match="token ids"):
+            llm.score([_tokens(5), [1, bad, 2]])
+    assert llm.cache.free_pages == llm.cache.num_pages
