@@ -23,8 +23,8 @@
 // the result does not depend on the order of anything, and rows in ascending order
 // are slow, not wrong.
 //
-// Bound: HBM for many rows (2048 x 151936 bf16: 102 us, 6.1 TB/s; top 5 125 us, 20
-// 170, 64 420, of the lists' first keys), a lane's 8.5 slots a value close behind (4 of
+// Bound: HBM for many rows (2048 x 151936 bf16: 102 us, 6.1 TB/s; top 5 124 us, 20
+// 162, 64 380, of the lists' first keys), a lane's 8.5 slots a value close behind (4 of
 // them exp's); for one row (top 5: 13 us) latency, of two launches.
 #include <math.h>
 
@@ -138,7 +138,7 @@ __device__ __forceinline__ uint64_t kth_of_lanes(uint64_t key, int k) {
 // What at least k keys reach (all of them, if there are fewer), from the lanes'
 // largest values: the k-th of these, its lowest six bits cleared.  Those hold the
 // lane for the ranks.  (By 64-bit keys of the values themselves, three times the
-// instructions: 2048 rows of 151936, top 5, 135 us, 125 so.)
+// instructions: 2048 rows of 151936, top 5, 135 us for 125.)
 __device__ __forceinline__ uint64_t first_threshold(float top, int k, int lane) {
   const uint32_t o = (ordered(top) & ~63u) | (uint32_t)lane;
   int above = 0;
@@ -263,16 +263,22 @@ __device__ __forceinline__ Part block_sums(BlockState &b, Part p, int lane, int 
 }
 
 // f(place, key) of the k largest of the wavefronts' lists, which are in order (a
-// barrier lies behind them): a key's place is the number of larger ones.
+// barrier lies behind them): a key's place is the number of larger ones, which a
+// search by halves counts in each other list.
 template <class F>
 __device__ __forceinline__ void block_top(const BlockState &b, int k, int lane, int wv, F f) {
   for (int i = lane; i < b.n[wv]; i += 64) {
     const uint64_t v = b.keys[wv][i];
-    int place = i;
-    for (int w = 0; w < kWaves; ++w) {
-      if (w == wv) continue;
-      for (int j = 0; j < b.n[w]; ++j) place += b.keys[w][j] > v;
-    }
+    int larger[kWaves] = {};
+    for (int step = 1 << (31 - __builtin_clz(k)); step > 0; step >>= 1)
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const int at = larger[w] + step;
+        if (at <= b.n[w] && b.keys[w][at - 1] > v) larger[w] = at;
+      }
+    int place = 0;  // (in its own list, too)
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) place += larger[w];
     if (place < k) f(place, v);
   }
 }
@@ -296,7 +302,7 @@ __device__ __forceinline__ void block_threshold(BlockState &b, TopList &list, in
 
 template <int DT>
 __device__ __forceinline__ void store_row(const LogprobArgs &a, BlockState &b, int64_t row,
-                                          const Part &p, int lane, int wv) {
+                                          const Part &p, float xt, int lane, int wv) {
   // (x L - m first, exactly: of values of 1e38 their difference is all that counts)
   const double lz = log2(p.z);
   // (neither above zero nor, the entropy, below it by an error of exp2)
@@ -306,7 +312,7 @@ __device__ __forceinline__ void store_row(const LogprobArgs &a, BlockState &b, i
   };
   if (threadIdx.x == 0) {
     const int64_t t = a.tokens[row];
-    a.lp[row] = t >= 0 && t < a.V ? logprob(Logits<DT>::one(a.x, row * a.ld + t)) : 0.f;
+    a.lp[row] = t >= 0 && t < a.V ? logprob(xt) : 0.f;
     const double h = (lz - p.s / p.z) / (double)kLog2e;
     a.ent[row] = h < 0.0 ? 0.f : (float)h;
   }
@@ -315,6 +321,14 @@ __device__ __forceinline__ void store_row(const LogprobArgs &a, BlockState &b, i
       a.ids[row * a.k + place] = id_of(v);
       a.top[row * a.k + place] = logprob(value_of(v));
     });
+}
+
+// The logit of a row's token, or of token 0: asked for at the start, since it is two
+// trips to memory away.
+template <int DT>
+__device__ __forceinline__ float token_logit(const LogprobArgs &a, int64_t row) {
+  const int64_t t = a.tokens[row];
+  return Logits<DT>::one(a.x, row * a.ld + (t >= 0 && t < a.V ? t : 0));
 }
 
 // Grid: rows, splits.
@@ -337,6 +351,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
   const int end = min(first + per, nv);
   if (threadIdx.x == 0) s_b.T = 0;
   __syncthreads();
+  const float xt = a.S == 1 ? token_logit<DT>(a, row) : 0.f;
 
   auto load = [&](int v0, u32x4 (&raw)[kUnroll]) {
 #pragma unroll
@@ -419,8 +434,6 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
           for (int u = 0; u < kUnroll; ++u)
             hit[u] &= __builtin_amdgcn_ballot_w64(
                 tmax[u] != limit || (int64_t)(v0 + 64 * u + lane) * PER - lead <= idT);
-          // one lane's vector after the other, a value a lane: few have one that counts
-          const int e = lane & (PER - 1);
 #pragma unroll 1
           for (int u = 0; u < kUnroll; ++u) {
             uint64_t h = hit[0];
@@ -428,9 +441,12 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
 #pragma unroll
             for (int w = 1; w < kUnroll; ++w)
               if (u == w) h = hit[w], r = raw[w];
+            // one lane's vector after the other, a value a lane: few have one that counts
+            // (a second path, by value, for vectors of four lanes and more: top 64 of
+            // 2048 rows of 151936 323 us for 380, but top 5 128 for 124, 20 178 for 162)
 #pragma unroll 1
             while (h) {
-              const int from = __builtin_ctzll(h);
+              const int from = __builtin_ctzll(h), e = lane & (PER - 1);
               h &= h - 1;
               u32x4 one;
 #pragma unroll
@@ -478,7 +494,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
   if (lane == 0) s_b.n[wv] = list.n;
   p = block_sums(s_b, p, lane, wv);
   if (a.S == 1) {
-    store_row<DT>(a, s_b, row, p, lane, wv);
+    store_row<DT>(a, s_b, row, p, xt, lane, wv);
     return;
   }
   const int64_t at = row * a.S + blockIdx.y;
@@ -500,6 +516,7 @@ __global__ __launch_bounds__(64 * kWaves) void logprobs_merge_kernel(LogprobArgs
   __shared__ BlockState s_b;
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = blockIdx.x;
+  const float xt = token_logit<DT>(a, row);
   Part p = {-1e39, 0.0, 0.0};
   if (threadIdx.x < a.S) {
     const double *o = a.part_sums + (row * a.S + threadIdx.x) * 3;
@@ -518,7 +535,7 @@ __global__ __launch_bounds__(64 * kWaves) void logprobs_merge_kernel(LogprobArgs
   }
   if (lane == 0) s_b.n[wv] = list.n;
   p = block_sums(s_b, p, lane, wv);
-  store_row<DT>(a, s_b, row, p, lane, wv);
+  store_row<DT>(a, s_b, row, p, xt, lane, wv);
 }
 
 template <int DT>
