@@ -22,7 +22,7 @@
 //   The next tile's keys are requested when this one's are converted, the next
 //   values when these are in LDS.  Bound: for long contexts HBM (16 requests of 40000
 //   positions, 32/4 heads of 128: 62 us, 5.5 TB/s of codes and scales); for short ones
-//   the chain of trips to memory, code among them: one request of 700 positions 7.3 us
+//   the chain of trips to memory, code among them: one request of 700 positions 6.9 us
 //   with the merge, of 100 4.1 without.
 // mx_rows_kernel: any head dim, one wavefront per query row.  A position's row
 //   of codes goes to a group of GL lanes (eight values, one dword, a lane), so
@@ -448,7 +448,10 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
 // row: lane s takes split s's maximum and sum, then each lane D / 64 dims of those
 // with a weight (others were perhaps not written).
 constexpr int kMaxSplits = 64;
-template <int DH>
+// ONE: of single query rows, few and late: the first splits' outputs are asked for
+// beside the maxima, whether they count or not (one request of 32768 positions 15.0 us
+// for 16.4; of 3 x 100 rows, whose splits are a few MB, 17.8 for 16.7).
+template <int DH, bool ONE>
 __global__ __launch_bounds__(kRowThreads) void mx_combine_kernel(const float *__restrict__ part_o,
                                                                  const float *__restrict__ part_ml,
                                                                  int64_t rows, int S, void *out,
@@ -458,6 +461,15 @@ __global__ __launch_bounds__(kRowThreads) void mx_combine_kernel(const float *__
   if (n >= rows) return;
   const int lane = threadIdx.x & 63;
   const float *po = part_o + n * S * DH + PD * lane;
+  constexpr int kAhead = 8;
+  float v[kAhead][PD];
+  auto load = [&](int s0, int end) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+      for (int d = 0; d < PD; ++d) v[j][d] = po[(int64_t)min(s0 + j, end - 1) * DH + d];
+  };
+  if constexpr (ONE) load(0, S);
   float ms = -INFINITY, ls = 0.f;
   if (lane < S) {
     ms = part_ml[(n * S + lane) * 2];
@@ -471,13 +483,8 @@ __global__ __launch_bounds__(kRowThreads) void mx_combine_kernel(const float *__
   const uint64_t on = __builtin_amdgcn_ballot_w64(w != 0.f);
   const int last = on ? 64 - __builtin_clzll(on) : 0;
   float acc[PD] = {};
-  constexpr int kAhead = 8;
   for (int s0 = 0; s0 < last; s0 += kAhead) {
-    float v[kAhead][PD];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-#pragma unroll
-      for (int d = 0; d < PD; ++d) v[j][d] = po[(int64_t)min(s0 + j, last - 1) * DH + d];
+    if (!ONE || s0 > 0) load(s0, last);
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), (s0 + j) & 63));
@@ -575,8 +582,14 @@ hipError_t launch_combine(const MxAttnArgs &a, hipStream_t st) {
   if (a.S == 1) return hipSuccess;
   const int64_t rows = (int64_t)a.B * a.L * a.Hq;
   const unsigned blocks = (unsigned)((rows + kRowThreads / 64 - 1) / (kRowThreads / 64));
-  hipLaunchKernelGGL(a.D == 128 ? mx_combine_kernel<128> : mx_combine_kernel<64>, dim3(blocks),
-                     dim3(kRowThreads), 0, st, a.part_o, a.part_ml, rows, a.S, a.out, a.out_dt);
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3(blocks), dim3(kRowThreads), 0, st, a.part_o, a.part_ml, rows, a.S,
+                       a.out, a.out_dt);
+  };
+  if (a.L == 1)
+    a.D == 128 ? go(mx_combine_kernel<128, true>) : go(mx_combine_kernel<64, true>);
+  else
+    a.D == 128 ? go(mx_combine_kernel<128, false>) : go(mx_combine_kernel<64, false>);
   return hipGetLastError();
 }
 
