@@ -399,3 +399,29 @@ def test_attention_extreme_scales(L):
     q[..., 32:64] *= 2.0 ** -100
     v[1][:, :, :, 0], v[1][:, :, :, 1] = 8, 220
     _check_attention(q, k, v, bt, lens, True, odt=torch.float32)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("code", [0x22, 0x00])
+@pytest.mark.parametrize("L", [1, 3])
+@pytest.mark.parametrize("D", [64, 128, 96])
+@pytest.mark.parametrize("odt", ACTS)
+def test_key_block_of_nans_whatever_its_codes(odt, D, L, code, sign):
+    """A scale of 255 is a NaN, no infinity that a score of one sign would hide:
+    rows that see the position are NaN, others are not."""
+    from nano_vllm_metal_amd import paged_attention_mx
+
+    q, k, v, bt, lens = _attention_case(9, 2, 4, 2, D, 4, [37, 20], L, odt)
+    q = torch.full_like(q, sign)
+    at = 37 - L  # the first row's last position of request 0
+    page, slot = int(bt[0, at // 4]), at % 4
+    k[0][page, 1, slot] = code
+    k[1][page, 1, slot, 0] = 255
+    got = paged_attention_mx(q.to(DEV), _pages(k), _pages(v), bt.to(DEV), lens.to(DEV),
+                             mask="causal").cpu()
+    nan = torch.zeros(got.shape, dtype=torch.bool)
+    nan[0, 2:] = True
+    assert torch.equal(got.isnan(), nan)
+    got = paged_attention_mx(q.to(DEV), _pages(k), _pages(v), bt.to(DEV),
+                             torch.tensor([at, 20], dtype=torch.int32, device=DEV)).cpu()
+    assert not got.isnan().any()
