@@ -2,8 +2,8 @@
 // rows of logits (declared in include/nvm_logprobs.h).
 //
 // One pass over a row, or over a part of it where there are few rows.  With L =
-// log2 e as a float32 a lane keeps a reference m (the largest x L, at first, and
-// another only where one exceeds it by kSlack), Z = sum 2^(x L - m) and S = sum
+// log2 e as a float32 a lane keeps a reference m (the largest x L so far, so that
+// the largest term is exact; one that moves by steps of 16 only was no faster), Z = sum 2^(x L - m) and S = sum
 // 2^(x L - m) (x L - m); then log p(t) = (x_t L - m - log2 Z) / L and the entropy is
 // (log2 Z - S / Z) / L.  x L - m is one fma, whose product is exact.  A vector's few
 // terms are summed in float32, everything beyond in float64.
@@ -39,7 +39,6 @@ namespace nvm {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 4.f;
 constexpr int kWaves = 4;
 constexpr int kUnroll = 4;                    // vectors of a lane's tile
 constexpr int kMaxTop = NVM_MAX_TOP_LOGPROBS;
@@ -388,7 +387,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
         tmax[u] = t;
         top = max_nan(top, t);
       }
-      const bool above = top * kLog2e > m + kSlack;
+      const bool above = top * kLog2e > m;
       if (__any(above)) {
         const float mn = fmaxf(m, top * kLog2e);
         const double d = (double)m - (double)mn, alpha = __builtin_amdgcn_exp2f((float)d);

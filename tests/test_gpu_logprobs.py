@@ -2,9 +2,8 @@
 
 Ids are exact: a stable descending sort of the logits.  With d = x - max and u =
 2^-24, the exponent of a term is off by 3 u |d| (a difference, a product, and
-log2 e itself; as one fma x log2 e - m with the reference m at most 4 below the
-largest, u (|d| + 2.8)), exp2 by one unit (2 u) more; float32 sums of at most
-eight terms by 7 u.  So log Z is off by Z' = sum p (3 u |d| + 4 u) + 8 u, and the
+log2 e itself; one fma x log2 e - m, m the largest so far, less), exp2 by one
+unit (2 u) more; float32 sums of at most eight terms by 7 u.  So log Z is off by Z' = sum p (3 u |d| + 4 u) + 8 u, and the
 entropy by that, by sum p |d| (3 u |d| + 8 u) and by sum p |d| (Z' + 8 u); each
 result is rounded once (u of itself, and to infinity beyond float32's largest
 value: the difference of that type's largest and lowest is 6.8e38).
