@@ -72,10 +72,9 @@ int nvm_paged_kv_read_mx(const void *key_codes, const uint8_t *key_scales,
  *   out  [B, L, num_heads, D] of out_dtype (the same three)
  * Codes times scales are exact, so are the products with q, and sums are
  * float32.  For D of 64 or 128 the softmax weights go into the product with the
- * values as two bf16 parts (2^-17 of each weight), with several rows and a bf16
- * output as one f16 (2^-11).  Workspace: nvm_paged_attention_mx_workspace_size, on the device
- * that the call runs on (zero bytes if no context is split; workspace may
- * then be NULL).
+ * values as two bf16 parts (2^-17 of each weight), whatever out_dtype is.
+ * Workspace: nvm_paged_attention_mx_workspace_size, on the device that the call
+ * runs on (zero bytes if no context is split; workspace may then be NULL).
  */
 int nvm_paged_attention_mx_workspace_size(int64_t B, int64_t L, int64_t D, int64_t max_pages,
                                           int64_t page_size, int num_kv_heads, int num_heads,

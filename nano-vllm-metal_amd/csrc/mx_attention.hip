@@ -518,11 +518,15 @@ MxPlan mx_plan(int64_t B, int64_t L, int64_t D, int64_t max_pages, int64_t page_
   if ((D != 64 && D != 128) || B == 0) return p;
   const int R = Hq / Hkv;
   if (L > 1) {
-    // The splits of the least time: a tile of 64 positions takes a block 1.55 us, half
-    // as much more beside another block of its CU; a merge 3 us and its outputs'
-    // way there and back at 5 TB/s.  (us with 1, 2, 4, 8, 16, 32 splits, 32/4 heads of
-    // 128: 512 rows over 4096 positions 102, 69, 60, 70, 98, 161; 4 x 256 over 1280 42,
-    // 55, 64, 89, 158; 16 over 8192 193, 104, 57, 35, 25, 23.)
+    // The splits of the least time, a tile of 64 positions taken as 1.55 us of a block,
+    // half as much more beside another block of its CU, a merge as 3 us and its outputs'
+    // way there and back at 5 TB/s.  A tile takes 1.75 us with a bf16 query of 128 dims,
+    // 2.0 with f16, 1.6 with 64 dims; the smaller figure for all leaves a few splits
+    // fewer, and the choice lies within 8 % of the best of these.  (us with 1, 2, 4, 8, 16, 32 splits.
+    // bf16, 32/4 heads of 128: 512 rows over 4096 positions 117, 74, 68, 76, 102, 166; 4 x
+    // 256 over 1280 44, 55, 65, 94, 158, 210; 16 over 8192 222, 118, 64, 38, 26, 23.  f16:
+    // 512 over 4096 130, 81, 75, 83, 107, 172.  bf16, 16/8 heads of 64: 512 over 4096 102,
+    // 59, 37, 35, 40, 52; f16, 14/2 of 64: 3 x 100 over 1501 42, 28, 19, 18, 19, 22.)
     const int64_t blocks = mx_prefill_blocks(L, R), cu = cu_count();
     if (B > 0xFFFF || blocks * Hkv > 0x7FFFFF) return p;
     p.prefill = true;

@@ -12,11 +12,11 @@
 //   * Softmax in base 2, two lanes a column.  The maximum moves only where a score
 //     exceeds it by more than 2^kSlack, so the sums are rarely rescaled.
 //   * O^T += V^T . P^T: the scores lie as the operand P^T wants them; values come out
-//     of LDS transposed (ds_read_b64_tr_b16).  P is two bf16 parts (2^-17).  For a bf16
-//     output it is one f16 (2^-11 of each weight, a quarter of the output's own
-//     rounding) and values are f16, exact for scales of 2^-23 to 2^13 and blocks of
-//     zeros: a third fewer products (2048 rows over 6144 positions 201 us for 252).  A block
-//     that meets another scale starts again with the two parts.
+//     of LDS transposed (ds_read_b64_tr_b16).  P is two bf16 parts: a weight loses
+//     2^-17 of itself, so a result at most 2^-16 of its column's largest value.  (One f16
+//     part would lose 2^-11 of each weight, which shows beside a bf16 output's own 2^-8
+//     where values cancel; it took 193 us where two take 249: 2048 rows over 6144
+//     positions, 32/4 heads of 128.)
 // Positions that are not there are row 0 with a finite scale, and masked.  So are the
 // scales of value blocks of NaNs, since a zero weight would not hide them from rows
 // that do not see their position; those that do are told at the end.
@@ -38,15 +38,6 @@ constexpr int kCW = 4;             // wavefronts of a block (two blocks a CU)
 constexpr int kCols = 32 * kCW;    // its columns
 constexpr int kKeys = 64;          // positions of a tile
 constexpr float kSlack = 6.f;
-constexpr uint32_t kLowScale = 127 - 23, kHighScale = 127 + 13;  // of f16 values
-
-// Eight codes times a scale as f16.
-__device__ __forceinline__ u32x4 codes_f16(uint32_t d, float s) {
-  return u32x4{mx_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, s, 0)),
-               mx_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, s, 1)),
-               mx_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, s, 2)),
-               mx_bits(__builtin_amdgcn_cvt_scalef32_pk_f16_fp4(d, s, 3))};
-}
 
 template <int QT, int DH>
 __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, int blocks) {
@@ -55,7 +46,6 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
   constexpr int NC = DH / 16;  // steps of a score MFMA
   constexpr int NT = DH / 32;  // tiles of the output
   // LDS pitch of a row: the four rows of a transposed read lie in banks of their own
-  // (with 8 in place of 16 in pairs: 2048 rows over 6144 positions 205 us for 199.6)
   constexpr int VP = DH + 16;
   constexpr int NB = DH / 32;  // scales of a row; dwords of codes of a quarter of it
   static_assert(4 * kKeys == 64 * kCW, "a quarter of a row a thread");
@@ -117,20 +107,14 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
     ksc = a.ks[(uint64_t)row * NB + (DH / 4) * part / 32];
     vsc = a.vs[(uint64_t)row * NB + (DH / 4) * part / 32];
   };
-  bool beyond = false;  // a scale that f16 values do not take
-  auto stage_store = [&](int buf, auto f16) {
+  auto stage_store = [&](int buf) {
     const bool nan = ok & (vsc == 255u);
-    uint32_t any = 0;
-#pragma unroll
-    for (int j = 0; j < NB; ++j) any |= vd[j] & 0x77777777u;
-    beyond |= ok & !nan & (any != 0u) & (vsc - kLowScale > kHighScale - kLowScale);
     const float f = __uint_as_float(ok ? ksc << 23 : 0u);
     const float g = __uint_as_float(ok & !nan ? vsc << 23 : 0u);
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       *(u32x4 *)&s_k[buf][key][(DH / 4) * part + 8 * j] = codes_bf16(kd[j], f);
-      *(u32x4 *)&s_v[buf][key][(DH / 4) * part + 8 * j] =
-          decltype(f16)::value ? codes_f16(vd[j], g) : codes_bf16(vd[j], g);
+      *(u32x4 *)&s_v[buf][key][(DH / 4) * part + 8 * j] = codes_bf16(vd[j], g);
     }
     // (lane i of the first sixteen: position i of the wavefront's)
     const uint64_t there = __builtin_amdgcn_ballot_w64(__shfl((int)ok, 4 * lane & 63) != 0);
@@ -145,130 +129,106 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
     }
   };
 
-  float m_run, l_run;  // column c32's; l_run this lane's share
-  uint32_t seen_nan;   // value blocks of NaNs that the column sees
-  f32x16 oacc[NT];     // O^T: column c32, dims 32 t + 8 j + 4 h + i
+  float m_run = -INFINITY, l_run = 0.f;  // column c32's; l_run this lane's share
+  uint32_t seen_nan = 0;                 // value blocks of NaNs that the column sees
+  f32x16 oacc[NT];                       // O^T: column c32, dims 32 t + 8 j + 4 h + i
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) oacc[t][i] = 0.f;
   // (-1, 0) and (0, -1), which pick out of a pair (in registers: as a constant the
   // second is taken for the inline constant -1.0, in the other half)
   uint32_t pick0 = 0x0000BF80u, pick1 = 0xBF800000u;
   asm volatile("" : "+v"(pick0), "+v"(pick1));
-  // All tiles.  With f16 weights these are up to 2^(kSlack + 8), so that they lose
-  // bits only from 2^-28 of the largest on.
-  auto run = [&](auto f16) {
-    constexpr bool F16 = decltype(f16)::value;
-    constexpr float kShift = F16 ? 8.f : 0.f;
-    m_run = -INFINITY;
-    l_run = 0.f;
-    seen_nan = 0;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) oacc[t][i] = 0.f;
-    page_id(t0);
-    stage_load(t0);
-    page_id(t0 + 1);
-    stage_store(0, f16);
-    __syncthreads();
-    for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
-      stage_load(t + 1);  // (past the last one: row 0, or another split's)
-      page_id(t + 2);
+  page_id(t0);
+  stage_load(t0);
+  page_id(t0 + 1);
+  stage_store(0);
+  __syncthreads();
+  for (int t = t0; t < t1; ++t) {
+    const int buf = (t - t0) & 1;
+    stage_load(t + 1);  // (past the last one: row 0, or another split's)
+    page_id(t + 2);
 
-      f32x16 acc[2];
+    f32x16 acc[2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[u][i] = 0.f;
+      for (int i = 0; i < 16; ++i) acc[u][i] = 0.f;
 #pragma unroll
-        for (int k = 0; k < NC; ++k) {
-          const u32x4 kb = *(const u32x4 *)&s_k[buf][32 * u + c32][16 * k + 8 * h];
+      for (int k = 0; k < NC; ++k) {
+        const u32x4 kb = *(const u32x4 *)&s_k[buf][32 * u + c32][16 * k + 8 * h];
 #pragma unroll
-          for (int p = 0; p < QP; ++p) acc[u] = A::mfma32(kb, qop[k][p], acc[u]);
-        }
+        for (int p = 0; p < QP; ++p) acc[u] = A::mfma32(kb, qop[k][p], acc[u]);
       }
-      const uint64_t there = *(const uint64_t *)s_ok[buf];
-      if (there != ~0ull || kKeys * (t + 1) > all_see) {  // uniform
-        // bits of what this column sees; those of this lane's element i of part u are
-        // 8 (i / 4) + i % 4 of the word
-        const int n = bound - kKeys * t + 1;
-        const uint64_t seen = n >= 64 ? there : n <= 0 ? 0 : there & ((1ull << n) - 1);
-        const uint32_t w[2] = {(uint32_t)seen >> (4 * h), (uint32_t)(seen >> 32) >> (4 * h)};
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)w[u], 8 * (i >> 2) + (i & 3), 1);
-            acc[u][i] = __uint_as_float((__float_as_uint(acc[u][i]) & m) | (~m & 0xFF800000u));
-          }
-      }
-      if (s_any[buf][0] | s_any[buf][1] | s_any[buf][2] | s_any[buf][3]) {  // uniform
-#pragma unroll 1
-        for (int kl = 0; kl < kKeys; ++kl)
-          if (kKeys * t + kl <= bound) seen_nan |= s_nan[buf][kl];
-      }
-      float tmax = acc[0][0];
+    }
+    const uint64_t there = *(const uint64_t *)s_ok[buf];
+    if (there != ~0ull || kKeys * (t + 1) > all_see) {  // uniform
+      // bits of what this column sees; those of this lane's element i of part u are
+      // 8 (i / 4) + i % 4 of the word
+      const int n = bound - kKeys * t + 1;
+      const uint64_t seen = n >= 64 ? there : n <= 0 ? 0 : there & ((1ull << n) - 1);
+      const uint32_t w[2] = {(uint32_t)seen >> (4 * h), (uint32_t)(seen >> 32) >> (4 * h)};
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, acc[u][i]);
-      tmax *= a.scale2;
-      if (__any(tmax > m_run + kSlack)) {
-        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax),
-                                                        false, false);
-        const float m_new =
-            fmaxf(m_run, fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
-        const float alpha = exp2_below(m_run, m_new);
-        l_run *= alpha;
-#pragma unroll
-        for (int k = 0; k < NT; ++k) oacc[k] *= alpha;
-        m_run = m_new;
-      }
-      const float m_sub = m_run == -INFINITY ? 0.f : m_run - kShift;
-      // P^T: slot 8 h + j of 16 positions' product is position 4 h + j, or 8 + 4 h + j
-      // - 4 from j = 4 on
-      u32x4 hi[4], lo[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = 8 * (c & 1) + 2 * j;
-          const float x = __builtin_amdgcn_exp2f(fmaf(acc[c >> 1][i], a.scale2, -m_sub));
-          const float y = __builtin_amdgcn_exp2f(fmaf(acc[c >> 1][i + 1], a.scale2, -m_sub));
-          l_run += x + y;
-          if constexpr (F16) {
-            hi[c][j] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x, (_Float16)y});
-          } else {
-            hi[c][j] = A::pack2(x, y);
-            lo[c][j] = A::pack2(A::dot2(hi[c][j], pick0, x), A::dot2(hi[c][j], pick1, y));
-          }
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)w[u], 8 * (i >> 2) + (i & 3), 1);
+          acc[u][i] = __uint_as_float((__float_as_uint(acc[u][i]) & m) | (~m & 0xFF800000u));
         }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint16_t *v0 = &s_v[buf][16 * c + 4 * h + ((lane & 15) >> 2)]
-                                 [16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
-#pragma unroll
-        for (int k = 0; k < NT; ++k) {
-          const u32x2 x = lds_read_tr(v0 + 32 * k), y = lds_read_tr(v0 + 8 * VP + 32 * k);
-          const u32x4 va = {x.x, x.y, y.x, y.y};
-          if constexpr (F16) {
-            oacc[k] = Act<DT_F16>::mfma32(va, hi[c], oacc[k]);
-          } else {
-            oacc[k] = A::mfma32(va, hi[c], oacc[k]);
-            oacc[k] = A::mfma32(va, lo[c], oacc[k]);
-          }
-        }
-      }
-      stage_store(buf ^ 1, f16);
-      __syncthreads();
     }
-    m_run -= kShift;
-  };
-  bool parts = a.out_dt != NVM_KV_BF16;
-  if (!parts) {
-    run(MxInt<1>{});
-    parts = __syncthreads_or(beyond);
+    if (s_any[buf][0] | s_any[buf][1] | s_any[buf][2] | s_any[buf][3]) {  // uniform
+#pragma unroll 1
+      for (int kl = 0; kl < kKeys; ++kl)
+        if (kKeys * t + kl <= bound) seen_nan |= s_nan[buf][kl];
+    }
+    float tmax = acc[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) tmax = fmaxf(tmax, acc[u][i]);
+    tmax *= a.scale2;
+    if (__any(tmax > m_run + kSlack)) {
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(tmax), __float_as_uint(tmax),
+                                                      false, false);
+      const float m_new =
+          fmaxf(m_run, fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])));
+      const float alpha = exp2_below(m_run, m_new);
+      l_run *= alpha;
+#pragma unroll
+      for (int k = 0; k < NT; ++k) oacc[k] *= alpha;
+      m_run = m_new;
+    }
+    const float m_sub = m_run == -INFINITY ? 0.f : m_run;
+    // P^T: slot 8 h + j of 16 positions' product is position 4 h + j, or 8 + 4 h + j
+    // - 4 from j = 4 on
+    u32x4 hi[4], lo[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = 8 * (c & 1) + 2 * j;
+        const float x = __builtin_amdgcn_exp2f(fmaf(acc[c >> 1][i], a.scale2, -m_sub));
+        const float y = __builtin_amdgcn_exp2f(fmaf(acc[c >> 1][i + 1], a.scale2, -m_sub));
+        l_run += x + y;
+        hi[c][j] = A::pack2(x, y);
+        lo[c][j] = A::pack2(A::dot2(hi[c][j], pick0, x), A::dot2(hi[c][j], pick1, y));
+      }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint16_t *v0 = &s_v[buf][16 * c + 4 * h + ((lane & 15) >> 2)]
+                               [16 * ((lane >> 4) & 1) + 4 * (lane & 3)];
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        const u32x2 x = lds_read_tr(v0 + 32 * k), y = lds_read_tr(v0 + 8 * VP + 32 * k);
+        const u32x4 va = {x.x, x.y, y.x, y.y};
+        oacc[k] = A::mfma32(va, hi[c], oacc[k]);
+        oacc[k] = A::mfma32(va, lo[c], oacc[k]);
+      }
+    }
+    stage_store(buf ^ 1);
+    __syncthreads();
   }
-  if (parts) run(MxInt<0>{});
 
   l_run += __shfl_xor(l_run, 32);
   if (!col_ok) return;
