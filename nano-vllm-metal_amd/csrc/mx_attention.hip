@@ -446,7 +446,9 @@ __global__ __launch_bounds__(64 * NW, 4) void mx_decode_kernel(MxAttnArgs a) {
 
 // Splits of a row: sum_s 2^(M_s - M) O_s / sum_s 2^(M_s - M) L_s, a wavefront a
 // row: lane s takes split s's maximum and sum, then each lane D / 64 dims of those
-// with a weight (others were perhaps not written).
+// that saw a position (others were perhaps not written).  A weight of zero does not
+// leave a split out: its outputs may be NaN, and zero times NaN is NaN, as it is
+// where a context is not split.
 constexpr int kMaxSplits = 64;
 // ONE: of single query rows, few and late: the first splits' outputs are asked for
 // beside the maxima, whether they count or not (one request of 32768 positions 15.0 us
@@ -480,7 +482,7 @@ __global__ __launch_bounds__(kRowThreads) void mx_combine_kernel(const float *__
   for (int x = 32; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor(M, x));
   const float w = exp2_below(ms, M);
   const float L = wave_sum(w * ls);
-  const uint64_t on = __builtin_amdgcn_ballot_w64(w != 0.f);
+  const uint64_t on = __builtin_amdgcn_ballot_w64(ms != -INFINITY || ls != 0.f);
   const int last = on ? 64 - __builtin_clzll(on) : 0;
   float acc[PD] = {};
   for (int s0 = 0; s0 < last; s0 += kAhead) {
@@ -489,7 +491,8 @@ __global__ __launch_bounds__(kRowThreads) void mx_combine_kernel(const float *__
     for (int j = 0; j < kAhead; ++j) {
       const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), (s0 + j) & 63));
 #pragma unroll
-      for (int d = 0; d < PD; ++d) acc[d] += s0 + j < last && f != 0.f ? f * v[j][d] : 0.f;
+      for (int d = 0; d < PD; ++d)
+        acc[d] += s0 + j < last && (on >> ((s0 + j) & 63) & 1) ? f * v[j][d] : 0.f;
     }
   }
 #pragma unroll

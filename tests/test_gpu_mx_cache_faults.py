@@ -52,3 +52,41 @@ def test_weights_of_values_that_cancel(L, D, dt):
     bt = torch.tensor([[2], [1]], dtype=torch.int32)
     lens = torch.tensor([8, 8], dtype=torch.int32)
     _check(_run(q, k, v, bt, lens), q, k, v, bt, lens)
+
+
+@pytest.mark.parametrize("nan,top", [(3, 1999), (1990, 5), (700, 701), (0, 1000)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("L", [1, 2, 40])
+def test_nan_value_far_below_the_largest_score(L, D, nan, top):
+    """A value block of NaNs at a position whose weight is 2^-430 of the row's largest,
+    which float32 holds as zero: it shows in its 32 dims of the rows that see it,
+    however many splits lie between the two."""
+    g = torch.Generator().manual_seed(nan)
+    q = torch.ones(1, 4, L, D, dtype=torch.bfloat16)
+    k = (torch.zeros(128, 2, 16, D // 2, dtype=torch.uint8),
+         torch.full((128, 2, 16, D // 32), 127, dtype=torch.uint8))
+    v = C.random_pages(g, 128, 2, 16, D)
+    bt = torch.randperm(128, generator=g)[:125][None].int()
+    lens = torch.tensor([2000], dtype=torch.int32)
+    k[0][int(bt[0, top // 16]), :, top % 16] = 0x22  # ones
+    scale = 300.0 / D
+    _check(_run(q, k, v, bt, lens, False, scale), q, k, v, bt, lens, False, scale)
+    clean = _run(q, k, v, bt, lens, False, scale)
+    v[1][int(bt[0, nan // 16]), 1, nan % 16, 1] = 255
+    got = _run(q, k, v, bt, lens, False, scale)
+    assert got[:, 2:, :, 32:64].isnan().all()
+    got[:, 2:, :, 32:64] = clean[:, 2:, :, 32:64]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("L", [1, 2])
+def test_nan_key_far_from_the_largest_score(L):
+    """A key block of NaNs: the whole row, wherever the largest score is."""
+    g = torch.Generator().manual_seed(L)
+    q = torch.ones(1, 2, L, 128, dtype=torch.float16)
+    k, v = (C.random_pages(g, 128, 1, 16, 128) for _ in range(2))
+    bt = torch.randperm(128, generator=g)[:125][None].int()
+    lens = torch.tensor([2000], dtype=torch.int32)
+    k[0][int(bt[0, 1999 // 16]), :, 1999 % 16], k[1][int(bt[0, 1999 // 16]), :, 1999 % 16] = 0x22, 132
+    k[1][int(bt[0, 0]), 0, 7, 2] = 255
+    assert _run(q, k, v, bt, lens).isnan().all()
