@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
   const int col = blk * kCols + 32 * wv + c32;
   const bool col_ok = col < a.L * a.R;
   const int qrow = col / a.R, head = kvh * a.R + col - qrow * a.R;
-  const int len = a.lens[b], ctx = context_of(a, len), off = len - a.L;
+  const int len = max(a.lens[b], 0), ctx = context_of(a, len), off = len - a.L;
   const int32_t *bt = a.bt + (int64_t)b * a.max_pages;
   // positions that a column of the block may see, of these this split's tiles
   const int last_row = min((blk * kCols + kCols - 1) / a.R, a.L - 1);
@@ -75,7 +75,8 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
   // of the wavefront's columns: up to which tile all see everything
   const int first_row = min((blk * kCols + 32 * wv) / a.R, a.L - 1);
   const int all_see = a.causal ? first_row + off + 1 : 0x7FFFFFFF;
-  const int bound = a.causal ? qrow + off : 0x7FFFFFFF;
+  // the column's last position (any of the last row's for a column that is none)
+  const int bound = a.causal ? min(qrow, a.L - 1) + off : 0x7FFFFFFF;
 
   u32x4 qop[NC][QP];
   {
@@ -166,8 +167,8 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
     if (there != ~0ull || kKeys * (t + 1) > all_see) {  // uniform
       // bits of what this column sees; those of this lane's element i of part u are
       // 8 (i / 4) + i % 4 of the word
-      const int n = bound - kKeys * t + 1;
-      const uint64_t seen = n >= 64 ? there : n <= 0 ? 0 : there & ((1ull << n) - 1);
+      const int n = bound - kKeys * t;  // (the last of them; one more might not fit an int)
+      const uint64_t seen = n >= 63 ? there : n < 0 ? 0 : there & ((2ull << n) - 1);
       const uint32_t w[2] = {(uint32_t)seen >> (4 * h), (uint32_t)(seen >> 32) >> (4 * h)};
 #pragma unroll
       for (int u = 0; u < 2; ++u)

@@ -90,3 +90,20 @@ def test_nan_key_far_from_the_largest_score(L):
     k[0][int(bt[0, 1999 // 16]), :, 1999 % 16], k[1][int(bt[0, 1999 // 16]), :, 1999 % 16] = 0x22, 132
     k[1][int(bt[0, 0]), 0, 7, 2] = 255
     assert _run(q, k, v, bt, lens).isnan().all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("L", [2, 33])
+@pytest.mark.parametrize("causal", [False, True])
+def test_several_rows_first_tile_incomplete(causal, L, D, dt):
+    """Several rows over contexts of 0, 1, 63, 64 and 65 positions, a negative length, one
+    beyond the table, and one whose first page is not there; every column sees the first
+    64 positions where there is no mask."""
+    g = torch.Generator().manual_seed(L + D)
+    lens = torch.tensor([1, 63, 64, 65, 200, 0, -2 ** 31, 2 ** 31 - 1], dtype=torch.int32)
+    q = torch.randn(len(lens), 4, L, D, generator=g).to(dt)
+    k, v = (C.random_pages(g, 120, 2, 16, D) for _ in range(2))
+    bt = torch.randperm(120, generator=g)[:13 * len(lens)].reshape(len(lens), 13).int()
+    bt[4, 0] = -1
+    _check(_run(q, k, v, bt, lens, causal), q, k, v, bt, lens, causal)
