@@ -30,7 +30,9 @@ enum { NVM_MAX_TOP_LOGPROBS = 64 };
  *                 descending order, equal ones by ascending id, and their log p
  * tokens [N] int64; top_k from 0 (both top outputs may then be NULL) to the
  * smaller of V and NVM_MAX_TOP_LOGPROBS.  Sums are float32 of few terms and
- * float64 beyond, rounded to float32 once.  A row with a NaN or +infinity, or
+ * float64 beyond, rounded to float32 once; the largest logit's term is exactly 1
+ * and summed in float64, so that results next to zero (a token that is all but
+ * certain) are no less exact than others.  A row with a NaN or +infinity, or
  * of -infinities only, has NaN log probabilities (but for tokens outside) and
  * entropy; among the largest logits a NaN is the first.  V below 2^31 - 64, N below
  * 2^24.  Rows are read in aligned pieces of 16 bytes, so up to 15 bytes around one

@@ -2,16 +2,22 @@
 // rows of logits (declared in include/nvm_logprobs.h).
 //
 // One pass over a row, or over a part of it where there are few rows.  With L =
-// log2 e as a float32 a lane keeps a reference m (the largest x L so far, so that
-// the largest term is exact; one that moves by steps of 16 only was no faster), Z = sum 2^(x L - m) and S = sum
-// 2^(x L - m) (x L - m); then log p(t) = (x_t L - m - log2 Z) / L and the entropy is
-// (log2 Z - S / Z) / L.  x L - m is one fma, whose product is exact.  A vector's few
-// terms are summed in float32, everything beyond in float64.
+// log2 e as a float32 a lane keeps its largest value X and, of all its other ones, Z =
+// sum 2^(x L - m) and S = sum 2^(x L - m) (x L - m), m being X L as a float32 (one that
+// moves by steps of 16 only was no faster).  x L - m is one fma, whose product is exact.
+// A vector's few terms are summed in float32, everything beyond in float64, where X
+// joins them as a term of 1 at the reference X L, exact in float64.  So the row's
+// largest term is exactly 1 and none of the others is lost beside it: a token that is
+// all but certain has its log probability and entropy to float32's own precision (with
+// X among the other terms both were off by 1e-7, more than they are).  At the end
+// log p(t) = (x_t L - m - log2 Z) / L and the entropy H = (log2 Z - S / Z) / L.  L is
+// log2 e less 1.3e-8 of itself, a temperature that far from 1: log p gets back the 1.3e-8 H
+// that it takes away; the entropy is off by 1.3e-8 of the logits' variance.
 //
 // That fails for values beyond 2.3e38, whose x L is none, and S for -infinity: a
 // tile whose S comes out NaN takes its terms again with the difference clamped, and
-// a part whose Z is not a positive number is read again with x - m in place of x L -
-// m (a row of the type's lowest values, or nothing but -infinities).
+// a part with an X like that is read again with x - X in place of x L - m (a row of
+// bf16's or float32's lowest values; a lane that sees nothing else suffices).
 //
 // The largest logits, in the same pass, by a wavefront each: keys of 64 bits
 // (the value's order, then the lower id), which are all different.  A threshold
@@ -23,9 +29,11 @@
 // the result does not depend on the order of anything, and rows in ascending order
 // are slow, not wrong.
 //
-// Bound: HBM for many rows (2048 x 151936 bf16: 102 us, 6.1 TB/s; top 5 124 us, 20
-// 162, 64 380, of the lists' first keys), a lane's 8.5 slots a value close behind (4 of
-// them exp's); for one row (top 5: 13 us) latency, of two launches.
+// Bound: HBM for many rows (2048 x 151936 bf16: 105 us, 5.9 TB/s; top 5 129 us, 20
+// 172, 64 391, of the lists' first keys), a lane's 10 slots a value close behind (4 of
+// them exp's, 1.5 to keep X out: 104 us for 103.5, top 5 129 for 125.5; with all of a
+// tile's other values in registers, 110 for 94, 116 and 151); for one row (top 5: 13 us)
+// latency, of two launches.
 #include <math.h>
 
 #include <algorithm>
@@ -39,6 +47,7 @@ namespace nvm {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2eOff = 1.0 - (double)kLog2e / 1.4426950408889634;
 constexpr int kWaves = 4;
 constexpr int kUnroll = 4;                    // vectors of a lane's tile
 constexpr int kMaxTop = NVM_MAX_TOP_LOGPROBS;
@@ -98,6 +107,11 @@ struct Logits {
 // The larger, NaN if one of them is.
 __device__ __forceinline__ float max_nan(float a, float b) {
   return __builtin_elementwise_maximum(a, b);
+}
+
+// The smallest of values without NaNs.
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  return __builtin_elementwise_minimum(__builtin_elementwise_minimum(a, b), c);
 }
 
 // Order of float32 values as that of unsigned integers: NaNs above +infinity,
@@ -303,16 +317,16 @@ template <int DT>
 __device__ __forceinline__ void store_row(const LogprobArgs &a, BlockState &b, int64_t row,
                                           const Part &p, float xt, int lane, int wv) {
   // (x L - m first, exactly: of values of 1e38 their difference is all that counts)
-  const double lz = log2(p.z);
+  const double lz = log2(p.z), h = (lz - p.s / p.z) / (double)kLog2e;
+  const double off = kLog2eOff * h;
   // (neither above zero nor, the entropy, below it by an error of exp2)
   auto logprob = [&](float v) {
-    const double d = ((double)v * (double)kLog2e - p.m - lz) / (double)kLog2e;
+    const double d = ((double)v * (double)kLog2e - p.m - lz) / (double)kLog2e + off;
     return d > 0.0 ? 0.f : (float)d;
   };
   if (threadIdx.x == 0) {
     const int64_t t = a.tokens[row];
     a.lp[row] = t >= 0 && t < a.V ? logprob(xt) : 0.f;
-    const double h = (lz - p.s / p.z) / (double)kLog2e;
     a.ent[row] = h < 0.0 ? 0.f : (float)h;
   }
   if (a.k > 0)
@@ -378,18 +392,18 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
     if (v0 < end) {  // uniform
       u32x4 raw[kUnroll];
       load(v0, raw);
-      float tmax[kUnroll];
+      float tmax[kUnroll], most = top;
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         float t = X::at(raw[u], 0);
 #pragma unroll
         for (int i = 1; i < PER; ++i) t = max_nan(t, X::at(raw[u], i));
         tmax[u] = t;
-        top = max_nan(top, t);
+        most = max_nan(most, t);
       }
-      const bool above = top * kLog2e > m;
+      const bool above = most * kLog2e > m;
       if (__any(above)) {
-        const float mn = fmaxf(m, top * kLog2e);
+        const float mn = fmaxf(m, most * kLog2e);
         const double d = (double)m - (double)mn, alpha = __builtin_amdgcn_exp2f((float)d);
         p.s = alpha * (p.s + p.z * d);
         p.z *= alpha;
@@ -397,10 +411,18 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
       }
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
-        float z = 0.f, s = 0.f;
+        // the vector's values and X less the largest of them, which is X from here on
+        float rest[PER], z = 0.f, s = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; i += 2) {
+          const float v = X::at(raw[u], i), w = X::at(raw[u], i + 1);
+          rest[i] = min3(top, v, w);
+          rest[i + 1] = __builtin_amdgcn_fmed3f(top, v, w);
+          top = max_nan(max_nan(top, v), w);
+        }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const float d = fmaf(X::at(raw[u], i), kLog2e, -m);
+          const float d = fmaf(rest[i], kLog2e, -m);
           const float e = __builtin_amdgcn_exp2f(d);
           z += e;
           s = fmaf(e, d, s);
@@ -409,7 +431,7 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
           s = 0.f;
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
-            const float d = fmaf(X::at(raw[u], i), kLog2e, -m);
+            const float d = fmaf(rest[i], kLog2e, -m);
             s = fmaf(__builtin_amdgcn_exp2f(d), fmaxf(d, -1e30f), s);
           }
         }
@@ -464,9 +486,14 @@ __global__ __launch_bounds__(64 * kWaves) void token_logprobs_kernel(LogprobArgs
     if (a.k > 0 && ((it == 0 && rounds > 2) || (it == 3 && rounds > 6)))
       block_threshold(s_b, list, a.k, lane, wv);
   }
-  if (p.z > 0.0) p.m = (double)m;
-  // (a sum that is none, or nothing of values that are there)
-  if (__any(p.z > 0.0 ? !(p.z < INFINITY) : top != -INFINITY)) {
+  // (top: none of the values that are there, or one whose product with L is one)
+  if (!__any(top != -INFINITY && !(fabsf(top * kLog2e) < INFINITY))) {
+    if (top != -INFINITY) {
+      const double r = (double)top * (double)kLog2e, d = (double)m - r;
+      const double f = __builtin_amdgcn_exp2f((float)d);
+      p = {r, 1.0 + f * p.z, f * (p.s + p.z * d)};
+    }
+  } else {
     p = {-1e39, 0.0, 0.0};
     top = -3.402823466e38f;
     for (int v0 = first + wv * kTile; v0 < end; v0 += kWaves * kTile) {
