@@ -25,9 +25,11 @@ class MxPages:
     """Pages ``[P, num_kv_heads, page_size, D]`` of keys or values in MXFP4:
     ``codes`` uint8 ``[..., D / 2]`` (E2M1, the even value in the low half) and
     ``scales`` uint8 ``[..., D / 32]``, byte b standing for ``2 ** (b - 127)``,
-    255 for NaN.  Both contiguous: the store writes into them."""
+    255 for NaN.  Both contiguous: the store writes into them, wherever they lie at
+    the call."""
 
-    __slots__ = ("codes", "scales", "shape", "device", "_index", "_at")
+    # _at: the addresses that were checked
+    __slots__ = ("_codes", "_scales", "shape", "device", "_index", "_at")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
@@ -45,11 +47,30 @@ class MxPages:
             raise ValueError("MxPages: codes and scales must be contiguous")
         if codes.data_ptr() % 16 or scales.data_ptr() % 16:
             raise ValueError("MxPages: codes and scales must be 16-byte aligned")
-        self.codes, self.scales = codes, scales
+        self._codes, self._scales = codes, scales
         self.shape = torch.Size((*codes.shape[:3], D))
         self.device = codes.device
         self._index = codes.get_device()
         self._at = (codes.data_ptr(), scales.data_ptr())
+
+    @property
+    def codes(self) -> torch.Tensor:
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        return self._scales
+
+    def _refresh(self) -> None:
+        """Checks again what has got another storage (``set_``, ``data``)."""
+        codes, scales = self._codes, self._scales
+        if (codes.data_ptr(), scales.data_ptr()) != self._at:
+            shape = self.shape
+            self.__init__(codes, scales)
+            if self.shape != shape:
+                now, self.shape = self.shape, shape
+                self._at = (0, 0)
+                raise ValueError(f"MxPages: pages of {tuple(shape)} have become {tuple(now)}")
 
     @classmethod
     def zeros(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int,
@@ -75,6 +96,8 @@ def _check_pages(op: str, key_pages: MxPages, value_pages: MxPages) -> int:
     """The one GPU of both."""
     if type(key_pages) is not MxPages or type(value_pages) is not MxPages:
         raise ValueError(f"{op}: key_pages and value_pages must be MxPages")
+    key_pages._refresh()
+    value_pages._refresh()
     if key_pages.shape != value_pages.shape:
         raise ValueError(f"{op}: key and value pages differ in shape")
     index = key_pages._index

@@ -107,3 +107,33 @@ def test_several_rows_first_tile_incomplete(causal, L, D, dt):
     bt = torch.randperm(120, generator=g)[:13 * len(lens)].reshape(len(lens), 13).int()
     bt[4, 0] = -1
     _check(_run(q, k, v, bt, lens, causal), q, k, v, bt, lens, causal)
+
+
+def test_store_into_the_pages_present_storage():
+    """Codes and scales with another storage (as after moving a cache): the step writes
+    there, and nothing into the storage before."""
+    from nano_vllm_metal_amd import MxPages, paged_kv_read_mx, qk_norm_rope_store_mx
+
+    T, D = 5, 64
+    g = torch.Generator(device=DEV).manual_seed(1)
+    qkv = torch.randn(T, 4 * D, device=DEV, generator=g).bfloat16()
+    one, pos = torch.ones(D, device=DEV).bfloat16(), torch.arange(T, device=DEV).int()
+    cos, sin = torch.ones(9, D // 2, device=DEV), torch.zeros(9, D // 2, device=DEV)
+
+    def store(kp, vp):
+        qk_norm_rope_store_mx(qkv, 2, 1, D, one, one, 1e-6, pos, cos, sin, pos % 3, pos, kp, vp)
+
+    want = [MxPages.zeros(3, 1, 16, D, DEV) for _ in range(2)]
+    store(*want)
+    got = [MxPages.zeros(3, 1, 16, D, DEV) for _ in range(2)]
+    before = []
+    for p in got:
+        for t in (p.codes, p.scales):
+            before.append(t.detach().view(t.shape))
+            t.data = torch.zeros_like(t)
+    store(*got)
+    for a, b in zip(got, want):
+        assert torch.equal(a.codes, b.codes) and torch.equal(a.scales, b.scales) and b.codes.any()
+    assert not any(t.any() for t in before)
+    for x, y in zip(paged_kv_read_mx(*got, pos % 3, pos), paged_kv_read_mx(*want, pos % 3, pos)):
+        assert torch.equal(x, y)
