@@ -18,6 +18,8 @@ import torch
 from . import _lib
 from .mx import MX_BLOCK, MxTensor, _current_device, _raw_stream, mx_dequantize
 
+_INT_TYPES = {torch.uint8, torch.int8, torch.uint16, torch.int16, torch.uint32, torch.int32,
+              torch.int64}
 _CODES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # nvm_kv_dtype
 
 
@@ -109,10 +111,10 @@ def _check_pages(op: str, key_pages: MxPages, value_pages: MxPages) -> int:
 def _ints(op: str, name: str, t: torch.Tensor, n: int, index: int) -> torch.Tensor:
     """`n` int32 values in a row, on device `index`."""
     if t.dtype != torch.int32:
-        if t.dtype == torch.int64:  # (what 32 bits would wrap stays outside)
-            t = t.clamp(-1, 0x7FFFFFFF)
-        elif t.dtype.is_floating_point or t.dtype.is_complex:
-            raise ValueError(f"{op}: {name} must be integers, got {t.dtype}")
+        if t.dtype not in _INT_TYPES:
+            raise ValueError(f"{op}: {name} must be integers of at most 63 bits, got {t.dtype}")
+        if t.dtype in (torch.int64, torch.uint32):  # (what 32 bits would wrap stays outside)
+            t = t.to(torch.int64).clamp(-1, 0x7FFFFFFF)
         t = t.to(torch.int32)
     if t.numel() != n:
         raise ValueError(f"{op}: {name} must have {n} elements, got {t.numel()}")

@@ -137,3 +137,22 @@ def test_store_into_the_pages_present_storage():
     assert not any(t.any() for t in before)
     for x, y in zip(paged_kv_read_mx(*got, pos % 3, pos), paged_kv_read_mx(*want, pos % 3, pos)):
         assert torch.equal(x, y)
+
+
+def test_unsigned_indices():
+    """Page ids and lengths of 32 unsigned bits: those beyond 2^31 are no page, and a
+    length beyond everything."""
+    from nano_vllm_metal_amd import paged_attention_mx, paged_kv_read_mx
+
+    g = torch.Generator().manual_seed(2)
+    k, v = (C.random_pages(g, 4, 2, 16, 64) for _ in range(2))
+    kp, vp = _pages(k), _pages(v)
+    ids = torch.tensor([1, 2 ** 31 + 1, 2 ** 32 - 1, 3], dtype=torch.uint32, device=DEV)
+    slots = torch.tensor([3, 3, 3, 3], dtype=torch.uint32, device=DEV)
+    got = paged_kv_read_mx(kp, vp, ids, slots)[0]
+    want = paged_kv_read_mx(kp, vp, torch.tensor([1, -1, -1, 3], device=DEV), slots.int())[0]
+    assert torch.equal(got, want) and got[0].any() and not got[1:3].any()
+    q = torch.randn(1, 4, 1, 64, generator=g).bfloat16()
+    bt, lens = torch.tensor([[2, 0]], dtype=torch.int32), torch.tensor([2 ** 31 + 7], dtype=torch.uint32)
+    got = paged_attention_mx(q.to(DEV), kp, vp, bt.to(DEV), lens.to(DEV)).cpu()
+    _check(got, q, k, v, bt, torch.tensor([32]))

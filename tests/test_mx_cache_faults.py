@@ -36,3 +36,21 @@ def test_pages_follow_their_tensors():
     refused("MxPages: codes")
     p.scales.data = _bytes(3, 2, 16, 2)
     refused("GPU only")
+
+
+def test_indices_of_every_type():
+    """Values that 32 bits do not hold stay beyond every page, position and length;
+    types that cannot be converted so are refused."""
+    from nano_vllm_metal_amd.mx_cache import _ints
+
+    for dt in (torch.uint8, torch.int8, torch.uint16, torch.int16, torch.uint32, torch.int32,
+               torch.int64):
+        got = _ints("op", "slots", torch.tensor([0, 1, 100], dtype=dt), 3, -1)
+        assert got.dtype == torch.int32 and got.tolist() == [0, 1, 100]
+    big = torch.tensor([2 ** 31, 2 ** 32 - 1, 2 ** 31 - 1], dtype=torch.uint32)
+    assert _ints("op", "slots", big, 3, -1).tolist() == [2 ** 31 - 1] * 3
+    big = torch.tensor([2 ** 31, 2 ** 32 + 5, -2 ** 32], dtype=torch.int64)
+    assert _ints("op", "slots", big, 3, -1).tolist() == [2 ** 31 - 1, 2 ** 31 - 1, -1]
+    for dt in (torch.uint64, torch.bool, torch.float32, torch.complex64):
+        with pytest.raises(ValueError, match="slots must be integers"):
+            _ints("op", "slots", torch.zeros(3, dtype=dt), 3, -1)
