@@ -500,7 +500,8 @@ __global__ __launch_bounds__(kRowThreads) void mx_combine_kernel(const float *__
     store_out(out, out_dt, n * DH + PD * lane + d, L == 0.f ? 0.f : acc[d] / L);
 }
 
-constexpr int64_t kMaxRows = 0x3FFFFFF;  // query rows of a call: wavefronts of a launch
+// query rows of a call: wavefronts of a launch, which has below 2^32 threads in whole blocks
+constexpr int64_t kMaxRows = 0x3FFFFFC;
 
 // Wavefronts a block and most splits of a context (which the kernel shares out by
 // length).  us, 32/4 heads of 128: 64 requests of 4096 positions in blocks of 8 x 1

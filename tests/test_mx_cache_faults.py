@@ -54,3 +54,21 @@ def test_indices_of_every_type():
     for dt in (torch.uint64, torch.bool, torch.float32, torch.complex64):
         with pytest.raises(ValueError, match="slots must be integers"):
             _ints("op", "slots", torch.zeros(3, dtype=dt), 3, -1)
+
+
+def test_most_query_rows():
+    """A wavefront a query row: more than 2^32 - 256 threads are refused by name."""
+    import ctypes
+
+    from nano_vllm_metal_amd import _lib
+
+    lib, size = _lib.load(), ctypes.c_size_t(7)
+
+    def ask(rows):
+        return lib.nvm_paged_attention_mx_workspace_size(rows, 1, 32, 1, 16, 1, 1, ctypes.byref(size))
+
+    most = (2 ** 32 - 256) // 64
+    assert ask(most) == _lib.NVM_OK and size.value == 0
+    for rows in (most + 1, most + 3, 2 ** 26):
+        assert ask(rows) == _lib.NVM_ERR_UNSUPPORTED
+        assert "too many query rows" in lib.nvm_last_error().decode()
