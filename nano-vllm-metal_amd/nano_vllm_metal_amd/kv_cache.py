@@ -18,7 +18,7 @@ from typing import Dict, List, Sequence, Tuple
 
 import torch
 
-from .mx import mx_quantize
+from .mx import MX_DTYPES, mx_quantize
 from .mx_cache import MxPages, paged_kv_read_mx
 
 
@@ -107,17 +107,18 @@ class PagedKVCache:
               slots: torch.Tensor) -> None:
         """Store ``k``/``v [B, L, num_kv_heads, D]`` at the mapped slots (for
         callers that compute k/v themselves; the model's fused q/k kernel
-        stores them directly)."""
-        kk = k.reshape(-1, self.num_kv_heads, self.head_dim).to(self.dtype)
-        vv = v.reshape(-1, self.num_kv_heads, self.head_dim).to(self.dtype)
+        stores them directly).  Four bits are taken of the values as they come,
+        without a rounding to the cache's dtype before it (of float64 ones as
+        float32)."""
         page_ids, slots = page_ids.long(), slots.long()
-        for pages, x in ((self.key_pages[layer], kk), (self.value_pages[layer], vv)):
+        for pages, x in ((self.key_pages[layer], k), (self.value_pages[layer], v)):
+            x = x.reshape(-1, self.num_kv_heads, self.head_dim)
             if self.kv_bits == 4:
-                t = mx_quantize(x, "mxfp4")
+                t = mx_quantize(x if x.dtype in MX_DTYPES else x.float(), "mxfp4")
                 pages.codes[page_ids, :, slots] = t.codes
                 pages.scales[page_ids, :, slots] = t.scales
             else:
-                pages[page_ids, :, slots, :] = x
+                pages[page_ids, :, slots, :] = x.to(self.dtype)
 
     def read(self, layer: int, page_ids: torch.Tensor, slots: torch.Tensor
              ) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -156,3 +156,25 @@ def test_unsigned_indices():
     bt, lens = torch.tensor([[2, 0]], dtype=torch.int32), torch.tensor([2 ** 31 + 7], dtype=torch.uint32)
     got = paged_attention_mx(q.to(DEV), kp, vp, bt.to(DEV), lens.to(DEV)).cpu()
     _check(got, q, k, v, bt, torch.tensor([32]))
+
+
+@pytest.mark.parametrize("dt", [torch.float64, torch.float32, torch.float16, torch.bfloat16])
+def test_cache_write_rounds_once(dt):
+    """Values next to a border of E2M1 (2.5 and 2.5 + 2^-10 in a block of 6: 2 and 3), which
+    a rounding to bf16 before would put on it."""
+    from nano_vllm_metal_amd import PagedKVCache
+    from oracle import mx_oracle as MX
+
+    cache = PagedKVCache(1, 2, 64, 3, 16, torch.bfloat16, DEV, kv_bits=4)
+    x = torch.randn(1, 5, 2, 64, generator=torch.Generator().manual_seed(3), dtype=torch.float64)
+    x[..., ::4], x[..., 1::4] = 6.0, 2.5 + 2.0 ** -10
+    x[0, 2:] *= 2.0 ** -5
+    x = x.to(dt)
+    ids, slots = torch.tensor([0, 0, 2, 1, 1]), torch.tensor([0, 1, 15, 3, 4])
+    cache.write(0, x.to(DEV), -x.to(DEV), ids.to(DEV), slots.to(DEV))
+    for pages, y in ((cache.key_pages[0], x), (cache.value_pages[0], -x)):
+        c, b = MX.quantize(y.reshape(5, 2, 64).double(), "mxfp4")
+        assert torch.equal(MX.pack(c, "mxfp4"), pages.codes.cpu()[ids, :, slots])
+        assert torch.equal(b.to(torch.uint8), pages.scales.cpu()[ids, :, slots])
+    if dt == torch.float32:
+        assert (cache.read(0, ids.to(DEV), slots.to(DEV))[0][0, :, 1::4] == 3).all()
