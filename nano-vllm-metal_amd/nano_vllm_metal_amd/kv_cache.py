@@ -103,14 +103,24 @@ class PagedKVCache:
         return (torch.tensor(pages, dtype=torch.int32, device=dev),
                 torch.tensor(slots, dtype=torch.int32, device=dev))
 
+    def _mapped(self, page_ids: torch.Tensor, slots: torch.Tensor):
+        """Which slots exist, and 64-bit indices of theirs (0 for others): indexing
+        out of bounds would end the process, and below zero it counts from the end."""
+        page_ids, slots = page_ids.long(), slots.long()
+        there = ((page_ids >= 0) & (page_ids <= self.num_pages) & (slots >= 0)
+                 & (slots < self.page_size))
+        return there, page_ids * there, slots * there
+
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, page_ids: torch.Tensor,
               slots: torch.Tensor) -> None:
         """Store ``k``/``v [B, L, num_kv_heads, D]`` at the mapped slots (for
         callers that compute k/v themselves; the model's fused q/k kernel
         stores them directly).  Four bits are taken of the values as they come,
         without a rounding to the cache's dtype before it (of float64 ones as
-        float32)."""
-        page_ids, slots = page_ids.long(), slots.long()
+        float32).  Slots outside the pages are not stored (their values go to the
+        scratch page)."""
+        there, page_ids, slots = self._mapped(page_ids, slots)
+        page_ids = torch.where(there, page_ids, self.scratch_page)
         for pages, x in ((self.key_pages[layer], k), (self.value_pages[layer], v)):
             x = x.reshape(-1, self.num_kv_heads, self.head_dim)
             if self.kv_bits == 4:
@@ -123,12 +133,13 @@ class PagedKVCache:
     def read(self, layer: int, page_ids: torch.Tensor, slots: torch.Tensor
              ) -> Tuple[torch.Tensor, torch.Tensor]:
         """What the mapped slots hold: ``k, v [T, num_kv_heads, D]`` of the
-        cache's dtype."""
+        cache's dtype.  Slots outside the pages give zeros."""
         kp, vp = self.key_pages[layer], self.value_pages[layer]
         if self.kv_bits == 4:
             return paged_kv_read_mx(kp, vp, page_ids, slots, self.dtype)
-        page_ids, slots = page_ids.long(), slots.long()
-        return kp[page_ids, :, slots, :], vp[page_ids, :, slots, :]
+        there, page_ids, slots = self._mapped(page_ids, slots)
+        gone = ~there[:, None, None]
+        return tuple(pages[page_ids, :, slots, :].masked_fill(gone, 0) for pages in (kp, vp))
 
     def advance(self, seq_ids: Sequence[int], n_new: int) -> None:
         for s in seq_ids:

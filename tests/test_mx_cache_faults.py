@@ -72,3 +72,22 @@ def test_most_query_rows():
     for rows in (most + 1, most + 3, 2 ** 26):
         assert ask(rows) == _lib.NVM_ERR_UNSUPPORTED
         assert "too many query rows" in lib.nvm_last_error().decode()
+
+
+def test_cache_slots_outside_the_pages():
+    """Sixteen bits, on the CPU: slots that are not there are not stored, nor taken for
+    others counted from the end, and read as zeros."""
+    from nano_vllm_metal_amd import PagedKVCache
+
+    cache = PagedKVCache(1, 2, 8, 3, 4, torch.float32, "cpu")
+    x = torch.arange(1.0, 1 + 6 * 16).reshape(1, 6, 2, 8)
+    ids = torch.tensor([1, -1, 0, 4, 2, 2 ** 40])
+    slots = torch.tensor([3, 0, -1, 0, 4, 1])
+    cache.write(0, x, 2 * x, ids, slots)
+    want = torch.zeros(3, 2, 4, 8)
+    want[1, :, 3] = x[0, 0]
+    assert torch.equal(cache.key_pages[0][:3], want)
+    assert torch.equal(cache.value_pages[0][:3], 2 * want)
+    k, v = cache.read(0, ids, slots)
+    assert torch.equal(k[0], x[0, 0]) and torch.equal(v[0], 2 * x[0, 0])
+    assert k.shape == (6, 2, 8) and not k[1:].any() and not v[1:].any()
