@@ -19,6 +19,7 @@ the checkpoint directory; loaded with ``local_files_only``, no hub access).
 
 from __future__ import annotations
 
+import numbers
 import time
 from collections import deque
 from dataclasses import dataclass, field
@@ -110,8 +111,11 @@ def _pick(logits: torch.Tensor, sp: SamplingParams):
 
 
 def _check_top(name: str, n: Optional[int], vocab: int) -> None:
-    if n is not None and not 0 <= n <= min(MAX_TOP_LOGPROBS, vocab):
-        raise ValueError(f"{name} must be in [0, {min(MAX_TOP_LOGPROBS, vocab)}], got {n}")
+    """Before anything runs: a refusal in the middle of a step leaves its requests'
+    pages in the cache."""
+    most = min(MAX_TOP_LOGPROBS, vocab)
+    if n is not None and not (isinstance(n, numbers.Integral) and 0 <= n <= most):
+        raise ValueError(f"{name} must be a whole number in [0, {most}], got {n!r}")
 
 
 class _DecodeGraph:

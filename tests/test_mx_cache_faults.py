@@ -1,4 +1,5 @@
-"""The 4-bit cache without a GPU: calls that went wrong before any kernel ran."""
+"""The 4-bit cache and log probabilities without a GPU: calls that went wrong before
+any kernel ran."""
 
 from __future__ import annotations
 
@@ -91,3 +92,16 @@ def test_cache_slots_outside_the_pages():
     k, v = cache.read(0, ids, slots)
     assert torch.equal(k[0], x[0, 0]) and torch.equal(v[0], 2 * x[0, 0])
     assert k.shape == (6, 2, 8) and not k[1:].any() and not v[1:].any()
+
+
+def test_counts_of_alternatives_are_whole_numbers():
+    """Refused before a request has pages, which it would keep."""
+    import numpy as np
+
+    from nano_vllm_metal_amd.llm import _check_top
+
+    for n in (None, 0, 5, 64, np.int64(3)):
+        _check_top("x", n, 1000)
+    for n in (2.5, 3.0, "3", float("nan"), [1], torch.tensor(2.0)):
+        with pytest.raises(ValueError, match="x must be a whole number"):
+            _check_top("x", n, 1000)
