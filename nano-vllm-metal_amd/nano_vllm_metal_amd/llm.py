@@ -115,7 +115,7 @@ def _check_top(name: str, n: Optional[int], vocab: int) -> None:
     pages in the cache."""
     most = min(MAX_TOP_LOGPROBS, vocab)
     if n is not None and not (isinstance(n, numbers.Integral) and 0 <= n <= most):
-        raise ValueError(f"{name} must be a whole number in [0, {most}], got {n!r}")
+        raise ValueError(f"{name} must be in [0, {most}], a whole number, got {n!r}")
 
 
 class _DecodeGraph:

@@ -103,5 +103,5 @@ def test_counts_of_alternatives_are_whole_numbers():
     for n in (None, 0, 5, 64, np.int64(3)):
         _check_top("x", n, 1000)
     for n in (2.5, 3.0, "3", float("nan"), [1], torch.tensor(2.0)):
-        with pytest.raises(ValueError, match="x must be a whole number"):
+        with pytest.raises(ValueError, match="x must be in .*a whole number"):
             _check_top("x", n, 1000)
