@@ -1,9 +1,12 @@
-"""GPU tests of the 4-bit cache where single results went wrong: weights that lost
-bits.  Against the 64-bit results and bounds of ``oracle/mx_cache_oracle.py``, and
-one rounding of the result.
+"""GPU tests of the 4-bit cache where results went wrong or no test could have told:
+weights that lost bits, NaNs lost between splits, incomplete first tiles, storage
+exchanged under the pages, indices of unusual types.  Against the 64-bit results and
+bounds of ``oracle/mx_cache_oracle.py``, and one rounding of the result.
 """
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
@@ -178,3 +181,33 @@ def test_cache_write_rounds_once(dt):
         assert torch.equal(b.to(torch.uint8), pages.scales.cpu()[ids, :, slots])
     if dt == torch.float32:
         assert (cache.read(0, ids.to(DEV), slots.to(DEV))[0][0, :, 1::4] == 3).all()
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("L", [1, 2])
+@pytest.mark.parametrize("s,top", [(13, 100), (22, 2000), (27, 5), (40, 2999), (100, 1500)])
+def test_small_weights_are_all_of_the_result(s, top, L, D, dt):
+    """One position of a weight of 1 and a value of zero, 2999 of weights 2^-s and values
+    of one size: the result is these alone, and is compared relative to itself.  With
+    u = 2^-23 their exponents are off by u (|s| + |m|) log2 e and (D + 4) u |s| (2^-9 at
+    s = 100), exp2 by 2 u, the parts of a weight by 2^-16, sums of n terms by
+    2 n u; then one rounding."""
+    n, u = 3000, 2.0 ** -23
+    g = torch.Generator().manual_seed(s)
+    q = torch.ones(1, 2, L, D).to(dt)
+    k, v = ((torch.full((190, 1, 16, D // 2), 0x22, dtype=torch.uint8),
+             torch.full((190, 1, 16, D // 32), 127, dtype=torch.uint8)) for _ in range(2))
+    bt = torch.randperm(190, generator=g)[:188][None].int()
+    lens = torch.tensor([n], dtype=torch.int32)
+    at = int(bt[0, top // 16]), 0, top % 16
+    k[1][at] = 128          # a score of D above the others
+    v[1][:] = 127 + s - 11  # (results of about 1.5)
+    v[0][at] = 0
+    scale = s * math.log(2.0) / D
+    got = _run(q, k, v, bt, lens, False, scale).double()
+    w = 2.0 ** -s
+    want = (n - 1) * w / (1 + (n - 1) * w) * 2.0 ** (s - 11)
+    m = 2 * s * math.log(2.0)  # the largest score; the others' are half of it
+    rel = (1.5 * m * 1.45 + (D + 4) * m + 2) * u + 2.0 ** -16 + 2 * n * u + torch.finfo(dt).eps / 2
+    assert ((got - want).abs() <= rel * want).all()
