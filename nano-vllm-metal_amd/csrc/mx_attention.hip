@@ -75,7 +75,8 @@ __global__ __launch_bounds__(kRowThreads) void mx_rows_kernel(MxAttnArgs a, int6
   const bool on = lane < n8;
   const int64_t len = a.lens[b];
   const int64_t cap = min(len, (int64_t)a.max_pages * a.page_size);
-  const int last = (int)(a.causal ? min(cap, i + len - a.L + 1) : cap);
+  // (from 0 on: below -2^31, of a length next to it, an int would come out positive)
+  const int last = (int)max((int64_t)0, a.causal ? min(cap, i + len - a.L + 1) : cap);
   const int32_t *bt = a.bt + (int64_t)b * a.max_pages;
   float qv[8], ov[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll

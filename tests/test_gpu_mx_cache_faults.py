@@ -211,3 +211,18 @@ def test_small_weights_are_all_of_the_result(s, top, L, D, dt):
     m = 2 * s * math.log(2.0)  # the largest score; the others' are half of it
     rel = (1.5 * m * 1.45 + (D + 4) * m + 2) * u + 2.0 ** -16 + 2 * n * u + torch.finfo(dt).eps / 2
     assert ((got - want).abs() <= rel * want).all()
+
+
+@pytest.mark.parametrize("D", [32, 96, 256])
+@pytest.mark.parametrize("causal", [True, False])
+def test_lengths_next_to_the_least_integer(causal, D):
+    """Other head dims, several rows: lengths from -2^31 on are empty contexts (the first
+    rows' bounds lie below -2^31), those up to 2^31 - 1 all of the table."""
+    g = torch.Generator().manual_seed(D)
+    lens = torch.tensor([-2 ** 31, -2 ** 31 + 3, -1, 2 ** 31 - 1, 30], dtype=torch.int32)
+    q = torch.randn(5, 4, 6, D, generator=g).bfloat16()
+    k, v = (C.random_pages(g, 20, 2, 16, D) for _ in range(2))
+    bt = torch.randperm(20, generator=g)[:15].reshape(5, 3).int()
+    got = _run(q, k, v, bt, lens, causal)
+    assert (got[:3] == 0).all()
+    _check(got, q, k, v, bt, lens, causal)
