@@ -64,15 +64,13 @@ class MxPages:
         return self._scales
 
     def _refresh(self) -> None:
-        """Checks again what has got another storage (``set_``, ``data``)."""
-        codes, scales = self._codes, self._scales
-        if (codes.data_ptr(), scales.data_ptr()) != self._at:
-            shape = self.shape
-            self.__init__(codes, scales)
-            if self.shape != shape:
-                now, self.shape = self.shape, shape
-                self._at = (0, 0)
-                raise ValueError(f"MxPages: pages of {tuple(shape)} have become {tuple(now)}")
+        """Checks codes and scales that lie elsewhere than before (``set_``, ``data``)."""
+        shape = self.shape
+        self.__init__(self._codes, self._scales)
+        if self.shape != shape:
+            now, self.shape = self.shape, shape
+            self._at = (0, 0)
+            raise ValueError(f"MxPages: pages of {tuple(shape)} have become {tuple(now)}")
 
     @classmethod
     def zeros(cls, num_pages: int, num_kv_heads: int, page_size: int, head_dim: int,
@@ -98,8 +96,10 @@ def _check_pages(op: str, key_pages: MxPages, value_pages: MxPages) -> int:
     """The one GPU of both."""
     if type(key_pages) is not MxPages or type(value_pages) is not MxPages:
         raise ValueError(f"{op}: key_pages and value_pages must be MxPages")
-    key_pages._refresh()
-    value_pages._refresh()
+    for p in (key_pages, value_pages):
+        codes, scales = p._at
+        if p._codes.data_ptr() != codes or p._scales.data_ptr() != scales:
+            p._refresh()
     if key_pages.shape != value_pages.shape:
         raise ValueError(f"{op}: key and value pages differ in shape")
     index = key_pages._index
