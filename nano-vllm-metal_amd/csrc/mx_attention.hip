@@ -15,15 +15,19 @@
 //     a score exceeds it.
 //   * O^T += V^T . P^T: the scores' layout is that of the operand P^T.  Value rows
 //     go to LDS as bf16 and come back transposed (ds_read_b64_tr_b16).  P is two
-//     bf16 parts (2^-17): with up to eight query heads the MFMA's other eight
-//     columns hold the second part, so both cost one product.
+//     bf16 parts (2^-17 of each weight, below a 16-bit output's rounding by 2^6 or
+//     more, and for a float32 one what a third product would take away): with up to
+//     eight query heads the MFMA's other eight columns hold the second part, so both
+//     cost one product.
 //   * A masked position has a finite scale and any codes: its weight is zero, and
 //     zero times a finite value is zero.
 //   The next tile's keys are requested when this one's are converted, the next
 //   values when these are in LDS.  Bound: for long contexts HBM (16 requests of 40000
 //   positions, 32/4 heads of 128: 62 us, 5.5 TB/s of codes and scales); for short ones
-//   the chain of trips to memory, code among them: one request of 700 positions 6.9 us
-//   with the merge, of 100 4.1 without.
+//   the chain of trips to memory, code among them: one request of 700 positions 7.0 us
+//   with the merge, of 100 4.0 without (in a table for 4096 positions, as a captured
+//   step has, 6.9: the merge's launch goes by the table).  With f16 queries, 128 dims and
+//   blocks of eight wavefronts six registers spill.
 // mx_rows_kernel: any head dim, one wavefront per query row.  A position's row
 //   of codes goes to a group of GL lanes (eight values, one dword, a lane), so
 //   64 / GL positions are in flight side by side, each group with a running

@@ -10,8 +10,8 @@
 //   rounding border of E2M1 is a quarter of itself off if it falls on the wrong
 //   side, and float32 sums in another order put one in some 10^5 there.  That
 //   concerns Hkv of the Hq + 2 Hkv heads.
-// paged_kv_read_mx_kernel: eight values a lane (4096 rows of 4 heads of 128: 5.4 us,
-//   1.9 TB/s, of which the launch is 1.4).
+// paged_kv_read_mx_kernel: eight values a lane (4096 rows of 4 heads of 128: 4.3 us,
+//   2.4 TB/s, of which the launch is 1.4; a dword of codes a lane keeps it from more).
 #include <math.h>
 
 #include "common.h"
@@ -107,8 +107,10 @@ __device__ __forceinline__ void norm_rope(u32x4 x, u32x4 p, u32x4 wx, u32x4 wp, 
 
 // Items of a token: U query heads each (the last may be fewer), then a key or a
 // value head each.  Bound: for one token the launch and one load's latency, 2 us;
-// for 4096 of 32/4 heads of 128 the 80 MB read and written, 19 us, 4.2 TB/s.  (Loads
-// with the non-temporal hint: 25.4 -> 24.3 us with the read of the rows.)
+// for 4096 of 32/4 heads of 128 the 80 MB read and written, 20 us, 4.0 TB/s, and with
+// keys and values handed on and all of it in float32 (a prompt's first pass) 130 MB,
+// 29.4 us, 4.4 TB/s.  (Loads with the non-temporal hint: 25.4 -> 24.3 us with the read
+// of the rows.)
 template <int DT, bool F32, int GL, int U>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_store_mx_kernel(StoreArgs a) {
   using A = Act<DT>;

@@ -15,8 +15,12 @@
 //     of LDS transposed (ds_read_b64_tr_b16).  P is two bf16 parts: a weight loses
 //     2^-17 of itself, so a result at most 2^-16 of its column's largest value.  (One f16
 //     part would lose 2^-11 of each weight, which shows beside a bf16 output's own 2^-8
-//     where values cancel; it took 193 us where two take 249: 2048 rows over 6144
+//     where values cancel; it took 193 us where two take 247: 2048 rows over 6144
 //     positions, 32/4 heads of 128.)
+// Bound, at that size: the matrix cores are busy 52 % of the time and the vector
+// instructions fill as much, with two wavefronts a SIMD to overlap them; LDS is active 54 %
+// of it, half of that for bank conflicts of the keys' reads and of the stores.  With a
+// float32 query of 128 dims, three parts, nine registers spill.
 // Positions that are not there are row 0 with a finite scale, and masked.  So are the
 // scales of value blocks of NaNs, since a zero weight would not hide them from rows
 // that do not see their position; those that do are told at the end.
@@ -46,6 +50,7 @@ __global__ __launch_bounds__(64 * kCW, 2) void mx_prefill_kernel(MxAttnArgs a, i
   constexpr int NC = DH / 16;  // steps of a score MFMA
   constexpr int NT = DH / 32;  // tiles of the output
   // LDS pitch of a row: the four rows of a transposed read lie in banks of their own
+  // (with 8 in place of 16 in pairs, and the keys' reads apart: 249 us for 247)
   constexpr int VP = DH + 16;
   constexpr int NB = DH / 32;  // scales of a row; dwords of codes of a quarter of it
   static_assert(4 * kKeys == 64 * kCW, "a quarter of a row a thread");
